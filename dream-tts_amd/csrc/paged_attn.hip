@@ -1,0 +1,467 @@
+// Attention of each sequence's new tokens over its paged f16 cache: out_i = sum_j softmax_j(scale
+// q_i . k_j) v_j over p_i - window < j <= p_i, a ragged batch of chunks and single tokens.
+//
+// A row is one (new token, query head). The heads / n_kv query heads of a kv head read the same keys,
+// so rows are numbered token * gqa + head within (sequence, kv head), and a tile of 16 consecutive
+// rows goes to one workgroup (paged_attn_rows). A query's scores, softmax state (running maximum,
+// running sum) and output sums are f32; q, k, v are f16 as the cache and the matrix cores hold them;
+// the weights e^(s - max) are rounded to f16 for the second product (at most 2^-11 of each weight,
+// as the output's own rounding), and the output is rounded once.
+#include "paged.hpp"
+
+namespace dtts {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct AttnArgs {
+    PagedBatch batch;
+    const half_t *q, *k, *v;
+    half_t *out;
+    float *part;       // per (row, chunk): D weighted sums, the weight sum, the maximum (log2)
+    int64_t q_stride;  // elements between tokens
+    int heads, n_kv, gqa, window;
+    float scale2;      // scale * log2(e): the softmax runs in base 2
+    int chunk, nsplit; // keys per chunk, chunks at most (the last takes what is left)
+};
+
+// The keys that sequence s's rows see, in chunks: [lo, hi), lo a multiple of 64, `n` chunks. hi stops
+// at the table's end, whatever the context says.
+struct Span {
+    int lo, hi, n;
+    __device__ __forceinline__ Span(const AttnArgs &a, int s, int n_new, int ctx) {
+        const int64_t cap = static_cast<int64_t>(a.batch.max_pages) << a.batch.page_shift;
+        hi = ctx < 0 ? 0 : ctx < cap ? ctx : static_cast<int>(cap);
+        lo = a.window > 0 && ctx - n_new - a.window + 1 > 0 ? (ctx - n_new - a.window + 1) & ~63 : 0;
+        if (lo > hi) lo = hi & ~63;
+        n = (hi - lo + a.chunk - 1) / a.chunk;
+        n = n < 1 ? 1 : n > a.nsplit ? a.nsplit : n;
+    }
+    __device__ __forceinline__ void chunk_keys(const AttnArgs &a, int c, int &k0, int &k1) const {
+        k0 = lo + c * a.chunk;
+        k1 = c == n - 1 ? hi : k0 + a.chunk;
+    }
+};
+
+// The tile-th tile of `rows` rows over the sequences, counted in order (every wave for itself).
+// Returns the sequence, or -1 past the last; `at` is the tile's place in it.
+__device__ __forceinline__ int find_tile(const AttnArgs &a, int rows, int tile, int &at) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < a.batch.b; s0 += 64) {
+        int tiles = 0;
+        if (s0 + lane < a.batch.b) {
+            int first, n;
+            a.batch.rows(s0 + lane, first, n);
+            tiles = static_cast<int>((static_cast<int64_t>(n) * a.gqa + rows - 1) / rows);
+        }
+        int upto = tiles;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int v = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += v;
+        }
+        const uint64_t past = __ballot(upto > tile);
+        if (past) {
+            const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            at = tile - __builtin_amdgcn_readlane(upto - tiles, l);
+            return s0 + l;
+        }
+        tile -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return -1;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// One row over keys [k0, k1) alone, by one wave (D / 64 dimensions a lane): the sums a tile's row
+// would have, without the products with weight 0 of keys that other rows of the tile see. Used where
+// such a product made a NaN (0 times a value that is not finite).
+template <int D>
+__device__ void attend_alone(const AttnArgs &a, int s, int kh, const half_t *qr, int k0, int k1, float (&o)[D / 64], float &l,
+                             float &m) {
+    constexpr int PER = D / 64;
+    const int d0 = (threadIdx.x & 63) * PER;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int r = 0; r < PER; ++r) o[r] = 0.0f;
+    for (int j = k0; j < k1 && l == l; ++j) {  // a NaN sum stays one
+        const int page = a.batch.page(s, j >> a.batch.page_shift);
+        if (page < 0) continue;
+        const int64_t at = page * a.batch.page_stride +
+                           ((static_cast<int64_t>(kh) << a.batch.page_shift) + (j & ((1 << a.batch.page_shift) - 1))) * D + d0;
+        float dot = 0.0f, v[PER];
+#pragma unroll
+        for (int r = 0; r < PER; ++r) {
+            dot += static_cast<float>(qr[d0 + r]) * static_cast<float>(a.k[at + r]);
+            v[r] = static_cast<float>(a.v[at + r]);
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
+        const float sc = dot * a.scale2, mx = fmaxf(m, sc), mu = mx == -INFINITY ? 0.0f : mx;
+        const float c = exp2_fast(m - mu), p = exp2_fast(sc - mu);
+        m = mx;
+        l = l * c + p;
+#pragma unroll
+        for (int r = 0; r < PER; ++r) o[r] = o[r] * c + p * v[r];
+    }
+}
+
+// Row rr of (s, kh) again, its keys of [k0, k1) alone, into the place where its tile left it. pos0: the
+// position of the sequence's first new token.
+template <int D>
+__device__ void store_alone(const AttnArgs &a, int s, int kh, int first, int pos0, int rr, int k0, int k1, int chunks,
+                                         int c) {
+    constexpr int PER = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int tok = rr / a.gqa, head = kh * a.gqa + rr - tok * a.gqa, pos = pos0 + tok;
+    const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+    float o[PER], l, m;
+    attend_alone<D>(a, s, kh, a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D, k0 > lo ? k0 : lo < 0 ? 0 : lo,
+                    k1 <= pos ? k1 : pos + 1, o, l, m);
+    const int64_t trow = static_cast<int64_t>(first + tok) * a.heads + head;
+    if (chunks > 1) {
+        float *pr = a.part + (trow * a.nsplit + c) * (D + 4);
+#pragma unroll
+        for (int r = 0; r < PER; ++r) pr[lane * PER + r] = o[r];
+        if (lane == 0) {
+            pr[D] = l;
+            pr[D + 1] = m;
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < PER; ++r) a.out[trow * D + lane * PER + r] = static_cast<half_t>(l == 0.0f ? 0.0f : o[r] / l);
+    }
+}
+
+// ---------------------------------------------------------------- few rows: 16 a tile
+
+// Four waves, each with its own tiles of 32 keys and its own softmax state; the states meet in LDS at
+// the end. A score tile is K . Q^T on 16x16x32 MFMAs: a lane holds 4 keys (4g + i of 16, g = lane / 16)
+// of one row (lane % 16), two such tiles make 8, and those 8 weights are, as they stand, the lane's
+// operand of out^T = V^T . P^T (the k index of a product may name the keys in any order, so long as
+// both operands do: 8g + j is key 4g + j for j < 4 and 16 + 4g + j - 4 from there). V^T's operand is
+// 8 keys of one dimension; a lane loads those 8 keys' rows 16 bytes wide (dimensions 8h .. 8h + 7, h =
+// lane % 16) and the 8 columns of that block are 8 products' operands, product e making the
+// dimensions 8h + e. So K, V and the scores go from memory to the matrix cores without LDS.
+template <int D>
+struct KvTile {
+    static constexpr int E = D / 16;  // dimensions a lane holds of each of its 8 value rows
+    typedef half_t ve __attribute__((ext_vector_type(E)));
+    half8_t k[2][D / 32];
+    ve v[8];
+    int ok;  // bit u: keys 16u .. 16u + 15 have a page
+};
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
+    constexpr int C = D / 32, E = D / 16, ROWS = 16;
+    __shared__ __attribute__((aligned(16))) float sm_o[4][ROWS][D + 4];
+    __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
+    const int kh = blockIdx.x % a.n_kv;
+    int at;
+    const int s = find_tile(a, ROWS, static_cast<int>(blockIdx.x) / a.n_kv, at);
+    if (s < 0) return;
+    int first, n_new;
+    a.batch.rows(s, first, n_new);
+    const int ctx = a.batch.context[s];
+    const Span span(a, s, n_new, ctx);
+    const int c = blockIdx.y;
+    if (c >= span.n) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+    const int n_rows = n_new * a.gqa - at * ROWS < ROWS ? n_new * a.gqa - at * ROWS : ROWS;
+    // the lane's row: token `tok` of the sequence, query head kh * gqa + head
+    const int row = at * ROWS + (l16 < n_rows ? l16 : n_rows - 1);
+    const int tok = row / a.gqa, head = kh * a.gqa + row - tok * a.gqa;
+    const int pos = ctx - n_new + tok;
+    const int first_tok = at * ROWS / a.gqa, last_tok = (at * ROWS + n_rows - 1) / a.gqa;
+    int k0, k1;  // the tile's keys in this chunk
+    span.chunk_keys(a, c, k0, k1);
+    const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
+    {
+        const int top = ctx - n_new + last_tok + 1, bottom = a.window > 0 ? ctx - n_new + first_tok - a.window + 1 : 0;
+        if (k1 > top) k1 = top;
+        if (k0 < bottom) k0 = bottom & ~31;
+    }
+    half8_t qf[C];
+    {
+        const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+        for (int i = 0; i < C; ++i) qf[i] = *reinterpret_cast<const half8_t *>(qr + 32 * i + 8 * g);
+    }
+    const int in_page = (1 << a.batch.page_shift) - 1;
+    const int64_t head_at = (static_cast<int64_t>(kh) << a.batch.page_shift) * D;
+    auto load = [&](int kb, KvTile<D> &t) {
+        t.ok = 0;
+        int64_t base[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int key = kb + 16 * u;
+            const int page = key < k1 ? a.batch.page(s, key >> a.batch.page_shift) : -1;
+            if (page >= 0) t.ok |= 1 << u;
+            base[u] = (page < 0 ? 0 : page) * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                t.k[u][i] = *reinterpret_cast<const half8_t *>(a.k + base[u] + l16 * D + 32 * i + 8 * g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            t.v[j] = *reinterpret_cast<const typename KvTile<D>::ve *>(a.v + base[j >> 2] + (4 * g + (j & 3)) * D + E * l16);
+    };
+    float m = -INFINITY, l = 0.0f;
+    float4_t o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int kb, KvTile<D> &t) {
+        float4_t sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            sc[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < C; ++i) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[u][i], qf[i], sc[u], 0, 0, 0);
+        }
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = kb + 16 * u + 4 * g + i;
+                const bool seen = key <= pos && key >= row_lo && key < k1 && (t.ok >> u & 1);
+                sc[u][i] = seen ? sc[u][i] * a.scale2 : -INFINITY;
+                mx = fmaxf(mx, sc[u][i]);
+            }
+        // the row's other keys are 16 and 32 lanes away
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        if (__any(mx > m)) {
+            const float f = exp2_fast(m - mu);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= f;
+            m = mx;
+        }
+        half8_t p;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = exp2_fast(sc[u][i] - mu);
+                l += x;
+                p[4 * u + i] = static_cast<half_t>(x);
+            }
+        // slots past the last key and of missing pages hold anything: 0 times it may be NaN
+        if (kb + 32 > k1 || t.ok != 3) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
+                if (key >= k1 || !(t.ok >> (j >> 2) & 1)) t.v[j] = typename KvTile<D>::ve{};
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            half8_t f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = t.v[j][e];
+            o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[e], 0, 0, 0);
+        }
+    };
+    KvTile<D> t;
+    for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) {
+        load(kb, t);
+        compute(kb, t);
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    // product e's row r is dimension E r + e: a lane holds 4 runs of E dimensions of its row
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<float4_t *>(&sm_o[w][l16][E * (4 * g + i) + e]) = float4_t{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+    if (g == 0) {
+        sm_m[w][l16] = m;
+        sm_l[w][l16] = l;
+    }
+    __syncthreads();
+    // the waves' states: 16 lanes a row, E dimensions each
+    const int r = threadIdx.x >> 4;
+    float mt = -INFINITY, den = 0.0f, num[E] = {};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mt = fmaxf(mt, sm_m[u][r]);
+    const float mu = mt == -INFINITY ? 0.0f : mt;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const float f = exp2_fast(sm_m[u][r] - mu);
+        den += sm_l[u][r] * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) num[e] += sm_o[u][r][E * l16 + e] * f;
+    }
+    const int rr = at * ROWS + (r < n_rows ? r : n_rows - 1), rtok = rr / a.gqa, rhead = kh * a.gqa + rr - rtok * a.gqa;
+    const int64_t trow = static_cast<int64_t>(first + rtok) * a.heads + rhead;
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) nan |= num[e] != num[e];
+    if (r < n_rows) {
+        if (span.n > 1) {
+            float *pr = a.part + (trow * a.nsplit + c) * (D + 4);
+#pragma unroll
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<float4_t *>(pr + E * l16 + e) = float4_t{num[e], num[e + 1], num[e + 2], num[e + 3]};
+            if (l16 == 0) {
+                pr[D] = den;
+                pr[D + 1] = mt;
+            }
+        } else {
+            const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // a row that sees no key is zero
+            typename KvTile<D>::ve y;
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = static_cast<half_t>(num[e] * inv);
+            *reinterpret_cast<typename KvTile<D>::ve *>(a.out + trow * D + E * l16) = y;
+        }
+    }
+    const uint64_t redo = __ballot(nan && r < n_rows);
+    if (redo == 0) return;
+    for (int i = 0; i < 4; ++i)
+        if (redo >> (16 * i) & 0xffff) store_alone<D>(a, s, kh, first, ctx - n_new, at * ROWS + 4 * w + i, k0, k1, span.n, c);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
+    constexpr int PER = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t trow = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
+    const int t = static_cast<int>((trow < rows ? trow : rows - 1) / a.heads);
+    const int s = a.batch.sequence_of<64>(t);
+    if (trow >= rows || s >= a.batch.b) return;
+    int first, n_new;
+    a.batch.rows(s, first, n_new);
+    const int i = t - first;
+    if (i < 0 || i >= n_new) return;
+    const int ctx = a.batch.context[s];
+    const Span span(a, s, n_new, ctx);
+    if (span.n <= 1) return;
+    const float *pr = a.part + trow * a.nsplit * (D + 4);
+    float num[PER] = {}, den = 0.0f, m = -INFINITY;
+    for (int c = 0; c < span.n; ++c) {
+        const float *pc = pr + c * (D + 4);
+        const float mc = pc[D + 1], mx = fmaxf(m, mc), mu = mx == -INFINITY ? 0.0f : mx;
+        const float f = exp2_fast(m - mu), fc = exp2_fast(mc - mu);
+        m = mx;
+        den = den * f + pc[D] * fc;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) num[e] = num[e] * f + pc[lane * PER + e] * fc;
+    }
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) a.out[trow * D + lane * PER + e] = static_cast<half_t>(num[e] * inv);
+}
+
+// ---------------------------------------------------------------- the launch
+
+struct Plan {
+    int64_t tiles;  // of 16 rows, at most
+    int chunk, nsplit;
+};
+
+// Chunks of the keys: enough for kFill workgroups where the tiles alone are fewer, none under
+// kMinChunk keys.
+constexpr int64_t kFill = 1024, kMinChunk = 128;
+
+inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window) {
+    Plan p;
+    p.tiles = (tokens * gqa + 15 * (b < tokens ? b : tokens)) / 16;
+    int64_t span = window > 0 && window + max_q + 63 < max_context ? window + max_q + 63 : max_context;
+    if (span < 1) span = 1;
+    const int64_t wgs = p.tiles * n_kv > 0 ? p.tiles * n_kv : 1;
+    int64_t n = (kFill + wgs - 1) / wgs;
+    const int64_t most = (span + kMinChunk - 1) / kMinChunk;
+    if (n > most) n = most;
+    p.chunk = static_cast<int>(((span + n - 1) / n + 63) / 64 * 64);
+    p.nsplit = static_cast<int>((span + p.chunk - 1) / p.chunk);
+    return p;
+}
+
+inline size_t part_bytes(const Plan &p, int64_t tokens, int64_t heads, int64_t hd) {
+    return p.nsplit > 1 ? static_cast<size_t>(tokens * heads * p.nsplit * (hd + 4)) * sizeof(float) : 0;
+}
+
+template <int D>
+hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
+    paged_attn_rows<D><<<dim3(static_cast<unsigned>(p.tiles * a.n_kv), a.nsplit), 256, 0, stream>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.nsplit == 1) return e;
+    const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
+    paged_attn_merge<D><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+inline bool plannable(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t hd, int64_t max_q, int64_t max_context,
+                      int64_t window) {
+    return tokens > 0 && b > 0 && n_kv > 0 && heads > 0 && heads % n_kv == 0 && hd > 0 && max_q > 0 && max_context > 0 && window >= 0 &&
+           tokens < (int64_t(1) << 24) && b <= kMaxSeqs && heads <= 65536 && hd <= 128 && max_q < (int64_t(1) << 31) &&
+           max_context < (int64_t(1) << 31) && window < (int64_t(1) << 31);
+}
+
+}  // namespace
+}  // namespace dtts
+
+extern "C" size_t dtts_paged_attention_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
+                                                       int64_t max_q, int64_t max_context, int64_t window) {
+    using namespace dtts;
+    if (!plannable(tokens, b, heads, n_kv, head_dim, max_q, max_context, window)) return 0;
+    return part_bytes(plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window), tokens, heads, head_dim);
+}
+
+extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dtts_f16 *vpages, const int32_t *q_start,
+                                        const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens,
+                                        int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages,
+                                        int64_t max_pages, int64_t page_stride, int64_t q_stride, int64_t max_q,
+                                        int64_t max_context, int64_t window, float scale, void *workspace, size_t ws_bytes,
+                                        hipStream_t stream) {
+    using namespace dtts;
+    const char *name = "dtts_paged_attention_f16";
+    DTTS_REQUIRE_PAGED(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride);
+    DTTS_REQUIRE(heads > 0 && heads <= 65536 && heads % n_kv == 0, "%s: %lld heads over %lld kv heads", name, (long long)heads,
+                 (long long)n_kv);
+    DTTS_REQUIRE(q_stride >= heads * head_dim && q_stride % 8 == 0, "%s: q_stride %lld (a multiple of 8, at least heads * head_dim)",
+                 name, (long long)q_stride);
+    DTTS_REQUIRE(window >= 0 && window < (int64_t(1) << 31), "%s: window %lld", name, (long long)window);
+    if (tokens == 0 || b == 0) return DTTS_OK;
+    DTTS_REQUIRE(max_q > 0 && max_context > 0 && max_q < (int64_t(1) << 31) && max_context < (int64_t(1) << 31),
+                 "%s: max_q %lld, max_context %lld", name, (long long)max_q, (long long)max_context);
+    DTTS_REQUIRE(q && kpages && vpages && q_start && context && page_table && out, "%s: null pointer", name);
+    DTTS_REQUIRE(aligned(q, 16) && aligned(kpages, 16) && aligned(vpages, 16) && aligned(out, 16) && aligned(q_start, 4) &&
+                     aligned(context, 4) && aligned(page_table, 4),
+                 "%s: misaligned operand", name);
+    DTTS_REQUIRE(out != q, "%s: the output may not be the queries", name);
+    Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window);
+    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && p.tiles * n_kv < (int64_t(1) << 31), "%s: too many rows", name);
+    AttnArgs a;
+    a.batch = PagedBatch{q_start, context, page_table, static_cast<int>(tokens), static_cast<int>(b), log2_of(page),
+                         static_cast<int>(n_pages), static_cast<int>(max_pages), page_stride};
+    a.q = reinterpret_cast<const half_t *>(q);
+    a.k = reinterpret_cast<const half_t *>(kpages);
+    a.v = reinterpret_cast<const half_t *>(vpages);
+    a.out = reinterpret_cast<half_t *>(out);
+    a.q_stride = q_stride;
+    a.heads = static_cast<int>(heads);
+    a.n_kv = static_cast<int>(n_kv);
+    a.gqa = static_cast<int>(heads / n_kv);
+    a.window = static_cast<int>(window);
+    a.scale2 = scale * kLog2e;
+    a.part = nullptr;
+    if (p.nsplit > 1 && workspace && ws_bytes >= part_bytes(p, tokens, heads, head_dim)) {
+        DTTS_REQUIRE(aligned(workspace, 16), "%s: misaligned workspace", name);
+        a.part = static_cast<float *>(workspace);
+    } else {
+        p.nsplit = 1;  // one workgroup takes all of a tile's keys
+    }
+    a.chunk = p.chunk;
+    a.nsplit = p.nsplit;
+    DTTS_HIP_CHECK(head_dim == 128 ? launch<128>(a, p, stream) : launch<64>(a, p, stream), name);
+    return DTTS_OK;
+}

@@ -67,6 +67,16 @@ SIGNATURES = {
     "dtts_decode_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64],
     "dtts_decode_attention_f16": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _SZ, _P],
     "dtts_decode_attention_f32": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _SZ, _P],
+    "dtts_rope_table_scaled_f32": [_I64, _I64, _F64, _I32, _F64, _I64, _F64, _F64, _F64, _P, _P],
+    "dtts_rotary_f32": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I64, _I64, _I64, _P],
+    "dtts_rotary_f16": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _I64, _I64, _I64, _P],
+    "dtts_qk_rope_append_paged_f32": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],
+    "dtts_qk_rope_append_paged_f16": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],
+    "dtts_paged_attention_workspace_bytes": [_I64] * 8,
+    "dtts_paged_attention_f16": [_P] * 7 + [_I64] * 13 + [_F32, _P, _SZ, _P],
+    "dtts_sample_workspace_bytes": [_I64, _I64],
+    "dtts_sample_f32": [_P] * 8 + [_I64] * 3 + [_P, _SZ, _P],
+    "dtts_sample_f16": [_P] * 8 + [_I64] * 3 + [_P, _SZ, _P],
     "dtts_rvq_lookup_sum_f16": [_P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P],
     "dtts_depthwise_layernorm_nlc_f16": [_P, _P, _P, _P, _P, _F32, _P, _I64, _I64, _I64, _I64, _P],
     "dtts_rms_norm_rows_f16": [_P, _P, _P, _I64, _I64, _F32, _P],
@@ -142,6 +152,7 @@ SIGNATURES = {
 _RESTYPES = {"dtts_last_error": ctypes.c_char_p, "dtts_codec_destroy": None,
              "dtts_codec_hop": ctypes.c_int64, "dtts_codec_workspace_bytes": ctypes.c_size_t,
              "dtts_decode_attention_workspace_bytes": ctypes.c_size_t,
+             "dtts_paged_attention_workspace_bytes": ctypes.c_size_t, "dtts_sample_workspace_bytes": ctypes.c_size_t,
              "dtts_gemm_f16_workspace_bytes": ctypes.c_size_t, "dtts_stack_destroy": None,
              "dtts_stack_workspace_bytes": ctypes.c_size_t, "dtts_gemm_f32_nt_workspace_bytes": ctypes.c_size_t, "dtts_stack_prefill_workspace_bytes": ctypes.c_size_t, "dtts_codec_front_destroy": None,
              "dtts_codec_front_workspace_bytes": ctypes.c_size_t,

@@ -429,6 +429,122 @@ int dtts_stack_prefill(dtts_stack *stack, const float *x, float *out, const dtts
                        int64_t t, int64_t start, int64_t cap, void *workspace, size_t workspace_bytes,
                        hipStream_t stream);
 
+/* ------------------------------------------------------------------ serving: rotary positions, paged cache, sampling
+ *
+ * What a server of many requests needs beside the ops above; the reference has no counterpart (it
+ * serves one batch at one position over rectangular caches). Every index, length and setting here is
+ * a DEVICE array, so a captured graph stays valid while they change; the host checks sizes, and the
+ * kernels check every value where they use it. */
+
+/* cos and sin tables for contexts longer than the trained one, [len, rot_dim / 2] f32 on the host:
+ * angle t * freq_i in f64, freq_i = base^(-2i / rot_dim) and
+ *   DTTS_ROPE_SCALE_NONE    as it is (dtts_rope_table_f32 bit for bit);
+ *   DTTS_ROPE_SCALE_LINEAR  freq_i / factor (position interpolation);
+ *   DTTS_ROPE_SCALE_NTK     base * factor^(rot_dim / (rot_dim - 2)) in the place of base;
+ *   DTTS_ROPE_SCALE_YARN    from freq_i to freq_i / factor by wavelength: unchanged for pairs that turn
+ *                           beta_fast times or more over original_len, divided for beta_slow or less,
+ *                           a linear ramp over the pair index between; cos and sin times attn_factor
+ *                           (0: 0.1 ln(factor) + 1).
+ * factor >= 1; original_len and the betas count for YaRN only. */
+#define DTTS_ROPE_SCALE_NONE 0
+#define DTTS_ROPE_SCALE_LINEAR 1
+#define DTTS_ROPE_SCALE_NTK 2
+#define DTTS_ROPE_SCALE_YARN 3
+int dtts_rope_table_scaled_f32(int64_t len, int64_t rot_dim, double base, int32_t scaling, double factor,
+                               int64_t original_len, double beta_fast, double beta_slow, double attn_factor,
+                               float *cos_out, float *sin_out);
+
+/* Rotary positions on x [rows, heads, D]: the first rot_dim dimensions of every head turned by the
+ * row's position, o1 = x1 c - x2 s, o2 = x2 c + x1 s over pairs (i, i + rot_dim / 2)
+ * (DTTS_ROPE_HALF) or (2i, 2i + 1) (DTTS_ROPE_INTERLEAVED); the rest copied. Products rounded
+ * separately in f32, one rounding on the store. pos DEVICE int32[rows]; a row whose position is
+ * outside [0, table_len) is padding: its y is left as it was. cos / sin [table_len, rot_dim / 2].
+ * x_stride and y_stride: elements from row to row (>= heads * D), so the queries or keys inside a qkv
+ * tensor can be turned where they are; x == y (in place, equal strides) is allowed, any other overlap
+ * is not. Any even rot_dim <= D; interleaved pairs need an even D, even strides and pair-aligned
+ * addresses. Fastest when D, rot_dim, strides and addresses are multiples of 16 bytes (rot_dim: 32
+ * half-split). */
+#define DTTS_ROPE_HALF 0
+#define DTTS_ROPE_INTERLEAVED 1
+int dtts_rotary_f32(const float *x, const float *cos_t, const float *sin_t, const int32_t *pos, float *y, int64_t rows,
+                    int64_t heads, int64_t head_dim, int64_t rot_dim, int32_t layout, int64_t x_stride, int64_t y_stride,
+                    int64_t table_len, hipStream_t stream);
+int dtts_rotary_f16(const dtts_f16 *x, const float *cos_t, const float *sin_t, const int32_t *pos, dtts_f16 *y,
+                    int64_t rows, int64_t heads, int64_t head_dim, int64_t rot_dim, int32_t layout, int64_t x_stride,
+                    int64_t y_stride, int64_t table_len, hipStream_t stream);
+
+/* A ragged batch over a paged f16 KV cache. kpages and vpages hold n_pages pages [n_kv, page, D],
+ * page_stride elements apart (n_kv * page * D when they are packed; more when k and v, or several layers,
+ * share a pool); page is a power of two, 16 to 65536; D is 64 or 128. page_table DEVICE int32
+ * [b, max_pages]: position p of sequence s is row p % page of page page_table[s, p / page]. q_start
+ * DEVICE int32[b + 1], rising: sequence s's new tokens are rows q_start[s] .. q_start[s + 1] - 1 of the
+ * batch (none: an idle slot). context DEVICE int32[b]: the sequence's length with its new tokens, so
+ * its i-th of n new tokens is at position context[s] - n + i. Rows from q_start[b] on are padding:
+ * left as they were by both calls. Page ids outside [0, n_pages) hold no position.
+ * tokens < 2^24, b <= 65536, max_pages * page < 2^31.
+ *
+ * dtts_qk_rope_append_paged_*: QK-norm (norms [2, D] f32, q's weight then k's, or NULL for none),
+ * rotary positions and the write of the new keys and values. qkv [tokens, (heads + 2 n_kv) * D] (q
+ * heads, then k, then v); q_out [tokens, heads, D] f16; k and v go to the pages. f32 arithmetic, one
+ * rounding to f16. rot_dim a multiple of 8. A token whose position is outside [0, table_len) or has no
+ * page is left out whole: its q_out row and every page stay as they were. */
+int dtts_qk_rope_append_paged_f32(const float *qkv, const float *norms, const float *cos_t, const float *sin_t,
+                                  const int32_t *q_start, const int32_t *context, const int32_t *page_table,
+                                  dtts_f16 *q_out, dtts_f16 *kpages, dtts_f16 *vpages, int64_t tokens, int64_t b,
+                                  int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
+                                  int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
+                                  int64_t table_len, float eps, hipStream_t stream);
+int dtts_qk_rope_append_paged_f16(const dtts_f16 *qkv, const float *norms, const float *cos_t, const float *sin_t,
+                                  const int32_t *q_start, const int32_t *context, const int32_t *page_table,
+                                  dtts_f16 *q_out, dtts_f16 *kpages, dtts_f16 *vpages, int64_t tokens, int64_t b,
+                                  int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
+                                  int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
+                                  int64_t table_len, float eps, hipStream_t stream);
+
+/* Attention of the new tokens over the cache, their own keys included:
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / (heads / n_kv)]) v[j, ..]
+ * over positions max(0, p - window + 1) <= j <= p of the token's sequence, p its position (window 0: all of
+ * them). q [tokens, heads, D] f16 with q_stride elements between tokens (a multiple of 8), out
+ * [tokens, heads, D] f16, not q. heads is any multiple of n_kv. Scores, softmax state and sums in f32;
+ * the weights are rounded to f16 for the product with v. A token that sees no position (p < 0, or no page
+ * of its window is there) gets zeros. Positions without a page are not attended to, slots past a
+ * sequence's context are never used, and a value that is not finite reaches only the tokens that see it.
+ * max_q and max_context are what the caller knows of the batch: the longest chunk and context. They
+ * choose the kernels and how far contexts are split over workgroups, never what is computed.
+ * workspace (device, 16-byte aligned) of dtts_paged_attention_workspace_bytes bytes lets contexts split,
+ * a second launch joining the chunks in order; without it (NULL or fewer bytes) none does. Calls that may
+ * overlap must not share one. */
+size_t dtts_paged_attention_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
+                                            int64_t max_q, int64_t max_context, int64_t window);
+int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dtts_f16 *vpages, const int32_t *q_start,
+                             const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens, int64_t b,
+                             int64_t heads, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages,
+                             int64_t max_pages, int64_t page_stride, int64_t q_stride, int64_t max_q, int64_t max_context,
+                             int64_t window, float scale, void *workspace, size_t ws_bytes, hipStream_t stream);
+
+/* Sampling: one token per row of logits [rows, vocab] (row_stride elements apart), from a given uniform
+ * random number. Per row, with the settings of the DEVICE arrays [rows] (each may be NULL: off):
+ *   w_i = exp((l_i - max l) / temperature); tokens in order of logit, equal ones by index;
+ *   top_k: the first top_k tokens (0, negative, or >= vocab: all);
+ *   top_p: of those, the shortest prefix with top_p of their weight or more (>= 1: all);
+ *   min_p: of those, the ones with w_i >= min_p (<= 0: all); the first token is always kept;
+ *   token[r] = the smallest index whose kept weight up to and including it, in index order, exceeds
+ *   u[r] times the kept weight. u in [0, 1) (others are clipped).
+ * temperature 0 (or negative, or not a number): the largest logit, the lower index of equals.
+ * logprob (or NULL): the token's log-probability among the kept ones (0 for temperature 0). NaN logits count
+ * as -inf; a row of nothing else gives token -1 and logprob -inf; +inf logits share all the weight.
+ * Weights are f64 and their sums integers (units of 2^-42 of the largest), so a result depends on nothing
+ * but the row. vocab <= 2^20. workspace (device, 16-byte aligned) of dtts_sample_workspace_bytes bytes lets
+ * several workgroups share a long row; without it (NULL or fewer bytes) one workgroup takes a row, with the
+ * same result. Calls that may overlap must not share one. */
+size_t dtts_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int dtts_sample_f32(const float *logits, const float *temperature, const int32_t *top_k, const float *top_p,
+                    const float *min_p, const float *u, int32_t *token, float *logprob, int64_t rows, int64_t vocab,
+                    int64_t row_stride, void *workspace, size_t ws_bytes, hipStream_t stream);
+int dtts_sample_f16(const dtts_f16 *logits, const float *temperature, const int32_t *top_k, const float *top_p,
+                    const float *min_p, const float *u, int32_t *token, float *logprob, int64_t rows, int64_t vocab,
+                    int64_t row_stride, void *workspace, size_t ws_bytes, hipStream_t stream);
+
 /* ------------------------------------------------------------------ f-3 codec front half */
 
 /* Rvq::decode's lookups (crates/qwen3tts/src/codec.rs:296-313) for both quantizer stacks at
