@@ -11,34 +11,45 @@ Every tensor of a call is on one device; the work goes to that device's current 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
-from ._lib import DttsError, call, lib, ptr, stream_handle
+from ._lib import DttsError, call, lib
 
 _F16, _F32, _I32 = torch.float16, torch.float32, torch.int32
 _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+_Tensor = torch.Tensor
 
 
-def _check(name, device, **tensors):
-    """what=(tensor, dtypes): a contiguous tensor of one of them, on `device`."""
-    for what, (t, dtypes) in tensors.items():
-        if not isinstance(t, torch.Tensor):
-            raise DttsError(f"{name}: {what} must be a tensor")
-        if t.device != device or device.type != "cuda":
-            raise DttsError(f"{name}: {what} must be on the device ({t.device}, {device})")
-        if t.dtype not in dtypes:
-            raise DttsError(f"{name}: {what} dtype {t.dtype} not in {dtypes}")
-        if not t.is_contiguous():
-            raise DttsError(f"{name}: {what} must be contiguous")
+def _need(name, device, what, t, dtypes, contiguous=True):
+    """Raises unless t is a (contiguous) tensor of one of dtypes on GPU number `device`. The callers pass
+    their tensors through one test that holds for all of a right call (a step is a few microseconds of GPU
+    work, and so is each of these calls on the host) and come here to say what is wrong."""
+    if not isinstance(t, _Tensor):
+        raise DttsError(f"{name}: {what} must be a tensor")
+    if device < 0 or t.get_device() != device:
+        raise DttsError(f"{name}: {what} must be on the device ({t.device}, GPU {device})")
+    if t.dtype not in dtypes:
+        raise DttsError(f"{name}: {what} dtype {t.dtype} not in {dtypes}")
+    if contiguous and not t.is_contiguous():
+        raise DttsError(f"{name}: {what} must be contiguous")
+
+
+def _is(t, dtype, device):
+    return isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and t.is_contiguous()
 
 
 def _enqueue(fn, device, *args):
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            call(fn, *args, stream_handle(device))
+    """The call on GPU number `device`'s current stream (as the raw handle: building a Stream object takes
+    longer than the launch)."""
+    if device == torch._C._cuda_getDevice():
+        status = getattr(lib(), fn)(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        call(fn, *args, stream_handle(device))
+        with torch.cuda.device(device):
+            status = getattr(lib(), fn)(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status != 0:
+        raise DttsError(f"{fn} failed ({status}): {lib().dtts_last_error().decode(errors='replace')}")
 
 
 # ---------------------------------------------------------------- rotary positions
@@ -59,18 +70,22 @@ def rope_table_scaled(length, rot_dim, base, scaling="none", factor=1.0, origina
     return c, s
 
 
-def _tables(name, cos, sin):
-    if cos.dim() != 2 or cos.shape != sin.shape:
-        raise DttsError(f"{name}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [positions, rot_dim / 2]")
-    return cos.shape
+def _tables(name, device, cos, sin):
+    if not (_is(cos, _F32, device) and _is(sin, _F32, device)):
+        _need(name, device, "cos", cos, (_F32,))
+        _need(name, device, "sin", sin, (_F32,))
+    n, sn = cos.shape, sin.shape
+    if len(n) != 2 or n != sn:
+        raise DttsError(f"{name}: cos {tuple(n)} and sin {tuple(sn)} must be [positions, rot_dim / 2]")
+    return n
 
 
 def _rows(name, t, what):
-    """[rows, heads, D], each row contiguous: the elements between rows."""
-    if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
-        raise DttsError(f"{name}: {what} must be [rows, heads, D] with contiguous rows, got {tuple(t.shape)} {t.stride()}")
-    width = t.shape[1] * t.shape[2]
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    """[rows, heads, D] with contiguous rows: its sizes, and the elements between rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or stride[2] != 1 or stride[1] != shape[2]:
+        raise DttsError(f"{name}: {what} must be [rows, heads, D] with contiguous rows, got {tuple(shape)} {stride}")
+    return shape, stride[0] if shape[0] > 1 else max(stride[0], shape[1] * shape[2])
 
 
 def rotary(x, cos, sin, pos, interleaved=False, out=None):
@@ -79,39 +94,70 @@ def rotary(x, cos, sin, pos, interleaved=False, out=None):
     position outside the tables is padding: that row of `out` is left as it was (of a new one: unset).
     out may be x."""
     name = "rotary"
-    if not isinstance(x, torch.Tensor) or x.dtype not in (_F32, _F16):
+    if not isinstance(x, _Tensor) or (x.dtype is not _F32 and x.dtype is not _F16):
         raise DttsError(f"{name}: x must be an f32 or f16 tensor")
-    xs = _rows(name, x, "x")
-    _check(name, x.device, cos=(cos, (_F32,)), sin=(sin, (_F32,)), pos=(pos, (_I32,)))
-    n, half = _tables(name, cos, sin)
-    rows, heads, hd = x.shape
+    dev = x.get_device()
+    if dev < 0:
+        _need(name, dev, "x", x, (x.dtype,), contiguous=False)
+    (rows, heads, hd), xs = _rows(name, x, "x")
+    n, half = _tables(name, dev, cos, sin)
+    if not _is(pos, _I32, dev):
+        _need(name, dev, "pos", pos, (_I32,))
     if pos.numel() != rows:
         raise DttsError(f"{name}: {pos.numel()} positions for {rows} rows")
     if out is None:
-        out = torch.empty((rows, heads, hd), dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise DttsError(f"{name}: out {tuple(out.shape)} {out.dtype} for x {tuple(x.shape)} {x.dtype}")
-    ys = _rows(name, out, "out")
-    _enqueue("dtts_rotary_f32" if x.dtype == _F32 else "dtts_rotary_f16", x.device, ptr(x), ptr(cos), ptr(sin), ptr(pos),
-             ptr(out), rows, heads, hd, 2 * half, int(interleaved), xs, ys, n)
+        out, ys = torch.empty(x.shape, dtype=x.dtype, device=x.device), heads * hd
+    else:
+        _need(name, dev, "out", out, (x.dtype,), contiguous=False)
+        if out.shape != x.shape:
+            raise DttsError(f"{name}: out {tuple(out.shape)} for x {tuple(x.shape)}")
+        ys = _rows(name, out, "out")[1]
+    _enqueue("dtts_rotary_f32" if x.dtype is _F32 else "dtts_rotary_f16", dev, x.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+             pos.data_ptr(), out.data_ptr(), rows, heads, hd, 2 * half, 1 if interleaved else 0, xs, ys, n)
     return out
 
 
 # ---------------------------------------------------------------- the paged cache
 
-def _paged(name, k_pages, v_pages, q_start, context, pages):
-    """The cache's and the batch's sizes: pages [n_pages, n_kv, page, D], each contiguous."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
-        raise DttsError(f"{name}: k pages {tuple(k_pages.shape)} and v pages {tuple(v_pages.shape)}")
-    if k_pages.dtype != _F16 or v_pages.dtype != _F16:
-        raise DttsError(f"{name}: pages are f16")
-    n_pages, n_kv, page, hd = k_pages.shape
-    st = k_pages.stride()
-    if st[1:] != (page * hd, hd, 1):
+def _paged(name, device, k_pages, v_pages, q_start, context, pages):
+    """Checks the cache [n_pages, n_kv, page, D] (each page contiguous) and the batch's arrays: b, n_kv, D,
+    page, n_pages, max_pages and the elements between pages."""
+    if not (_is(q_start, _I32, device) and _is(context, _I32, device) and _is(pages, _I32, device)):
+        _need(name, device, "q_start", q_start, (_I32,))
+        _need(name, device, "context", context, (_I32,))
+        _need(name, device, "pages", pages, (_I32,))
+    _need(name, device, "k_pages", k_pages, (_F16,), contiguous=False)
+    _need(name, device, "v_pages", v_pages, (_F16,), contiguous=False)
+    shape, st = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or st != v_pages.stride():
+        raise DttsError(f"{name}: k pages {tuple(shape)} and v pages {tuple(v_pages.shape)}")
+    n_pages, n_kv, page, hd = shape
+    if st[3] != 1 or st[2] != hd or st[1] != page * hd:
         raise DttsError(f"{name}: a page must be contiguous, got strides {st}")
-    if pages.dim() != 2 or pages.shape[0] != context.numel() or q_start.numel() != pages.shape[0] + 1:
-        raise DttsError(f"{name}: page table {tuple(pages.shape)}, {context.numel()} contexts, {q_start.numel()} starts")
-    return pages.shape[0], n_kv, hd, page, n_pages, pages.shape[1], max(st[0], n_kv * page * hd) if n_pages == 1 else st[0]
+    table = pages.shape
+    if len(table) != 2 or table[0] != context.numel() or q_start.numel() != table[0] + 1:
+        raise DttsError(f"{name}: page table {tuple(table)}, {context.numel()} contexts, {q_start.numel()} starts")
+    return table[0], n_kv, hd, page, n_pages, table[1], st[0] if n_pages > 1 else max(st[0], n_kv * page * hd)
+
+
+def _out(name, device, out, like, tokens, heads, hd):
+    if out is None:
+        return torch.empty((tokens, heads, hd), dtype=_F16, device=like.device)
+    _need(name, device, "out", out, (_F16,))
+    if out.numel() != tokens * heads * hd:
+        raise DttsError(f"{name}: out {tuple(out.shape)} is not [{tokens}, {heads}, {hd}]")
+    return out
+
+
+def _bytes(name, device, workspace, need, like):
+    """(tensor kept alive, address, bytes) of a call's workspace."""
+    if workspace is None:
+        if not need:
+            return None, None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    else:
+        _need(name, device, "workspace", workspace, (torch.uint8,))
+    return workspace, workspace.data_ptr(), workspace.numel()
 
 
 def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, pages, heads, norms=None, eps=1e-6,
@@ -122,32 +168,28 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
     included) and pages [b, max_pages] are int32; see dtts.h for what each selects. Rows of `out` that
     belong to no sequence are left as they were."""
     name = "qk_rope_append_paged"
-    dev = k_pages.device
-    _check(name, dev, qkv=(qkv, (_F32, _F16)), cos=(cos, (_F32,)), sin=(sin, (_F32,)), q_start=(q_start, (_I32,)),
-           context=(context, (_I32,)), pages=(pages, (_I32,)))
-    if v_pages.device != dev:
-        raise DttsError(f"{name}: v_pages must be on the device ({v_pages.device}, {dev})")
-    n, half = _tables(name, cos, sin)
-    b, n_kv, hd, page, n_pages, max_pages, stride = _paged(name, k_pages, v_pages, q_start, context, pages)
-    if qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * n_kv) * hd:
+    if not isinstance(qkv, _Tensor):
+        raise DttsError(f"{name}: qkv must be a tensor")
+    dev = qkv.get_device()
+    _need(name, dev, "qkv", qkv, (_F32, _F16))
+    b, n_kv, hd, page, n_pages, max_pages, stride = _paged(name, dev, k_pages, v_pages, q_start, context, pages)
+    n, half = _tables(name, dev, cos, sin)
+    if len(qkv.shape) != 2 or qkv.shape[1] != (heads + 2 * n_kv) * hd:
         raise DttsError(f"{name}: qkv {tuple(qkv.shape)} is not [tokens, ({heads} + 2 * {n_kv}) * {hd}]")
     if norms is not None:
-        _check(name, dev, norms=(norms, (_F32,)))
+        _need(name, dev, "norms", norms, (_F32,))
         if norms.numel() != 2 * hd:
             raise DttsError(f"{name}: norms {tuple(norms.shape)} is not [2, {hd}]")
     tokens = qkv.shape[0]
-    if out is None:
-        out = torch.empty((tokens, heads, hd), dtype=_F16, device=dev)
-    else:
-        _check(name, dev, out=(out, (_F16,)))
-        if out.numel() != tokens * heads * hd:
-            raise DttsError(f"{name}: out {tuple(out.shape)} is not [{tokens}, {heads}, {hd}]")
-    _enqueue("dtts_qk_rope_append_paged_f32" if qkv.dtype == _F32 else "dtts_qk_rope_append_paged_f16", dev, ptr(qkv),
-             ptr(norms), ptr(cos), ptr(sin), ptr(q_start), ptr(context), ptr(pages), ptr(out), ptr(k_pages), ptr(v_pages),
-             tokens, b, heads, n_kv, hd, 2 * half, int(interleaved), page, n_pages, max_pages, stride, n, float(eps))
+    out = _out(name, dev, out, qkv, tokens, heads, hd)
+    _enqueue("dtts_qk_rope_append_paged_f32" if qkv.dtype is _F32 else "dtts_qk_rope_append_paged_f16", dev, qkv.data_ptr(),
+             None if norms is None else norms.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_start.data_ptr(),
+             context.data_ptr(), pages.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tokens, b, heads,
+             n_kv, hd, 2 * half, 1 if interleaved else 0, page, n_pages, max_pages, stride, n, eps)
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window=0):
     """Workspace bytes paged_attention splits contexts over workgroups with."""
     return int(lib().dtts_paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window))
@@ -162,37 +204,40 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
     paged_attention_workspace_bytes (allocated when not given). Rows of `out` that belong to no sequence are
     left as they were; a token that sees no position gets zeros."""
     name = "paged_attention"
-    dev = q.device
-    if q.dtype != _F16:
-        raise DttsError(f"{name}: q must be f16")
-    qs = _rows(name, q, "q")
-    _check(name, dev, q_start=(q_start, (_I32,)), context=(context, (_I32,)), pages=(pages, (_I32,)))
-    if k_pages.device != dev or v_pages.device != dev:
-        raise DttsError(f"{name}: the pages must be on the device ({k_pages.device}, {v_pages.device}, {dev})")
-    b, n_kv, hd, page, n_pages, max_pages, stride = _paged(name, k_pages, v_pages, q_start, context, pages)
-    tokens, heads, qd = q.shape
+    if not isinstance(q, _Tensor) or q.dtype is not _F16:
+        raise DttsError(f"{name}: q must be an f16 tensor")
+    dev = q.get_device()
+    if dev < 0:
+        _need(name, dev, "q", q, (_F16,), contiguous=False)
+    (tokens, heads, qd), qs = _rows(name, q, "q")
+    b, n_kv, hd, page, n_pages, max_pages, stride = _paged(name, dev, k_pages, v_pages, q_start, context, pages)
     if qd != hd:
         raise DttsError(f"{name}: q {tuple(q.shape)} over pages of head_dim {hd}")
-    if out is None:
-        out = torch.empty((tokens, heads, hd), dtype=_F16, device=dev)
-    else:
-        _check(name, dev, out=(out, (_F16,)))
-        if out.numel() != tokens * heads * hd:
-            raise DttsError(f"{name}: out {tuple(out.shape)} is not [{tokens}, {heads}, {hd}]")
-    if workspace is None:
-        need = paged_attention_workspace_bytes(tokens, b, heads, n_kv, hd, max_q, max_context, window)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _enqueue("dtts_paged_attention_f16", dev, ptr(q), ptr(k_pages), ptr(v_pages), ptr(q_start), ptr(context), ptr(pages),
-             ptr(out), tokens, b, heads, n_kv, hd, page, n_pages, max_pages, stride, qs, max_q, max_context, window,
-             float(scale), ptr(workspace), workspace.numel() if workspace is not None else 0)
+    out = _out(name, dev, out, q, tokens, heads, hd)
+    need = 0 if workspace is not None else paged_attention_workspace_bytes(tokens, b, heads, n_kv, hd, max_q, max_context, window)
+    keep, ws, ws_bytes = _bytes(name, dev, workspace, need, q)
+    _enqueue("dtts_paged_attention_f16", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_start.data_ptr(),
+             context.data_ptr(), pages.data_ptr(), out.data_ptr(), tokens, b, heads, n_kv, hd, page, n_pages, max_pages, stride,
+             qs, max_q, max_context, window, scale, ws, ws_bytes)
     return out
 
 
 # ---------------------------------------------------------------- sampling
 
+@functools.lru_cache(maxsize=4096)
 def sample_workspace_bytes(rows, vocab):
     """Workspace bytes sample splits a long row over workgroups with."""
     return int(lib().dtts_sample_workspace_bytes(rows, vocab))
+
+
+def _setting(name, device, what, t, dtype, rows):
+    if t is None:
+        return None
+    if not _is(t, dtype, device):
+        _need(name, device, what, t, (dtype,))
+    if t.numel() != rows:
+        raise DttsError(f"{name}: {t.numel()} of {what} for {rows} rows")
+    return t.data_ptr()
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, workspace=None):
@@ -200,30 +245,28 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, work
     numbers u [rows] in [0, 1): (tokens int32 [rows], log-probabilities f32 [rows] under the distribution
     sampled from). temperature, top_p, min_p f32 [rows] and top_k int32 [rows] are each row's settings or
     None; temperature 0 takes the largest logit, top_k 0, top_p 1 and min_p 0 filter nothing. A row without
-    a finite (or +inf) logit gives token -1."""
+    a finite (or +inf) logit gives token -1. `workspace`: a device byte tensor of sample_workspace_bytes
+    (allocated when not given)."""
     name = "sample"
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (_F32, _F16) or logits.dim() != 2:
+    if not isinstance(logits, _Tensor) or (logits.dtype is not _F32 and logits.dtype is not _F16) or logits.dim() != 2:
         raise DttsError(f"{name}: logits must be an f32 or f16 tensor [rows, vocab]")
     rows, vocab = logits.shape
-    if logits.stride(1) != 1 and vocab > 1:
-        raise DttsError(f"{name}: a row of logits must be contiguous, got strides {logits.stride()}")
-    dev = logits.device
-    _check(name, dev, u=(u, (_F32,)))
-    for what, t, dtype in (("temperature", temperature, _F32), ("top_k", top_k, _I32), ("top_p", top_p, _F32),
-                           ("min_p", min_p, _F32)):
-        if t is not None:
-            _check(name, dev, **{what: (t, (dtype,))})
-            if t.numel() != rows:
-                raise DttsError(f"{name}: {t.numel()} of {what} for {rows} rows")
-    if u.numel() != rows:
-        raise DttsError(f"{name}: {u.numel()} random numbers for {rows} rows")
-    token = torch.empty(rows, dtype=_I32, device=dev)
-    logprob = torch.empty(rows, dtype=_F32, device=dev)
-    if workspace is None:
-        need = sample_workspace_bytes(rows, vocab)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _enqueue("dtts_sample_f32" if logits.dtype == _F32 else "dtts_sample_f16", dev, ptr(logits), ptr(temperature), ptr(top_k),
-             ptr(top_p), ptr(min_p), ptr(u), ptr(token), ptr(logprob), rows, vocab,
-             logits.stride(0) if rows > 1 else max(logits.stride(0), vocab), ptr(workspace),
-             workspace.numel() if workspace is not None else 0)
+    stride = logits.stride()
+    if stride[1] != 1 and vocab > 1:
+        raise DttsError(f"{name}: a row of logits must be contiguous, got strides {stride}")
+    dev = logits.get_device()
+    if dev < 0:
+        _need(name, dev, "logits", logits, (logits.dtype,), contiguous=False)
+    if u is None:
+        raise DttsError(f"{name}: u must be a tensor")
+    pu = _setting(name, dev, "random numbers", u, _F32, rows)
+    pt = _setting(name, dev, "temperature", temperature, _F32, rows)
+    pk = _setting(name, dev, "top_k", top_k, _I32, rows)
+    pp = _setting(name, dev, "top_p", top_p, _F32, rows)
+    pm = _setting(name, dev, "min_p", min_p, _F32, rows)
+    token = torch.empty(rows, dtype=_I32, device=logits.device)
+    logprob = torch.empty(rows, dtype=_F32, device=logits.device)
+    keep, ws, ws_bytes = _bytes(name, dev, workspace, sample_workspace_bytes(rows, vocab), logits)
+    _enqueue("dtts_sample_f32" if logits.dtype is _F32 else "dtts_sample_f16", dev, logits.data_ptr(), pt, pk, pp, pm, pu,
+             token.data_ptr(), logprob.data_ptr(), rows, vocab, stride[0] if rows > 1 else max(stride[0], vocab), ws, ws_bytes)
     return token, logprob
