@@ -23,6 +23,7 @@ struct AttnArgs {
     int heads, n_kv, gqa, window;
     float scale2;      // scale * log2(e): the softmax runs in base 2
     int chunk, nsplit; // keys per chunk, chunks at most (the last takes what is left)
+    int64_t few;       // sequences of at most this many rows go to the 16-row tiles
 };
 
 // The keys that sequence s's rows see, in chunks: [lo, hi), lo a multiple of 64, `n` chunks. hi stops
@@ -43,30 +44,32 @@ struct Span {
     }
 };
 
-// The tile-th tile of `rows` rows over the sequences, counted in order (every wave for itself).
-// Returns the sequence, or -1 past the last; `at` is the tile's place in it.
-__device__ __forceinline__ int find_tile(const AttnArgs &a, int rows, int tile, int &at) {
+// The tile-th tile of `rows` rows over the sequences of more than `above` and at most `upto` rows,
+// counted in order (every wave for itself; a sequence's last tile first, which under a causal mask is its
+// longest). Returns the sequence, or -1 past the last; `at` is the tile's place in it.
+__device__ __forceinline__ int find_tile(const AttnArgs &a, int rows, int64_t above, int64_t upto, int tile, int &at) {
     const int lane = threadIdx.x & 63;
     for (int s0 = 0; s0 < a.batch.b; s0 += 64) {
         int tiles = 0;
         if (s0 + lane < a.batch.b) {
             int first, n;
             a.batch.rows(s0 + lane, first, n);
-            tiles = static_cast<int>((static_cast<int64_t>(n) * a.gqa + rows - 1) / rows);
+            const int64_t of = static_cast<int64_t>(n) * a.gqa;
+            if (of > above && of <= upto) tiles = static_cast<int>((of + rows - 1) / rows);
         }
-        int upto = tiles;
+        int sum = tiles;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
-            const int v = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += v;
+            const int v = __shfl_up(sum, off, 64);
+            if (lane >= off) sum += v;
         }
-        const uint64_t past = __ballot(upto > tile);
+        const uint64_t past = __ballot(sum > tile);
         if (past) {
             const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            at = tile - __builtin_amdgcn_readlane(upto - tiles, l);
+            at = __builtin_amdgcn_readlane(sum, l) - 1 - tile;
             return s0 + l;
         }
-        tile -= __builtin_amdgcn_readlane(upto, 63);
+        tile -= __builtin_amdgcn_readlane(sum, 63);
     }
     return -1;
 }
@@ -160,7 +163,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
     __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
     const int kh = blockIdx.x % a.n_kv;
     int at;
-    const int s = find_tile(a, ROWS, static_cast<int>(blockIdx.x) / a.n_kv, at);
+    const int s = find_tile(a, ROWS, 0, a.few, static_cast<int>(blockIdx.x) / a.n_kv, at);
     if (s < 0) return;
     int first, n_new;
     a.batch.rows(s, first, n_new);
@@ -304,7 +307,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
     bool nan = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) nan |= num[e] != num[e];
-    if (r < n_rows) {
+    const uint64_t redo = __ballot(nan && r < n_rows);
+    if (r < n_rows && (redo >> (lane & 48) & 0xffff) == 0) {
         if (span.n > 1) {
             float *pr = a.part + (trow * a.nsplit + c) * (D + 4);
 #pragma unroll
@@ -322,10 +326,224 @@ __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
             *reinterpret_cast<typename KvTile<D>::ve *>(a.out + trow * D + E * l16) = y;
         }
     }
-    const uint64_t redo = __ballot(nan && r < n_rows);
     if (redo == 0) return;
     for (int i = 0; i < 4; ++i)
         if (redo >> (16 * i) & 0xffff) store_alone<D>(a, s, kh, first, ctx - n_new, at * ROWS + 4 * w + i, k0, k1, span.n, c);
+}
+
+// ---------------------------------------------------------------- chunks: 128 rows a tile
+
+// Four waves of 32 rows each share every 64 keys through LDS. A score block is K . Q^T on 32x32x16
+// MFMAs: a lane holds 16 keys (8 (r >> 2) + 4g + (r & 3), g = lane / 32) of one row (lane % 32), and
+// registers 8h .. 8h + 7 are, as they stand, its operand of out^T = V^T . P^T for keys 16h .. 16h + 15,
+// whose k index 8g + j then names key 4g + j for j < 4 and 8 + 4g + j - 4 from there. V is stored
+// transposed in that key order as it is staged (a thread takes 4 keys of E dimensions, so the turn is
+// made once for the four waves), and both operands are single 16-byte LDS reads. Rows of both tiles are
+// XOR-swizzled in 16-byte pieces: neighbouring lanes read different banks.
+//
+// Two buffers: the next keys' rows are requested before a tile's products and stored after them, one
+// barrier a tile. Per 64 keys a wave has 1024 cycles of MFMA and about as many of softmax.
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
+    constexpr int ROWS = 128, KT = 64, E = D / 16, C = D / 16, KL = D / 32;  // C: k steps, KL: 16-byte key loads a thread
+    constexpr int KCH = D / 8;                                               // 16-byte pieces of a key row
+    typedef half_t ve __attribute__((ext_vector_type(E)));
+    __shared__ __attribute__((aligned(16))) half_t sk[2][KT * D], sv[2][D * KT];
+    __shared__ int s_ok[2][4];
+    const int kh = blockIdx.x % a.n_kv;
+    int at;
+    const int s = find_tile(a, ROWS, a.few, INT64_MAX, static_cast<int>(blockIdx.x) / a.n_kv, at);
+    if (s < 0) return;
+    int first, n_new;
+    a.batch.rows(s, first, n_new);
+    const int ctx = a.batch.context[s], pos0 = ctx - n_new;
+    const Span span(a, s, n_new, ctx);
+    const int c = blockIdx.y;
+    if (c >= span.n) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
+    const int r0 = at * ROWS, n_rows = n_new * a.gqa - r0 < ROWS ? n_new * a.gqa - r0 : ROWS;
+    int k0, k1;
+    span.chunk_keys(a, c, k0, k1);
+    {
+        const int top = pos0 + (r0 + n_rows - 1) / a.gqa + 1, bottom = a.window > 0 ? pos0 + r0 / a.gqa - a.window + 1 : 0;
+        if (k1 > top) k1 = top;
+        if (k0 < bottom) k0 = bottom & ~(KT - 1);
+    }
+    // the wave's rows and the lane's
+    const int wrows = n_rows - 32 * w < 32 ? n_rows - 32 * w : 32;
+    const int row = r0 + 32 * w + (l32 < wrows ? l32 : wrows > 0 ? wrows - 1 : -32 * w);
+    const int tok = row / a.gqa, head = kh * a.gqa + row - tok * a.gqa, pos = pos0 + tok;
+    const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
+    const int wfirst = pos0 + (r0 + 32 * w) / a.gqa, wlast = pos0 + (r0 + 32 * w + wrows - 1) / a.gqa;
+    half8_t qf[C];
+    {
+        const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+        for (int i = 0; i < C; ++i) qf[i] = *reinterpret_cast<const half8_t *>(qr + 16 * i + 8 * g);
+    }
+    const int in_page = (1 << a.batch.page_shift) - 1;
+    const int64_t head_at = (static_cast<int64_t>(kh) << a.batch.page_shift) * D;
+    // staging: wave w takes keys 16w .. 16w + 15 of a tile, one page
+    half8_t gk[KL];
+    ve gv[4];
+    int g_ok = 0;
+    const int krow = lane / KCH, kch = lane % KCH, a4 = lane >> 4, db = lane & 15;
+    auto load = [&](int kb) {
+        const int key = kb + 16 * w;
+        const int page = key < k1 ? a.batch.page(s, key >> a.batch.page_shift) : -1;
+        g_ok = page >= 0;
+        const int64_t base = (page < 0 ? 0 : page) * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D;
+#pragma unroll
+        for (int i = 0; i < KL; ++i)
+            gk[i] = *reinterpret_cast<const half8_t *>(a.k + base + (krow + i * (64 / KCH)) * D + kch * 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) gv[j] = *reinterpret_cast<const ve *>(a.v + base + (4 * a4 + j) * D + E * db);
+    };
+    auto store = [&](int kb, int buf) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+            const int r = 16 * w + krow + i * (64 / KCH);
+            *reinterpret_cast<half8_t *>(&sk[buf][r * D + ((kch ^ r) & (KCH - 1)) * 8]) = gk[i];
+        }
+        if (!g_ok || kb + 16 * w + 16 > k1) {  // slots that hold no position: 0 times what is there may be NaN
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (!g_ok || kb + 16 * w + 4 * a4 + j >= k1) gv[j] = ve{};
+        }
+        const int kk = 16 * w + ((a4 & 1) << 3 | (a4 >> 1) << 2);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int d = E * db + e;
+            *reinterpret_cast<half4_t *>(&sv[buf][d * KT + (((kk >> 3) ^ d ^ (d >> 3)) & 7) * 8 + (kk & 4)]) =
+                half4_t{gv[0][e], gv[1][e], gv[2][e], gv[3][e]};
+        }
+        if (lane == 0) s_ok[buf][w] = g_ok;
+    };
+    float m = -INFINITY, l = 0.0f;
+    float16_t o[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    auto compute = [&](int kb, int buf) {
+        float16_t sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = 32 * u + l32;
+                const half8_t kf = *reinterpret_cast<const half8_t *>(&sk[buf][r * D + (((2 * i + g) ^ r) & (KCH - 1)) * 8]);
+                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], sc[u], 0, 0, 0);
+            }
+        int ok[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) ok[t] = __builtin_amdgcn_readfirstlane(s_ok[buf][t]);
+        const bool whole = kb + KT - 1 <= wfirst && kb + KT <= k1 && (a.window == 0 || kb > wlast - a.window) &&
+                           (ok[0] & ok[1] & ok[2] & ok[3]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[u][r] *= a.scale2;
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = kb + 32 * u + 8 * (r >> 2) + 4 * g + (r & 3);
+                    if (!(key <= pos && key >= row_lo && key < k1 && ok[2 * u + (r >> 3)])) sc[u][r] = -INFINITY;
+                }
+        }
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        if (__any(mx > m)) {
+            const float f = exp2_fast(m - mu);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= f;
+            m = mx;
+        }
+        half8_t pf[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = exp2_fast(sc[t >> 1][8 * (t & 1) + j] - mu);
+                l += x;
+                pf[t][j] = static_cast<half_t>(x);
+            }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                const int dd = 32 * d + l32;
+                const half8_t vf = *reinterpret_cast<const half8_t *>(&sv[buf][dd * KT + (((2 * t + g) ^ dd ^ (dd >> 3)) & 7) * 8]);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[t], o[d], 0, 0, 0);
+            }
+    };
+    int kb = k0 & ~(KT - 1), buf = 0;
+    if (kb < k1) {
+        load(kb);
+        store(kb, 0);
+        if (kb + KT < k1) load(kb + KT);
+        __syncthreads();
+        for (; kb < k1; kb += KT, buf ^= 1) {
+            if (wrows > 0 && kb <= wlast && (a.window == 0 || kb + KT > wfirst - a.window + 1)) compute(kb, buf);
+            if (kb + KT < k1) {
+                store(kb + KT, buf ^ 1);
+                if (kb + 2 * KT < k1) load(kb + 2 * KT);
+            }
+            __syncthreads();
+        }
+    }
+    if (wrows <= 0) return;
+    l += __shfl_xor(l, 32, 64);
+    const int64_t trow = static_cast<int64_t>(first + tok) * a.heads + head;
+    bool nan = false;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nan |= o[d][r] != o[d][r];
+    const uint64_t bad = __ballot(nan && l32 < wrows);
+    const uint32_t redo = static_cast<uint32_t>(bad | bad >> 32);
+    if (l32 < wrows && !(redo >> l32 & 1)) {
+        if (span.n > 1) {
+            float *pr = a.part + (trow * a.nsplit + c) * (D + 4);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<float4_t *>(pr + 32 * d + 2 * r + 4 * g) = float4_t{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+            if (g == 0) {
+                pr[D] = l;
+                pr[D + 1] = m;
+            }
+        } else {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees no key is zero
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    half4_t y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = static_cast<half_t>(o[d][r + i] * inv);
+                    *reinterpret_cast<half4_t *>(a.out + trow * D + 32 * d + 2 * r + 4 * g) = y;
+                }
+        }
+    }
+    if (redo == 0) return;
+    for (int i = 0; i < wrows; ++i)
+        if (redo >> i & 1) store_alone<D>(a, s, kh, first, pos0, r0 + 32 * w + i, k0, k1, span.n, c);
 }
 
 template <int D>
@@ -363,20 +581,38 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
 // ---------------------------------------------------------------- the launch
 
 struct Plan {
-    int64_t tiles;  // of 16 rows, at most
+    int64_t small, large;  // tiles of 16 and of 128 rows, at most
+    int64_t few;           // rows of a sequence up to which it goes to the small ones
     int chunk, nsplit;
 };
 
+// Sequences of up to kFew rows go to the 16-row tiles. A batch without longer chunks has no 128-row
+// launch; one sequence alone goes where its chunk does.
+constexpr int64_t kFew = 32;
 // Chunks of the keys: enough for kFill workgroups where the tiles alone are fewer, none under
 // kMinChunk keys.
 constexpr int64_t kFill = 1024, kMinChunk = 128;
 
 inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window) {
     Plan p;
-    p.tiles = (tokens * gqa + 15 * (b < tokens ? b : tokens)) / 16;
+    const int64_t rows = tokens * gqa, live = b < tokens ? b : tokens;
+    if (max_q * gqa <= kFew) {
+        p.few = INT64_MAX;
+        p.small = (rows + 15 * live) / 16;
+        p.large = 0;
+    } else if (b == 1) {
+        p.few = 0;
+        p.small = 0;
+        p.large = (rows + 127) / 128;
+    } else {
+        p.few = kFew;
+        p.small = (rows + 15 * live) / 16 < live * (kFew / 16) ? (rows + 15 * live) / 16 : live * (kFew / 16);
+        const int64_t most = rows / (kFew + 1) < live ? rows / (kFew + 1) : live;  // sequences of that many rows
+        p.large = (rows + 127 * most) / 128;
+    }
     int64_t span = window > 0 && window + max_q + 63 < max_context ? window + max_q + 63 : max_context;
     if (span < 1) span = 1;
-    const int64_t wgs = p.tiles * n_kv > 0 ? p.tiles * n_kv : 1;
+    const int64_t wgs = (p.small + p.large) * n_kv > 0 ? (p.small + p.large) * n_kv : 1;
     int64_t n = (kFill + wgs - 1) / wgs;
     const int64_t most = (span + kMinChunk - 1) / kMinChunk;
     if (n > most) n = most;
@@ -391,8 +627,15 @@ inline size_t part_bytes(const Plan &p, int64_t tokens, int64_t heads, int64_t h
 
 template <int D>
 hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
-    paged_attn_rows<D><<<dim3(static_cast<unsigned>(p.tiles * a.n_kv), a.nsplit), 256, 0, stream>>>(a);
-    hipError_t e = hipGetLastError();
+    hipError_t e = hipSuccess;
+    if (p.large > 0) {
+        paged_attn_chunk<D><<<dim3(static_cast<unsigned>(p.large * a.n_kv), a.nsplit), 256, 0, stream>>>(a);
+        e = hipGetLastError();
+    }
+    if (p.small > 0 && e == hipSuccess) {
+        paged_attn_rows<D><<<dim3(static_cast<unsigned>(p.small * a.n_kv), a.nsplit), 256, 0, stream>>>(a);
+        e = hipGetLastError();
+    }
     if (e != hipSuccess || a.nsplit == 1) return e;
     const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
     paged_attn_merge<D><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
@@ -439,7 +682,7 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
                  "%s: misaligned operand", name);
     DTTS_REQUIRE(out != q, "%s: the output may not be the queries", name);
     Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window);
-    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && p.tiles * n_kv < (int64_t(1) << 31), "%s: too many rows", name);
+    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large) * n_kv < (int64_t(1) << 31), "%s: too many rows", name);
     AttnArgs a;
     a.batch = PagedBatch{q_start, context, page_table, static_cast<int>(tokens), static_cast<int>(b), log2_of(page),
                          static_cast<int>(n_pages), static_cast<int>(max_pages), page_stride};
@@ -453,6 +696,7 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
     a.gqa = static_cast<int>(heads / n_kv);
     a.window = static_cast<int>(window);
     a.scale2 = scale * kLog2e;
+    a.few = p.few;
     a.part = nullptr;
     if (p.nsplit > 1 && workspace && ws_bytes >= part_bytes(p, tokens, heads, head_dim)) {
         DTTS_REQUIRE(aligned(workspace, 16), "%s: misaligned workspace", name);
