@@ -14,6 +14,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+
 struct AttnArgs {
     PagedBatch batch;
     const half_t *q, *k, *v;
@@ -44,15 +45,20 @@ struct Span {
     }
 };
 
+// A tile of rows: its sequence (-1: none), place in it, the sequence's first row and new tokens, context.
+struct Tile {
+    int s, at, first, n_new, ctx;
+};
+
 // The tile-th tile of `rows` rows over the sequences of more than `above` and at most `upto` rows,
 // counted in order (every wave for itself; a sequence's last tile first, which under a causal mask is its
-// longest). Returns the sequence, or -1 past the last; `at` is the tile's place in it.
-__device__ __forceinline__ int find_tile(const AttnArgs &a, int rows, int64_t above, int64_t upto, int tile, int &at) {
+// longest). What the lanes have read of the sequence comes along: one memory round trip in all.
+__device__ __forceinline__ Tile find_tile(const AttnArgs &a, int rows, int64_t above, int64_t upto, int tile) {
     const int lane = threadIdx.x & 63;
     for (int s0 = 0; s0 < a.batch.b; s0 += 64) {
-        int tiles = 0;
+        int tiles = 0, first = 0, n = 0, ctx = 0;
         if (s0 + lane < a.batch.b) {
-            int first, n;
+            ctx = a.batch.context[s0 + lane];
             a.batch.rows(s0 + lane, first, n);
             const int64_t of = static_cast<int64_t>(n) * a.gqa;
             if (of > above && of <= upto) tiles = static_cast<int>((of + rows - 1) / rows);
@@ -66,12 +72,12 @@ __device__ __forceinline__ int find_tile(const AttnArgs &a, int rows, int64_t ab
         const uint64_t past = __ballot(sum > tile);
         if (past) {
             const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            at = __builtin_amdgcn_readlane(sum, l) - 1 - tile;
-            return s0 + l;
+            return Tile{s0 + l, __builtin_amdgcn_readlane(sum, l) - 1 - tile, __builtin_amdgcn_readlane(first, l),
+                        __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(ctx, l)};
         }
         tile -= __builtin_amdgcn_readlane(sum, 63);
     }
-    return -1;
+    return Tile{-1, 0, 0, 0, 0};
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -162,12 +168,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) float sm_o[4][ROWS][D + 4];
     __shared__ float sm_m[4][ROWS], sm_l[4][ROWS];
     const int kh = blockIdx.x % a.n_kv;
-    int at;
-    const int s = find_tile(a, ROWS, 0, a.few, static_cast<int>(blockIdx.x) / a.n_kv, at);
-    if (s < 0) return;
-    int first, n_new;
-    a.batch.rows(s, first, n_new);
-    const int ctx = a.batch.context[s];
+    const Tile tile = find_tile(a, ROWS, 0, a.few, static_cast<int>(blockIdx.x) / a.n_kv);
+    if (tile.s < 0) return;
+    const int s = tile.s, at = tile.at, first = tile.first, n_new = tile.n_new, ctx = tile.ctx;
     const Span span(a, s, n_new, ctx);
     const int c = blockIdx.y;
     if (c >= span.n) return;
@@ -351,12 +354,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) half_t sk[2][KT * D], sv[2][D * KT];
     __shared__ int s_ok[2][4];
     const int kh = blockIdx.x % a.n_kv;
-    int at;
-    const int s = find_tile(a, ROWS, a.few, INT64_MAX, static_cast<int>(blockIdx.x) / a.n_kv, at);
-    if (s < 0) return;
-    int first, n_new;
-    a.batch.rows(s, first, n_new);
-    const int ctx = a.batch.context[s], pos0 = ctx - n_new;
+    const Tile tile = find_tile(a, ROWS, a.few, INT64_MAX, static_cast<int>(blockIdx.x) / a.n_kv);
+    if (tile.s < 0) return;
+    const int s = tile.s, at = tile.at, first = tile.first, n_new = tile.n_new, ctx = tile.ctx, pos0 = ctx - n_new;
     const Span span(a, s, n_new, ctx);
     const int c = blockIdx.y;
     if (c >= span.n) return;
@@ -546,33 +546,116 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
         if (redo >> i & 1) store_alone<D>(a, s, kh, first, pos0, r0 + 32 * w + i, k0, k1, span.n, c);
 }
 
-template <int D>
+// ---------------------------------------------------------------- the chunks' states
+
+// Joins a row's chunks: out = sum_c num_c 2^(m_c - M) / sum_c den_c 2^(m_c - M), M the largest m_c. Up to
+// kFewChunks: a wave a row, everything requested at once. More: W waves a row, wave w taking chunks w,
+// w + W, ..; 64 of its chunks at a time have their maxima and sums read by a lane each, then their rows
+// follow with U requests in flight (5 tokens of 32 heads, 51 chunks: 19.6 us with a loop that carries the
+// maximum along and waits for each, 5.1 so).
+constexpr int kFewChunks = 8;
+
+template <int D, int W>
 __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
-    constexpr int PER = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t trow = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    constexpr int PER = D / 64, U = 8;
+    __shared__ float sm[4][D + 2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % W;
+    const int64_t trow = static_cast<int64_t>(blockIdx.x) * (4 / W) + wave / W;
     const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
     const int t = static_cast<int>((trow < rows ? trow : rows - 1) / a.heads);
     const int s = a.batch.sequence_of<64>(t);
-    if (trow >= rows || s >= a.batch.b) return;
-    int first, n_new;
-    a.batch.rows(s, first, n_new);
-    const int i = t - first;
-    if (i < 0 || i >= n_new) return;
-    const int ctx = a.batch.context[s];
-    const Span span(a, s, n_new, ctx);
-    if (span.n <= 1) return;
-    const float *pr = a.part + trow * a.nsplit * (D + 4);
-    float num[PER] = {}, den = 0.0f, m = -INFINITY;
-    for (int c = 0; c < span.n; ++c) {
-        const float *pc = pr + c * (D + 4);
-        const float mc = pc[D + 1], mx = fmaxf(m, mc), mu = mx == -INFINITY ? 0.0f : mx;
-        const float f = exp2_fast(m - mu), fc = exp2_fast(mc - mu);
-        m = mx;
-        den = den * f + pc[D] * fc;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) num[e] = num[e] * f + pc[lane * PER + e] * fc;
+    int first = 0, n_new = 0, n = 0;
+    if (trow < rows && s < a.batch.b) {
+        a.batch.rows(s, first, n_new);
+        if (t >= first && t - first < n_new) n = Span(a, s, n_new, a.batch.context[s]).n;
     }
+    float num[PER] = {}, den = 0.0f, m = -INFINITY;
+    const float *pr = a.part + trow * a.nsplit * (D + 4);
+    if (W == 1 && n > 1) {  // kFewChunks at most
+        float mc[kFewChunks], lc[kFewChunks], v[kFewChunks][PER];
+#pragma unroll
+        for (int c = 0; c < kFewChunks; ++c)
+            if (c < n) {
+                const float *pc = pr + c * (D + 4);
+                mc[c] = pc[D + 1];
+                lc[c] = pc[D];
+#pragma unroll
+                for (int e = 0; e < PER; ++e) v[c][e] = pc[lane * PER + e];
+            }
+#pragma unroll
+        for (int c = 0; c < kFewChunks; ++c)
+            if (c < n) m = fmaxf(m, mc[c]);
+        const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int c = 0; c < kFewChunks; ++c)
+            if (c < n) {
+                const float f = exp2_fast(mc[c] - mu);
+                den += lc[c] * f;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) num[e] += v[c][e] * f;
+            }
+    }
+    if (W > 1 && n > 1) {
+        for (int c0 = w; c0 < n; c0 += 64 * W) {
+            const int mine = c0 + lane * W;
+            const float mc = mine < n ? pr[static_cast<int64_t>(mine) * (D + 4) + D + 1] : -INFINITY;
+            const float lc = mine < n ? pr[static_cast<int64_t>(mine) * (D + 4) + D] : 0.0f;
+            float mx = mc;
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+            mx = fmaxf(mx, m);
+            const float mu = mx == -INFINITY ? 0.0f : mx, back = exp2_fast(m - mu), f = exp2_fast(mc - mu);
+            float dl = lc * f;
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) dl += __shfl_xor(dl, off, 64);
+            den = den * back + dl;
+            m = mx;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) num[e] *= back;
+            const int left = (n - c0 + W - 1) / W, count = left < 64 ? left : 64;
+            const float *pc = pr + static_cast<int64_t>(c0) * (D + 4) + lane * PER;
+            for (int i = 0; i < count; i += U) {
+                float v[U][PER];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+                        v[u][e] = pc[static_cast<int64_t>((i + u < count ? i + u : count - 1) * W) * (D + 4) + e];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float fu = i + u < count ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + u)) : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+                        if (i + u < count) num[e] += v[u][e] * fu;
+                }
+            }
+        }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sm[w][lane * PER + e] = num[e];
+        if (lane == 0) {
+            sm[w][D] = den;
+            sm[w][D + 1] = m;
+        }
+        __syncthreads();
+        if (w != 0) return;
+        float mx = m;
+#pragma unroll
+        for (int u = 1; u < W; ++u) mx = fmaxf(mx, sm[u][D + 1]);
+        const float mu = mx == -INFINITY ? 0.0f : mx, f0 = exp2_fast(m - mu);
+        den *= f0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) num[e] *= f0;
+#pragma unroll
+        for (int u = 1; u < W; ++u) {
+            const float f = exp2_fast(sm[u][D + 1] - mu);
+            den += sm[u][D] * f;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) num[e] += sm[u][lane * PER + e] * f;
+        }
+    }
+    if (n <= 1) return;
     const float inv = den == 0.0f ? 0.0f : 1.0f / den;
 #pragma unroll
     for (int e = 0; e < PER; ++e) a.out[trow * D + lane * PER + e] = static_cast<half_t>(num[e] * inv);
@@ -589,9 +672,9 @@ struct Plan {
 // Sequences of up to kFew rows go to the 16-row tiles. A batch without longer chunks has no 128-row
 // launch; one sequence alone goes where its chunk does.
 constexpr int64_t kFew = 32;
-// Chunks of the keys: enough for kFill workgroups where the tiles alone are fewer, none under
+// Chunks of the keys: enough to fill the chip's workgroups where the tiles alone do not, none under
 // kMinChunk keys.
-constexpr int64_t kFill = 1024, kMinChunk = 128;
+constexpr int64_t kFillSmall = 1024, kFillLarge = 512, kMinChunk = 128, kWhole = 384;
 
 inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window) {
     Plan p;
@@ -613,8 +696,8 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
     int64_t span = window > 0 && window + max_q + 63 < max_context ? window + max_q + 63 : max_context;
     if (span < 1) span = 1;
     const int64_t wgs = (p.small + p.large) * n_kv > 0 ? (p.small + p.large) * n_kv : 1;
-    int64_t n = (kFill + wgs - 1) / wgs;
-    const int64_t most = (span + kMinChunk - 1) / kMinChunk;
+    int64_t n = ((p.large > 0 ? kFillLarge : kFillSmall) + wgs - 1) / wgs;
+    const int64_t most = span <= kWhole ? 1 : (span + kMinChunk - 1) / kMinChunk;
     if (n > most) n = most;
     p.chunk = static_cast<int>(((span + n - 1) / n + 63) / 64 * 64);
     p.nsplit = static_cast<int>((span + p.chunk - 1) / p.chunk);
@@ -638,7 +721,10 @@ hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
     }
     if (e != hipSuccess || a.nsplit == 1) return e;
     const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
-    paged_attn_merge<D><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+    if (a.nsplit <= kFewChunks)
+        paged_attn_merge<D, 1><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+    else
+        paged_attn_merge<D, 4><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
