@@ -7,6 +7,10 @@
 // running sum) and output sums are f32; q, k, v are f16 as the cache and the matrix cores hold them;
 // the weights e^(s - max) are rounded to f16 for the second product (at most 2^-11 of each weight,
 // as the output's own rounding), and the output is rounded once.
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
 #include "paged.hpp"
 
 namespace dtts {
@@ -22,7 +26,8 @@ struct AttnArgs {
     float *part;       // per (row, chunk): D weighted sums, the weight sum, the maximum (log2)
     int64_t q_stride;  // elements between tokens
     int heads, n_kv, gqa, window;
-    float scale2;      // scale * log2(e): the softmax runs in base 2
+    float scale2;      // |scale| * log2(e), above 0: the softmax runs in base 2
+    bool negate;       // scale < 0: the queries change sign
     int chunk, nsplit; // keys per chunk, chunks at most (the last takes what is left)
     int64_t few;       // sequences of at most this many rows go to the 16-row tiles
 };
@@ -107,7 +112,7 @@ __device__ void attend_alone(const AttnArgs &a, int s, int kh, const half_t *qr,
         }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
-        const float sc = dot * a.scale2, mx = fmaxf(m, sc), mu = mx == -INFINITY ? 0.0f : mx;
+        const float sc = (a.negate ? -dot : dot) * a.scale2, mx = fmaxf(m, sc), mu = mx == -INFINITY ? 0.0f : mx;
         const float c = exp2_fast(m - mu), p = exp2_fast(sc - mu);
         m = mx;
         l = l * c + p;
@@ -193,7 +198,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
     {
         const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
-        for (int i = 0; i < C; ++i) qf[i] = *reinterpret_cast<const half8_t *>(qr + 32 * i + 8 * g);
+        for (int i = 0; i < C; ++i) {
+            qf[i] = *reinterpret_cast<const half8_t *>(qr + 32 * i + 8 * g);
+            if (a.negate) qf[i] = -qf[i];
+        }
     }
     const int in_page = (1 << a.batch.page_shift) - 1;
     const int64_t head_at = (static_cast<int64_t>(kh) << a.batch.page_shift) * D;
@@ -346,12 +354,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
 //
 // Two buffers: the next keys' rows are requested before a tile's products and stored after them, one
 // barrier a tile. Per 64 keys a wave has 1024 cycles of MFMA and about as many of softmax.
+constexpr float kSlack = 8.0f;
+
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
     constexpr int ROWS = 128, KT = 64, E = D / 16, C = D / 16, KL = D / 32;  // C: k steps, KL: 16-byte key loads a thread
     constexpr int KCH = D / 8;                                               // 16-byte pieces of a key row
     typedef half_t ve __attribute__((ext_vector_type(E)));
-    __shared__ __attribute__((aligned(16))) half_t sk[2][KT * D], sv[2][D * KT];
+    constexpr int KP = D + 8;  // elements from key row to key row in LDS
+    __shared__ __attribute__((aligned(16))) half_t sk[2][KT * KP], sv[2][D * KT];
     __shared__ int s_ok[2][4];
     const int kh = blockIdx.x % a.n_kv;
     const Tile tile = find_tile(a, ROWS, a.few, INT64_MAX, static_cast<int>(blockIdx.x) / a.n_kv);
@@ -379,7 +390,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
     {
         const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
-        for (int i = 0; i < C; ++i) qf[i] = *reinterpret_cast<const half8_t *>(qr + 16 * i + 8 * g);
+        for (int i = 0; i < C; ++i) {
+            qf[i] = *reinterpret_cast<const half8_t *>(qr + 16 * i + 8 * g);
+            if (a.negate) qf[i] = -qf[i];
+        }
     }
     const int in_page = (1 << a.batch.page_shift) - 1;
     const int64_t head_at = (static_cast<int64_t>(kh) << a.batch.page_shift) * D;
@@ -403,7 +417,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int r = 16 * w + krow + i * (64 / KCH);
-            *reinterpret_cast<half8_t *>(&sk[buf][r * D + ((kch ^ r) & (KCH - 1)) * 8]) = gk[i];
+            *reinterpret_cast<half8_t *>(&sk[buf][r * KP + kch * 8]) = gk[i];
         }
         if (!g_ok || kb + 16 * w + 16 > k1) {  // slots that hold no position: 0 times what is there may be NaN
 #pragma unroll
@@ -419,35 +433,41 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
         }
         if (lane == 0) s_ok[buf][w] = g_ok;
     };
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, m2 = 0.0f, l = 0.0f;  // m2: m in log2, 0 while there is none
     float16_t o[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-    auto compute = [&](int kb, int buf) {
+    auto compute = [&](int kb, auto which) {
+        constexpr int buf = decltype(which)::value;
         float16_t sc[2];
+        half8_t kf[C][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int i = 0; i < C; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
+            for (int u = 0; u < 2; ++u) kf[i][u] = *reinterpret_cast<const half8_t *>(&sk[buf][(32 * u + l32) * KP + 16 * i + 8 * g]);
 #pragma unroll
         for (int i = 0; i < C; ++i)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int r = 32 * u + l32;
-                const half8_t kf = *reinterpret_cast<const half8_t *>(&sk[buf][r * D + (((2 * i + g) ^ r) & (KCH - 1)) * 8]);
-                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], sc[u], 0, 0, 0);
+                if (i == 0)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
+                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i][u], qf[i], sc[u], 0, 0, 0);
             }
         int ok[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) ok[t] = __builtin_amdgcn_readfirstlane(s_ok[buf][t]);
+        // reads run four ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * C; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
         const bool whole = kb + KT - 1 <= wfirst && kb + KT <= k1 && (a.window == 0 || kb > wlast - a.window) &&
                            (ok[0] & ok[1] & ok[2] & ok[3]);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[u][r] *= a.scale2;
         if (!whole) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -457,28 +477,29 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
                     if (!(key <= pos && key >= row_lo && key < k1 && ok[2 * u + (r >> 3)])) sc[u][r] = -INFINITY;
                 }
         }
-        float mx = m;
+        float mx = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[u][r]);
+        for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, sc[0][r]), sc[1][r]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mu = mx == -INFINITY ? 0.0f : mx;
-        if (__any(mx > m)) {
-            const float f = exp2_fast(m - mu);
+        // weights are taken relative to m, an earlier maximum, until a row outgrows it by 2^kSlack: the sums
+        // hold that as well, and few tiles after the first move it
+        if (__any((mx - m) * a.scale2 > kSlack)) {
+            mx = fmaxf(mx, m);
+            const float f = exp2_fast(mx == -INFINITY ? 0.0f : (m - mx) * a.scale2);
             l *= f;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= f;
             m = mx;
+            m2 = m == -INFINITY ? 0.0f : m * a.scale2;
         }
         half8_t pf[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float x = exp2_fast(sc[t >> 1][8 * (t & 1) + j] - mu);
+                const float x = exp2_fast(__builtin_fmaf(sc[t >> 1][8 * (t & 1) + j], a.scale2, -m2));
                 l += x;
                 pf[t][j] = static_cast<half_t>(x);
             }
@@ -491,19 +512,25 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[t], o[d], 0, 0, 0);
             }
     };
-    int kb = k0 & ~(KT - 1), buf = 0;
+    int kb = k0 & ~(KT - 1);
+    auto turn = [&](auto which) {
+        constexpr int buf = decltype(which)::value;
+        if (wrows > 0 && kb <= wlast && (a.window == 0 || kb + KT > wfirst - a.window + 1)) compute(kb, which);
+        if (kb + KT < k1) {
+            store(kb + KT, buf ^ 1);
+            if (kb + 2 * KT < k1) load(kb + 2 * KT);
+        }
+        __syncthreads();
+        kb += KT;
+    };
     if (kb < k1) {
         load(kb);
         store(kb, 0);
         if (kb + KT < k1) load(kb + KT);
         __syncthreads();
-        for (; kb < k1; kb += KT, buf ^= 1) {
-            if (wrows > 0 && kb <= wlast && (a.window == 0 || kb + KT > wfirst - a.window + 1)) compute(kb, buf);
-            if (kb + KT < k1) {
-                store(kb + KT, buf ^ 1);
-                if (kb + 2 * KT < k1) load(kb + 2 * KT);
-            }
-            __syncthreads();
+        while (kb < k1) {
+            turn(std::integral_constant<int, 0>{});
+            if (kb < k1) turn(std::integral_constant<int, 1>{});
         }
     }
     if (wrows <= 0) return;
@@ -526,7 +553,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
                     *reinterpret_cast<float4_t *>(pr + 32 * d + 2 * r + 4 * g) = float4_t{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
             if (g == 0) {
                 pr[D] = l;
-                pr[D + 1] = m;
+                pr[D + 1] = m == -INFINITY ? m : m2;
             }
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees no key is zero
@@ -781,7 +808,9 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
     a.n_kv = static_cast<int>(n_kv);
     a.gqa = static_cast<int>(heads / n_kv);
     a.window = static_cast<int>(window);
-    a.scale2 = scale * kLog2e;
+    // a scale of 0 is the smallest number: every score then is 0, and a masked one still -inf
+    a.scale2 = fmaxf(fabsf(scale) * kLog2e, FLT_MIN);
+    a.negate = scale < 0.0f;
     a.few = p.few;
     a.part = nullptr;
     if (p.nsplit > 1 && workspace && ws_bytes >= part_bytes(p, tokens, heads, head_dim)) {
