@@ -400,13 +400,19 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
     // staging: wave w takes keys 16w .. 16w + 15 of a tile, one page
     half8_t gk[KL];
     ve gv[4];
-    int g_ok = 0;
+    bool g_ok = false;
     const int krow = lane / KCH, kch = lane % KCH, a4 = lane >> 4, db = lane & 15;
-    auto load = [&](int kb) {
-        const int key = kb + 16 * w;
-        const int page = key < k1 ? a.batch.page(s, key >> a.batch.page_shift) : -1;
-        g_ok = page >= 0;
-        const int64_t base = (page < 0 ? 0 : page) * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D;
+    const int32_t *table = a.batch.table + static_cast<int64_t>(s) * a.batch.max_pages;
+    auto id_of = [&](int kb) {
+        const int block = (kb + 16 * w) >> a.batch.page_shift;
+        return table[block < a.batch.max_pages ? block : a.batch.max_pages - 1];
+    };
+    int next_id = id_of(k0 & ~(KT - 1));  // of the tile to be requested next
+    auto load = [&](int kb) {  // past the last key: somewhere in page 0, for nothing, so that no branch holds a request
+        const int key = kb + 16 * w, id = next_id;
+        next_id = id_of(kb + KT);
+        g_ok = key < k1 && id >= 0 && id < a.batch.n_pages;
+        const int64_t base = (g_ok ? id : 0) * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D;
 #pragma unroll
         for (int i = 0; i < KL; ++i)
             gk[i] = *reinterpret_cast<const half8_t *>(a.k + base + (krow + i * (64 / KCH)) * D + kch * 8);
@@ -469,12 +475,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
         const bool whole = kb + KT - 1 <= wfirst && kb + KT <= k1 && (a.window == 0 || kb > wlast - a.window) &&
                            (ok[0] & ok[1] & ok[2] & ok[3]);
         if (!whole) {
+            const int hi = (pos < k1 ? pos : k1 - 1) - kb - 4 * g, lo = row_lo - kb - 4 * g;  // of the key's place in the tile
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int key = kb + 32 * u + 8 * (r >> 2) + 4 * g + (r & 3);
-                    if (!(key <= pos && key >= row_lo && key < k1 && ok[2 * u + (r >> 3)])) sc[u][r] = -INFINITY;
+                    const int at_key = 32 * u + 8 * (r >> 2) + (r & 3);
+                    if (at_key > hi || at_key < lo || !ok[2 * u + (r >> 3)]) sc[u][r] = -INFINITY;
                 }
         }
         float mx = fmaxf(sc[0][0], sc[1][0]);
@@ -516,17 +523,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk(AttnArgs a) {
     auto turn = [&](auto which) {
         constexpr int buf = decltype(which)::value;
         if (wrows > 0 && kb <= wlast && (a.window == 0 || kb + KT > wfirst - a.window + 1)) compute(kb, which);
-        if (kb + KT < k1) {
-            store(kb + KT, buf ^ 1);
-            if (kb + 2 * KT < k1) load(kb + 2 * KT);
-        }
+        store(kb + KT, buf ^ 1);
+        load(kb + 2 * KT);
         __syncthreads();
         kb += KT;
     };
     if (kb < k1) {
         load(kb);
         store(kb, 0);
-        if (kb + KT < k1) load(kb + KT);
+        load(kb + KT);
         __syncthreads();
         while (kb < k1) {
             turn(std::integral_constant<int, 0>{});
