@@ -53,7 +53,7 @@ struct Row {  // one row's settings, made safe
     int k;
     double u, inv_t;
     bool greedy;
-    __device__ __forceinline__ bool filters() const { return k > 0 || (p < 1.0f && p > 0.0f); }
+    __device__ __forceinline__ bool filters() const { return k > 0 || p < 1.0f; }
 };
 
 template <typename T>
@@ -62,8 +62,8 @@ __device__ __forceinline__ Row row_of(const SampleArgs<T> &a, int r) {
     const float t = a.temperature ? a.temperature[r] : 1.0f;
     const int k = a.top_k ? a.top_k[r] : 0;
     const float p = a.top_p ? a.top_p[r] : 1.0f, m = a.min_p ? a.min_p[r] : 0.0f, u = a.u[r];
-    s.greedy = !(t > 0.0f);
-    s.inv_t = 1.0 / static_cast<double>(s.greedy ? 1.0f : t);
+    s.greedy = !(t > 0.0f) || p <= 0.0f;  // a top-p of nothing keeps the first token alone
+    s.inv_t = 1.0 / static_cast<double>(t > 0.0f ? t : 1.0f);
     s.per_unit = kBins / (kRange * fmaxf(t, 1.0f));
     s.k = k <= 0 || k >= a.vocab ? 0 : k;  // 0: all
     s.p = p < 1.0f ? p : 1.0f;             // 1 (or not a number): all
@@ -498,22 +498,92 @@ __device__ u64 threshold(Shared<NT> &sh, const Held<T, NT, E> &row, float top, c
 
 // ---------------------------------------------------------------- one workgroup a row
 
+// The weight of logit i if it is kept.
+__device__ __forceinline__ u64 kept_mass(float l, int i, float top, const Row &s, u64 best, u64 cut) {
+    if (l == -INFINITY) return 0;
+    const u64 k = pack(l, i);
+    if (k < cut) return 0;
+    const double x = weight(l, top, s.inv_t);
+    return x >= static_cast<double>(s.m) || k == best ? mass(x) : 0;
+}
+
+// The kept weight of the w-th of each NW runs of 256 logits from i0 on, to sh.seg.
+template <typename T, int NT>
+__device__ __forceinline__ void sum_runs(Shared<NT> &sh, const T *row, int i0, int i1, float top, const Row &s, u64 best, u64 cut) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, segs = (i1 - i0 + 255) / 256;
+    const bool vec = reinterpret_cast<uintptr_t>(row + i0) % (4 * sizeof(T)) == 0;
+    for (int seg = w; seg < segs; seg += NT / 64) {
+        const int i = i0 + seg * 256 + lane * 4;
+        u64 m = 0;
+        if (vec && i + 4 <= i1) {
+            const v4 v = *reinterpret_cast<const v4 *>(row + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m += kept_mass(logit(v[e]), i + e, top, s, best, cut);
+        } else {
+            for (int e = 0; e < 4 && i + e < i1; ++e) m += kept_mass(logit(row[i + e]), i + e, top, s, best, cut);
+        }
+        m = last_lane(wave_scan(m));
+        if (lane == 0) sh.seg[seg] = m;
+    }
+}
+
+// The token where the kept weight passes `target`, from the runs' weights in sh.seg: logits [i0, i1), `upto`
+// the kept weight before them. z: the whole row's.
+template <typename T, int NT, int MOST>
+__device__ __forceinline__ void find_token(Shared<NT> &sh, const SampleArgs<T> &a, const T *row, int r, const Row &s, u64 best, u64 cut,
+                                           int i0, int i1, u64 upto, u64 target, u64 z, u64 t, u64 before) {
+    constexpr int SP = (MOST + NT - 1) / NT;  // runs a thread, whose weight is t, after `before`
+    const int lane = threadIdx.x & 63;
+    const float top = logit_of(best);
+    before += upto;
+    if (before <= target && target < before + t) {  // one thread
+        for (int i = 0; i < SP; ++i) {
+            const u64 m = sh.seg[threadIdx.x * SP + i];
+            if (target < before + m) {
+                sh.n = threadIdx.x * SP + i;
+                sh.out0 = before;
+                break;
+            }
+            before += m;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const int i = i0 + sh.n * 256 + lane * 4;
+    u64 m[4], mine = 0;
+    float l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        l[e] = i + e < i1 ? logit(row[i + e]) : -INFINITY;
+        mine += m[e] = kept_mass(l[e], i + e, top, s, best, cut);
+    }
+    u64 run = sh.out0 + wave_scan(mine) - mine;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (run <= target && target < run + m[e]) {
+            a.token[r] = i + e;
+            if (a.logprob) {
+                const double d = l[e] == top ? 0.0 : (static_cast<double>(l[e]) - static_cast<double>(top)) * s.inv_t;
+                a.logprob[r] = static_cast<float>(d - log(static_cast<double>(z) / kUnit));
+            }
+        }
+        run += m[e];
+    }
+}
+
+__device__ __forceinline__ u64 target_of(const Row &s, u64 z) {
+    const u64 t = static_cast<u64>(s.u * static_cast<double>(z));
+    return t >= z ? z - 1 : t;
+}
+
 // The row's token from its kept tokens' weights: in runs of 256 logits, then inside the run that u falls into.
 template <typename T, int NT, int E>
 __device__ __forceinline__ void choose(Shared<NT> &sh, const SampleArgs<T> &a, const Held<T, NT, E> &row, int r, const Row &s, u64 best,
                                        u64 cut) {
-    constexpr int NW = NT / 64;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, vocab = a.vocab;
+    constexpr int NW = NT / 64, MOST = E > 0 ? E / 4 * NW : kSegs, SP = (MOST + NT - 1) / NT;
     const float top = logit_of(best);
-    const double min_p = static_cast<double>(s.m);
-    auto kept = [&](float l, int i) -> u64 {
-        if (l == -INFINITY) return 0;
-        const u64 k = pack(l, i);
-        if (k < cut) return 0;
-        const double x = weight(l, top, s.inv_t);
-        return x >= min_p || k == best ? mass(x) : 0;
-    };
-    const int segs = (vocab + 255) / 256;
+    const int segs = (a.vocab + 255) / 256;
     if constexpr (E > 0) {
 #pragma unroll
         for (int q = 0; q < E / 4; ++q) {
@@ -524,66 +594,21 @@ __device__ __forceinline__ void choose(Shared<NT> &sh, const SampleArgs<T> &a, c
                 const float l = row.l[4 * q + e];
                 if (l == -INFINITY) continue;
                 const u64 k = pack(l, i);
-                if (k >= cut && (s.m == 0.0f || k == best || weight(l, top, s.inv_t) >= min_p)) m += row.m[4 * q + e];
+                if (k >= cut && (s.m == 0.0f || k == best || weight(l, top, s.inv_t) >= static_cast<double>(s.m))) m += row.m[4 * q + e];
             }
             m = last_lane(wave_scan(m));
-            if (lane == 0 && q * NW + w < kSegs) sh.seg[q * NW + w] = m;
+            if ((threadIdx.x & 63) == 0) sh.seg[q * NW + (threadIdx.x >> 6)] = m;
         }
     } else {
-        for (int seg = w; seg < segs; seg += NW) {
-            u64 m = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = seg * 256 + lane * 4 + e;
-                if (i < vocab) m += kept(logit(row.row[i]), i);
-            }
-            m = last_lane(wave_scan(m));
-            if (lane == 0) sh.seg[seg] = m;
-        }
+        sum_runs<T, NT>(sh, row.row, 0, a.vocab, top, s, best, cut);
     }
     __syncthreads();
-    constexpr int SP = E > 0 ? (E / 4 * NW + NT - 1) / NT : kSegs / NT;
     u64 t = 0, before, z, x, y;
 #pragma unroll
     for (int i = 0; i < SP; ++i)
         if (static_cast<int>(threadIdx.x) * SP + i < segs) t += sh.seg[threadIdx.x * SP + i];
     block_scan<NT>(sh, t, 0, before, x, z, y);
-    u64 target = static_cast<u64>(s.u * static_cast<double>(z));
-    if (target >= z) target = z - 1;
-    if (before <= target && target < before + t) {  // one thread
-        u64 upto = before;
-        for (int i = 0; i < SP; ++i) {
-            const u64 m = sh.seg[threadIdx.x * SP + i];
-            if (target < upto + m) {
-                sh.n = threadIdx.x * SP + i;
-                sh.out0 = upto;
-                break;
-            }
-            upto += m;
-        }
-    }
-    __syncthreads();
-    if (w != 0) return;
-    const int i0 = sh.n * 256 + lane * 4;
-    u64 m[4], mine = 0;
-    float l[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        l[e] = i0 + e < vocab ? logit(row.row[i0 + e]) : -INFINITY;
-        mine += m[e] = kept(l[e], i0 + e);
-    }
-    u64 upto = sh.out0 + wave_scan(mine) - mine;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (upto <= target && target < upto + m[e]) {
-            a.token[r] = i0 + e;
-            if (a.logprob) {
-                const double d = l[e] == top ? 0.0 : (static_cast<double>(l[e]) - static_cast<double>(top)) * s.inv_t;
-                a.logprob[r] = static_cast<float>(d - log(static_cast<double>(z) / kUnit));
-            }
-        }
-        upto += m[e];
-    }
+    find_token<T, NT, MOST>(sh, a, row.row, r, s, best, cut, 0, a.vocab, 0, target_of(s, z), z, t, before);
 }
 
 // Nothing to choose from, or no choice. True when that was so.
@@ -619,9 +644,7 @@ __device__ __forceinline__ void sample_whole(Shared<NT> &sh, const SampleArgs<T>
     const float top = logit_of(best);
     row.weigh(top, s.inv_t);
     u64 cut = 0;
-    if (s.p <= 0.0f) {
-        cut = best;
-    } else if (s.filters()) {
+    if (s.filters()) {
         row.all(top, s.inv_t, [&](float l, int, auto m) {
             const int b = bin_of(l, top, s.per_unit);
             atomicAdd(&sh.h.count[b], 1u);
@@ -640,6 +663,263 @@ __global__ __launch_bounds__(NT) void sample_row(SampleArgs<T> a) {
     sample_whole<T, NT, E>(sh, a, blockIdx.x);
 }
 
+// ---------------------------------------------------------------- several workgroups a row
+
+constexpr int kPartNT = 512;     // threads of the workgroups that share a row
+constexpr int kMostParts = 256;  // of a row
+
+// What the workgroups of a row leave each other. All but `mass` of a part and the candidates beyond
+// n_cand is written by one launch before the next reads it.
+struct RowState {
+    u64 hist_mass[kBins];
+    u64 best[kMostParts], part_mass[kMostParts];
+    u64 cand[kCand];
+    uint32_t hist_count[kBins];
+    uint32_t n_cand;
+    // the bins that hold the top-k threshold (-1: none) and may hold the top-p one (lo .. hi), the sums
+    // above them, the members of the first
+    int32_t k_bin, lo, hi;
+    u64 k_above_c, k_above_m, lo_above_m;
+    uint32_t k_count, pad;
+};
+
+template <typename T>
+struct PartArgs {
+    SampleArgs<T> a;
+    RowState *rows;
+    int part, parts;  // logits of a part (a multiple of 1024), parts of a row
+};
+
+template <int NT>
+__device__ __forceinline__ u64 best_of(Shared<NT> &sh, const RowState &st, int parts) {
+    return block_max<NT>(sh, static_cast<int>(threadIdx.x) < parts ? st.best[threadIdx.x] : 0);
+}
+
+// First launch: each part's largest; the histogram is cleared.
+template <typename T>
+__global__ __launch_bounds__(kPartNT) void sample_part_max(PartArgs<T> p) {
+    __shared__ Shared<kPartNT> sh;
+    const int g = blockIdx.x, r = blockIdx.y, i0 = g * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    RowState &st = p.rows[r];
+    for (int i = g * kPartNT + threadIdx.x; i < kBins; i += p.parts * kPartNT) {
+        st.hist_mass[i] = 0;
+        st.hist_count[i] = 0;
+    }
+    if (g == 0 && threadIdx.x == 0) st.n_cand = 0;
+    const T *row = p.a.logits + r * p.a.stride;
+    const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
+    u64 best = pack(-INFINITY, i0);
+    each<T, kPartNT>(row, i0, i1, vec, [&](float l, int i) {
+        const u64 k = pack(l, i);
+        best = k > best ? k : best;
+    });
+    best = block_max<kPartNT>(sh, best);
+    if (threadIdx.x == 0) st.best[g] = best;
+}
+
+// Second: the histogram of a row that filters by rank or weight, the part's kept weight of one that does not.
+template <typename T>
+__global__ __launch_bounds__(kPartNT) void sample_part_hist(PartArgs<T> p) {
+    __shared__ Shared<kPartNT> sh;
+    const int g = blockIdx.x, r = blockIdx.y, i0 = g * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    RowState &st = p.rows[r];
+    const Row s = row_of(p.a, r);
+    if (s.filters())
+        for (int i = threadIdx.x; i < kBins; i += kPartNT) {
+            sh.h.mass[i] = 0;
+            sh.h.count[i] = 0;
+        }
+    const u64 best = best_of<kPartNT>(sh, st, p.parts);
+    const float top = logit_of(best);
+    if (top == -INFINITY || s.greedy) return;
+    const T *row = p.a.logits + r * p.a.stride;
+    const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
+    if (!s.filters()) {
+        u64 m = 0, x, y, all, z;
+        each<T, kPartNT>(row, i0, i1, vec, [&](float l, int i) { m += kept_mass(l, i, top, s, best, 0); });
+        block_scan<kPartNT>(sh, m, 0, x, y, all, z);
+        if (threadIdx.x == 0) st.part_mass[g] = all;
+        return;
+    }
+    const bool by_mass = s.p < 1.0f;
+    each<T, kPartNT>(row, i0, i1, vec, [&](float l, int) {
+        if (l == -INFINITY) return;
+        const int b = bin_of(l, top, s.per_unit);
+        atomicAdd(&sh.h.count[b], 1u);
+        if (by_mass) {
+            const u64 m = mass(weight(l, top, s.inv_t));
+            if (m) atomicAdd(&sh.h.mass[b], m);
+        }
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kPartNT) {
+        if (sh.h.count[i]) atomicAdd(&st.hist_count[i], sh.h.count[i]);
+        if (sh.h.mass[i]) atomicAdd(&st.hist_mass[i], sh.h.mass[i]);
+    }
+}
+
+// Third: where the thresholds lie (every workgroup for itself, from the histogram), the members of those bins,
+// and the part's kept weight above them.
+template <typename T>
+__global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
+    __shared__ Shared<kPartNT> sh;
+    const int g = blockIdx.x, r = blockIdx.y, i0 = g * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    RowState &st = p.rows[r];
+    const Row s = row_of(p.a, r);
+    if (s.greedy || !s.filters()) return;
+    const u64 best = best_of<kPartNT>(sh, st, p.parts);
+    const float top = logit_of(best);
+    if (top == -INFINITY) return;
+    Bins<kPartNT> bins;
+    bins.scan(sh, st.hist_mass, st.hist_count);
+    int k_bin = -1, lo = kBins, hi = -1;
+    u64 k_above_c = 0, k_above_m = 0, lo_above_m = 0, x, y;
+    if (s.k) k_bin = bins.cross(sh, false, static_cast<double>(s.k), kBins - 1, ~0ull, k_above_c, k_above_m);
+    if (s.p < 1.0f) {
+        // the top-k's weight is between those of the bins above its threshold's and with it
+        const u64 least = k_bin >= 0 ? k_above_m : bins.m_all;
+        const u64 most = k_bin >= 0 ? k_above_m + st.hist_mass[k_bin] : bins.m_all;
+        const int last = k_bin >= 0 ? k_bin : kBins - 1;
+        const double p64 = static_cast<double>(s.p);
+        hi = bins.cross(sh, true, p64 * static_cast<double>(most), last, ~0ull, x, lo_above_m);
+        lo = hi;
+        if (least < most) {
+            lo = bins.cross(sh, true, p64 * static_cast<double>(least), last, ~0ull, x, y);
+            if (lo < 0) {
+                lo = 0;  // least is 0
+                y = 0;
+            }
+            lo_above_m = y;
+        }
+        if (hi < 0) lo = kBins;  // no threshold: all of the top-k
+    } else {
+        lo = hi = k_bin;
+        if (k_bin < 0) lo = kBins;
+        lo_above_m = k_above_m;
+    }
+    const int sure = k_bin >= 0 && k_bin < lo ? k_bin : lo;  // the bins before it are kept
+    if (g == 0 && threadIdx.x == 0) {
+        st.k_bin = k_bin;
+        st.lo = lo;
+        st.hi = hi;
+        st.k_above_c = k_above_c;
+        st.k_above_m = k_above_m;
+        st.lo_above_m = lo_above_m;
+        st.k_count = k_bin >= 0 ? st.hist_count[k_bin] : 0;
+    }
+    const T *row = p.a.logits + r * p.a.stride;
+    const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
+    u64 m = 0, all, z;
+    each<T, kPartNT>(row, i0, i1, vec, [&](float l, int i) {
+        if (l == -INFINITY) return;
+        const int b = bin_of(l, top, s.per_unit);
+        if (b < sure) {
+            m += kept_mass(l, i, top, s, best, 0);
+        } else if ((b >= lo && b <= hi) || b == k_bin) {
+            const uint32_t at = atomicAdd(&st.n_cand, 1u);
+            if (at < kCand) st.cand[at] = pack(l, i);
+        }
+    });
+    block_scan<kPartNT>(sh, m, 0, x, y, all, z);
+    if (threadIdx.x == 0) st.part_mass[g] = all;
+}
+
+// Fourth, a workgroup a row: the thresholds among the members, the part that u falls into, the token.
+template <typename T>
+__global__ __launch_bounds__(1024) void sample_finish(PartArgs<T> p) {
+    constexpr int NT = 1024;
+    __shared__ Shared<NT> sh;
+    __shared__ u64 part_mass[kMostParts];
+    const int r = blockIdx.x;
+    RowState &st = p.rows[r];
+    const Row s = row_of(p.a, r);
+    const u64 best = best_of<NT>(sh, st, p.parts);
+    if (settled(p.a, r, s, best)) return;
+    const float top = logit_of(best);
+    if (static_cast<int>(threadIdx.x) < p.parts) part_mass[threadIdx.x] = st.part_mass[threadIdx.x];
+    u64 cut = 0;
+    if (s.filters()) {
+        const int n = static_cast<int>(st.n_cand);
+        if (n > kCand) {  // many members: equal logits, or a narrow spread
+            sample_whole<T, NT, 0>(sh, p.a, r);
+            return;
+        }
+        if (static_cast<int>(threadIdx.x) < n) sh.cand[threadIdx.x] = st.cand[threadIdx.x];
+        __syncthreads();
+        sort_desc<NT>(sh.cand, n);
+        // the top-k bin's members are the last of the list
+        u64 sum = st.k_above_m, upto;
+        u64 want_k = 0;
+        if (st.k_bin >= 0) {
+            const int from = n - static_cast<int>(st.k_count);
+            const int at = from + s.k - static_cast<int>(st.k_above_c) - 1;
+            cut = want_k = sh.cand[at];
+            u64 x, y, z;
+            const int i = threadIdx.x;
+            block_scan<NT>(sh, i >= from && i <= at ? mass(weight(logit_of(sh.cand[i]), top, s.inv_t)) : 0, 0, x, y, upto, z);
+            sum += upto;
+        } else if (s.p < 1.0f) {
+            u64 x, y, z, v = 0;
+            for (int i = threadIdx.x; i < kBins; i += NT) v += st.hist_mass[i];
+            block_scan<NT>(sh, v, 0, x, y, sum, z);
+        }
+        if (s.p < 1.0f && st.hi >= 0) {
+            const u64 c = cut_in<NT>(sh, n, true, 0, st.lo_above_m, static_cast<double>(s.p) * static_cast<double>(sum), top, s.inv_t, upto);
+            cut = c > cut ? c : cut;
+        }
+        // their weights to their parts
+        if (static_cast<int>(threadIdx.x) < n) {
+            const u64 k = sh.cand[threadIdx.x];
+            const u64 m = kept_mass(logit_of(k), index_of(k), top, s, best, cut);
+            if (m) atomicAdd(&part_mass[index_of(k) / p.part], m);
+        }
+    }
+    __syncthreads();
+    u64 before, z, x, y;
+    const u64 t = static_cast<int>(threadIdx.x) < p.parts ? part_mass[threadIdx.x] : 0;
+    block_scan<NT>(sh, t, 0, before, x, z, y);
+    const u64 target = target_of(s, z);
+    if (before <= target && target < before + t) {
+        sh.bin = threadIdx.x;
+        sh.out1 = before;
+    }
+    __syncthreads();
+    const int i0 = sh.bin * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    const u64 upto = sh.out1;
+    const T *row = p.a.logits + r * p.a.stride;
+    sum_runs<T, NT>(sh, row, i0, i1, top, s, best, cut);
+    __syncthreads();
+    constexpr int MOST = NT;  // runs of a part (kMostPart)
+    const u64 seg = static_cast<int>(threadIdx.x) * 256 < i1 - i0 ? sh.seg[threadIdx.x] : 0;
+    u64 part_all;
+    block_scan<NT>(sh, seg, 0, before, x, part_all, y);
+    find_token<T, NT, MOST>(sh, p.a, row, r, s, best, cut, i0, i1, upto, target, z, seg, before);
+}
+
+struct Parts {
+    int part, parts;
+};
+
+// Rows of up to kWholeVocab logits, and rows enough to fill the chip by themselves, are one workgroup each.
+constexpr int64_t kWholeVocab = 8192, kPartFill = 512;
+constexpr int64_t kMostPart = 1024 * 256;  // a run of 256 logits for each thread of the last launch
+
+inline Parts parts_of(int64_t rows, int64_t vocab) {
+    int64_t part = (rows * vocab + kPartFill - 1) / kPartFill;
+    if (part < 2048) part = 2048;
+    if (part < (vocab + kMostParts - 1) / kMostParts) part = (vocab + kMostParts - 1) / kMostParts;
+    part = (part + 1023) / 1024 * 1024;
+    Parts p;
+    p.part = static_cast<int>(part);
+    p.parts = static_cast<int>((vocab + part - 1) / part);
+    if (vocab <= kWholeVocab || part > kMostPart || p.parts < 2) p.parts = 1;
+    return p;
+}
+
+inline size_t sample_bytes(int64_t rows, int64_t vocab) {
+    return parts_of(rows, vocab).parts > 1 ? static_cast<size_t>(rows) * sizeof(RowState) : 0;
+}
+
 template <typename T>
 int sample(const char *name, const T *logits, const float *temperature, const int32_t *top_k, const float *top_p,
            const float *min_p, const float *u, int32_t *token, float *logprob, int64_t rows, int64_t vocab, int64_t stride,
@@ -653,19 +933,32 @@ int sample(const char *name, const T *logits, const float *temperature, const in
     DTTS_REQUIRE(aligned(logits, sizeof(T)) && aligned(temperature, 4) && aligned(top_k, 4) && aligned(top_p, 4) &&
                      aligned(min_p, 4) && aligned(u, 4) && aligned(token, 4) && aligned(logprob, 4),
                  "%s: misaligned operand", name);
-    (void)workspace;
-    (void)ws_bytes;
     SampleArgs<T> a{logits, stride, temperature, top_p, min_p, u, top_k, token, logprob, static_cast<int>(rows),
                     static_cast<int>(vocab)};
     const unsigned grid = static_cast<unsigned>(rows);
+    const Parts parts = parts_of(rows, vocab);
+    if (parts.parts > 1 && workspace && ws_bytes >= sample_bytes(rows, vocab)) {
+        DTTS_REQUIRE(aligned(workspace, 16), "%s: misaligned workspace", name);
+        const PartArgs<T> p{a, static_cast<RowState *>(workspace), parts.part, parts.parts};
+        const dim3 each_part(static_cast<unsigned>(parts.parts), grid);
+        sample_part_max<T><<<each_part, kPartNT, 0, stream>>>(p);
+        DTTS_LAUNCH_CHECK(name);
+        sample_part_hist<T><<<each_part, kPartNT, 0, stream>>>(p);
+        DTTS_LAUNCH_CHECK(name);
+        sample_part_collect<T><<<each_part, kPartNT, 0, stream>>>(p);
+        DTTS_LAUNCH_CHECK(name);
+        sample_finish<T><<<grid, 1024, 0, stream>>>(p);
+        DTTS_LAUNCH_CHECK(name);
+        return DTTS_OK;
+    }
     if (vocab <= 1024)
         sample_row<T, 256, 4><<<grid, 256, 0, stream>>>(a);
     else if (vocab <= 2048)
         sample_row<T, 256, 8><<<grid, 256, 0, stream>>>(a);
     else if (vocab <= 4096)
         sample_row<T, 512, 8><<<grid, 512, 0, stream>>>(a);
-    else if (vocab <= 16384)
-        sample_row<T, 1024, 16><<<grid, 1024, 0, stream>>>(a);
+    else if (vocab <= 8192)
+        sample_row<T, 1024, 8><<<grid, 1024, 0, stream>>>(a);
     else
         sample_row<T, 1024, 0><<<grid, 1024, 0, stream>>>(a);
     DTTS_LAUNCH_CHECK(name);
@@ -676,9 +969,7 @@ int sample(const char *name, const T *logits, const float *temperature, const in
 }  // namespace dtts
 
 extern "C" size_t dtts_sample_workspace_bytes(int64_t rows, int64_t vocab) {
-    (void)rows;
-    (void)vocab;
-    return 0;
+    return rows > 0 && vocab > 0 && rows < (int64_t(1) << 24) && vocab <= dtts::kMaxVocab ? dtts::sample_bytes(rows, vocab) : 0;
 }
 
 extern "C" int dtts_sample_f32(const float *logits, const float *temperature, const int32_t *top_k, const float *top_p,
