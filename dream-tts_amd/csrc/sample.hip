@@ -21,6 +21,7 @@
 // every pass over the logits after the first from L2 or the MALL. What bounds them: a short row the chain
 // of block-wide steps, a long one the f64 exponentials and the launches.
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -157,6 +158,8 @@ __device__ __forceinline__ u64 wave_max(u64 v) {
 
 constexpr int kSegs = 4096;  // runs of 256 logits: vocabularies of up to 2^20
 
+// One barrier a sum: the waves' parts go to the two halves of `red` in turn, and every other value that one
+// thread leaves the rest has a place of its own (k: [0], p: [1]).
 template <int NT>
 struct Shared {
     static constexpr int NW = NT / 64;
@@ -170,30 +173,40 @@ struct Shared {
     u64 cand[kCand];
     u64 digit_mass[256];
     uint32_t digit_count[256];
-    u64 red[2][NW];
-    u64 out0, out1;
-    int n, bin;
+    u64 red[2][2][NW];
+    u64 above_c[2], above_m[2], cut[2], upto[2];  // of a threshold: the sums before its bin, itself, the sum with it
+    int bin[2], n[2];                             // its bin (-1: none), the bin's members
+    u64 run_before;                               // the run that u falls into
+    int run, digit;
+
+    // By any thread before the first barrier.
+    __device__ __forceinline__ void clear() {
+        if (threadIdx.x < 2) {
+            bin[threadIdx.x] = -1;
+            n[threadIdx.x] = 0;
+        }
+    }
 };
 
 template <int NT>
-__device__ __forceinline__ u64 block_max(Shared<NT> &sh, u64 v) {
+__device__ __forceinline__ u64 block_max(Shared<NT> &sh, int &half, u64 v) {
     v = wave_max(v);
-    if ((threadIdx.x & 63) == 0) sh.red[0][threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) sh.red[half][0][threadIdx.x >> 6] = v;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < Shared<NT>::NW; ++i) v = sh.red[0][i] > v ? sh.red[0][i] : v;
-    __syncthreads();
+    for (int i = 0; i < Shared<NT>::NW; ++i) v = sh.red[half][0][i] > v ? sh.red[half][0][i] : v;
+    half ^= 1;
     return v;
 }
 
 // The workgroup's sums of a and b, and each thread's sum over the threads before it.
 template <int NT>
-__device__ __forceinline__ void block_scan(Shared<NT> &sh, u64 a, u64 b, u64 &a_before, u64 &b_before, u64 &a_all, u64 &b_all) {
+__device__ __forceinline__ void block_scan(Shared<NT> &sh, int &half, u64 a, u64 b, u64 &a_before, u64 &b_before, u64 &a_all, u64 &b_all) {
     const int w = threadIdx.x >> 6;
     const u64 au = wave_scan(a), bu = wave_scan(b);
     if ((threadIdx.x & 63) == 63) {
-        sh.red[0][w] = au;
-        sh.red[1][w] = bu;
+        sh.red[half][0][w] = au;
+        sh.red[half][1][w] = bu;
     }
     __syncthreads();
     a_before = au - a;
@@ -201,7 +214,7 @@ __device__ __forceinline__ void block_scan(Shared<NT> &sh, u64 a, u64 b, u64 &a_
     a_all = b_all = 0;
 #pragma unroll
     for (int i = 0; i < Shared<NT>::NW; ++i) {
-        const u64 x = sh.red[0][i], y = sh.red[1][i];
+        const u64 x = sh.red[half][0][i], y = sh.red[half][1][i];
         if (i < w) {
             a_before += x;
             b_before += y;
@@ -209,7 +222,13 @@ __device__ __forceinline__ void block_scan(Shared<NT> &sh, u64 a, u64 b, u64 &a_
         a_all += x;
         b_all += y;
     }
-    __syncthreads();
+    half ^= 1;
+}
+template <int NT>
+__device__ __forceinline__ u64 block_scan(Shared<NT> &sh, int &half, u64 a, u64 &before) {
+    u64 x, all, y;
+    block_scan<NT>(sh, half, a, 0, before, x, all, y);
+    return all;
 }
 
 // ---------------------------------------------------------------- a row as a workgroup sees it
@@ -277,24 +296,43 @@ struct Held {
     }
 };
 
-// Descending, in place; the first n of a power of two at least n are given, the rest are filled. Up to 64:
-// the first wave's lanes hold them.
+// The first wave's lanes' values, descending; the others' are 0. All 64 lanes of it call.
+__device__ __forceinline__ u64 wave_sort_desc(u64 v, int size) {
+    const int i = threadIdx.x & 63;
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const u64 o = __shfl_xor(v, j, 64);
+            const bool keep_max = ((i & j) == 0) == ((i & k) == 0);
+            v = keep_max == (o > v) ? o : v;
+        }
+    return v;
+}
+
+// c[0 .. n), n > 64, descending, in place (bitonic). With a thread for each, steps inside a wave are lane
+// exchanges.
 template <int NT>
 __device__ __forceinline__ void sort_desc(u64 *c, int n) {
-    int size = 1;
+    int size = 128;
     while (size < n) size <<= 1;
-    if (size <= 64) {
-        if (threadIdx.x < 64) {
-            const int i = threadIdx.x;
-            u64 v = i < n ? c[i] : 0;
-            for (int k = 2; k <= size; k <<= 1)
-                for (int j = k >> 1; j > 0; j >>= 1) {
-                    const u64 o = __shfl_xor(v, j, 64);
-                    const bool keep_max = ((i & j) == 0) == ((i & k) == 0);
-                    v = keep_max == (o > v) ? o : v;
+    if (size <= NT) {
+        const int i = threadIdx.x;
+        u64 v = i < n ? c[i] : 0;
+        for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                u64 o;
+                if (j >= 64) {
+                    __syncthreads();
+                    if (i < size) c[i] = v;
+                    __syncthreads();
+                    o = i < size ? c[i ^ j] : 0;
+                } else {
+                    o = __shfl_xor(v, j, 64);
                 }
-            if (i < n) c[i] = v;
-        }
+                const bool keep_max = ((i & j) == 0) == ((i & k) == 0);
+                v = keep_max == (o > v) ? o : v;
+            }
+        __syncthreads();
+        if (i < n) c[i] = v;
         __syncthreads();
         return;
     }
@@ -316,46 +354,62 @@ __device__ __forceinline__ void sort_desc(u64 *c, int n) {
         }
 }
 
-// The member of the sorted cand[0 .. n) where the running count (from above_c) or weight (from above_m)
-// reaches `want`; upto: the weight up to and including it.
-template <int NT>
-__device__ __forceinline__ u64 cut_in(Shared<NT> &sh, int n, bool by_mass, u64 above_c, u64 above_m, double want, float top,
-                                      double inv_t, u64 &upto) {
+// Sorts cand[0 .. n) (given unsorted when `sort`) and leaves in cut[WHICH] and upto[WHICH] the member where
+// the running count (WHICH 0, from above_c) or weight (1, from above_m) reaches `want`, and the weight up to
+// and including it.
+template <int NT, int WHICH>
+__device__ __forceinline__ void cut_in(Shared<NT> &sh, int &half, int n, bool sort, u64 above_c, u64 above_m, double want, float top,
+                                       double inv_t) {
+    if (n <= 64) {  // the first wave does it alone
+        if (threadIdx.x < 64) {
+            const int i = threadIdx.x;
+            u64 k = i < n ? sh.cand[i] : 0;
+            if (sort) {
+                int size = 1;
+                while (size < n) size <<= 1;
+                k = wave_sort_desc(k, size);
+                if (i < n) sh.cand[i] = k;
+            }
+            const u64 v = i < n ? mass(weight(logit_of(k), top, inv_t)) : 0, run = above_m + wave_scan(v);
+            const double lo = static_cast<double>(WHICH ? run - v : above_c + i), hi = static_cast<double>(WHICH ? run : above_c + i + 1);
+            if (i < n && ((lo < want && hi >= want) || (i == n - 1 && hi < want))) {
+                sh.cut[WHICH] = k;
+                sh.upto[WHICH] = run;
+            }
+        }
+        __syncthreads();
+        return;
+    }
+    if (sort) sort_desc<NT>(sh.cand, n);
     constexpr int CP = (kCand + NT - 1) / NT;
-    u64 v[CP], t = 0, before, all, x, y;
+    u64 v[CP], t = 0, before;
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
         const int at = threadIdx.x * CP + i;
         t += v[i] = at < n ? mass(weight(logit_of(sh.cand[at]), top, inv_t)) : 0;
     }
-    block_scan<NT>(sh, t, 0, before, x, all, y);
+    block_scan<NT>(sh, half, t, before);
     u64 run = above_m + before;
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
         const int at = threadIdx.x * CP + i;
         const u64 prev = run;
         run += v[i];
-        if (at < n) {
-            const double lo = static_cast<double>(by_mass ? prev : above_c + at);
-            const double hi = static_cast<double>(by_mass ? run : above_c + at + 1);
-            if ((lo < want && hi >= want) || (at == n - 1 && hi < want)) {
-                sh.n = at;
-                sh.out1 = run;
-            }
+        const double lo = static_cast<double>(WHICH ? prev : above_c + at), hi = static_cast<double>(WHICH ? run : above_c + at + 1);
+        if (at < n && ((lo < want && hi >= want) || (at == n - 1 && hi < want))) {
+            sh.cut[WHICH] = sh.cand[at];
+            sh.upto[WHICH] = run;
         }
     }
     __syncthreads();
-    const u64 cut = sh.cand[sh.n];
-    upto = sh.out1;
-    __syncthreads();
-    return cut;
 }
 
-// The same among the many members of a bin that are `floor` or more: eight bits of the packed token at a
-// time, keeping the digit where the running sum crosses. Many members: equal logits, or a narrow spread.
-template <typename T, int NT>
-__device__ __noinline__ u64 cut_by_digits(Shared<NT> &sh, const T *row, int vocab, int bin, u64 floor, bool by_mass, u64 above_c,
-                                          u64 above_m, double want, float top, float per_unit, double inv_t) {
+// The same among the many members of a bin that are `floor` or more, from memory: eight bits of the packed
+// token at a time, keeping the digit where the running sum crosses. Many members: equal logits, or a narrow
+// spread.
+template <typename T, int NT, int WHICH>
+__device__ __noinline__ void cut_by_digits(Shared<NT> &sh, const T *row, int vocab, int bin, u64 floor, u64 above_c, u64 above_m,
+                                           double want, float top, float per_unit, double inv_t) {
     const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
     u64 prefix = 0;
     for (int shift = 56; shift >= 0; shift -= 8) {
@@ -375,29 +429,26 @@ __device__ __noinline__ u64 cut_by_digits(Shared<NT> &sh, const T *row, int voca
         __syncthreads();
         if (threadIdx.x == 0) {
             u64 cc = above_c, mm = above_m;
-            int last = -1;
-            sh.out0 = cc;
-            sh.out1 = mm;
+            int last = 255;
             for (int d = 0; d < 256; ++d) {
                 if (!sh.digit_count[d]) continue;
                 last = d;
-                sh.out0 = cc;
-                sh.out1 = mm;
+                sh.above_c[WHICH] = cc;
+                sh.above_m[WHICH] = mm;
                 cc += sh.digit_count[d];
                 mm += sh.digit_mass[d];
-                if (static_cast<double>(by_mass ? mm : cc) >= want) break;
+                if (static_cast<double>(WHICH ? mm : cc) >= want) break;
             }
-            sh.n = last < 0 ? 255 : last;
+            sh.digit = last;
+            sh.upto[WHICH] = mm;
         }
         __syncthreads();
-        prefix = prefix << 8 | static_cast<u64>(255 - sh.n);
-        above_c = sh.out0;
-        above_m = sh.out1;
-        __syncthreads();
-        if (threadIdx.x == 0) sh.out1 = above_m + sh.digit_mass[sh.n];
-        __syncthreads();
+        prefix = prefix << 8 | static_cast<u64>(255 - sh.digit);
+        above_c = sh.above_c[WHICH];
+        above_m = sh.above_m[WHICH];
     }
-    return prefix;  // sh.out1: the weight up to and including it
+    if (threadIdx.x == 0) sh.cut[WHICH] = prefix;
+    __syncthreads();
 }
 
 // A thread's bins of the histogram and the sums over the bins before them.
@@ -405,92 +456,84 @@ template <int NT>
 struct Bins {
     static constexpr int PER = kBins / NT;
     u64 c[PER], m[PER], c_before, m_before, c_all, m_all;
-    __device__ __forceinline__ void scan(Shared<NT> &sh, const u64 *mass_of, const uint32_t *count_of) {
+    __device__ __forceinline__ void scan(Shared<NT> &sh, int &half, const u64 *mass_of, const uint32_t *count_of) {
         u64 ct = 0, mt = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             ct += c[i] = count_of[threadIdx.x * PER + i];
             mt += m[i] = mass_of[threadIdx.x * PER + i];
         }
-        block_scan<NT>(sh, ct, mt, c_before, m_before, c_all, m_all);
+        block_scan<NT>(sh, half, ct, mt, c_before, m_before, c_all, m_all);
     }
-    // The bin whose running count or weight reaches `want` (-1: none does), and the sums before it. Bins
-    // past `last` hold nothing, and that one `last_mass` (~0: what it has).
-    __device__ __forceinline__ int cross(Shared<NT> &sh, bool by_mass, double want, int last, u64 last_mass, u64 &above_c,
-                                         u64 &above_m) const {
-        if (threadIdx.x == 0) sh.bin = -1;
-        __syncthreads();
+    // bin[WHICH]: the one whose running count (BY_MASS false) or weight reaches `want` (it stays -1 where none
+    // does), above_c and above_m the sums before it. Bins past `last` hold nothing, and that one `last_mass`
+    // (~0: what it has). The caller's next barrier shows them.
+    template <int WHICH, bool BY_MASS>
+    __device__ __forceinline__ void cross(Shared<NT> &sh, double want, int last, u64 last_mass) const {
         u64 cc = c_before, mm = m_before;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int b = threadIdx.x * PER + i;
             const u64 more = b == last && last_mass != ~0ull ? last_mass : m[i];
-            const double lo = static_cast<double>(by_mass ? mm : cc), hi = static_cast<double>(by_mass ? mm + more : cc + c[i]);
+            const double lo = static_cast<double>(BY_MASS ? mm : cc), hi = static_cast<double>(BY_MASS ? mm + more : cc + c[i]);
             if (b <= last && lo < want && hi >= want) {  // one bin at most: the sums only rise
-                sh.bin = b;
-                sh.out0 = cc;
-                sh.out1 = mm;
+                sh.bin[WHICH] = b;
+                sh.above_c[WHICH] = cc;
+                sh.above_m[WHICH] = mm;
             }
             cc += c[i];
             mm += m[i];
         }
-        __syncthreads();
-        above_c = sh.out0;
-        above_m = sh.out1;
-        const int bin = sh.bin;
-        __syncthreads();
-        return bin;
     }
 };
 
 // The threshold of a row's kept tokens by top-k and top-p: a packed token is kept when it is >= the result.
 // The histogram is in sh.h.
 template <typename T, int NT, int E>
-__device__ u64 threshold(Shared<NT> &sh, const Held<T, NT, E> &row, float top, const Row &s) {
+__device__ __forceinline__ u64 threshold(Shared<NT> &sh, int &half, const Held<T, NT, E> &row, float top, const Row &s) {
     Bins<NT> bins;
-    bins.scan(sh, sh.h.mass, sh.h.count);
-    u64 cut = 0, sum = bins.m_all, above_c, above_m;
+    bins.scan(sh, half, sh.h.mass, sh.h.count);
+    u64 cut = 0, sum = bins.m_all, k_bin_mass = ~0ull;
     int k_bin = kBins - 1, n = 0, held = -1;  // held: the bin whose members are in sh.cand, sorted
-    u64 k_bin_mass = ~0ull;
-    auto cut_of = [&](int bin, bool by_mass, double want, u64 floor, u64 &upto) {
-        if (held != bin) {
-            if (threadIdx.x == 0) sh.n = 0;
-            __syncthreads();
+    auto settle = [&](auto which, double want, u64 floor) {
+        constexpr int W = decltype(which)::value;
+        const int bin = sh.bin[W];
+        const bool fresh = held != bin;
+        if (fresh) {
             row.all(top, s.inv_t, [&](float l, int i, auto) {
                 if (bin_of(l, top, s.per_unit) != bin) return;
-                const int at = atomicAdd(&sh.n, 1);
+                const int at = atomicAdd(&sh.n[W], 1);
                 if (at < kCand) sh.cand[at] = pack(l, i);
             });
             __syncthreads();
-            n = sh.n;
-            __syncthreads();
-            if (n <= kCand) {
-                sort_desc<NT>(sh.cand, n);
-                held = bin;
-            }
+            n = sh.n[W];
+            if (n <= kCand) held = bin;
         }
-        if (n <= kCand) return cut_in<NT>(sh, n, by_mass, above_c, above_m, want, top, s.inv_t, upto);
-        const u64 c = cut_by_digits<T, NT>(sh, row.row, row.vocab, bin, floor, by_mass, above_c, above_m, want, top, s.per_unit, s.inv_t);
-        upto = sh.out1;
-        __syncthreads();
-        return c;
+        if (n <= kCand)
+            cut_in<NT, W>(sh, half, n, fresh, sh.above_c[W], sh.above_m[W], want, top, s.inv_t);
+        else
+            cut_by_digits<T, NT, W>(sh, row.row, row.vocab, bin, floor, sh.above_c[W], sh.above_m[W], want, top, s.per_unit, s.inv_t);
     };
     if (s.k) {
         const double want = static_cast<double>(s.k);
-        const int bin = bins.cross(sh, false, want, kBins - 1, ~0ull, above_c, above_m);
-        if (bin >= 0) {
-            cut = cut_of(bin, false, want, 0, sum);
-            k_bin = bin;
-            k_bin_mass = sum - above_m;
+        bins.template cross<0, false>(sh, want, kBins - 1, ~0ull);
+        __syncthreads();
+        if (sh.bin[0] >= 0) {
+            k_bin = sh.bin[0];
+            const u64 above = sh.above_m[0];
+            settle(std::integral_constant<int, 0>{}, want, 0);
+            cut = sh.cut[0];
+            sum = sh.upto[0];
+            k_bin_mass = sum - above;
         }
     }
     if (s.p < 1.0f) {
         const double want = static_cast<double>(s.p) * static_cast<double>(sum);
-        const int bin = bins.cross(sh, true, want, k_bin, k_bin_mass, above_c, above_m);
-        if (bin >= 0) {
-            u64 upto;
-            const u64 c = cut_of(bin, true, want, cut, upto);
-            cut = c > cut ? c : cut;
+        bins.template cross<1, true>(sh, want, k_bin, k_bin_mass);
+        __syncthreads();
+        if (sh.bin[1] >= 0) {
+            settle(std::integral_constant<int, 1>{}, want, cut);
+            cut = sh.cut[1] > cut ? sh.cut[1] : cut;
         }
     }
     return cut;
@@ -528,29 +571,13 @@ __device__ __forceinline__ void sum_runs(Shared<NT> &sh, const T *row, int i0, i
     }
 }
 
-// The token where the kept weight passes `target`, from the runs' weights in sh.seg: logits [i0, i1), `upto`
-// the kept weight before them. z: the whole row's.
-template <typename T, int NT, int MOST>
-__device__ __forceinline__ void find_token(Shared<NT> &sh, const SampleArgs<T> &a, const T *row, int r, const Row &s, u64 best, u64 cut,
-                                           int i0, int i1, u64 upto, u64 target, u64 z, u64 t, u64 before) {
-    constexpr int SP = (MOST + NT - 1) / NT;  // runs a thread, whose weight is t, after `before`
-    const int lane = threadIdx.x & 63;
+// The token where the kept weight passes `target`, inside the run of 256 logits of [.., i1) from i on, `before`
+// the kept weight before it; by one wave. z: the whole row's.
+template <typename T>
+__device__ __forceinline__ void find_token(const SampleArgs<T> &a, const T *row, int r, const Row &s, u64 best, u64 cut, int i, int i1,
+                                           u64 before, u64 target, u64 z) {
     const float top = logit_of(best);
-    before += upto;
-    if (before <= target && target < before + t) {  // one thread
-        for (int i = 0; i < SP; ++i) {
-            const u64 m = sh.seg[threadIdx.x * SP + i];
-            if (target < before + m) {
-                sh.n = threadIdx.x * SP + i;
-                sh.out0 = before;
-                break;
-            }
-            before += m;
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x >= 64) return;
-    const int i = i0 + sh.n * 256 + lane * 4;
+    i += (threadIdx.x & 63) * 4;
     u64 m[4], mine = 0;
     float l[4];
 #pragma unroll
@@ -558,7 +585,7 @@ __device__ __forceinline__ void find_token(Shared<NT> &sh, const SampleArgs<T> &
         l[e] = i + e < i1 ? logit(row[i + e]) : -INFINITY;
         mine += m[e] = kept_mass(l[e], i + e, top, s, best, cut);
     }
-    u64 run = sh.out0 + wave_scan(mine) - mine;
+    u64 run = before + wave_scan(mine) - mine;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         if (run <= target && target < run + m[e]) {
@@ -579,8 +606,8 @@ __device__ __forceinline__ u64 target_of(const Row &s, u64 z) {
 
 // The row's token from its kept tokens' weights: in runs of 256 logits, then inside the run that u falls into.
 template <typename T, int NT, int E>
-__device__ __forceinline__ void choose(Shared<NT> &sh, const SampleArgs<T> &a, const Held<T, NT, E> &row, int r, const Row &s, u64 best,
-                                       u64 cut) {
+__device__ __forceinline__ void choose(Shared<NT> &sh, int &half, const SampleArgs<T> &a, const Held<T, NT, E> &row, int r, const Row &s,
+                                       u64 best, u64 cut) {
     constexpr int NW = NT / 64, MOST = E > 0 ? E / 4 * NW : kSegs, SP = (MOST + NT - 1) / NT;
     const float top = logit_of(best);
     const int segs = (a.vocab + 255) / 256;
@@ -603,12 +630,35 @@ __device__ __forceinline__ void choose(Shared<NT> &sh, const SampleArgs<T> &a, c
         sum_runs<T, NT>(sh, row.row, 0, a.vocab, top, s, best, cut);
     }
     __syncthreads();
-    u64 t = 0, before, z, x, y;
+    if constexpr (MOST <= 64) {  // the first wave has a run a lane
+        if (threadIdx.x >= 64) return;
+        const u64 m = static_cast<int>(threadIdx.x) < segs ? sh.seg[threadIdx.x] : 0, upto = wave_scan(m), z = last_lane(upto);
+        const u64 target = target_of(s, z);
+        const int at = __ffsll(static_cast<unsigned long long>(__ballot(target < upto))) - 1;
+        const u64 before = upto - m;
+        const u64 b = static_cast<u64>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before >> 32), at))) << 32 |
+                      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before), at));
+        find_token<T>(a, row.row, r, s, best, cut, at * 256, a.vocab, b, target, z);
+    } else {
+        u64 t = 0, before;
 #pragma unroll
-    for (int i = 0; i < SP; ++i)
-        if (static_cast<int>(threadIdx.x) * SP + i < segs) t += sh.seg[threadIdx.x * SP + i];
-    block_scan<NT>(sh, t, 0, before, x, z, y);
-    find_token<T, NT, MOST>(sh, a, row.row, r, s, best, cut, 0, a.vocab, 0, target_of(s, z), z, t, before);
+        for (int i = 0; i < SP; ++i)
+            if (static_cast<int>(threadIdx.x) * SP + i < segs) t += sh.seg[threadIdx.x * SP + i];
+        const u64 z = block_scan<NT>(sh, half, t, before), target = target_of(s, z);
+        if (before <= target && target < before + t) {  // one thread
+            for (int i = 0; i < SP; ++i) {
+                const u64 m = sh.seg[threadIdx.x * SP + i];
+                if (target < before + m) {
+                    sh.run = threadIdx.x * SP + i;
+                    sh.run_before = before;
+                    break;
+                }
+                before += m;
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) find_token<T>(a, row.row, r, s, best, cut, sh.run * 256, a.vocab, sh.run_before, target, z);
+    }
 }
 
 // Nothing to choose from, or no choice. True when that was so.
@@ -623,23 +673,25 @@ __device__ __forceinline__ bool settled(const SampleArgs<T> &a, int r, const Row
     return true;
 }
 
+// Calls follow a barrier or start the kernel.
 template <typename T, int NT, int E>
 __device__ __forceinline__ void sample_whole(Shared<NT> &sh, const SampleArgs<T> &a, int r) {
     Held<T, NT, E> row(a.logits + r * a.stride, a.vocab);
     const Row s = row_of(a, r);
+    int half = 0;
+    sh.clear();
     if (s.filters()) {
         for (int i = threadIdx.x; i < kBins; i += NT) {
             sh.h.mass[i] = 0;
             sh.h.count[i] = 0;
         }
     }
-    u64 best = 0;
+    u64 best = pack(-INFINITY, 0);
     row.all(0.0f, 1.0, [&](float l, int i, auto) {
         const u64 k = pack(l, i);
         best = k > best ? k : best;
     });
-    best = block_max<NT>(sh, best);
-    if (best == 0) best = pack(-INFINITY, 0);
+    best = block_max<NT>(sh, half, best);
     if (settled(a, r, s, best)) return;
     const float top = logit_of(best);
     row.weigh(top, s.inv_t);
@@ -651,10 +703,9 @@ __device__ __forceinline__ void sample_whole(Shared<NT> &sh, const SampleArgs<T>
             atomicAdd(&sh.h.mass[b], m());
         });
         __syncthreads();
-        cut = threshold<T, NT, E>(sh, row, top, s);
-        __syncthreads();
+        cut = threshold<T, NT, E>(sh, half, row, top, s);
     }
-    choose<T, NT, E>(sh, a, row, r, s, best, cut);
+    choose<T, NT, E>(sh, half, a, row, r, s, best, cut);
 }
 
 template <typename T, int NT, int E>
@@ -691,8 +742,8 @@ struct PartArgs {
 };
 
 template <int NT>
-__device__ __forceinline__ u64 best_of(Shared<NT> &sh, const RowState &st, int parts) {
-    return block_max<NT>(sh, static_cast<int>(threadIdx.x) < parts ? st.best[threadIdx.x] : 0);
+__device__ __forceinline__ u64 best_of(Shared<NT> &sh, int &half, const RowState &st, int parts) {
+    return block_max<NT>(sh, half, static_cast<int>(threadIdx.x) < parts ? st.best[threadIdx.x] : 0);
 }
 
 // First launch: each part's largest; the histogram is cleared.
@@ -713,7 +764,8 @@ __global__ __launch_bounds__(kPartNT) void sample_part_max(PartArgs<T> p) {
         const u64 k = pack(l, i);
         best = k > best ? k : best;
     });
-    best = block_max<kPartNT>(sh, best);
+    int half = 0;
+    best = block_max<kPartNT>(sh, half, best);
     if (threadIdx.x == 0) st.best[g] = best;
 }
 
@@ -729,15 +781,16 @@ __global__ __launch_bounds__(kPartNT) void sample_part_hist(PartArgs<T> p) {
             sh.h.mass[i] = 0;
             sh.h.count[i] = 0;
         }
-    const u64 best = best_of<kPartNT>(sh, st, p.parts);
+    int half = 0;
+    const u64 best = best_of<kPartNT>(sh, half, st, p.parts);
     const float top = logit_of(best);
     if (top == -INFINITY || s.greedy) return;
     const T *row = p.a.logits + r * p.a.stride;
     const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
     if (!s.filters()) {
-        u64 m = 0, x, y, all, z;
+        u64 m = 0, before;
         each<T, kPartNT>(row, i0, i1, vec, [&](float l, int i) { m += kept_mass(l, i, top, s, best, 0); });
-        block_scan<kPartNT>(sh, m, 0, x, y, all, z);
+        const u64 all = block_scan<kPartNT>(sh, half, m, before);
         if (threadIdx.x == 0) st.part_mass[g] = all;
         return;
     }
@@ -767,29 +820,41 @@ __global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
     RowState &st = p.rows[r];
     const Row s = row_of(p.a, r);
     if (s.greedy || !s.filters()) return;
-    const u64 best = best_of<kPartNT>(sh, st, p.parts);
+    int half = 0;
+    sh.clear();
+    if (threadIdx.x == 0) sh.digit = 0;
+    const u64 best = best_of<kPartNT>(sh, half, st, p.parts);
     const float top = logit_of(best);
     if (top == -INFINITY) return;
     Bins<kPartNT> bins;
-    bins.scan(sh, st.hist_mass, st.hist_count);
+    bins.scan(sh, half, st.hist_mass, st.hist_count);
     int k_bin = -1, lo = kBins, hi = -1;
-    u64 k_above_c = 0, k_above_m = 0, lo_above_m = 0, x, y;
-    if (s.k) k_bin = bins.cross(sh, false, static_cast<double>(s.k), kBins - 1, ~0ull, k_above_c, k_above_m);
+    u64 k_above_c = 0, k_above_m = 0, lo_above_m = 0;
+    if (s.k) {
+        bins.template cross<0, false>(sh, static_cast<double>(s.k), kBins - 1, ~0ull);
+        __syncthreads();
+        k_bin = sh.bin[0];
+        k_above_c = sh.above_c[0];
+        k_above_m = sh.above_m[0];
+        __syncthreads();
+    }
     if (s.p < 1.0f) {
         // the top-k's weight is between those of the bins above its threshold's and with it
         const u64 least = k_bin >= 0 ? k_above_m : bins.m_all;
         const u64 most = k_bin >= 0 ? k_above_m + st.hist_mass[k_bin] : bins.m_all;
         const int last = k_bin >= 0 ? k_bin : kBins - 1;
         const double p64 = static_cast<double>(s.p);
-        hi = bins.cross(sh, true, p64 * static_cast<double>(most), last, ~0ull, x, lo_above_m);
-        lo = hi;
-        if (least < most) {
-            lo = bins.cross(sh, true, p64 * static_cast<double>(least), last, ~0ull, x, y);
-            if (lo < 0) {
-                lo = 0;  // least is 0
-                y = 0;
-            }
-            lo_above_m = y;
+        if (threadIdx.x == 0) sh.bin[0] = -1;
+        __syncthreads();
+        bins.template cross<0, true>(sh, p64 * static_cast<double>(least), last, ~0ull);
+        bins.template cross<1, true>(sh, p64 * static_cast<double>(most), last, ~0ull);
+        __syncthreads();
+        lo = sh.bin[0];
+        hi = sh.bin[1];
+        lo_above_m = sh.above_m[0];
+        if (lo < 0) {  // least is 0
+            lo = 0;
+            lo_above_m = 0;
         }
         if (hi < 0) lo = kBins;  // no threshold: all of the top-k
     } else {
@@ -809,19 +874,27 @@ __global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
     }
     const T *row = p.a.logits + r * p.a.stride;
     const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
-    u64 m = 0, all, z;
+    u64 m = 0;
     each<T, kPartNT>(row, i0, i1, vec, [&](float l, int i) {
         if (l == -INFINITY) return;
         const int b = bin_of(l, top, s.per_unit);
         if (b < sure) {
             m += kept_mass(l, i, top, s, best, 0);
         } else if ((b >= lo && b <= hi) || b == k_bin) {
-            const uint32_t at = atomicAdd(&st.n_cand, 1u);
-            if (at < kCand) st.cand[at] = pack(l, i);
+            const int at = atomicAdd(&sh.digit, 1);
+            if (at < kCand) sh.cand[at] = pack(l, i);
         }
     });
-    block_scan<kPartNT>(sh, m, 0, x, y, all, z);
-    if (threadIdx.x == 0) st.part_mass[g] = all;
+    u64 before;
+    const u64 all = block_scan<kPartNT>(sh, half, m, before);
+    const int n = sh.digit;  // the part's members: a place for all of them at once
+    if (threadIdx.x == 0) {
+        st.part_mass[g] = all;
+        sh.run = n ? static_cast<int>(atomicAdd(&st.n_cand, static_cast<uint32_t>(n))) : 0;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n && i < kCand; i += kPartNT)
+        if (sh.run + i < kCand) st.cand[sh.run + i] = sh.cand[i];
 }
 
 // Fourth, a workgroup a row: the thresholds among the members, the part that u falls into, the token.
@@ -833,67 +906,71 @@ __global__ __launch_bounds__(1024) void sample_finish(PartArgs<T> p) {
     const int r = blockIdx.x;
     RowState &st = p.rows[r];
     const Row s = row_of(p.a, r);
-    const u64 best = best_of<NT>(sh, st, p.parts);
+    int half = 0;
+    const u64 best = best_of<NT>(sh, half, st, p.parts);
     if (settled(p.a, r, s, best)) return;
     const float top = logit_of(best);
-    if (static_cast<int>(threadIdx.x) < p.parts) part_mass[threadIdx.x] = st.part_mass[threadIdx.x];
-    u64 cut = 0;
+    const int i = threadIdx.x;
+    if (i < p.parts) part_mass[i] = st.part_mass[i];
+    u64 cut = 0, before;
     if (s.filters()) {
         const int n = static_cast<int>(st.n_cand);
         if (n > kCand) {  // many members: equal logits, or a narrow spread
+            __syncthreads();
             sample_whole<T, NT, 0>(sh, p.a, r);
             return;
         }
-        if (static_cast<int>(threadIdx.x) < n) sh.cand[threadIdx.x] = st.cand[threadIdx.x];
+        if (i < n) sh.cand[i] = st.cand[i];
         __syncthreads();
-        sort_desc<NT>(sh.cand, n);
+        if (n > 64) {
+            sort_desc<NT>(sh.cand, n);
+        } else {
+            if (i < 64) {
+                const u64 v = wave_sort_desc(i < n ? sh.cand[i] : 0, 64);
+                if (i < n) sh.cand[i] = v;
+            }
+            __syncthreads();
+        }
         // the top-k bin's members are the last of the list
-        u64 sum = st.k_above_m, upto;
-        u64 want_k = 0;
+        u64 sum = st.k_above_m;
+        const u64 mine = i < n ? sh.cand[i] : 0, weighs = i < n ? mass(weight(logit_of(mine), top, s.inv_t)) : 0;
         if (st.k_bin >= 0) {
-            const int from = n - static_cast<int>(st.k_count);
-            const int at = from + s.k - static_cast<int>(st.k_above_c) - 1;
-            cut = want_k = sh.cand[at];
-            u64 x, y, z;
-            const int i = threadIdx.x;
-            block_scan<NT>(sh, i >= from && i <= at ? mass(weight(logit_of(sh.cand[i]), top, s.inv_t)) : 0, 0, x, y, upto, z);
-            sum += upto;
+            const int from = n - static_cast<int>(st.k_count), at = from + s.k - static_cast<int>(st.k_above_c) - 1;
+            cut = sh.cand[at];
+            sum += block_scan<NT>(sh, half, i >= from && i <= at ? weighs : 0, before);
         } else if (s.p < 1.0f) {
-            u64 x, y, z, v = 0;
-            for (int i = threadIdx.x; i < kBins; i += NT) v += st.hist_mass[i];
-            block_scan<NT>(sh, v, 0, x, y, sum, z);
+            sum = block_scan<NT>(sh, half, st.hist_mass[i] + st.hist_mass[i + NT], before);
         }
         if (s.p < 1.0f && st.hi >= 0) {
-            const u64 c = cut_in<NT>(sh, n, true, 0, st.lo_above_m, static_cast<double>(s.p) * static_cast<double>(sum), top, s.inv_t, upto);
-            cut = c > cut ? c : cut;
+            cut_in<NT, 1>(sh, half, n, false, 0, st.lo_above_m, static_cast<double>(s.p) * static_cast<double>(sum), top, s.inv_t);
+            cut = sh.cut[1] > cut ? sh.cut[1] : cut;
         }
         // their weights to their parts
-        if (static_cast<int>(threadIdx.x) < n) {
-            const u64 k = sh.cand[threadIdx.x];
-            const u64 m = kept_mass(logit_of(k), index_of(k), top, s, best, cut);
-            if (m) atomicAdd(&part_mass[index_of(k) / p.part], m);
-        }
+        if (i < n && mine >= cut && (weight(logit_of(mine), top, s.inv_t) >= static_cast<double>(s.m) || mine == best))
+            atomicAdd(&part_mass[index_of(mine) / p.part], weighs);
     }
     __syncthreads();
-    u64 before, z, x, y;
-    const u64 t = static_cast<int>(threadIdx.x) < p.parts ? part_mass[threadIdx.x] : 0;
-    block_scan<NT>(sh, t, 0, before, x, z, y);
-    const u64 target = target_of(s, z);
+    const u64 t = i < p.parts ? part_mass[i] : 0, z = block_scan<NT>(sh, half, t, before), target = target_of(s, z);
     if (before <= target && target < before + t) {
-        sh.bin = threadIdx.x;
-        sh.out1 = before;
+        sh.run = i;
+        sh.run_before = before;
     }
     __syncthreads();
-    const int i0 = sh.bin * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
-    const u64 upto = sh.out1;
+    const int i0 = sh.run * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    const u64 upto = sh.run_before;
     const T *row = p.a.logits + r * p.a.stride;
     sum_runs<T, NT>(sh, row, i0, i1, top, s, best, cut);
     __syncthreads();
-    constexpr int MOST = NT;  // runs of a part (kMostPart)
-    const u64 seg = static_cast<int>(threadIdx.x) * 256 < i1 - i0 ? sh.seg[threadIdx.x] : 0;
-    u64 part_all;
-    block_scan<NT>(sh, seg, 0, before, x, part_all, y);
-    find_token<T, NT, MOST>(sh, p.a, row, r, s, best, cut, i0, i1, upto, target, z, seg, before);
+    // a run of the part a thread (kMostPart)
+    const u64 seg = i * 256 < i1 - i0 ? sh.seg[i] : 0;
+    block_scan<NT>(sh, half, seg, before);
+    before += upto;
+    if (before <= target && target < before + seg) {
+        sh.run = i;
+        sh.run_before = before;
+    }
+    __syncthreads();
+    if (i < 64) find_token<T>(p.a, row, r, s, best, cut, i0 + sh.run * 256, i1, sh.run_before, target, z);
 }
 
 struct Parts {
@@ -954,9 +1031,9 @@ int sample(const char *name, const T *logits, const float *temperature, const in
     if (vocab <= 1024)
         sample_row<T, 256, 4><<<grid, 256, 0, stream>>>(a);
     else if (vocab <= 2048)
-        sample_row<T, 256, 8><<<grid, 256, 0, stream>>>(a);
+        sample_row<T, 512, 4><<<grid, 512, 0, stream>>>(a);
     else if (vocab <= 4096)
-        sample_row<T, 512, 8><<<grid, 512, 0, stream>>>(a);
+        sample_row<T, 1024, 4><<<grid, 1024, 0, stream>>>(a);
     else if (vocab <= 8192)
         sample_row<T, 1024, 8><<<grid, 1024, 0, stream>>>(a);
     else
