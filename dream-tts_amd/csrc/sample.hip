@@ -52,7 +52,7 @@ struct SampleArgs {
 struct Row {  // one row's settings, made safe
     float p, m, per_unit;  // per_unit: bins per logit
     int k;
-    double u, inv_t;
+    double u, inv_t;         // log2(e) / T
     bool greedy;
     __device__ __forceinline__ bool filters() const { return k > 0 || p < 1.0f; }
 };
@@ -63,8 +63,8 @@ __device__ __forceinline__ Row row_of(const SampleArgs<T> &a, int r) {
     const float t = a.temperature ? a.temperature[r] : 1.0f;
     const int k = a.top_k ? a.top_k[r] : 0;
     const float p = a.top_p ? a.top_p[r] : 1.0f, m = a.min_p ? a.min_p[r] : 0.0f, u = a.u[r];
-    s.greedy = !(t > 0.0f) || p <= 0.0f;  // a top-p of nothing keeps the first token alone
-    s.inv_t = 1.0 / static_cast<double>(t > 0.0f ? t : 1.0f);
+    s.greedy = !(t > 0.0f) || p <= 0.0f || m > 1.0f;  // such a top-p or min-p keeps the first token alone
+    s.inv_t = 1.4426950408889634074 / static_cast<double>(t > 0.0f ? t : 1.0f);
     s.per_unit = kBins / (kRange * fmaxf(t, 1.0f));
     s.k = k <= 0 || k >= a.vocab ? 0 : k;  // 0: all
     s.p = p < 1.0f ? p : 1.0f;             // 1 (or not a number): all
@@ -91,27 +91,29 @@ __device__ __forceinline__ float logit_of(u64 k) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// e^((l - top) / T) for l <= top: 2^n 2^f with n the nearest integer to the exponent and 2^f by its Taylor
-// series, whose remainder at |f| <= 1/2 is (ln 2 / 2)^11 / 11! = 2.2e-13, the sums' own unit. (The
-// library's exp carries 53 bits, at twice the instructions.)
+// e^((l - top) / T) for l <= top, inv_t = log2(e) / T: 2^n 2^f with n the exponent's nearest integer and 2^f
+// by its Taylor series in f ln 2, whose remainder at |f| <= 1/2 is (ln 2 / 2)^11 / 11! = 2.2e-13, the sums'
+// own unit. (The library's exp carries 53 bits.) Adding 1.5 * 2^52 leaves n in the low word; n goes straight
+// into the result's exponent.
 __device__ __forceinline__ double weight(float l, float top, double inv_t) {
-    if (l == top) return 1.0;
-    if (top == INFINITY) return 0.0;
-    const double y = (static_cast<double>(l) - static_cast<double>(top)) * inv_t * 1.4426950408889634074;
-    if (!(y > -64.0)) return 0.0;  // under half a unit
-    const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-    double r = 1.0 / 3628800;
-    r = fma(r, f, 1.0 / 362880);
-    r = fma(r, f, 1.0 / 40320);
-    r = fma(r, f, 1.0 / 5040);
-    r = fma(r, f, 1.0 / 720);
-    r = fma(r, f, 1.0 / 120);
-    r = fma(r, f, 1.0 / 24);
-    r = fma(r, f, 1.0 / 6);
-    r = fma(r, f, 0.5);
+    constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5,
+                     c6 = c5 * c1 / 6, c7 = c6 * c1 / 7, c8 = c7 * c1 / 8, c9 = c8 * c1 / 9, c10 = c9 * c1 / 10;
+    constexpr double kRound = 6755399441055744.0;
+    const double y = (static_cast<double>(l) - static_cast<double>(top)) * inv_t;
+    const double t = y + kRound, f = y - (t - kRound);
+    double r = fma(c10, f, c9);
+    r = fma(r, f, c8);
+    r = fma(r, f, c7);
+    r = fma(r, f, c6);
+    r = fma(r, f, c5);
+    r = fma(r, f, c4);
+    r = fma(r, f, c3);
+    r = fma(r, f, c2);
+    r = fma(r, f, c1);
     r = fma(r, f, 1.0);
-    r = fma(r, f, 1.0);
-    return ldexp(r, static_cast<int>(n));
+    const uint64_t n = static_cast<uint64_t>(__double_as_longlong(t)) << 52;
+    const double w = __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(__double_as_longlong(r)) + n));
+    return l == top ? 1.0 : y > -64.0 ? w : 0.0;  // under half a unit: nothing (and so where top is +inf)
 }
 // The nearest number of units: added to 2^52, an f64's last place is one unit.
 __device__ __forceinline__ u64 mass(double w) {
@@ -541,30 +543,30 @@ __device__ __forceinline__ u64 threshold(Shared<NT> &sh, int &half, const Held<T
 
 // ---------------------------------------------------------------- one workgroup a row
 
-// The weight of logit i if it is kept.
-__device__ __forceinline__ u64 kept_mass(float l, int i, float top, const Row &s, u64 best, u64 cut) {
-    if (l == -INFINITY) return 0;
-    const u64 k = pack(l, i);
-    if (k < cut) return 0;
+// A logit's weight if min-p keeps it (the largest's is 1, and min-p at most 1 here); and if the threshold does too.
+__device__ __forceinline__ u64 min_p_mass(float l, float top, const Row &s) {
     const double x = weight(l, top, s.inv_t);
-    return x >= static_cast<double>(s.m) || k == best ? mass(x) : 0;
+    return l != -INFINITY && x >= static_cast<double>(s.m) ? mass(x) : 0;
+}
+__device__ __forceinline__ u64 kept_mass(float l, int i, float top, const Row &s, u64 cut) {
+    return pack(l, i) >= cut ? min_p_mass(l, top, s) : 0;
 }
 
-// The kept weight of the w-th of each NW runs of 256 logits from i0 on, to sh.seg.
+// The kept weights of a row's runs of 256 logits, to sh.seg.
 template <typename T, int NT>
-__device__ __forceinline__ void sum_runs(Shared<NT> &sh, const T *row, int i0, int i1, float top, const Row &s, u64 best, u64 cut) {
+__device__ __forceinline__ void sum_runs(Shared<NT> &sh, const T *row, int i1, float top, const Row &s, u64 cut) {
     typedef T v4 __attribute__((ext_vector_type(4)));
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, segs = (i1 - i0 + 255) / 256;
-    const bool vec = reinterpret_cast<uintptr_t>(row + i0) % (4 * sizeof(T)) == 0;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, segs = (i1 + 255) / 256;
+    const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
     for (int seg = w; seg < segs; seg += NT / 64) {
-        const int i = i0 + seg * 256 + lane * 4;
+        const int i = seg * 256 + lane * 4;
         u64 m = 0;
         if (vec && i + 4 <= i1) {
             const v4 v = *reinterpret_cast<const v4 *>(row + i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) m += kept_mass(logit(v[e]), i + e, top, s, best, cut);
+            for (int e = 0; e < 4; ++e) m += kept_mass(logit(v[e]), i + e, top, s, cut);
         } else {
-            for (int e = 0; e < 4 && i + e < i1; ++e) m += kept_mass(logit(row[i + e]), i + e, top, s, best, cut);
+            for (int e = 0; e < 4 && i + e < i1; ++e) m += kept_mass(logit(row[i + e]), i + e, top, s, cut);
         }
         m = last_lane(wave_scan(m));
         if (lane == 0) sh.seg[seg] = m;
@@ -583,7 +585,7 @@ __device__ __forceinline__ void find_token(const SampleArgs<T> &a, const T *row,
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         l[e] = i + e < i1 ? logit(row[i + e]) : -INFINITY;
-        mine += m[e] = kept_mass(l[e], i + e, top, s, best, cut);
+        mine += m[e] = kept_mass(l[e], i + e, top, s, cut);
     }
     u64 run = before + wave_scan(mine) - mine;
 #pragma unroll
@@ -592,7 +594,7 @@ __device__ __forceinline__ void find_token(const SampleArgs<T> &a, const T *row,
             a.token[r] = i + e;
             if (a.logprob) {
                 const double d = l[e] == top ? 0.0 : (static_cast<double>(l[e]) - static_cast<double>(top)) * s.inv_t;
-                a.logprob[r] = static_cast<float>(d - log(static_cast<double>(z) / kUnit));
+                a.logprob[r] = static_cast<float>(d * 0.69314718055994530942 - log(static_cast<double>(z) / kUnit));
             }
         }
         run += m[e];
@@ -621,13 +623,13 @@ __device__ __forceinline__ void choose(Shared<NT> &sh, int &half, const SampleAr
                 const float l = row.l[4 * q + e];
                 if (l == -INFINITY) continue;
                 const u64 k = pack(l, i);
-                if (k >= cut && (s.m == 0.0f || k == best || weight(l, top, s.inv_t) >= static_cast<double>(s.m))) m += row.m[4 * q + e];
+                if (k >= cut && (s.m == 0.0f || weight(l, top, s.inv_t) >= static_cast<double>(s.m))) m += row.m[4 * q + e];
             }
             m = last_lane(wave_scan(m));
             if ((threadIdx.x & 63) == 0) sh.seg[q * NW + (threadIdx.x >> 6)] = m;
         }
     } else {
-        sum_runs<T, NT>(sh, row.row, 0, a.vocab, top, s, best, cut);
+        sum_runs<T, NT>(sh, row.row, a.vocab, top, s, cut);
     }
     __syncthreads();
     if constexpr (MOST <= 64) {  // the first wave has a run a lane
@@ -719,11 +721,12 @@ __global__ __launch_bounds__(NT) void sample_row(SampleArgs<T> a) {
 constexpr int kPartNT = 512;     // threads of the workgroups that share a row
 constexpr int kMostParts = 256;  // of a row
 
-// What the workgroups of a row leave each other. All but `mass` of a part and the candidates beyond
-// n_cand is written by one launch before the next reads it.
+// What the workgroups of a row leave each other. All but the candidates beyond n_cand is written by one
+// launch before the next reads it.
 struct RowState {
     u64 hist_mass[kBins];
-    u64 best[kMostParts], part_mass[kMostParts];
+    u64 run_mass[kSegs];  // the kept weight of each run of 256 logits
+    u64 best[kMostParts];
     u64 cand[kCand];
     uint32_t hist_count[kBins];
     uint32_t n_cand;
@@ -746,11 +749,60 @@ __device__ __forceinline__ u64 best_of(Shared<NT> &sh, int &half, const RowState
     return block_max<NT>(sh, half, static_cast<int>(threadIdx.x) < parts ? st.best[threadIdx.x] : 0);
 }
 
+// A part of a row, in steps of four logits a thread (a wave's are a run of 256). Eight steps are requested
+// together, the first eight before anything else: a launch's chain of small reads runs under them.
+template <typename T>
+struct Part {
+    static constexpr int STEP = kPartNT * 4, BATCH = 8;
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    const T *row;
+    int i0, i1;
+    bool vec;
+    float l[BATCH][4];
+
+    __device__ __forceinline__ Part(const PartArgs<T> &p, int g, int r) : row(p.a.logits + r * p.a.stride), i0(g * p.part) {
+        i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+        vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
+        load(i0);
+    }
+    __device__ __forceinline__ void load(int from) {
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q) {
+            const int i = from + q * STEP + static_cast<int>(threadIdx.x) * 4;
+            if (vec && i + 4 <= i1) {
+                const v4 v = *reinterpret_cast<const v4 *>(row + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l[q][e] = static_cast<float>(v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l[q][e] = i + e < i1 ? static_cast<float>(row[i + e]) : -INFINITY;
+            }
+        }
+    }
+    // f(logit, index) for every logit of the part and, past its end, some masked ones; after every step, end(index
+    // of the wave's run) by whole waves.
+    template <typename F, typename G>
+    __device__ __forceinline__ void all(F f, G end) {
+        for (int from = i0; from < i1; from += BATCH * STEP) {
+            if (from != i0) load(from);
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q) {
+                const int run = from + q * STEP + (static_cast<int>(threadIdx.x) & ~63) * 4;
+                if (run >= i1) break;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f(logit(l[q][e]), from + q * STEP + static_cast<int>(threadIdx.x) * 4 + e);
+                end(run / 256);
+            }
+        }
+    }
+};
+
 // First launch: each part's largest; the histogram is cleared.
 template <typename T>
 __global__ __launch_bounds__(kPartNT) void sample_part_max(PartArgs<T> p) {
     __shared__ Shared<kPartNT> sh;
-    const int g = blockIdx.x, r = blockIdx.y, i0 = g * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    const int g = blockIdx.x, r = blockIdx.y;
+    const int i0 = g * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
     RowState &st = p.rows[r];
     for (int i = g * kPartNT + threadIdx.x; i < kBins; i += p.parts * kPartNT) {
         st.hist_mass[i] = 0;
@@ -769,11 +821,12 @@ __global__ __launch_bounds__(kPartNT) void sample_part_max(PartArgs<T> p) {
     if (threadIdx.x == 0) st.best[g] = best;
 }
 
-// Second: the histogram of a row that filters by rank or weight, the part's kept weight of one that does not.
+// Second: the histogram of a row that filters by rank or weight, the runs' kept weights of one that does not.
 template <typename T>
 __global__ __launch_bounds__(kPartNT) void sample_part_hist(PartArgs<T> p) {
     __shared__ Shared<kPartNT> sh;
-    const int g = blockIdx.x, r = blockIdx.y, i0 = g * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    const int r = blockIdx.y;
+    Part<T> part(p, blockIdx.x, r);
     RowState &st = p.rows[r];
     const Row s = row_of(p.a, r);
     if (s.filters())
@@ -785,25 +838,28 @@ __global__ __launch_bounds__(kPartNT) void sample_part_hist(PartArgs<T> p) {
     const u64 best = best_of<kPartNT>(sh, half, st, p.parts);
     const float top = logit_of(best);
     if (top == -INFINITY || s.greedy) return;
-    const T *row = p.a.logits + r * p.a.stride;
-    const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
     if (!s.filters()) {
-        u64 m = 0, before;
-        each<T, kPartNT>(row, i0, i1, vec, [&](float l, int i) { m += kept_mass(l, i, top, s, best, 0); });
-        const u64 all = block_scan<kPartNT>(sh, half, m, before);
-        if (threadIdx.x == 0) st.part_mass[g] = all;
+        u64 m = 0;
+        part.all([&](float l, int) { m += min_p_mass(l, top, s); },
+                 [&](int run) {
+                     if (__any(m != 0)) m = last_lane(wave_scan(m));
+                     if ((threadIdx.x & 63) == 0) st.run_mass[run] = m;
+                     m = 0;
+                 });
         return;
     }
     const bool by_mass = s.p < 1.0f;
-    each<T, kPartNT>(row, i0, i1, vec, [&](float l, int) {
-        if (l == -INFINITY) return;
-        const int b = bin_of(l, top, s.per_unit);
-        atomicAdd(&sh.h.count[b], 1u);
-        if (by_mass) {
-            const u64 m = mass(weight(l, top, s.inv_t));
-            if (m) atomicAdd(&sh.h.mass[b], m);
-        }
-    });
+    part.all(
+        [&](float l, int) {
+            if (l == -INFINITY) return;
+            const int b = bin_of(l, top, s.per_unit);
+            atomicAdd(&sh.h.count[b], 1u);
+            if (by_mass) {
+                const u64 m = mass(weight(l, top, s.inv_t));
+                if (m) atomicAdd(&sh.h.mass[b], m);
+            }
+        },
+        [](int) {});
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kPartNT) {
         if (sh.h.count[i]) atomicAdd(&st.hist_count[i], sh.h.count[i]);
@@ -812,14 +868,15 @@ __global__ __launch_bounds__(kPartNT) void sample_part_hist(PartArgs<T> p) {
 }
 
 // Third: where the thresholds lie (every workgroup for itself, from the histogram), the members of those bins,
-// and the part's kept weight above them.
+// and the runs' kept weights above them.
 template <typename T>
 __global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
     __shared__ Shared<kPartNT> sh;
-    const int g = blockIdx.x, r = blockIdx.y, i0 = g * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
+    const int r = blockIdx.y;
     RowState &st = p.rows[r];
     const Row s = row_of(p.a, r);
     if (s.greedy || !s.filters()) return;
+    Part<T> part(p, blockIdx.x, r);
     int half = 0;
     sh.clear();
     if (threadIdx.x == 0) sh.digit = 0;
@@ -863,7 +920,7 @@ __global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
         lo_above_m = k_above_m;
     }
     const int sure = k_bin >= 0 && k_bin < lo ? k_bin : lo;  // the bins before it are kept
-    if (g == 0 && threadIdx.x == 0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
         st.k_bin = k_bin;
         st.lo = lo;
         st.hi = hi;
@@ -872,46 +929,44 @@ __global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
         st.lo_above_m = lo_above_m;
         st.k_count = k_bin >= 0 ? st.hist_count[k_bin] : 0;
     }
-    const T *row = p.a.logits + r * p.a.stride;
-    const bool vec = reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0;
     u64 m = 0;
-    each<T, kPartNT>(row, i0, i1, vec, [&](float l, int i) {
-        if (l == -INFINITY) return;
-        const int b = bin_of(l, top, s.per_unit);
-        if (b < sure) {
-            m += kept_mass(l, i, top, s, best, 0);
-        } else if ((b >= lo && b <= hi) || b == k_bin) {
-            const int at = atomicAdd(&sh.digit, 1);
-            if (at < kCand) sh.cand[at] = pack(l, i);
-        }
-    });
-    u64 before;
-    const u64 all = block_scan<kPartNT>(sh, half, m, before);
+    part.all(
+        [&](float l, int i) {
+            if (l == -INFINITY) return;
+            const int b = bin_of(l, top, s.per_unit);
+            if (b < sure) {
+                m += min_p_mass(l, top, s);
+            } else if ((b >= lo && b <= hi) || b == k_bin) {
+                const int at = atomicAdd(&sh.digit, 1);
+                if (at < kCand) sh.cand[at] = pack(l, i);
+            }
+        },
+        [&](int run) {
+            if (__any(m != 0)) m = last_lane(wave_scan(m));
+            if ((threadIdx.x & 63) == 0) st.run_mass[run] = m;
+            m = 0;
+        });
+    __syncthreads();
     const int n = sh.digit;  // the part's members: a place for all of them at once
-    if (threadIdx.x == 0) {
-        st.part_mass[g] = all;
-        sh.run = n ? static_cast<int>(atomicAdd(&st.n_cand, static_cast<uint32_t>(n))) : 0;
-    }
+    if (threadIdx.x == 0) sh.run = n ? static_cast<int>(atomicAdd(&st.n_cand, static_cast<uint32_t>(n))) : 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n && i < kCand; i += kPartNT)
         if (sh.run + i < kCand) st.cand[sh.run + i] = sh.cand[i];
 }
 
-// Fourth, a workgroup a row: the thresholds among the members, the part that u falls into, the token.
+// Fourth, a workgroup a row: the thresholds among the members, the run that u falls into, the token.
 template <typename T>
 __global__ __launch_bounds__(1024) void sample_finish(PartArgs<T> p) {
-    constexpr int NT = 1024;
+    constexpr int NT = 1024, SP = kSegs / NT;
     __shared__ Shared<NT> sh;
-    __shared__ u64 part_mass[kMostParts];
-    const int r = blockIdx.x;
+    const int r = blockIdx.x, i = threadIdx.x, runs = (p.a.vocab + 255) / 256;
     RowState &st = p.rows[r];
     const Row s = row_of(p.a, r);
     int half = 0;
     const u64 best = best_of<NT>(sh, half, st, p.parts);
     if (settled(p.a, r, s, best)) return;
     const float top = logit_of(best);
-    const int i = threadIdx.x;
-    if (i < p.parts) part_mass[i] = st.part_mass[i];
+    for (int q = i; q < runs; q += NT) sh.seg[q] = st.run_mass[q];
     u64 cut = 0, before;
     if (s.filters()) {
         const int n = static_cast<int>(st.n_cand);
@@ -945,32 +1000,29 @@ __global__ __launch_bounds__(1024) void sample_finish(PartArgs<T> p) {
             cut_in<NT, 1>(sh, half, n, false, 0, st.lo_above_m, static_cast<double>(s.p) * static_cast<double>(sum), top, s.inv_t);
             cut = sh.cut[1] > cut ? sh.cut[1] : cut;
         }
-        // their weights to their parts
-        if (i < n && mine >= cut && (weight(logit_of(mine), top, s.inv_t) >= static_cast<double>(s.m) || mine == best))
-            atomicAdd(&part_mass[index_of(mine) / p.part], weighs);
+        // their weights to their runs
+        if (i < n && mine >= cut && weight(logit_of(mine), top, s.inv_t) >= static_cast<double>(s.m))
+            atomicAdd(&sh.seg[index_of(mine) / 256], weighs);
     }
     __syncthreads();
-    const u64 t = i < p.parts ? part_mass[i] : 0, z = block_scan<NT>(sh, half, t, before), target = target_of(s, z);
-    if (before <= target && target < before + t) {
-        sh.run = i;
-        sh.run_before = before;
+    u64 t = 0;
+#pragma unroll
+    for (int q = 0; q < SP; ++q)
+        if (i * SP + q < runs) t += sh.seg[i * SP + q];
+    const u64 z = block_scan<NT>(sh, half, t, before), target = target_of(s, z);
+    if (before <= target && target < before + t) {  // one thread
+        for (int q = 0; q < SP; ++q) {
+            const u64 m = sh.seg[i * SP + q];
+            if (target < before + m) {
+                sh.run = i * SP + q;
+                sh.run_before = before;
+                break;
+            }
+            before += m;
+        }
     }
     __syncthreads();
-    const int i0 = sh.run * p.part, i1 = i0 + p.part < p.a.vocab ? i0 + p.part : p.a.vocab;
-    const u64 upto = sh.run_before;
-    const T *row = p.a.logits + r * p.a.stride;
-    sum_runs<T, NT>(sh, row, i0, i1, top, s, best, cut);
-    __syncthreads();
-    // a run of the part a thread (kMostPart)
-    const u64 seg = i * 256 < i1 - i0 ? sh.seg[i] : 0;
-    block_scan<NT>(sh, half, seg, before);
-    before += upto;
-    if (before <= target && target < before + seg) {
-        sh.run = i;
-        sh.run_before = before;
-    }
-    __syncthreads();
-    if (i < 64) find_token<T>(p.a, row, r, s, best, cut, i0 + sh.run * 256, i1, sh.run_before, target, z);
+    if (i < 64) find_token<T>(p.a, p.a.logits + r * p.a.stride, r, s, best, cut, sh.run * 256, p.a.vocab, sh.run_before, target, z);
 }
 
 struct Parts {
@@ -979,7 +1031,6 @@ struct Parts {
 
 // Rows of up to kWholeVocab logits, and rows enough to fill the chip by themselves, are one workgroup each.
 constexpr int64_t kWholeVocab = 8192, kPartFill = 512;
-constexpr int64_t kMostPart = 1024 * 256;  // a run of 256 logits for each thread of the last launch
 
 inline Parts parts_of(int64_t rows, int64_t vocab) {
     int64_t part = (rows * vocab + kPartFill - 1) / kPartFill;
@@ -989,7 +1040,7 @@ inline Parts parts_of(int64_t rows, int64_t vocab) {
     Parts p;
     p.part = static_cast<int>(part);
     p.parts = static_cast<int>((vocab + part - 1) / part);
-    if (vocab <= kWholeVocab || part > kMostPart || p.parts < 2) p.parts = 1;
+    if (vocab <= kWholeVocab || p.parts < 2) p.parts = 1;
     return p;
 }
 
