@@ -727,7 +727,8 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
     }
     int64_t span = window > 0 && window + max_q + 63 < max_context ? window + max_q + 63 : max_context;
     if (span < 1) span = 1;
-    const int64_t wgs = (p.small + p.large) * n_kv > 0 ? (p.small + p.large) * n_kv : 1;
+    // the launch is sized for the most tiles there can be; the chunks go by what a batch of long chunks has
+    const int64_t wgs = (p.large > 0 ? rows / 128 + 1 : p.small) * n_kv;
     int64_t n = ((p.large > 0 ? kFillLarge : kFillSmall) + wgs - 1) / wgs;
     const int64_t most = span <= kWhole ? 1 : (span + kMinChunk - 1) / kMinChunk;
     if (n > most) n = most;
