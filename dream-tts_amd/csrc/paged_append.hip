@@ -30,7 +30,7 @@ struct AppendArgs {
     half_t *q_out, *kp, *vp;
     int heads, n_kv, half, table_len;
     float eps;
-    FastDiv per_row;  // heads + 2 n_kv
+    FastDiv parts;  // waves per token
 };
 
 template <typename T>
@@ -52,84 +52,108 @@ struct Four<half_t> {
     }
 };
 
+// A wave takes one token, or one of its `parts`: rows part * RW + its lane group's, then parts * RW further.
+// What a token's rows share (its sequence, position and page, and a lane's cos and sin, whatever the row) is
+// read once for all of them.
 template <typename T, int D, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv, AppendArgs a) {
-    constexpr int L = D / 8;  // lanes per head row
-    const uint32_t task = blockIdx.x * (256u / L) + threadIdx.x / L;
-    const int j = threadIdx.x % L;
-    const uint32_t tok = a.per_row.div(task);
-    const bool on = tok < static_cast<uint32_t>(a.batch.tokens);  // every lane takes part in the wave's steps
-    const int t = on ? static_cast<int>(tok) : a.batch.tokens - 1;
-    const int r = on ? static_cast<int>(task - tok * a.per_row.d) : 0;
+    constexpr int L = D / 8, RW = 64 / L, U = 4;  // lanes per head row, head rows per wave step, steps requested together
+    const uint32_t wid = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int t = static_cast<int>(a.parts.div(wid)), part = static_cast<int>(wid - static_cast<uint32_t>(t) * a.parts.d);
+    if (t >= a.batch.tokens) return;
+    const int lane = threadIdx.x & 63, j = lane % L, per = a.heads + 2 * a.n_kv, stride = static_cast<int>(a.parts.d) * RW;
     // element offsets of the lane's two groups; the dimensions past 2 half pass through
     const bool turns = 4 * j < a.half;
     const int rest = 2 * a.half + 8 * (j - a.half / 4);
     const int o1 = INTERLEAVED ? 8 * j : turns ? 4 * j : rest;
     const int o2 = INTERLEAVED ? 8 * j + 4 : turns ? a.half + 4 * j : rest + 4;
-    const T *src = qkv + (static_cast<int64_t>(t) * a.per_row.d + r) * D;
-    float x[4], y[4];
-    Four<T>::load(src + o1, x);
-    Four<T>::load(src + o2, y);
-    const int s = a.batch.sequence_of<L>(t);
-    if (!on || s >= a.batch.b) return;
+    const T *src = qkv + static_cast<int64_t>(t) * per * D;
+    float x[U][4], y[U][4];
+    auto load = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * stride < per ? r0 + u * stride : per - 1;
+            Four<T>::load(src + static_cast<int64_t>(r) * D + o1, x[u]);
+            Four<T>::load(src + static_cast<int64_t>(r) * D + o2, y[u]);
+        }
+    };
+    int r0 = part * RW + lane / L;
+    load(r0);
+    const int s = a.batch.sequence_of<64>(t);
+    if (s >= a.batch.b) return;
     int first, n;
     a.batch.rows(s, first, n);
     const int pos = a.batch.context[s] - n + (t - first);
     if (t < first || t >= first + n || pos < 0 || pos >= a.table_len) return;
     const int page = a.batch.page(s, pos >> a.batch.page_shift);
-    const bool is_q = r < a.heads, is_v = r >= a.heads + a.n_kv;
     if (page < 0) return;
-    if (!is_v) {
-        if (a.norms) {
-            float ss = 0.0f;
+    float c[4] = {}, sn[4] = {};
+    if (turns) {
+        Four<float>::load(a.cos_t + static_cast<int64_t>(pos) * a.half + 4 * j, c);
+        Four<float>::load(a.sin_t + static_cast<int64_t>(pos) * a.half + 4 * j, sn);
+    }
+    const int64_t slot = page * a.batch.page_stride + static_cast<int64_t>(pos & ((1 << a.batch.page_shift) - 1)) * D;
+    for (;;) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss += x[i] * x[i] + y[i] * y[i];
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * stride;
+            if (r >= per) break;
+            const bool is_q = r < a.heads, is_v = r >= a.heads + a.n_kv;
+            if (!is_v) {
+                if (a.norms) {
+                    float ss = 0.0f;
 #pragma unroll
-            for (int off = L / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
-            const float inv = 1.0f / sqrtf(ss / static_cast<float>(D) + a.eps);
-            float w[4], u[4];
-            const float *wr = a.norms + (is_q ? 0 : D);
-            Four<float>::load(wr + o1, w);
-            Four<float>::load(wr + o2, u);
+                    for (int i = 0; i < 4; ++i) ss += x[u][i] * x[u][i] + y[u][i] * y[u][i];
+#pragma unroll
+                    for (int off = L / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
+                    const float inv = 1.0f / sqrtf(ss / static_cast<float>(D) + a.eps);
+                    float w[4], v[4];
+                    const float *wr = a.norms + (is_q ? 0 : D);
+                    Four<float>::load(wr + o1, w);
+                    Four<float>::load(wr + o2, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[u][i] = x[u][i] * inv * w[i];
+                        y[u][i] = y[u][i] * inv * v[i];
+                    }
+                }
+                if (turns) {
+                    if constexpr (INTERLEAVED) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            rope_pair(x[u][2 * i], x[u][2 * i + 1], c[i], sn[i], x[u][2 * i], x[u][2 * i + 1]);
+                            rope_pair(y[u][2 * i], y[u][2 * i + 1], c[2 + i], sn[2 + i], y[u][2 * i], y[u][2 * i + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) rope_pair(x[u][i], y[u][i], c[i], sn[i], x[u][i], y[u][i]);
+                    }
+                }
+            }
+            half_t *dst;
+            if (is_q)
+                dst = a.q_out + (static_cast<int64_t>(t) * a.heads + r) * D;
+            else
+                dst = (is_v ? a.vp : a.kp) + slot +
+                      (static_cast<int64_t>(r - a.heads - (is_v ? a.n_kv : 0)) << a.batch.page_shift) * D;
+            h4 p, q;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = x[i] * inv * w[i];
-                y[i] = y[i] * inv * u[i];
+                p[i] = static_cast<half_t>(x[u][i]);
+                q[i] = static_cast<half_t>(y[u][i]);
             }
+            *reinterpret_cast<h4 *>(dst + o1) = p;
+            *reinterpret_cast<h4 *>(dst + o2) = q;
         }
-        if (turns) {
-            float c[4], sn[4];
-            Four<float>::load(a.cos_t + static_cast<int64_t>(pos) * a.half + 4 * j, c);
-            Four<float>::load(a.sin_t + static_cast<int64_t>(pos) * a.half + 4 * j, sn);
-            if constexpr (INTERLEAVED) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    rope_pair(x[2 * i], x[2 * i + 1], c[i], sn[i], x[2 * i], x[2 * i + 1]);
-                    rope_pair(y[2 * i], y[2 * i + 1], c[2 + i], sn[2 + i], y[2 * i], y[2 * i + 1]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) rope_pair(x[i], y[i], c[i], sn[i], x[i], y[i]);
-            }
-        }
+        r0 += U * stride;
+        if (r0 - lane / L >= per) return;
+        load(r0);
     }
-    half_t *dst;
-    if (is_q) {
-        dst = a.q_out + (static_cast<int64_t>(t) * a.heads + r) * D;
-    } else {
-        const int kh = r - a.heads - (is_v ? a.n_kv : 0);
-        const int64_t slot = (static_cast<int64_t>(kh) << a.batch.page_shift) + (pos & ((1 << a.batch.page_shift) - 1));
-        dst = (is_v ? a.vp : a.kp) + page * a.batch.page_stride + slot * D;
-    }
-    h4 p, q;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        p[i] = static_cast<half_t>(x[i]);
-        q[i] = static_cast<half_t>(y[i]);
-    }
-    *reinterpret_cast<h4 *>(dst + o1) = p;
-    *reinterpret_cast<h4 *>(dst + o2) = q;
 }
+
+// 5700 tokens, f16, 32 + 2 * 8 rows of 64 (82 MB): 14.3 us with 2048 or 4096, 15.6 with 8192 or more (each
+// repeats the token's lookups; a row a lane group and no sharing 18.7); 48 f32 tokens of 32 rows of 128 the same.
+constexpr int64_t kFillWaves = 4096;
 
 template <typename T>
 int append(const char *name, const T *qkv, const float *norms, const float *cos_t, const float *sin_t,
@@ -148,8 +172,12 @@ int append(const char *name, const T *qkv, const float *norms, const float *cos_
     DTTS_REQUIRE(aligned(qkv, 4 * sizeof(T)) && aligned(cos_t, 16) && aligned(sin_t, 16) && aligned(q_out, 8) && aligned(kp, 8) &&
                      aligned(vp, 8) && aligned(norms, 16) && aligned(q_start, 4) && aligned(context, 4) && aligned(page_table, 4),
                  "%s: misaligned operand", name);
-    const int64_t per = heads + 2 * n_kv, groups = 256 / (hd / 8);
-    DTTS_REQUIRE(tokens * per + groups < (int64_t(1) << 31), "%s: too many rows", name);
+    // Steps of RW head rows a token has, shared by enough waves to fill the chip (kFillWaves, 16 a CU): few tokens
+    // spread over many, each with one step; many tokens have a wave each.
+    const int64_t per = heads + 2 * n_kv, rw = 64 / (hd / 8), steps = (per + rw - 1) / rw;
+    int64_t parts = (kFillWaves + tokens - 1) / tokens;
+    if (parts > steps) parts = steps;
+    DTTS_REQUIRE(tokens * parts < (int64_t(1) << 31), "%s: too many rows", name);
     AppendArgs a;
     a.batch = PagedBatch{q_start, context, page_table, static_cast<int>(tokens), static_cast<int>(b), log2_of(page),
                          static_cast<int>(n_pages), static_cast<int>(max_pages), page_stride};
@@ -164,8 +192,8 @@ int append(const char *name, const T *qkv, const float *norms, const float *cos_
     a.half = static_cast<int>(rot / 2);
     a.table_len = static_cast<int>(table_len);
     a.eps = eps;
-    a.per_row = FastDiv(static_cast<uint32_t>(per));
-    const unsigned blocks = static_cast<unsigned>((tokens * per + groups - 1) / groups);
+    a.parts = FastDiv(static_cast<uint32_t>(parts));
+    const unsigned blocks = static_cast<unsigned>((tokens * parts + 3) / 4);
     const bool inter = layout == DTTS_ROPE_INTERLEAVED;
     if (hd == 128 && inter)
         qk_rope_append_paged_kernel<T, 128, true><<<blocks, 256, 0, stream>>>(qkv, a);
