@@ -22,10 +22,11 @@ _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 _Tensor = torch.Tensor
 
 
+
 def _need(name, device, what, t, dtypes, contiguous=True):
-    """Raises unless t is a (contiguous) tensor of one of dtypes on GPU number `device`. The callers pass
-    their tensors through one test that holds for all of a right call (a step is a few microseconds of GPU
-    work, and so is each of these calls on the host) and come here to say what is wrong."""
+    """Raises unless t is a (contiguous) tensor of one of dtypes on GPU number `device`. A step is a few
+    microseconds of GPU work, and so is each of these calls on the host: the callers pass their tensors
+    through one condition that holds for all of a right call, and come here to say what is wrong."""
     if not isinstance(t, _Tensor):
         raise DttsError(f"{name}: {what} must be a tensor")
     if device < 0 or t.get_device() != device:
@@ -34,10 +35,6 @@ def _need(name, device, what, t, dtypes, contiguous=True):
         raise DttsError(f"{name}: {what} dtype {t.dtype} not in {dtypes}")
     if contiguous and not t.is_contiguous():
         raise DttsError(f"{name}: {what} must be contiguous")
-
-
-def _is(t, dtype, device):
-    return isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and t.is_contiguous()
 
 
 def _enqueue(fn, device, *args):
@@ -71,12 +68,13 @@ def rope_table_scaled(length, rot_dim, base, scaling="none", factor=1.0, origina
 
 
 def _tables(name, device, cos, sin):
-    if not (_is(cos, _F32, device) and _is(sin, _F32, device)):
+    if not (isinstance(cos, _Tensor) and isinstance(sin, _Tensor) and cos.dtype is _F32 and sin.dtype is _F32
+            and cos.get_device() == device and sin.get_device() == device and cos.is_contiguous() and sin.is_contiguous()):
         _need(name, device, "cos", cos, (_F32,))
         _need(name, device, "sin", sin, (_F32,))
-    n, sn = cos.shape, sin.shape
-    if len(n) != 2 or n != sn:
-        raise DttsError(f"{name}: cos {tuple(n)} and sin {tuple(sn)} must be [positions, rot_dim / 2]")
+    n = cos.shape
+    if len(n) != 2 or n != sin.shape:
+        raise DttsError(f"{name}: cos {tuple(n)} and sin {tuple(sin.shape)} must be [positions, rot_dim / 2]")
     return n
 
 
@@ -101,12 +99,13 @@ def rotary(x, cos, sin, pos, interleaved=False, out=None):
         _need(name, dev, "x", x, (x.dtype,), contiguous=False)
     (rows, heads, hd), xs = _rows(name, x, "x")
     n, half = _tables(name, dev, cos, sin)
-    if not _is(pos, _I32, dev):
+    if not (isinstance(pos, _Tensor) and pos.dtype is _I32 and pos.get_device() == dev and pos.is_contiguous()):
         _need(name, dev, "pos", pos, (_I32,))
     if pos.numel() != rows:
         raise DttsError(f"{name}: {pos.numel()} positions for {rows} rows")
     if out is None:
-        out, ys = torch.empty(x.shape, dtype=x.dtype, device=x.device), heads * hd
+        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        ys = heads * hd
     else:
         _need(name, dev, "out", out, (x.dtype,), contiguous=False)
         if out.shape != x.shape:
@@ -122,12 +121,17 @@ def rotary(x, cos, sin, pos, interleaved=False, out=None):
 def _paged(name, device, k_pages, v_pages, q_start, context, pages):
     """Checks the cache [n_pages, n_kv, page, D] (each page contiguous) and the batch's arrays: b, n_kv, D,
     page, n_pages, max_pages and the elements between pages."""
-    if not (_is(q_start, _I32, device) and _is(context, _I32, device) and _is(pages, _I32, device)):
-        _need(name, device, "q_start", q_start, (_I32,))
-        _need(name, device, "context", context, (_I32,))
-        _need(name, device, "pages", pages, (_I32,))
-    _need(name, device, "k_pages", k_pages, (_F16,), contiguous=False)
-    _need(name, device, "v_pages", v_pages, (_F16,), contiguous=False)
+    tensors = (k_pages, v_pages, q_start, context, pages)
+    for t in tensors:
+        if not isinstance(t, _Tensor) or t.get_device() != device:
+            break
+    else:
+        if (k_pages.dtype is _F16 and v_pages.dtype is _F16 and q_start.dtype is _I32 and context.dtype is _I32
+                and pages.dtype is _I32 and q_start.is_contiguous() and context.is_contiguous() and pages.is_contiguous()):
+            tensors = None
+    if tensors is not None:
+        for t, what, dtype in zip(tensors, ("k_pages", "v_pages", "q_start", "context", "pages"), (_F16, _F16, _I32, _I32, _I32)):
+            _need(name, device, what, t, (dtype,), contiguous=dtype is _I32)
     shape, st = k_pages.shape, k_pages.stride()
     if len(shape) != 4 or shape != v_pages.shape or st != v_pages.stride():
         raise DttsError(f"{name}: k pages {tuple(shape)} and v pages {tuple(v_pages.shape)}")
@@ -142,6 +146,8 @@ def _paged(name, device, k_pages, v_pages, q_start, context, pages):
 
 def _out(name, device, out, like, tokens, heads, hd):
     if out is None:
+        if like.dtype is _F16 and like.dim() == 3 and like.is_contiguous():
+            return torch.empty_like(like)  # the queries' own shape, in half the time
         return torch.empty((tokens, heads, hd), dtype=_F16, device=like.device)
     _need(name, device, "out", out, (_F16,))
     if out.numel() != tokens * heads * hd:
@@ -171,18 +177,22 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
     if not isinstance(qkv, _Tensor):
         raise DttsError(f"{name}: qkv must be a tensor")
     dev = qkv.get_device()
-    _need(name, dev, "qkv", qkv, (_F32, _F16))
+    f32 = qkv.dtype is _F32
+    if dev < 0 or not (f32 or qkv.dtype is _F16) or not qkv.is_contiguous():
+        _need(name, dev, "qkv", qkv, (_F32, _F16))
     b, n_kv, hd, page, n_pages, max_pages, stride = _paged(name, dev, k_pages, v_pages, q_start, context, pages)
     n, half = _tables(name, dev, cos, sin)
-    if len(qkv.shape) != 2 or qkv.shape[1] != (heads + 2 * n_kv) * hd:
+    size = qkv.shape
+    if len(size) != 2 or size[1] != (heads + 2 * n_kv) * hd:
         raise DttsError(f"{name}: qkv {tuple(qkv.shape)} is not [tokens, ({heads} + 2 * {n_kv}) * {hd}]")
     if norms is not None:
-        _need(name, dev, "norms", norms, (_F32,))
+        if not (isinstance(norms, _Tensor) and norms.dtype is _F32 and norms.get_device() == dev and norms.is_contiguous()):
+            _need(name, dev, "norms", norms, (_F32,))
         if norms.numel() != 2 * hd:
             raise DttsError(f"{name}: norms {tuple(norms.shape)} is not [2, {hd}]")
-    tokens = qkv.shape[0]
+    tokens = size[0]
     out = _out(name, dev, out, qkv, tokens, heads, hd)
-    _enqueue("dtts_qk_rope_append_paged_f32" if qkv.dtype is _F32 else "dtts_qk_rope_append_paged_f16", dev, qkv.data_ptr(),
+    _enqueue("dtts_qk_rope_append_paged_f32" if f32 else "dtts_qk_rope_append_paged_f16", dev, qkv.data_ptr(),
              None if norms is None else norms.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_start.data_ptr(),
              context.data_ptr(), pages.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tokens, b, heads,
              n_kv, hd, 2 * half, 1 if interleaved else 0, page, n_pages, max_pages, stride, n, eps)
@@ -215,7 +225,10 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
         raise DttsError(f"{name}: q {tuple(q.shape)} over pages of head_dim {hd}")
     out = _out(name, dev, out, q, tokens, heads, hd)
     need = 0 if workspace is not None else paged_attention_workspace_bytes(tokens, b, heads, n_kv, hd, max_q, max_context, window)
-    keep, ws, ws_bytes = _bytes(name, dev, workspace, need, q)
+    keep = ws = None
+    ws_bytes = 0
+    if need or workspace is not None:
+        keep, ws, ws_bytes = _bytes(name, dev, workspace, need, q)
     _enqueue("dtts_paged_attention_f16", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_start.data_ptr(),
              context.data_ptr(), pages.data_ptr(), out.data_ptr(), tokens, b, heads, n_kv, hd, page, n_pages, max_pages, stride,
              qs, max_q, max_context, window, scale, ws, ws_bytes)
@@ -233,7 +246,7 @@ def sample_workspace_bytes(rows, vocab):
 def _setting(name, device, what, t, dtype, rows):
     if t is None:
         return None
-    if not _is(t, dtype, device):
+    if not (isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and t.is_contiguous()):
         _need(name, device, what, t, (dtype,))
     if t.numel() != rows:
         raise DttsError(f"{name}: {t.numel()} of {what} for {rows} rows")
@@ -265,8 +278,12 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, work
     pp = _setting(name, dev, "top_p", top_p, _F32, rows)
     pm = _setting(name, dev, "min_p", min_p, _F32, rows)
     token = torch.empty(rows, dtype=_I32, device=logits.device)
-    logprob = torch.empty(rows, dtype=_F32, device=logits.device)
-    keep, ws, ws_bytes = _bytes(name, dev, workspace, sample_workspace_bytes(rows, vocab), logits)
+    logprob = torch.empty_like(u) if u.dim() == 1 else torch.empty(rows, dtype=_F32, device=logits.device)
+    need = sample_workspace_bytes(rows, vocab)
+    keep = ws = None
+    ws_bytes = 0
+    if need or workspace is not None:
+        keep, ws, ws_bytes = _bytes(name, dev, workspace, need, logits)
     _enqueue("dtts_sample_f32" if logits.dtype is _F32 else "dtts_sample_f16", dev, logits.data_ptr(), pt, pk, pp, pm, pu,
              token.data_ptr(), logprob.data_ptr(), rows, vocab, stride[0] if rows > 1 else max(stride[0], vocab), ws, ws_bytes)
     return token, logprob
