@@ -85,6 +85,16 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs &a, int rows, int64_t a
     return Tile{-1, 0, 0, 0, 0};
 }
 
+// The largest of the lanes 32 apart (and 16 apart), by exchanging halves of registers: no trip through LDS.
+__device__ __forceinline__ float max_32_apart(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_16_32_apart(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_32_apart(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // One row over keys [k0, k1) alone, by one wave (D / 64 dimensions a lane): the sums a tile's row
@@ -253,8 +263,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
                 mx = fmaxf(mx, sc[u][i]);
             }
         // the row's other keys are 16 and 32 lanes away
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        mx = max_16_32_apart(mx);
         const float mu = mx == -INFINITY ? 0.0f : mx;
         if (__any(mx > m)) {
             const float f = exp2_fast(m - mu);
@@ -500,7 +509,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
         float mx = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, sc[0][r]), sc[1][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        mx = max_32_apart(mx);
         // weights are taken relative to m, an earlier maximum, until a row outgrows it by 2^kSlack: the sums
         // hold that as well, and few tiles after the first move it
         if (__any((mx - m) * a.scale2 > kSlack)) {
