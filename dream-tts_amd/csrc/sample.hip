@@ -718,7 +718,10 @@ __global__ __launch_bounds__(NT) void sample_row(SampleArgs<T> a) {
 
 // ---------------------------------------------------------------- several workgroups a row
 
-constexpr int kPartNT = 512;     // threads of the workgroups that share a row
+// Threads of the workgroups that share a row, and of the one that ends it, whose barriers cost more the more waves
+// meet (64 x 131072, 3 x 50021 f16: 512 and 512 threads 57 and 24 us; 256 and 512 68 and 26; 1024 and 512 69 and
+// 26; 512 and 256 65 and 25; 512 and 1024 60 and 25).
+constexpr int kPartNT = 512, kFinishNT = 512;
 constexpr int kMostParts = 256;  // of a row
 
 // What the workgroups of a row leave each other. All but the candidates beyond n_cand is written by one
@@ -956,8 +959,8 @@ __global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
 
 // Fourth, a workgroup a row: the thresholds among the members, the run that u falls into, the token.
 template <typename T>
-__global__ __launch_bounds__(1024) void sample_finish(PartArgs<T> p) {
-    constexpr int NT = 1024, SP = kSegs / NT;
+__global__ __launch_bounds__(kFinishNT) void sample_finish(PartArgs<T> p) {
+    constexpr int NT = kFinishNT, SP = kSegs / NT, CP = kCand / NT;
     __shared__ Shared<NT> sh;
     const int r = blockIdx.x, i = threadIdx.x, runs = (p.a.vocab + 255) / 256;
     RowState &st = p.rows[r];
@@ -975,34 +978,50 @@ __global__ __launch_bounds__(1024) void sample_finish(PartArgs<T> p) {
             sample_whole<T, NT, 0>(sh, p.a, r);
             return;
         }
-        if (i < n) sh.cand[i] = st.cand[i];
-        __syncthreads();
         if (n > 64) {
+            for (int q = i; q < n; q += NT) sh.cand[q] = st.cand[q];
+            __syncthreads();
             sort_desc<NT>(sh.cand, n);
         } else {
             if (i < 64) {
-                const u64 v = wave_sort_desc(i < n ? sh.cand[i] : 0, 64);
+                const u64 v = wave_sort_desc(i < n ? st.cand[i] : 0, 64);
                 if (i < n) sh.cand[i] = v;
             }
             __syncthreads();
         }
         // the top-k bin's members are the last of the list
-        u64 sum = st.k_above_m;
-        const u64 mine = i < n ? sh.cand[i] : 0, weighs = i < n ? mass(weight(logit_of(mine), top, s.inv_t)) : 0;
+        u64 sum = 0;
         if (st.k_bin >= 0) {
             const int from = n - static_cast<int>(st.k_count), at = from + s.k - static_cast<int>(st.k_above_c) - 1;
             cut = sh.cand[at];
-            sum += block_scan<NT>(sh, half, i >= from && i <= at ? weighs : 0, before);
+            if (s.p < 1.0f) {
+                u64 t = 0;
+#pragma unroll
+                for (int c = 0; c < CP; ++c) {
+                    const int q = c * NT + i;
+                    if (q >= from && q <= at) t += mass(weight(logit_of(sh.cand[q]), top, s.inv_t));
+                }
+                sum = st.k_above_m + block_scan<NT>(sh, half, t, before);
+            }
         } else if (s.p < 1.0f) {
-            sum = block_scan<NT>(sh, half, st.hist_mass[i] + st.hist_mass[i + NT], before);
+            u64 t = 0;
+#pragma unroll
+            for (int c = 0; c < kBins / NT; ++c) t += st.hist_mass[c * NT + i];
+            sum = block_scan<NT>(sh, half, t, before);
         }
         if (s.p < 1.0f && st.hi >= 0) {
             cut_in<NT, 1>(sh, half, n, false, 0, st.lo_above_m, static_cast<double>(s.p) * static_cast<double>(sum), top, s.inv_t);
             cut = sh.cut[1] > cut ? sh.cut[1] : cut;
         }
         // their weights to their runs
-        if (i < n && mine >= cut && weight(logit_of(mine), top, s.inv_t) >= static_cast<double>(s.m))
-            atomicAdd(&sh.seg[index_of(mine) / 256], weighs);
+#pragma unroll
+        for (int c = 0; c < CP; ++c) {
+            const u64 mine = c * NT + i < n ? sh.cand[c * NT + i] : 0;
+            if (c * NT + i < n && mine >= cut) {
+                const u64 m = min_p_mass(logit_of(mine), top, s);
+                if (m) atomicAdd(&sh.seg[index_of(mine) / 256], m);
+            }
+        }
     }
     __syncthreads();
     u64 t = 0;
@@ -1075,7 +1094,7 @@ int sample(const char *name, const T *logits, const float *temperature, const in
         DTTS_LAUNCH_CHECK(name);
         sample_part_collect<T><<<each_part, kPartNT, 0, stream>>>(p);
         DTTS_LAUNCH_CHECK(name);
-        sample_finish<T><<<grid, 1024, 0, stream>>>(p);
+        sample_finish<T><<<grid, kFinishNT, 0, stream>>>(p);
         DTTS_LAUNCH_CHECK(name);
         return DTTS_OK;
     }
