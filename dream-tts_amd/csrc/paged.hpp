@@ -61,6 +61,7 @@ struct PagedBatch {
     }
 };
 
+// Positions stay under 2^30, so that a kernel's look ahead of a few tiles cannot pass an int.
 #define DTTS_REQUIRE_PAGED(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride)                               \
     do {                                                                                                                          \
         DTTS_REQUIRE((tokens) >= 0 && (b) >= 0 && (n_kv) > 0 && (n_pages) > 0 && (max_pages) > 0,                                 \
@@ -70,11 +71,13 @@ struct PagedBatch {
                      (long long)(head_dim));                                                                                      \
         DTTS_REQUIRE((page) >= 16 && (page) <= 65536 && ((page) & ((page) - 1)) == 0,                                             \
                      "%s: page of %lld positions (a power of two from 16 to 65536)", name, (long long)(page));                    \
-        DTTS_REQUIRE((page_stride) >= (n_kv) * (page) * (head_dim) && (page_stride) % 8 == 0,                                     \
-                     "%s: page_stride %lld (a multiple of 8, at least n_kv * page * head_dim)", name, (long long)(page_stride));  \
         DTTS_REQUIRE((tokens) < (int64_t(1) << 24) && (b) <= kMaxSeqs && (n_kv) <= 4096 && (n_pages) < (int64_t(1) << 31) &&      \
-                         (max_pages) * (page) < (int64_t(1) << 31),                                                               \
+                         (max_pages) <= (int64_t(1) << 30) / (page),                                                              \
                      "%s: too many rows, sequences, heads or positions", name);                                                   \
+        DTTS_REQUIRE((page_stride) >= (n_kv) * (page) * (head_dim) && (page_stride) % 8 == 0 &&                                   \
+                         (page_stride) < (int64_t(1) << 32),                                                                      \
+                     "%s: page_stride %lld (a multiple of 8 under 2^32, at least n_kv * page * head_dim)", name,                  \
+                     (long long)(page_stride));                                                                                   \
     } while (0)
 
 inline int log2_of(int64_t page) {

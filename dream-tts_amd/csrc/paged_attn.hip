@@ -41,7 +41,7 @@ struct Span {
         hi = ctx < 0 ? 0 : ctx < cap ? ctx : static_cast<int>(cap);
         lo = a.window > 0 && ctx - n_new - a.window + 1 > 0 ? (ctx - n_new - a.window + 1) & ~63 : 0;
         if (lo > hi) lo = hi & ~63;
-        n = (hi - lo + a.chunk - 1) / a.chunk;
+        n = static_cast<int>((static_cast<int64_t>(hi) - lo + a.chunk - 1) / a.chunk);
         n = n < 1 ? 1 : n > a.nsplit ? a.nsplit : n;
     }
     __device__ __forceinline__ void chunk_keys(const AttnArgs &a, int c, int &k0, int &k1) const {
@@ -77,8 +77,10 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs &a, int rows, int64_t a
         const uint64_t past = __ballot(sum > tile);
         if (past) {
             const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            return Tile{s0 + l, __builtin_amdgcn_readlane(sum, l) - 1 - tile, __builtin_amdgcn_readlane(first, l),
-                        __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(ctx, l)};
+            const int at = __builtin_amdgcn_readlane(sum, l) - 1 - tile;
+            if (at < 0 || at >= __builtin_amdgcn_readlane(tiles, l)) break;  // starts that do not rise can pass any sum
+            return Tile{s0 + l, at, __builtin_amdgcn_readlane(first, l), __builtin_amdgcn_readlane(n, l),
+                        __builtin_amdgcn_readlane(ctx, l)};
         }
         tile -= __builtin_amdgcn_readlane(sum, 63);
     }
@@ -776,6 +778,7 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
     }
     int64_t span = window > 0 && window + max_q + 63 < max_context ? window + max_q + 63 : max_context;
     if (span < 1) span = 1;
+    if (span > int64_t(1) << 30) span = int64_t(1) << 30;  // no table holds more
     // the launch is sized for the most tiles there can be; the chunks go by what a batch of long chunks has
     const int64_t wgs = (p.large > 0 ? rows / 128 + 1 : p.small) * n_kv;
     int64_t n = ((p.large > 0 ? kFillLarge : kFillSmall) + wgs - 1) / wgs;
@@ -846,8 +849,9 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
                      aligned(context, 4) && aligned(page_table, 4),
                  "%s: misaligned operand", name);
     DTTS_REQUIRE(out != q, "%s: the output may not be the queries", name);
+    DTTS_REQUIRE(std::isfinite(scale * kLog2e), "%s: scale %g", name, static_cast<double>(scale));
     Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window);
-    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large) * n_kv < (int64_t(1) << 31), "%s: too many rows", name);
+    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large) * n_kv < (int64_t(1) << 24), "%s: too many rows", name);
     AttnArgs a;
     a.batch = PagedBatch{q_start, context, page_table, static_cast<int>(tokens), static_cast<int>(b), log2_of(page),
                          static_cast<int>(n_pages), static_cast<int>(max_pages), page_stride};

@@ -110,8 +110,9 @@ int rotary(const char *name, const T *x, const float *cos_t, const float *sin_t,
                  "%s: interleaved pairs need even sizes, strides and addresses", name);
     const int64_t v = wide ? V : inter ? 2 : 1;
     const int64_t per_head = (inter ? rot : half) / v + (x == y ? 0 : (hd - rot) / v);
+    DTTS_REQUIRE(rows < (int64_t(1) << 31) && heads * per_head < (int64_t(1) << 31), "%s: too many rows", name);
     const int64_t units = rows * heads * per_head;
-    DTTS_REQUIRE(rows < (int64_t(1) << 31) && units < (int64_t(1) << 31), "%s: too many rows", name);
+    DTTS_REQUIRE(units < (int64_t(1) << 31), "%s: too many rows", name);
     RotaryArgs a;
     a.cos_t = cos_t;
     a.sin_t = sin_t;

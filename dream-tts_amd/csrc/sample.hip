@@ -1071,7 +1071,7 @@ template <typename T>
 int sample(const char *name, const T *logits, const float *temperature, const int32_t *top_k, const float *top_p,
            const float *min_p, const float *u, int32_t *token, float *logprob, int64_t rows, int64_t vocab, int64_t stride,
            void *workspace, size_t ws_bytes, hipStream_t stream) {
-    DTTS_REQUIRE(rows >= 0 && rows < (int64_t(1) << 24) && vocab > 0, "%s: bad shape (%lld, %lld)", name, (long long)rows,
+    DTTS_REQUIRE(rows >= 0 && rows < (int64_t(1) << 20) && vocab > 0, "%s: bad shape (%lld, %lld)", name, (long long)rows,
                  (long long)vocab);
     DTTS_REQUIRE(vocab <= kMaxVocab, "%s: a vocabulary of %lld (2^20 at most)", name, (long long)vocab);
     DTTS_REQUIRE(stride >= vocab, "%s: row stride %lld under the vocabulary's %lld", name, (long long)stride, (long long)vocab);
@@ -1116,7 +1116,7 @@ int sample(const char *name, const T *logits, const float *temperature, const in
 }  // namespace dtts
 
 extern "C" size_t dtts_sample_workspace_bytes(int64_t rows, int64_t vocab) {
-    return rows > 0 && vocab > 0 && rows < (int64_t(1) << 24) && vocab <= dtts::kMaxVocab ? dtts::sample_bytes(rows, vocab) : 0;
+    return rows > 0 && vocab > 0 && rows < (int64_t(1) << 20) && vocab <= dtts::kMaxVocab ? dtts::sample_bytes(rows, vocab) : 0;
 }
 
 extern "C" int dtts_sample_f32(const float *logits, const float *temperature, const int32_t *top_k, const float *top_p,

@@ -480,8 +480,9 @@ int dtts_rotary_f16(const dtts_f16 *x, const float *cos_t, const float *sin_t, c
  * DEVICE int32[b + 1], rising: sequence s's new tokens are rows q_start[s] .. q_start[s + 1] - 1 of the
  * batch (none: an idle slot). context DEVICE int32[b]: the sequence's length with its new tokens, so
  * its i-th of n new tokens is at position context[s] - n + i. Rows from q_start[b] on are padding:
- * left as they were by both calls. Page ids outside [0, n_pages) hold no position.
- * tokens < 2^24, b <= 65536, max_pages * page < 2^31.
+ * left as they were by both calls. Page ids outside [0, n_pages) hold no position. Sequences may share
+ * pages (a common prefix) that none of them appends to.
+ * tokens < 2^24, b <= 65536, max_pages * page <= 2^30, page_stride < 2^32.
  *
  * dtts_qk_rope_append_paged_*: QK-norm (norms [2, D] f32, q's weight then k's, or NULL for none),
  * rotary positions and the write of the new keys and values. qkv [tokens, (heads + 2 n_kv) * D] (q
@@ -509,6 +510,7 @@ int dtts_qk_rope_append_paged_f16(const dtts_f16 *qkv, const float *norms, const
  * the weights are rounded to f16 for the product with v. A token that sees no position (p < 0, or no page
  * of its window is there) gets zeros. Positions without a page are not attended to, slots past a
  * sequence's context are never used, and a value that is not finite reaches only the tokens that see it.
+ * scale is finite (any sign).
  * max_q and max_context are what the caller knows of the batch: the longest chunk and context. They
  * choose the kernels and how far contexts are split over workgroups, never what is computed.
  * workspace (device, 16-byte aligned) of dtts_paged_attention_workspace_bytes bytes lets contexts split,
@@ -534,7 +536,7 @@ int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dt
  * logprob (or NULL): the token's log-probability among the kept ones (0 for temperature 0). NaN logits count
  * as -inf; a row of nothing else gives token -1 and logprob -inf; +inf logits share all the weight.
  * Weights are f64 and their sums integers (units of 2^-42 of the largest), so a result depends on nothing
- * but the row. vocab <= 2^20. workspace (device, 16-byte aligned) of dtts_sample_workspace_bytes bytes lets
+ * but the row. rows < 2^20, vocab <= 2^20. workspace (device, 16-byte aligned) of dtts_sample_workspace_bytes bytes lets
  * several workgroups share a long row; without it (NULL or fewer bytes) one workgroup takes a row, with the
  * same result. Calls that may overlap must not share one. */
 size_t dtts_sample_workspace_bytes(int64_t rows, int64_t vocab);

@@ -248,6 +248,34 @@ def test_attention_large_scores(dev):
     assert bool(((got.cpu().double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, -3.0, 1e-30])
+def test_attention_scales(dev, scale):
+    """A negative scale, none at all, one that leaves every weight equal."""
+    b = ref.Batch([1, 60, 2], [100, 200, 700], 2, 64, 16, dev)
+    _attend(b, _queries(b, 4, dev), dev, scale)
+
+
+def test_sequences_share_a_prefix(dev):
+    """Three sequences over the pages of one prefix and their own last page."""
+    b = ref.Batch([1, 20, 1], [70, 84, 66], 2, 128, 16, dev)
+    for s in (1, 2):
+        b.table[s, :4] = b.table[0, :4]
+    _attend(b, _queries(b, 4, dev), dev, 0.1)
+
+
+def test_attention_starts_that_do_not_rise(dev):
+    """Nonsense in q_start selects nothing outside the batch: the call ends, and later calls are right."""
+    b = ref.Batch([9, 1, 40], [90, 10, 100], 2, 64, 16, dev)
+    k, v, start, ctx, table = b.device()
+    q = _queries(b, 4, dev)
+    want = serving.paged_attention(q, k, v, start, ctx, table, 40, 100, 0.1)
+    for bad in ([50, 0, 50, 0], [-5, 99, -5, 99], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 0], [0, 50, 50, 50]):
+        odd = torch.tensor(bad, dtype=torch.int32, device=dev)
+        serving.paged_attention(q, k, v, odd, ctx, table, 40, 100, 0.1)
+        serving.paged_attention(q, k, v, odd, ctx, table, 1, 2000, 0.1)
+    assert torch.equal(serving.paged_attention(q, k, v, start, ctx, table, 40, 100, 0.1), want)
+
+
 def test_attention_strided_queries_and_pages(dev):
     """Queries inside a qkv tensor; pages of every third place of a larger pool."""
     b = ref.Batch([3, 1, 70], [90, 300, 100], 2, 64, 32, dev, stride_pages=3)

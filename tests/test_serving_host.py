@@ -82,6 +82,8 @@ def _rotary(x=P, cos=P, sin=P, pos=P, y=P, rows=4, heads=2, hd=64, rot=64, layou
     (dict(rot=66), "rotated dimensions"), (dict(rot=0), "rotated dimensions"), (dict(layout=2), "unknown layout"),
     (dict(xs=127), "row strides"), (dict(ys=0), "row strides"), (dict(pos=None), "null pointer"), (dict(ys=160), "equal row strides"),
     (dict(x=ctypes.c_void_p(4098)), "misaligned"), (dict(rows=1 << 31), "too many rows"),
+    # sizes whose products pass 64 bits
+    (dict(rows=1 << 62), "too many rows"), (dict(y=ctypes.c_void_p(8192), heads=1 << 19, hd=1 << 19, rot=2, xs=1 << 40, ys=1 << 40), "too many rows"),
     (dict(y=ctypes.c_void_p(8196), layout=1, hd=65, rot=2, xs=130, ys=130), "interleaved pairs"),
 ])
 def test_rotary_refusals(kw, match):
@@ -105,7 +107,9 @@ def _append(qkv=P, norms=None, cos=P, sin=P, start=P, ctx=P, table=P, q=P, k=P, 
 
 PAGED = [(dict(tokens=-1), "bad shape"), (dict(b=-1), "bad shape"), (dict(n_kv=0), "bad shape"), (dict(n_pages=0), "bad shape"),
          (dict(hd=96), "head_dim"), (dict(page=24), "power of two"), (dict(page=8), "power of two"), (dict(stride=2047), "page_stride"),
-         (dict(stride=2052), "page_stride"), (dict(b=1 << 17), "too many"), (dict(max_pages=1 << 28), "too many"),
+         (dict(stride=2052), "page_stride"), (dict(stride=1 << 33), "page_stride"), (dict(n_kv=1 << 60), "too many"),
+         (dict(max_pages=1 << 62), "too many"), (dict(max_pages=(1 << 26) + 1), "too many"), (dict(b=1 << 17), "too many"),
+         (dict(max_pages=1 << 28), "too many"),
          (dict(tokens=1 << 24), "too many"), (dict(start=None), "null pointer"), (dict(k=ctypes.c_void_p(4100)), "misaligned")]
 
 
@@ -119,14 +123,17 @@ def test_append_refusals(kw, match):
 
 
 def _attention(q=P, k=P, v=P, start=P, ctx=P, table=P, out=ctypes.c_void_p(8192), tokens=3, b=2, heads=4, n_kv=2, hd=64, page=16,
-               n_pages=8, max_pages=4, stride=2048, q_stride=256, max_q=2, max_context=40, window=0, ws=None, ws_bytes=0):
+               n_pages=8, max_pages=4, stride=2048, q_stride=256, max_q=2, max_context=40, window=0, ws=None, ws_bytes=0,
+               scale=1.0):
     return (q, k, v, start, ctx, table, out, tokens, b, heads, n_kv, hd, page, n_pages, max_pages, stride, q_stride, max_q,
-            max_context, window, 1.0, ws, ws_bytes, None)
+            max_context, window, scale, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("kw,match", PAGED + [
     (dict(heads=5), "heads over"), (dict(q_stride=255), "q_stride"), (dict(q_stride=260), "q_stride"), (dict(window=-1), "window"),
-    (dict(max_q=0), "max_q"), (dict(max_context=0), "max_context"), (dict(out=P), "may not be the queries"),
+    (dict(max_q=0), "max_q"), (dict(max_context=0), "max_context"), (dict(scale=float("nan")), "scale"),
+    (dict(scale=float("inf")), "scale"), (dict(scale=3e38), "scale"),
+    (dict(tokens=(1 << 24) - 1, heads=16, n_kv=16, stride=16384, q_stride=1024), "too many rows"), (dict(out=P), "may not be the queries"),
     (dict(out=ctypes.c_void_p(8200)), "misaligned"),
     (dict(max_context=60000, ws=ctypes.c_void_p(4100), ws_bytes=1 << 30), "misaligned workspace"),
 ])
@@ -139,7 +146,15 @@ def test_attention_workspace_sizes():
     assert f(48, 48, 16, 8, 128, 1, 100) == 0  # one chunk
     assert f(1, 1, 16, 8, 128, 1, 65536) >= 2 * 16 * 128 * 4
     assert f(1, 1, 16, 8, 128, 1, 65536, window=100) <= f(1, 1, 16, 8, 128, 1, 65536)
+    assert 0 < f(1, 1, 16, 8, 128, 1, (1 << 31) - 1) < 1 << 30  # a hint past every table
     assert f(0, 1, 16, 8, 128, 1, 65536) == 0 and f(4, 4, 15, 8, 128, 1, 65536) == 0 and f(-1, 1, 16, 8, 128, 1, 10) == 0
+
+
+def test_sample_workspace_sizes():
+    f = serving.sample_workspace_bytes
+    assert f(1, 2048) == 0 and f(4000, 131072) == 0  # one workgroup a row
+    assert 0 < f(1, 131072) == f(3, 131072) / 3
+    assert f(0, 131072) == 0 and f(-1, 131072) == 0 and f(1, 1 << 21) == 0
 
 
 def _sample(logits=P, t=None, k=None, p=None, m=None, u=P, token=P, logprob=None, rows=2, vocab=100, stride=100, ws=None, n=0):
@@ -147,7 +162,8 @@ def _sample(logits=P, t=None, k=None, p=None, m=None, u=P, token=P, logprob=None
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(rows=-1), "bad shape"), (dict(vocab=0), "bad shape"), (dict(vocab=(1 << 20) + 1, stride=1 << 21), "vocabulary"),
+    (dict(rows=-1), "bad shape"), (dict(rows=1 << 20), "bad shape"), (dict(vocab=0), "bad shape"),
+    (dict(vocab=(1 << 20) + 1, stride=1 << 21), "vocabulary"),
     (dict(stride=99), "row stride"), (dict(u=None), "null pointer"), (dict(token=None), "null pointer"),
     (dict(logits=ctypes.c_void_p(4097)), "misaligned"), (dict(k=ctypes.c_void_p(4098)), "misaligned"),
 ])
