@@ -863,7 +863,8 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
     a.heads = static_cast<int>(heads);
     a.n_kv = static_cast<int>(n_kv);
     a.gqa = static_cast<int>(heads / n_kv);
-    a.window = static_cast<int>(window);
+    // one of 2^30 reaches past every position that a table holds, and the differences below stay ints
+    a.window = window >= int64_t(1) << 30 ? 0 : static_cast<int>(window);
     // a scale of 0 is the smallest number: every score then is 0, and a masked one still -inf
     a.scale2 = fmaxf(fabsf(scale) * kLog2e, FLT_MIN);
     a.negate = scale < 0.0f;

@@ -90,8 +90,9 @@ def attention(q, k, v, start, context, table, page, scale, window):
                 if not torch.isfinite(vv).all() else list(p @ vv)
             o = torch.stack(rows)
             pv = p @ vv.nan_to_num(0, 0, 0).abs()
-            # scores: hd products summed in f32; weights: e^x of a score that far off, one ulp, and f16; sums
-            dots = (qq.nan_to_num(0, 0, 0).abs() @ kk.nan_to_num(0, 0, 0).abs().T).amax(-1, keepdim=True) * scale
+            # scores: hd products summed in f32; weights: e^x of a score that far off, one ulp, and f16; sums. A
+            # score's error is |scale| times its dot's, whatever the sign: |scale a - scale b| = |scale| |a - b|
+            dots = (qq.nan_to_num(0, 0, 0).abs() @ kk.nan_to_num(0, 0, 0).abs().T).amax(-1, keepdim=True) * abs(scale)
             rel = 2 * (hd + 4) * 2.0 ** -24 * dots + (len(keys) / 16 + 32) * 2.0 ** -24
             far = len(keys) * 2.0 ** -25 / l.clamp(min=1.0) * vv.nan_to_num(0, 0, 0).abs().amax()  # weights under f16's normal range
             out[a:e, h] = o

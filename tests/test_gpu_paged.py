@@ -255,6 +255,20 @@ def test_attention_scales(dev, scale):
     _attend(b, _queries(b, 4, dev), dev, scale)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 2 ** 30 - 1])
+def test_attention_windows_past_every_position(dev, window):
+    """With contexts shorter than their chunks, whose first tokens are before position 0."""
+    b = ref.Batch([200, 3, 60], [100, 3, 300], 2, 64, 16, dev)
+    _attend(b, _queries(b, 4, dev), dev, 0.1, window)
+
+
+@pytest.mark.parametrize("n", [[8, 1, 8], [9, 8, 1], [8, 7, 9, 17]])
+def test_attention_at_the_rows_that_choose_the_tile(dev, n):
+    """Four query heads a kv head: 32 rows of a sequence are the small tiles' last, 36 the large ones' first."""
+    b = ref.Batch(n, [x + 70 for x in n], 2, 128, 16, dev)
+    _attend(b, _queries(b, 8, dev), dev, 0.1)
+
+
 def test_sequences_share_a_prefix(dev):
     """Three sequences over the pages of one prefix and their own last page."""
     b = ref.Batch([1, 20, 1], [70, 84, 66], 2, 128, 16, dev)
@@ -305,6 +319,15 @@ def test_append_and_attention_past_4_gib(dev):
     o1 = serving.paged_attention(q1, sk, sv, start, ctx, table, 130, 300, 0.1)
     o2 = serving.paged_attention(q2, k, v, start, ctx, moved, 130, 300, 0.1)
     assert torch.equal(o1, o2) and bool(torch.isfinite(o1).all())
+
+
+def test_sizes_given_as_numpy_numbers(dev):
+    b = ref.Batch([3, 40], [90, 300], 2, 64, 16, dev)
+    k, v, start, ctx, table = b.device()
+    q = _queries(b, 4, dev)
+    want = serving.paged_attention(q, k, v, start, ctx, table, 40, 300, 0.125, 100)
+    got = serving.paged_attention(q, k, v, start, ctx, table, np.int64(40), np.int32(300), np.float32(0.125), np.int64(100))
+    assert torch.equal(got, want)
 
 
 def test_paged_python_refusals(dev):
