@@ -172,6 +172,7 @@ int append(const char *name, const T *qkv, const float *norms, const float *cos_
     DTTS_REQUIRE(aligned(qkv, 4 * sizeof(T)) && aligned(cos_t, 16) && aligned(sin_t, 16) && aligned(q_out, 8) && aligned(kp, 8) &&
                      aligned(vp, 8) && aligned(norms, 16) && aligned(q_start, 4) && aligned(context, 4) && aligned(page_table, 4),
                  "%s: misaligned operand", name);
+    DTTS_REQUIRE(static_cast<const void *>(qkv) != q_out, "%s: the queries may not replace qkv", name);
     // Steps of RW head rows a token has, shared by enough waves to fill the chip (kFillWaves, 16 a CU): few tokens
     // spread over many, each with one step; many tokens have a wave each.
     const int64_t per = heads + 2 * n_kv, rw = 64 / (hd / 8), steps = (per + rw - 1) / rw;

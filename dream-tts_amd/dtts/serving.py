@@ -195,14 +195,15 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
     _enqueue("dtts_qk_rope_append_paged_f32" if f32 else "dtts_qk_rope_append_paged_f16", dev, qkv.data_ptr(),
              None if norms is None else norms.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_start.data_ptr(),
              context.data_ptr(), pages.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tokens, b, heads,
-             n_kv, hd, 2 * half, 1 if interleaved else 0, page, n_pages, max_pages, stride, n, eps)
+             n_kv, hd, 2 * half, 1 if interleaved else 0, page, n_pages, max_pages, stride, n, float(eps))
     return out
 
 
 @functools.lru_cache(maxsize=4096)
 def paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window=0):
     """Workspace bytes paged_attention splits contexts over workgroups with."""
-    return int(lib().dtts_paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window))
+    return int(lib().dtts_paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, int(max_q), int(max_context),
+                                                          int(window)))
 
 
 def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale=1.0, window=0, out=None,
@@ -231,7 +232,7 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
         keep, ws, ws_bytes = _bytes(name, dev, workspace, need, q)
     _enqueue("dtts_paged_attention_f16", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_start.data_ptr(),
              context.data_ptr(), pages.data_ptr(), out.data_ptr(), tokens, b, heads, n_kv, hd, page, n_pages, max_pages, stride,
-             qs, max_q, max_context, window, scale, ws, ws_bytes)
+             qs, int(max_q), int(max_context), int(window), float(scale), ws, ws_bytes)
     return out
 
 

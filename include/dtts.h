@@ -486,7 +486,7 @@ int dtts_rotary_f16(const dtts_f16 *x, const float *cos_t, const float *sin_t, c
  *
  * dtts_qk_rope_append_paged_*: QK-norm (norms [2, D] f32, q's weight then k's, or NULL for none),
  * rotary positions and the write of the new keys and values. qkv [tokens, (heads + 2 n_kv) * D] (q
- * heads, then k, then v); q_out [tokens, heads, D] f16; k and v go to the pages. f32 arithmetic, one
+ * heads, then k, then v); q_out [tokens, heads, D] f16, no part of qkv; k and v go to the pages. f32 arithmetic, one
  * rounding to f16. rot_dim a multiple of 8. A token whose position is outside [0, table_len) or has no
  * page is left out whole: its q_out row and every page stay as they were. */
 int dtts_qk_rope_append_paged_f32(const float *qkv, const float *norms, const float *cos_t, const float *sin_t,
@@ -536,9 +536,9 @@ int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dt
  * logprob (or NULL): the token's log-probability among the kept ones (0 for temperature 0). NaN logits count
  * as -inf; a row of nothing else gives token -1 and logprob -inf; +inf logits share all the weight.
  * Weights are f64 and their sums integers (units of 2^-42 of the largest), so a result depends on nothing
- * but the row. rows < 2^20, vocab <= 2^20. workspace (device, 16-byte aligned) of dtts_sample_workspace_bytes bytes lets
- * several workgroups share a long row; without it (NULL or fewer bytes) one workgroup takes a row, with the
- * same result. Calls that may overlap must not share one. */
+ * but the row. rows < 2^20, vocab <= 2^20. workspace (device, 16-byte aligned) of
+ * dtts_sample_workspace_bytes bytes lets several workgroups share a long row; without it (NULL or fewer
+ * bytes) one workgroup takes a row, with the same result. Calls that may overlap must not share one. */
 size_t dtts_sample_workspace_bytes(int64_t rows, int64_t vocab);
 int dtts_sample_f32(const float *logits, const float *temperature, const int32_t *top_k, const float *top_p,
                     const float *min_p, const float *u, int32_t *token, float *logprob, int64_t rows, int64_t vocab,

@@ -158,6 +158,33 @@ def test_sample_follows_the_distribution(dev):
     assert np.array_equal(got, np.stack([np.arange(39), np.arange(1, 40)], 1))
 
 
+@pytest.mark.parametrize("vocab", [1024, 1025, 2049, 8191, 8192, 8193, 10240])
+def test_sample_where_the_kernel_changes(dev, vocab):
+    """The last and first sizes of each row length's kernel; a min_p that nothing but the first token reaches."""
+    x = _logits(dev, 6, vocab, torch.float32, vocab + 1)
+    for seed in range(2):
+        _run(dev, x, _u(6, seed), [1.0, 0.7, 1.0, 2.0, 1.0, 0.3], [0, 40, 0, vocab // 2, 0, 900], [1.0, 0.9, 0.7, 1.0, 1.0, 0.99],
+             [0.0, 0.0, 0.0, 0.0, 1.5, 0.01])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("vocab", [9001, 131072])
+def test_sample_without_a_workspace(dev, vocab, dtype):
+    """One workgroup a row, or several: the same tokens and the same bits."""
+    x = _logits(dev, 9, vocab, dtype, 3)
+    x[8] = 1.0
+    none = torch.empty(0, dtype=torch.uint8, device=dev)
+    f, i = torch.float32, torch.int32
+    t = torch.tensor([0.0, 1.0, 0.7, 1.0, 2.0, 0.1, 1.0, 1.0, 1.0], dtype=f, device=dev)
+    k = torch.tensor([0, 0, 50, 0, 2000, vocab // 2, 0, 1, 300], dtype=i, device=dev)
+    p = torch.tensor([1.0, 1.0, 0.9, 0.95, 0.5, 0.99, 1.0, 0.3, 0.5], dtype=f, device=dev)
+    m = torch.tensor([0.0, 0.0, 0.0, 0.01, 0.0, 0.0, 0.2, 0.0, 0.0], dtype=f, device=dev)
+    for seed in range(4):
+        u = torch.tensor(_u(9, seed), dtype=f, device=dev)
+        a, b = serving.sample(x, u, t, k, p, m), serving.sample(x, u, t, k, p, m, none)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_sample_refusals(dev):
     x = torch.zeros((2, 8), device=dev)
     u = torch.zeros(2, device=dev)

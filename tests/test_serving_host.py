@@ -116,6 +116,7 @@ PAGED = [(dict(tokens=-1), "bad shape"), (dict(b=-1), "bad shape"), (dict(n_kv=0
 @pytest.mark.parametrize("kw,match", PAGED + [
     (dict(heads=0), "heads"), (dict(rot=12), "rotated dimensions"), (dict(rot=72), "rotated dimensions"), (dict(layout=-1), "unknown layout"),
     (dict(table_len=0), "table"), (dict(cos=ctypes.c_void_p(4104)), "misaligned"), (dict(norms=ctypes.c_void_p(4104)), "misaligned"),
+    (dict(), "may not replace qkv"),
 ])
 def test_append_refusals(kw, match):
     for fn in ("dtts_qk_rope_append_paged_f32", "dtts_qk_rope_append_paged_f16"):
