@@ -1048,19 +1048,19 @@ struct Parts {
     int part, parts;
 };
 
-// Rows of up to kWholeVocab logits, and rows enough to fill the chip by themselves, are one workgroup each.
-constexpr int64_t kWholeVocab = 8192, kPartFill = 512;
+// Rows of up to kWholeVocab logits, which 1024 threads hold in registers, are one workgroup each (16384 logits,
+// 1 / 64 / 256 rows: 20 / 22 / 25 us, shared 22 / 33 / 40; the next size, 32 logits a thread, spills: 58 us for a row
+// of 32768, shared 23). Longer ones are shared by as many as the chip runs at once (kPartFill: two of 65 KB LDS a CU)
+// and none has under 2048 logits; from 257 rows on that is one (400 rows of 131072: 298 us, in two parts 336).
+constexpr int64_t kWholeVocab = 16384, kPartFill = 512;
 
 inline Parts parts_of(int64_t rows, int64_t vocab) {
-    int64_t part = (rows * vocab + kPartFill - 1) / kPartFill;
-    if (part < 2048) part = 2048;
-    if (part < (vocab + kMostParts - 1) / kMostParts) part = (vocab + kMostParts - 1) / kMostParts;
-    part = (part + 1023) / 1024 * 1024;
-    Parts p;
-    p.part = static_cast<int>(part);
-    p.parts = static_cast<int>((vocab + part - 1) / part);
-    if (vocab <= kWholeVocab || p.parts < 2) p.parts = 1;
-    return p;
+    int64_t parts = kPartFill / rows;
+    if (parts > vocab / 2048) parts = vocab / 2048;
+    if (parts > kMostParts) parts = kMostParts;
+    if (parts < 1 || vocab <= kWholeVocab) parts = 1;
+    const int64_t part = ((vocab + parts - 1) / parts + 1023) / 1024 * 1024;
+    return Parts{static_cast<int>(part), static_cast<int>((vocab + part - 1) / part)};
 }
 
 inline size_t sample_bytes(int64_t rows, int64_t vocab) {
@@ -1106,6 +1106,8 @@ int sample(const char *name, const T *logits, const float *temperature, const in
         sample_row<T, 1024, 4><<<grid, 1024, 0, stream>>>(a);
     else if (vocab <= 8192)
         sample_row<T, 1024, 8><<<grid, 1024, 0, stream>>>(a);
+    else if (vocab <= 16384)
+        sample_row<T, 1024, 16><<<grid, 1024, 0, stream>>>(a);
     else
         sample_row<T, 1024, 0><<<grid, 1024, 0, stream>>>(a);
     DTTS_LAUNCH_CHECK(name);

@@ -158,7 +158,7 @@ def test_sample_follows_the_distribution(dev):
     assert np.array_equal(got, np.stack([np.arange(39), np.arange(1, 40)], 1))
 
 
-@pytest.mark.parametrize("vocab", [1024, 1025, 2049, 8191, 8192, 8193, 10240])
+@pytest.mark.parametrize("vocab", [1024, 1025, 2049, 8191, 8192, 8193, 10240, 16384, 16385])
 def test_sample_where_the_kernel_changes(dev, vocab):
     """The last and first sizes of each row length's kernel; a min_p that nothing but the first token reaches."""
     x = _logits(dev, 6, vocab, torch.float32, vocab + 1)
@@ -168,7 +168,7 @@ def test_sample_where_the_kernel_changes(dev, vocab):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
-@pytest.mark.parametrize("vocab", [9001, 131072])
+@pytest.mark.parametrize("vocab", [9001, 16385, 131072])
 def test_sample_without_a_workspace(dev, vocab, dtype):
     """One workgroup a row, or several: the same tokens and the same bits."""
     x = _logits(dev, 9, vocab, dtype, 3)
