@@ -33,6 +33,14 @@ struct PagedBatch {
         n = end > first ? end - first : 0;
     }
 
+    // Sequence s's length. A table holds 2^30 positions at most and a batch 2^24 tokens: clipped so that positions,
+    // and a kernel's look ahead of them, stay ints, and none of an impossible length's is in a table.
+    __device__ __forceinline__ int length(int s) const {
+        constexpr int kMost = (1 << 30) + (1 << 24);
+        const int c = context[s];
+        return c < 0 ? 0 : c > kMost ? kMost : c;
+    }
+
     // The page of position-block `at` (position >> page_shift) of sequence s, or -1.
     __device__ __forceinline__ int page(int s, int at) const {
         if (at < 0 || at >= max_pages) return -1;
@@ -61,7 +69,6 @@ struct PagedBatch {
     }
 };
 
-// Positions stay under 2^30, so that a kernel's look ahead of a few tiles cannot pass an int.
 #define DTTS_REQUIRE_PAGED(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride)                               \
     do {                                                                                                                          \
         DTTS_REQUIRE((tokens) >= 0 && (b) >= 0 && (n_kv) > 0 && (n_pages) > 0 && (max_pages) > 0,                                 \

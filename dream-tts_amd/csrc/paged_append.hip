@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv,
     if (s >= a.batch.b) return;
     int first, n;
     a.batch.rows(s, first, n);
-    const int pos = a.batch.context[s] - n + (t - first);
+    const int pos = a.batch.length(s) - n + (t - first);
     if (t < first || t >= first + n || pos < 0 || pos >= a.table_len) return;
     const int page = a.batch.page(s, pos >> a.batch.page_shift);
     if (page < 0) return;

@@ -63,7 +63,7 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs &a, int rows, int64_t a
     for (int s0 = 0; s0 < a.batch.b; s0 += 64) {
         int tiles = 0, first = 0, n = 0, ctx = 0;
         if (s0 + lane < a.batch.b) {
-            ctx = a.batch.context[s0 + lane];
+            ctx = a.batch.length(s0 + lane);
             a.batch.rows(s0 + lane, first, n);
             const int64_t of = static_cast<int64_t>(n) * a.gqa;
             if (of > above && of <= upto) tiles = static_cast<int>((of + rows - 1) / rows);
@@ -650,7 +650,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     int first = 0, n_new = 0, n = 0;
     if (trow < rows && s < a.batch.b) {
         a.batch.rows(s, first, n_new);
-        if (t >= first && t - first < n_new) n = Span(a, s, n_new, a.batch.context[s]).n;
+        if (t >= first && t - first < n_new) n = Span(a, s, n_new, a.batch.length(s)).n;
     }
     float num[PER] = {}, den = 0.0f, m = -INFINITY;
     const float *pr = a.part + trow * a.nsplit * (D + 4);

@@ -262,6 +262,17 @@ def test_attention_windows_past_every_position(dev, window):
     _attend(b, _queries(b, 4, dev), dev, 0.1, window)
 
 
+@pytest.mark.parametrize("window", [0, 1, 7])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 30 + 2 ** 24 + 1, 2 ** 30 + 40, 2 ** 30, -1, -2 ** 31 + 1, -2 ** 31])
+def test_attention_of_impossible_lengths(dev, length, window):
+    """Positions no table holds, at the ends of an int: the chunk and the single token of such a length end, and
+    their neighbours are right. (A window's first key, rounded and 96 further, passed the int's end: the waves
+    then walked 2^31 keys.)"""
+    b = ref.Batch([1, 1, 50, 20], [60, 70, 100, 30], 2, 64, 16, dev)
+    b.c[1] = b.c[2] = length
+    _attend(b, _queries(b, 4, dev), dev, 0.1, window)
+
+
 @pytest.mark.parametrize("n", [[8, 1, 8], [9, 8, 1], [8, 7, 9, 17]])
 def test_attention_at_the_rows_that_choose_the_tile(dev, n):
     """Four query heads a kv head: 32 rows of a sequence are the small tiles' last, 36 the large ones' first."""
