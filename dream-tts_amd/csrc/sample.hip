@@ -19,8 +19,9 @@
 // A short row is one workgroup with its logits and weights in registers. A long one is shared by
 // workgroups in four launches (its largest logit; the histogram; the crossing bins' members; the token),
 // every pass over the logits after the first from L2 or the MALL. What bounds them: a short row the chain
-// of block-wide steps (48 rows of 2048: 10.4 us, of which the bytes are 0.1), a long one the f64 exponentials
-// and the launches (64 x 131072: 57 us = 8 + 18 + 17 + 14, the second with 8.4M exponentials; one row 24).
+// of block-wide steps (48 rows of 2048: 10 us, of which the bytes are 0.1), a long one the vector instructions of the
+// f64 exponentials and the launches' chains of small steps (64 x 131072 by top-p: 9 + 17 + 22 + 13 us, two passes of
+// 8.4M exponentials; one row 24).
 #include <cmath>
 #include <type_traits>
 
@@ -53,7 +54,7 @@ struct SampleArgs {
 struct Row {  // one row's settings, made safe
     float p, m, per_unit;  // per_unit: bins per logit
     int k;
-    double u, inv_t;         // log2(e) / T
+    double u, inv_t, least;  // log2(e) / T; min-p's weight in units
     bool greedy;
     __device__ __forceinline__ bool filters() const { return k > 0 || p < 1.0f; }
 };
@@ -65,11 +66,13 @@ __device__ __forceinline__ Row row_of(const SampleArgs<T> &a, int r) {
     const int k = a.top_k ? a.top_k[r] : 0;
     const float p = a.top_p ? a.top_p[r] : 1.0f, m = a.min_p ? a.min_p[r] : 0.0f, u = a.u[r];
     s.greedy = !(t > 0.0f) || p <= 0.0f || m > 1.0f;  // such a top-p or min-p keeps the first token alone
-    s.inv_t = 1.4426950408889634074 / static_cast<double>(t > 0.0f ? t : 1.0f);
+    // at least 1e-290, so that an infinite T leaves +inf above the rest
+    s.inv_t = fmax(1.4426950408889634074 / static_cast<double>(t > 0.0f ? t : 1.0f), 1e-290);
     s.per_unit = kBins / (kRange * fmaxf(t, 1.0f));
     s.k = k <= 0 || k >= a.vocab ? 0 : k;  // 0: all
     s.p = p < 1.0f ? p : 1.0f;             // 1 (or not a number): all
     s.m = m > 0.0f ? m : 0.0f;
+    s.least = static_cast<double>(s.m) * kUnit;
     s.u = u > 0.0f ? static_cast<double>(fminf(u, 1.0f)) : 0.0;
     return s;
 }
@@ -92,33 +95,37 @@ __device__ __forceinline__ float logit_of(u64 k) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// e^((l - top) / T) for l <= top, inv_t = log2(e) / T: 2^n 2^f with n the exponent's nearest integer and 2^f
-// by its Taylor series in f ln 2, whose remainder at |f| <= 1/2 is (ln 2 / 2)^11 / 11! = 2.2e-13, the sums'
-// own unit. (The library's exp carries 53 bits.) Adding 1.5 * 2^52 leaves n in the low word; n goes straight
-// into the result's exponent.
+// a b + c with c in scalar registers (the two-operand form that the compiler picks copies c first: 10 moves of 57
+// instructions a weight; with it, and four weights side by side, the histogram of 64 x 131072 takes 17 us for 21.5).
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+
+// e^((l - top) / T) for l <= top in units of 2^-42, inv_t = log2(e) / T: 2^(n + 42) 2^f with n the exponent's nearest
+// integer, 2^f - 1 = f P(f) by the P of degree 8 that meets (2^f - 1) / f at the nine Chebyshev nodes of |f| <= 1/2: off
+// by 4e-14 of the weight, a sixth of a unit at most. (The library's exp carries 53 bits.) Adding 1.5 * 2^52 + 42 leaves
+// n + 42 in the low word, which goes straight into the result's exponent. Exponents stop at -64, under half a unit, and
+// +inf counts as 1e300, so that no weight needs a branch: the largest is 1 and a masked one rounds to nothing.
 __device__ __forceinline__ double weight(float l, float top, double inv_t) {
-    constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5,
-                     c6 = c5 * c1 / 6, c7 = c6 * c1 / 7, c8 = c7 * c1 / 8, c9 = c8 * c1 / 9, c10 = c9 * c1 / 10;
-    constexpr double kRound = 6755399441055744.0;
-    const double y = (static_cast<double>(l) - static_cast<double>(top)) * inv_t;
-    const double t = y + kRound, f = y - (t - kRound);
-    double r = fma(c10, f, c9);
-    r = fma(r, f, c8);
-    r = fma(r, f, c7);
-    r = fma(r, f, c6);
-    r = fma(r, f, c5);
-    r = fma(r, f, c4);
-    r = fma(r, f, c3);
-    r = fma(r, f, c2);
-    r = fma(r, f, c1);
+    constexpr double kRound = 6755399441055744.0 + 42.0;
+    const double d = fmin(static_cast<double>(l), 1e300) - fmin(static_cast<double>(top), 1e300);
+    const double y = fmax(d * inv_t, -64.0), t = y + kRound, f = y - (t - kRound);
+    double r = fma_const(1.0203121063391729e-07, f, 1.3255224878668817e-06);
+    r = fma_const(r, f, 1.525268684626772e-05);
+    r = fma_const(r, f, 0.00015403455852453838);
+    r = fma_const(r, f, 0.0013333558179043112);
+    r = fma_const(r, f, 0.009618129159402558);
+    r = fma_const(r, f, 0.055504108664760424);
+    r = fma_const(r, f, 0.2402265069581299);
+    r = fma_const(r, f, 0.6931471805599453);
     r = fma(r, f, 1.0);
-    const uint64_t n = static_cast<uint64_t>(__double_as_longlong(t)) << 52;
-    const double w = __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(__double_as_longlong(r)) + n));
-    return l == top ? 1.0 : y > -64.0 ? w : 0.0;  // under half a unit: nothing (and so where top is +inf)
+    return __hiloint2double(__double2hiint(r) + (__double2loint(t) << 20), __double2loint(r));
 }
 // The nearest number of units: added to 2^52, an f64's last place is one unit.
 __device__ __forceinline__ u64 mass(double w) {
-    return static_cast<u64>(__double_as_longlong(fma(w, kUnit, 4503599627370496.0))) & 0xfffffffffffffull;
+    return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
 __device__ __forceinline__ int bin_of(float l, float top, float per_unit) {
@@ -281,7 +288,7 @@ struct Held {
     __device__ __forceinline__ void weigh(float top, double inv_t) {
         if constexpr (E > 0) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) m[e] = l[e] == -INFINITY ? 0 : mass(weight(l[e], top, inv_t));
+            for (int e = 0; e < E; ++e) m[e] = mass(weight(l[e], top, inv_t));
         }
     }
     // f(logit, index, mass()) for every logit that is not masked
@@ -547,7 +554,7 @@ __device__ __forceinline__ u64 threshold(Shared<NT> &sh, int &half, const Held<T
 // A logit's weight if min-p keeps it (the largest's is 1, and min-p at most 1 here); and if the threshold does too.
 __device__ __forceinline__ u64 min_p_mass(float l, float top, const Row &s) {
     const double x = weight(l, top, s.inv_t);
-    return l != -INFINITY && x >= static_cast<double>(s.m) ? mass(x) : 0;
+    return x >= s.least ? mass(x) : 0;
 }
 __device__ __forceinline__ u64 kept_mass(float l, int i, float top, const Row &s, u64 cut) {
     return pack(l, i) >= cut ? min_p_mass(l, top, s) : 0;
@@ -624,7 +631,7 @@ __device__ __forceinline__ void choose(Shared<NT> &sh, int &half, const SampleAr
                 const float l = row.l[4 * q + e];
                 if (l == -INFINITY) continue;
                 const u64 k = pack(l, i);
-                if (k >= cut && (s.m == 0.0f || weight(l, top, s.inv_t) >= static_cast<double>(s.m))) m += row.m[4 * q + e];
+                if (k >= cut && (s.m == 0.0f || weight(l, top, s.inv_t) >= s.least)) m += row.m[4 * q + e];
             }
             m = last_lane(wave_scan(m));
             if ((threadIdx.x & 63) == 0) sh.seg[q * NW + (threadIdx.x >> 6)] = m;
@@ -783,8 +790,8 @@ struct Part {
             }
         }
     }
-    // f(logit, index) for every logit of the part and, past its end, some masked ones; after every step, end(index
-    // of the wave's run) by whole waves.
+    // f(four logits, the first's index) for every logit of the part and, past its end, some masked ones; after every
+    // step, end(index of the wave's run) by whole waves.
     template <typename F, typename G>
     __device__ __forceinline__ void all(F f, G end) {
         for (int from = i0; from < i1; from += BATCH * STEP) {
@@ -793,8 +800,10 @@ struct Part {
             for (int q = 0; q < BATCH; ++q) {
                 const int run = from + q * STEP + (static_cast<int>(threadIdx.x) & ~63) * 4;
                 if (run >= i1) break;
+                float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f(logit(l[q][e]), from + q * STEP + static_cast<int>(threadIdx.x) * 4 + e);
+                for (int e = 0; e < 4; ++e) v[e] = logit(l[q][e]);
+                f(v, from + q * STEP + static_cast<int>(threadIdx.x) * 4);
                 end(run / 256);
             }
         }
@@ -844,7 +853,11 @@ __global__ __launch_bounds__(kPartNT) void sample_part_hist(PartArgs<T> p) {
     if (top == -INFINITY || s.greedy) return;
     if (!s.filters()) {
         u64 m = 0;
-        part.all([&](float l, int) { m += min_p_mass(l, top, s); },
+        part.all(
+            [&](const float(&l)[4], int) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m += min_p_mass(l[e], top, s);
+            },
                  [&](int run) {
                      if (__any(m != 0)) m = last_lane(wave_scan(m));
                      if ((threadIdx.x & 63) == 0) st.run_mass[run] = m;
@@ -852,16 +865,24 @@ __global__ __launch_bounds__(kPartNT) void sample_part_hist(PartArgs<T> p) {
                  });
         return;
     }
-    const bool by_mass = s.p < 1.0f;
+    const bool by_count = s.k > 0, by_mass = s.p < 1.0f;
     part.all(
-        [&](float l, int) {
-            if (l == -INFINITY) return;
-            const int b = bin_of(l, top, s.per_unit);
-            atomicAdd(&sh.h.count[b], 1u);
-            if (by_mass) {
-                const u64 m = mass(weight(l, top, s.inv_t));
-                if (m) atomicAdd(&sh.h.mass[b], m);
+        [&](const float(&l)[4], int) {
+            int b[4];
+            u64 m[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = bin_of(l[e], top, s.per_unit);
+            if (by_mass) {  // four chains of dependent f64 instructions side by side
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m[e] = mass(weight(l[e], top, s.inv_t));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (m[e]) atomicAdd(&sh.h.mass[b[e]], m[e]);
             }
+            if (by_count)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (l[e] != -INFINITY) atomicAdd(&sh.h.count[b[e]], 1u);
         },
         [](int) {});
     __syncthreads();
@@ -935,15 +956,27 @@ __global__ __launch_bounds__(kPartNT) void sample_part_collect(PartArgs<T> p) {
     }
     u64 m = 0;
     part.all(
-        [&](float l, int i) {
-            if (l == -INFINITY) return;
-            const int b = bin_of(l, top, s.per_unit);
-            if (b < sure) {
-                m += min_p_mass(l, top, s);
-            } else if ((b >= lo && b <= hi) || b == k_bin) {
-                const int at = atomicAdd(&sh.digit, 1);
-                if (at < kCand) sh.cand[at] = pack(l, i);
+        [&](const float(&l)[4], int i) {
+            int b[4];
+            bool above = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                b[e] = bin_of(l[e], top, s.per_unit);
+                above |= b[e] < sure;
             }
+            if (__any(above)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const u64 x = min_p_mass(l[e], top, s);
+                    m += b[e] < sure ? x : 0;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (l[e] != -INFINITY && b[e] >= sure && ((b[e] >= lo && b[e] <= hi) || b[e] == k_bin)) {
+                    const int at = atomicAdd(&sh.digit, 1);
+                    if (at < kCand) sh.cand[at] = pack(l[e], i + e);
+                }
         },
         [&](int run) {
             if (__any(m != 0)) m = last_lane(wave_scan(m));

@@ -158,6 +158,20 @@ def test_sample_follows_the_distribution(dev):
     assert np.array_equal(got, np.stack([np.arange(39), np.arange(1, 40)], 1))
 
 
+@pytest.mark.parametrize("vocab", [500, 9000, 30000])
+def test_sample_infinite_and_largest_logits(dev, vocab):
+    """+inf takes all the weight from the largest finite number, at any temperature; equal weights at an infinite one."""
+    x = _logits(dev, 4, vocab, torch.float32, 8)
+    x[:2, 7], x[:2, vocab // 2], x[:2, vocab - 1] = INF, -LOWEST, INF
+    x[3, 5:9] = -LOWEST
+    for seed in range(3):
+        u = _u(4, seed)
+        for t in ([1.0, INF, INF, 1.0], [1e38, 1e-38, 1e38, INF]):
+            got = _run(dev, x, u, t)
+            assert got[0] in (7, vocab - 1) and got[1] in (7, vocab - 1)
+            _run(dev, x, u, t, [0, 1, 9, 0], [0.5, 1.0, 0.9, 0.7], [0.0, 0.5, 0.1, 0.0])
+
+
 @pytest.mark.parametrize("vocab", [1024, 1025, 2049, 8191, 8192, 8193, 10240, 16384, 16385])
 def test_sample_where_the_kernel_changes(dev, vocab):
     """The last and first sizes of each row length's kernel; a min_p that nothing but the first token reaches."""
