@@ -7,6 +7,10 @@ their pages), ``paged_attention``, the output projection, and after the last lay
 captured into a graph is replayed while they change. Outputs are allocated unless given.
 
 Every tensor of a call is on one device; the work goes to that device's current stream.
+
+A right call on the current device is checked and enqueued by ``_serving`` (csrc/serving_py.cpp), since
+reading ten tensors' sizes and addresses in Python takes longer than the work. It returns None for any
+other, and the Python below makes the call or says what is wrong with it.
 """
 from __future__ import annotations
 
@@ -16,6 +20,11 @@ import functools
 import torch
 
 from ._lib import DttsError, call, lib
+
+try:
+    from . import _serving
+except ImportError as e:
+    raise DttsError(f"dtts/_serving.so is not built for this torch ({e}); run dream-tts_amd/build.py") from e
 
 _F16, _F32, _I32 = torch.float16, torch.float32, torch.int32
 _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
@@ -90,6 +99,9 @@ def rotary(x, cos, sin, pos, interleaved=False, out=None):
     2 * cos.shape[1] dimensions of each head turned by its row's position pos [rows] int32 (device). A
     position outside the tables is padding: that row of `out` is left as it was (of a new one: unset).
     out may be x."""
+    y = _serving.rotary(x, cos, sin, pos, interleaved, out)
+    if y is not None:
+        return y
     name = "rotary"
     if not isinstance(x, _Tensor) or (x.dtype is not _F32 and x.dtype is not _F16):
         raise DttsError(f"{name}: x must be an f32 or f16 tensor")
@@ -172,6 +184,9 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
     v_pages [n_pages, n_kv, page, D] f16 are written in place. q_start [b + 1], context [b] (new tokens
     included) and pages [b, max_pages] are int32; see dtts.h for what each selects. Rows of `out` that
     belong to no sequence are left as they were."""
+    y = _serving.qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, pages, heads, norms, eps, interleaved, out)
+    if y is not None:
+        return y
     name = "qk_rope_append_paged"
     if not isinstance(qkv, _Tensor):
         raise DttsError(f"{name}: qkv must be a tensor")
@@ -213,6 +228,9 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
     size the launch and never change what is computed. `workspace`: a device byte tensor of
     paged_attention_workspace_bytes (allocated when not given). Rows of `out` that belong to no sequence are
     left as they were; a token that sees no position gets zeros."""
+    y = _serving.paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale, window, out, workspace)
+    if y is not None:
+        return y
     name = "paged_attention"
     if not isinstance(q, _Tensor) or q.dtype is not _F16:
         raise DttsError(f"{name}: q must be an f16 tensor")
@@ -260,6 +278,9 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, work
     None; temperature 0 takes the largest logit, top_k 0, top_p 1 and min_p 0 filter nothing. A row without
     a finite (or +inf) logit gives token -1. `workspace`: a device byte tensor of sample_workspace_bytes
     (allocated when not given)."""
+    y = _serving.sample(logits, u, temperature, top_k, top_p, min_p, workspace)
+    if y is not None:
+        return y
     name = "sample"
     if not isinstance(logits, _Tensor) or (logits.dtype is not _F32 and logits.dtype is not _F16) or logits.dim() != 2:
         raise DttsError(f"{name}: logits must be an f32 or f16 tensor [rows, vocab]")

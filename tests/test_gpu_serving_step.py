@@ -183,3 +183,54 @@ def test_calls_on_a_stream_of_their_own(dev):
     torch.cuda.synchronize()
     for w, x in zip(want, got):
         assert all(torch.equal(p, q) for p, q in zip(w, x))
+
+
+def test_the_binding_and_the_python_path_make_the_same_calls(dev, monkeypatch):
+    """Every call here is one that the binding takes; through Python it gives the same bits, into new outputs and
+    given ones."""
+    b = ref.Batch([40, 1, 3], [90, 300, 70], 2, 64, 16, dev)
+    g = torch.Generator().manual_seed(3)
+    k, v, start, ctx, table = b.device()
+    heads, rows = 4, b.tokens
+    qkv = torch.randn((rows, (heads + 4) * 64), generator=g).half().to(dev)
+    cos, sin = (torch.from_numpy(t).to(dev) for t in serving.rope_table_scaled(400, 64, 1e4))
+    norms = (torch.rand((2, 64), generator=g) + 0.5).to(dev)
+    pos = torch.arange(rows, dtype=torch.int32, device=dev)
+    logits = (torch.randn((5, 20000), generator=g) * 3).to(dev)
+    u, t, p, m = (torch.rand(5, generator=g).to(dev) for _ in range(4))
+    top = torch.tensor([0, 1, 40, 5, 0], dtype=torch.int32, device=dev)
+    heads_of = qkv.view(rows, heads + 4, 64)
+    zeros = lambda *s: torch.zeros(s, dtype=torch.float16, device=dev)  # noqa: E731
+    byte = torch.empty(1 << 22, dtype=torch.uint8, device=dev)
+    calls = [
+        ("rotary", lambda: serving.rotary(heads_of[:, 1:5], cos, sin, pos)),
+        ("rotary", lambda: serving.rotary(heads_of[:, :6].float(), cos, sin, pos, True, torch.zeros((rows, 6, 64), device=dev))),
+        ("qk_rope_append_paged", lambda: serving.qk_rope_append_paged(qkv, cos, sin, k, v, start, ctx, table, heads)),
+        ("qk_rope_append_paged", lambda: serving.qk_rope_append_paged(qkv.float(), cos, sin, k, v, start, ctx, table, heads, norms,
+                                                                      1e-5, True, zeros(rows, heads, 64))),
+        ("paged_attention", lambda: serving.paged_attention(heads_of[:, :4], k, v, start, ctx, table, 40, 300, 0.125)),
+        ("paged_attention", lambda: serving.paged_attention(heads_of[:, :4], k, v, start, ctx, table, 40, 5000, 1, 50,
+                                                            zeros(rows, heads, 64), byte)),
+        ("sample", lambda: serving.sample(logits, u, t, top, p, m)),
+        ("sample", lambda: serving.sample(logits.half()[:, :9000], u, workspace=byte)),
+    ]
+    for name, call in calls:
+        taken, real = [], getattr(serving._serving, name)
+
+        def watched(*args, real=real, taken=taken):
+            taken.append(real(*args))
+            return taken[-1]
+
+        with monkeypatch.context() as mp:
+            mp.setattr(serving._serving, name, watched)
+            got = call()
+            cache = k.clone(), v.clone()
+        assert taken[0] is not None, name
+        with monkeypatch.context() as mp:
+            mp.setattr(serving._serving, name, lambda *args: None)
+            want = call()
+        for x, y in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert x.dtype == y.dtype and x.shape == y.shape and torch.equal(x, y), name
+        assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(cache, (k, v)))
+    out = zeros(rows, heads, 64)
+    assert serving.paged_attention(heads_of[:, :4], k, v, start, ctx, table, 40, 300, out=out) is out

@@ -182,3 +182,17 @@ def test_python_layer_refuses_host_tensors():
         serving.sample(torch.zeros((2, 9)), torch.zeros(2))
     with pytest.raises(DttsError, match="f16"):
         serving.paged_attention(x, x, x, x, x, x, 1, 1)
+
+
+def test_the_binding_takes_no_wrong_call():
+    """Anything that is not a right call on the current device is left to the Python path."""
+    b, x = serving._serving, torch.zeros(2, 3, 64)
+    i = torch.zeros(2, dtype=torch.int32)
+    assert b.rotary(x, x[0], x[0], i, False, None) is None  # not on a GPU
+    assert b.rotary(None, 1, "2", [], False, None) is None
+    assert b.qk_rope_append_paged(x, *[i] * 7, 4, None, 1e-6, False, None) is None
+    assert b.paged_attention(x, *[i] * 5, 1, 1, 1.0, 0, None, None) is None
+    assert b.sample(x[0], i, None, None, None, None, None) is None
+    for f in (b.rotary, b.qk_rope_append_paged, b.paged_attention, b.sample):
+        with pytest.raises(TypeError, match="arguments expected"):
+            f(x)
