@@ -637,114 +637,133 @@ __global__ __launch_bounds__(256, 2) void paged_attn_mixed(AttnArgs a, int large
 
 // ---------------------------------------------------------------- the chunks' states
 
-// Joins a row's chunks: out = sum_c num_c 2^(m_c - M) / sum_c den_c 2^(m_c - M), M the largest m_c. Up to
-// kFewChunks: a wave a row, everything requested at once. More: W waves a row, wave w taking chunks w,
-// w + W, ..; 64 of its chunks at a time have their maxima and sums read by a lane each, then their rows
-// follow with U requests in flight (5 tokens of 32 heads, 51 chunks: 19.6 us with a loop that carries the
-// maximum along and waits for each, 5.1 so).
+// Join a row's chunks: out = sum_c num_c 2^(m_c - M) / sum_c den_c 2^(m_c - M), M the largest m_c.
 constexpr int kFewChunks = 8;
 
-template <int D, int W>
-__global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
-    constexpr int PER = D / 64, U = 8;
-    __shared__ float sm[4][D + 2];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % W;
-    const int64_t trow = static_cast<int64_t>(blockIdx.x) * (4 / W) + wave / W;
-    const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
-    const int t = static_cast<int>((trow < rows ? trow : rows - 1) / a.heads);
-    const int s = a.batch.sequence_of<64>(t);
-    int first = 0, n_new = 0, n = 0;
-    if (trow < rows && s < a.batch.b) {
-        a.batch.rows(s, first, n_new);
-        if (t >= first && t - first < n_new) n = Span(a, s, n_new, a.batch.length(s)).n;
-    }
-    float num[PER] = {}, den = 0.0f, m = -INFINITY;
+// Up to kFewChunks: a wave for R heads of a token, which share its lookups, everything requested at once. 862 tokens of
+// 16 heads over four chunks with 1 / 2 / 4 heads a wave: 7.3 / 5.6 / 6.5 us; with the chunks requested before it is known
+// how many a row has 8.5.
+template <int D, int R>
+__global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
+    constexpr int PER = D / 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t trow = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * R, rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
+    if (trow >= rows) return;
+    const int t = static_cast<int>(trow / a.heads), s = a.batch.sequence_of<64>(t);
+    if (s >= a.batch.b) return;
+    int first, n_new;
+    a.batch.rows(s, first, n_new);
+    if (t < first || t - first >= n_new) return;
+    const int n = Span(a, s, n_new, a.batch.length(s)).n;
+    if (n <= 1) return;
     const float *pr = a.part + trow * a.nsplit * (D + 4);
-    if (W == 1 && n > 1) {  // kFewChunks at most
-        float mc[kFewChunks], lc[kFewChunks], v[kFewChunks][PER];
+    float mc[R][kFewChunks], lc[R][kFewChunks], v[R][kFewChunks][PER];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int c = 0; c < kFewChunks; ++c)
             if (c < n) {
-                const float *pc = pr + c * (D + 4);
-                mc[c] = pc[D + 1];
-                lc[c] = pc[D];
+                const float *pc = pr + static_cast<int64_t>(r * a.nsplit + c) * (D + 4);
+                mc[r][c] = pc[D + 1];
+                lc[r][c] = pc[D];
 #pragma unroll
-                for (int e = 0; e < PER; ++e) v[c][e] = pc[lane * PER + e];
+                for (int e = 0; e < PER; ++e) v[r][c][e] = pc[lane * PER + e];
             }
 #pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float num[PER] = {}, den = 0.0f, m = -INFINITY;
+#pragma unroll
         for (int c = 0; c < kFewChunks; ++c)
-            if (c < n) m = fmaxf(m, mc[c]);
+            if (c < n) m = fmaxf(m, mc[r][c]);
         const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int c = 0; c < kFewChunks; ++c)
             if (c < n) {
-                const float f = exp2_fast(mc[c] - mu);
-                den += lc[c] * f;
+                const float f = exp2_fast(mc[r][c] - mu);
+                den += lc[r][c] * f;
 #pragma unroll
-                for (int e = 0; e < PER; ++e) num[e] += v[c][e] * f;
+                for (int e = 0; e < PER; ++e) num[e] += v[r][c][e] * f;
             }
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) a.out[(trow + r) * D + lane * PER + e] = static_cast<half_t>(num[e] * inv);
     }
-    if (W > 1 && n > 1) {
-        for (int c0 = w; c0 < n; c0 += 64 * W) {
-            const int mine = c0 + lane * W;
-            const float mc = mine < n ? pr[static_cast<int64_t>(mine) * (D + 4) + D + 1] : -INFINITY;
-            const float lc = mine < n ? pr[static_cast<int64_t>(mine) * (D + 4) + D] : 0.0f;
-            float mx = mc;
-#pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-            mx = fmaxf(mx, m);
-            const float mu = mx == -INFINITY ? 0.0f : mx, back = exp2_fast(m - mu), f = exp2_fast(mc - mu);
-            float dl = lc * f;
-#pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) dl += __shfl_xor(dl, off, 64);
-            den = den * back + dl;
-            m = mx;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) num[e] *= back;
-            const int left = (n - c0 + W - 1) / W, count = left < 64 ? left : 64;
-            const float *pc = pr + static_cast<int64_t>(c0) * (D + 4) + lane * PER;
-            for (int i = 0; i < count; i += U) {
-                float v[U][PER];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int e = 0; e < PER; ++e)
-                        v[u][e] = pc[static_cast<int64_t>((i + u < count ? i + u : count - 1) * W) * (D + 4) + e];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float fu = i + u < count ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + u)) : 0.0f;
-#pragma unroll
-                    for (int e = 0; e < PER; ++e)
-                        if (i + u < count) num[e] += v[u][e] * fu;
-                }
-            }
-        }
-    }
-    if constexpr (W > 1) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) sm[w][lane * PER + e] = num[e];
-        if (lane == 0) {
-            sm[w][D] = den;
-            sm[w][D + 1] = m;
-        }
-        __syncthreads();
-        if (w != 0) return;
-        float mx = m;
-#pragma unroll
-        for (int u = 1; u < W; ++u) mx = fmaxf(mx, sm[u][D + 1]);
-        const float mu = mx == -INFINITY ? 0.0f : mx, f0 = exp2_fast(m - mu);
-        den *= f0;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) num[e] *= f0;
-#pragma unroll
-        for (int u = 1; u < W; ++u) {
-            const float f = exp2_fast(sm[u][D + 1] - mu);
-            den += sm[u][D] * f;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) num[e] += sm[u][lane * PER + e] * f;
-        }
-    }
+}
+
+// More: a workgroup a row, wave w taking chunks w, w + 4, ..; 64 of its chunks at a time have their maxima and sums read
+// by a lane each, then their rows follow with U requests in flight (5 tokens of 32 heads, 51 chunks: 19.6 us with a
+// loop that carries the maximum along and waits for each, 5.1 so).
+template <int D>
+__global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
+    constexpr int PER = D / 64, U = 8, W = 4;
+    __shared__ float sm[W][D + 2];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t trow = blockIdx.x;
+    const int t = static_cast<int>(trow / a.heads), s = a.batch.sequence_of<64>(t);
+    if (s >= a.batch.b) return;
+    int first, n_new;
+    a.batch.rows(s, first, n_new);
+    if (t < first || t - first >= n_new) return;
+    const int n = Span(a, s, n_new, a.batch.length(s)).n;
     if (n <= 1) return;
+    float num[PER] = {}, den = 0.0f, m = -INFINITY;
+    const float *pr = a.part + trow * a.nsplit * (D + 4);
+    for (int c0 = w; c0 < n; c0 += 64 * W) {
+        const int mine = c0 + lane * W;
+        const float mc = mine < n ? pr[static_cast<int64_t>(mine) * (D + 4) + D + 1] : -INFINITY;
+        const float lc = mine < n ? pr[static_cast<int64_t>(mine) * (D + 4) + D] : 0.0f;
+        float mx = mc;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+        mx = fmaxf(mx, m);
+        const float mu = mx == -INFINITY ? 0.0f : mx, back = exp2_fast(m - mu), f = exp2_fast(mc - mu);
+        float dl = lc * f;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) dl += __shfl_xor(dl, off, 64);
+        den = den * back + dl;
+        m = mx;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) num[e] *= back;
+        const int left = (n - c0 + W - 1) / W, count = left < 64 ? left : 64;
+        const float *pc = pr + static_cast<int64_t>(c0) * (D + 4) + lane * PER;
+        for (int i = 0; i < count; i += U) {
+            float v[U][PER];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < PER; ++e)
+                    v[u][e] = pc[static_cast<int64_t>((i + u < count ? i + u : count - 1) * W) * (D + 4) + e];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float fu = i + u < count ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + u)) : 0.0f;
+#pragma unroll
+                for (int e = 0; e < PER; ++e)
+                    if (i + u < count) num[e] += v[u][e] * fu;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sm[w][lane * PER + e] = num[e];
+    if (lane == 0) {
+        sm[w][D] = den;
+        sm[w][D + 1] = m;
+    }
+    __syncthreads();
+    if (w != 0) return;
+    float mx = m;
+#pragma unroll
+    for (int u = 1; u < W; ++u) mx = fmaxf(mx, sm[u][D + 1]);
+    const float mu = mx == -INFINITY ? 0.0f : mx, f0 = exp2_fast(m - mu);
+    den *= f0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) num[e] *= f0;
+#pragma unroll
+    for (int u = 1; u < W; ++u) {
+        const float f = exp2_fast(sm[u][D + 1] - mu);
+        den += sm[u][D] * f;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) num[e] += sm[u][lane * PER + e] * f;
+    }
     const float inv = den == 0.0f ? 0.0f : 1.0f / den;
 #pragma unroll
     for (int e = 0; e < PER; ++e) a.out[trow * D + lane * PER + e] = static_cast<half_t>(num[e] * inv);
@@ -815,10 +834,12 @@ hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
-    if (a.nsplit <= kFewChunks)
-        paged_attn_merge<D, 1><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+    if (a.nsplit <= kFewChunks && a.heads % 2 == 0)
+        paged_attn_merge_few<D, 2><<<static_cast<unsigned>((rows / 2 + 3) / 4), 256, 0, stream>>>(a);
+    else if (a.nsplit <= kFewChunks)
+        paged_attn_merge_few<D, 1><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
     else
-        paged_attn_merge<D, 4><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
+        paged_attn_merge<D><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 

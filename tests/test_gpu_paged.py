@@ -280,6 +280,15 @@ def test_attention_at_the_rows_that_choose_the_tile(dev, n):
     _attend(b, _queries(b, 8, dev), dev, 0.1)
 
 
+@pytest.mark.parametrize("c", [[900, 50, 0, 385], [2000, 129, 1500, 1]])
+@pytest.mark.parametrize("heads", [3, 6])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_joins_chunks_of_odd_and_even_heads(dev, c, heads, hd):
+    """Up to eight chunks a row and more, rows with one or none beside them, padding behind."""
+    b = ref.Batch([1, 1, 0, 2], c, 3, hd, 16, dev, extra_tokens=2)
+    _attend(b, _queries(b, heads, dev), dev, 0.1)
+
+
 def test_sequences_share_a_prefix(dev):
     """Three sequences over the pages of one prefix and their own last page."""
     b = ref.Batch([1, 20, 1], [70, 84, 66], 2, 128, 16, dev)
