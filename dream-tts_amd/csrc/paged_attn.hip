@@ -376,7 +376,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
 // Two buffers: the next keys' rows are requested a tile ahead and stored after the tile's products, one barrier a
 // tile. Bound by issue: two waves a SIMD take turns between the matrix cores and the softmax's 32 exponentials,
 // products with the scale and conversions a lane (matrix cores busy 41 % of the cycles, vector instructions 38 %,
-// LDS 37 %). 2048 tokens after 7952, 32 heads over 8, D = 128: 342 us, 880 TFLOP/s of the unmasked products.
+// LDS 37 %). 2048 tokens after 7952, 32 heads over 8, D = 128: 333 us, 900 TFLOP/s of the unmasked products.
 constexpr float kSlack = 8.0f;
 
 template <int D>
