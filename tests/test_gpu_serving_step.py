@@ -234,3 +234,41 @@ def test_the_binding_and_the_python_path_make_the_same_calls(dev, monkeypatch):
         assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(cache, (k, v)))
     out = zeros(rows, heads, 64)
     assert serving.paged_attention(heads_of[:, :4], k, v, start, ctx, table, 40, 300, out=out) is out
+
+
+def test_captured_long_rows_and_split_contexts(dev):
+    """The calls of several launches in two graphs, each with a workspace of its own, replayed in turn while logits,
+    settings, lengths and pages change, with eager calls between: every replay against the eager result."""
+    g = torch.Generator().manual_seed(5)
+    rows, vocab, heads = 5, 40000, 8
+    x, u = torch.zeros((rows, vocab), device=dev), torch.zeros(rows, device=dev)
+    t, p = torch.ones(rows, device=dev), torch.ones(rows, device=dev)
+    k = torch.zeros(rows, dtype=torch.int32, device=dev)
+    b = ref.Batch([1, 40, 1, 2], [900, 700, 64, 1500], 4, 64, 16, dev)
+    kp, vp, start, ctx, table = b.device()
+    q = torch.zeros((b.tokens, heads, 64), dtype=torch.float16, device=dev)
+    need = serving.paged_attention_workspace_bytes(b.tokens, 4, heads, 4, 64, 40, 1500), serving.sample_workspace_bytes(rows, vocab)
+    assert min(need) > 0
+    graphs = []
+    for _ in range(2):
+        ws = [torch.full((n,), 255, dtype=torch.uint8, device=dev) for n in need]
+        serving.sample(x, u, t, k, p, workspace=ws[1])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = serving.sample(x, u, t, k, p, workspace=ws[1]), serving.paged_attention(q, kp, vp, start, ctx, table, 40, 1500, 0.1,
+                                                                                           workspace=ws[0])
+        graphs.append((graph, out, ws))
+    for i in range(6):
+        x.copy_(torch.randn((rows, vocab), generator=g) * 3)
+        u.copy_(torch.rand(rows, generator=g))
+        t.copy_(torch.tensor([0.0, 1.0, 0.7, 1.3, 0.9]).roll(i))
+        k.copy_(torch.tensor([0, 50, 0, 3000, 1], dtype=torch.int32).roll(2 * i))
+        p.copy_(torch.tensor([1.0, 0.9, 0.5, 1.0, 0.99]).roll(3 * i))
+        q.copy_((torch.randn(q.shape, generator=g)).half())
+        ctx.copy_(torch.tensor([900 - 100 * i, 700 - 130 * i, 64 - i, 1500 - 7 * i], dtype=torch.int32))
+        graph, ((token, logprob), o), _ = graphs[i % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        (want, lp), wo = serving.sample(x, u, t, k, p), serving.paged_attention(q, kp, vp, start, ctx, table, 40, 1500, 0.1)
+        assert torch.equal(token, want) and torch.equal(logprob, lp) and torch.equal(o, wo), i
