@@ -5,8 +5,12 @@
 // so rows are numbered token * gqa + head within (sequence, kv head), and a tile of consecutive rows goes to one
 // workgroup: 16 rows where a sequence has few, 128 where it has a chunk. A query's scores, softmax state (running maximum,
 // running sum) and output sums are f32; q, k, v are f16 as the cache and the matrix cores hold them;
-// the weights e^(s - max) are rounded to f16 for the second product (at most 2^-11 of each weight,
-// as the output's own rounding), and the output is rounded once.
+// the weights e^(s - max) are rounded to f16 for the second product, and the output is rounded once. The weights are
+// held times 2^kBias (it cancels in the division by their sum), at the upper end of f16's range: down to 2^(-14 - kBias) of
+// the largest each is off by 2^-11 relative at most, as the output's own rounding is, and below that by 2^(-25 - kBias) of
+// the largest. Without it a flat tail far under one leading key would leave the numerator and stay in the denominator
+// (65000 keys e^-17.5 below one: all of their 0.16 %). For the same reason a tile's weights are summed before they meet
+// the running sum, next to which a single one may be nothing.
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -97,6 +101,11 @@ __device__ __forceinline__ float max_16_32_apart(float x) {
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What the exponents of the weights are raised by. The 16-row tiles' largest weight is 2^15, the 128-row ones' up to
+// 2^kSlack times 2^kChunkBias (their maximum may lag behind by that): both under f16's 65504. kSlack 1 / 4 / 8 (and a
+// bias that goes with it): 2048 tokens after 7952 335 / 333 / 335 us.
+constexpr float kBias = 15.0f, kSlack = 4.0f, kChunkBias = 11.0f;
 
 // One row over keys [k0, k1) alone, by one wave (D / 64 dimensions a lane): the sums a tile's row
 // would have, without the products with weight 0 of keys that other rows of the tile see. Used where
@@ -279,14 +288,16 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             m = mx;
         }
         half8_t p;
+        float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float x = exp2_fast(sc[u][i] - mu);
-                l += x;
+                const float x = exp2_fast(sc[u][i] - mu + kBias);
+                sum += x;
                 p[4 * u + i] = static_cast<half_t>(x);
             }
+        l += sum;
         // slots past the last key and of missing pages hold anything: 0 times it may be NaN
         if (kb + 32 > k1 || t.ok != 3) {
 #pragma unroll
@@ -348,7 +359,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
                 *reinterpret_cast<float4_t *>(pr + E * l16 + e) = float4_t{num[e], num[e + 1], num[e + 2], num[e + 3]};
             if (l16 == 0) {
                 pr[D] = den;
-                pr[D + 1] = mt;
+                pr[D + 1] = mt - kBias;  // a state's weights are relative to what it holds as its maximum
             }
         } else {
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // a row that sees no key is zero
@@ -377,8 +388,6 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
 // tile. Bound by issue: two waves a SIMD take turns between the matrix cores and the softmax's 32 exponentials,
 // products with the scale and conversions a lane (matrix cores busy 41 % of the cycles, vector instructions 38 %,
 // LDS 37 %). 2048 tokens after 7952, 32 heads over 8, D = 128: 333 us, 900 TFLOP/s of the unmasked products.
-constexpr float kSlack = 8.0f;
-
 template <int D>
 struct ChunkLds {
     static constexpr int KT = 64, KP = D + 8;  // keys a tile; elements from key row to key row
@@ -469,7 +478,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
         }
         if (lane == 0) s_ok[buf][w] = g_ok;
     };
-    float m = -INFINITY, m2 = 0.0f, l = 0.0f;  // m2: m in log2, 0 while there is none
+    float m = -INFINITY, m2 = 0.0f, l = 0.0f;  // m2: what the weights are relative to in log2, anything while there is no m
     float16_t o[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -529,20 +538,22 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= f;
             m = mx;
-            m2 = m == -INFINITY ? 0.0f : m * a.scale2;
+            m2 = (m == -INFINITY ? 0.0f : m * a.scale2) - kChunkBias;
         }
         half8_t pf[4];
         // the other workgroup's wave on this SIMD yields here, so that the two take turns between products and
         // softmax instead of meeting in both (2048 tokens after 7952: 363 -> 353 us)
         __builtin_amdgcn_s_setprio(1);
+        float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float x = exp2_fast(__builtin_fmaf(sc[t >> 1][8 * (t & 1) + j], a.scale2, -m2));
-                l += x;
+                sum += x;
                 pf[t][j] = static_cast<half_t>(x);
             }
+        l += sum;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll

@@ -507,8 +507,9 @@ int dtts_qk_rope_append_paged_f16(const dtts_f16 *qkv, const float *norms, const
  * over positions max(0, p - window + 1) <= j <= p of the token's sequence, p its position (window 0: all of
  * them). q [tokens, heads, D] f16 with q_stride elements between tokens (a multiple of 8), out
  * [tokens, heads, D] f16, not q. heads is any multiple of n_kv. Scores, softmax state and sums in f32;
- * the weights are rounded to f16 for the product with v. A token that sees no position (p < 0, or no page
- * of its window is there) gets zeros. Positions without a page are not attended to, slots past a
+ * the weights are rounded to f16 for the product with v (each off by 2^-11 of itself, or by 2^-36 of
+ * the largest where that is more). A token that sees no position (p < 0, or no page of its window is
+ * there) gets zeros. Positions without a page are not attended to, slots past a
  * sequence's context are never used, and a value that is not finite reaches only the tokens that see it.
  * scale is finite (any sign).
  * max_q and max_context are what the caller knows of the batch: the longest chunk and context. They

@@ -1,0 +1,73 @@
+"""dtts_paged_attention_f16 where the weights of a row span many orders: one or two keys ahead of a long flat tail, whose
+weights are each next to nothing and together are not."""
+import numpy as np
+import pytest
+import torch
+
+from dtts import serving
+
+pytestmark = pytest.mark.gpu
+PAGE = 64
+
+
+def _run(dev, scores, values, q_len, heads, n_kv, hd, workspace):
+    """Attention of q_len tokens at the end of keys whose scores (exact in f16) and values are one number each, for every
+    token alike; the 64-bit result of each token."""
+    n = len(scores)
+    pages = -(-n // PAGE)
+    s, v = np.zeros(pages * PAGE), np.full(pages * PAGE, np.nan)
+    s[:n], v[:n] = scores, values
+    k = torch.zeros((pages, n_kv, PAGE, hd), dtype=torch.float16)
+    k[..., 3] = torch.from_numpy(s).half().view(pages, 1, PAGE)
+    vv = torch.from_numpy(v).half().view(pages, 1, PAGE, 1).expand(pages, n_kv, PAGE, hd).contiguous()
+    assert np.array_equal(k[:, 0, :, 3].double().numpy().ravel(), s)
+    q = torch.zeros((q_len, heads, hd), dtype=torch.float16, device=dev)
+    q[..., 3] = 1.0
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    table = torch.arange(pages, dtype=torch.int32, device=dev)[None].contiguous()
+    ws = None if workspace else torch.empty(0, dtype=torch.uint8, device=dev)
+    got = serving.paged_attention(q, k.to(dev), vv.to(dev), i32([0, q_len]), i32([n]), table, q_len, n, 1.0, workspace=ws)
+    w = np.exp(s[:n] - s[:n].max())
+    v = vv[:, 0, :, 0].double().numpy().ravel()[:n]
+    num, den, mag = (np.cumsum(x)[n - q_len:] for x in (w * v, w, w * np.abs(v)))
+    return got.cpu().double().numpy().reshape(q_len, -1), num / den, mag / den
+
+
+def _check(got, want, mag, n, small):
+    """Half a step of f16 in every weight and in the output (2^-11 each); f32: a lane adds at most n / 16 products' or tiles'
+    sums to its running ones, numerator and denominator (2^-24 each), a tile's sum has 32 terms, the exponent's argument (up
+    to 64) is off by 2^-18; weights below f16's normal range by at most `small` of the largest each."""
+    rel = 2 * 2.0 ** -11 + (2 * n / 16 + 2 * 32) * 2.0 ** -24 + 2.0 ** -18
+    tol = rel * mag + n * small + 2.0 ** -25
+    err = np.abs(got - want[:, None]).max(1)
+    assert np.all(err <= tol), (float((err / tol).max()), got[-1, 0], want[-1])
+
+
+# half of f16's smallest number (2^-25) under a largest weight of 2^15 (16-row tiles) and of 2^11 at least (128-row ones)
+SMALL = {True: 2.0 ** -40, False: 2.0 ** -36}
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("q_len,heads,n_kv,hd", [(1, 1, 1, 128), (1, 8, 2, 64), (8, 4, 1, 128), (200, 4, 1, 128), (130, 1, 1, 64)])
+@pytest.mark.parametrize("below", [15.5, 17.0, 17.5, 20.0])
+def test_a_flat_tail_under_one_leading_key(dev, below, q_len, heads, n_kv, hd, workspace):
+    """65001 keys; the leading one (value 0) first, inside, or last that every token sees."""
+    n = 65001
+    for at in (0, 30011, n - q_len):
+        scores, values = np.full(n, -below), np.ones(n)
+        scores[at], values[at] = 0.0, 0.0
+        got, want, mag = _run(dev, scores, values, q_len, heads, n_kv, hd, workspace)
+        _check(got, want, mag, n, SMALL[q_len * heads // n_kv <= 32])
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("q_len,heads", [(1, 4), (200, 4)])
+def test_a_maximum_that_rises_in_small_steps(dev, q_len, heads, workspace):
+    """Leading keys 2.5 (under 2^4 in the weights) and 6 above the last: the 128-row tiles keep an earlier one as their
+    maximum, or move it."""
+    n = 30003
+    scores, values = np.full(n, -12.0), np.where(np.arange(n) % 2, 1.0, -0.5)
+    for i, (at, s) in enumerate([(2, 0.0), (500, 2.5), (9000, 8.5), (20000, 11.0)]):
+        scores[at], values[at] = s, i - 1.5
+    got, want, mag = _run(dev, scores, values, q_len, heads, 1, 128, workspace)
+    _check(got, want, mag, n, SMALL[q_len * heads <= 32])
