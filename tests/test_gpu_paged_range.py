@@ -71,3 +71,19 @@ def test_a_maximum_that_rises_in_small_steps(dev, q_len, heads, workspace):
         scores[at], values[at] = s, i - 1.5
     got, want, mag = _run(dev, scores, values, q_len, heads, 1, 128, workspace)
     _check(got, want, mag, n, SMALL[q_len * heads <= 32])
+
+
+@pytest.mark.parametrize("hd,heads", [(64, 1), (64, 8), (128, 1), (128, 8)])
+@pytest.mark.parametrize("n", [33000, 65000])
+def test_a_row_of_hundreds_of_chunks(dev, n, hd, heads):
+    """One token of one kv head is cut into more than 256 chunks, which its join takes in several rounds: with the largest
+    score in the first round, in the last one and in the chunk between them, the rest rising or falling."""
+    assert serving.paged_attention_workspace_bytes(1, 1, heads, 1, hd, 1, n) > 256 * heads * (hd + 4) * 4
+    rng = np.random.RandomState(n + hd)
+    values = rng.randint(-8, 9, n) / 4.0
+    for at in (5, n // 2, n - 3):
+        for slope in (0.0, 6.0, -6.0):
+            scores = np.round((rng.rand(n) * 2 + slope * np.arange(n) / n) * 64) / 64
+            scores[at] = 12.0
+            got, want, mag = _run(dev, scores, values, 1, heads, 1, hd, True)
+            _check(got, want, mag, n, SMALL[True])
