@@ -107,65 +107,35 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // bias that goes with it): 2048 tokens after 7952 335 / 333 / 335 us.
 constexpr float kBias = 15.0f, kSlack = 4.0f, kChunkBias = 11.0f;
 
-// One row over keys [k0, k1) alone, by one wave (D / 64 dimensions a lane): the sums a tile's row
-// would have, without the products with weight 0 of keys that other rows of the tile see. Used where
-// such a product made a NaN (0 times a value that is not finite).
-template <int D>
-__device__ void attend_alone(const AttnArgs &a, int s, int kh, const half_t *qr, int k0, int k1, float (&o)[D / 64], float &l,
-                             float &m) {
-    constexpr int PER = D / 64;
-    const int d0 = (threadIdx.x & 63) * PER;
-    m = -INFINITY;
-    l = 0.0f;
-#pragma unroll
-    for (int r = 0; r < PER; ++r) o[r] = 0.0f;
-    for (int j = k0; j < k1 && l == l; ++j) {  // a NaN sum stays one
-        const int page = a.batch.page(s, j >> a.batch.page_shift);
-        if (page < 0) continue;
-        const int64_t at = page * a.batch.page_stride +
-                           ((static_cast<int64_t>(kh) << a.batch.page_shift) + (j & ((1 << a.batch.page_shift) - 1))) * D + d0;
-        float dot = 0.0f, v[PER];
-#pragma unroll
-        for (int r = 0; r < PER; ++r) {
-            dot += static_cast<float>(qr[d0 + r]) * static_cast<float>(a.k[at + r]);
-            v[r] = static_cast<float>(a.v[at + r]);
-        }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
-        const float sc = (a.negate ? -dot : dot) * a.scale2, mx = fmaxf(m, sc), mu = mx == -INFINITY ? 0.0f : mx;
-        const float c = exp2_fast(m - mu), p = exp2_fast(sc - mu);
-        m = mx;
-        l = l * c + p;
-#pragma unroll
-        for (int r = 0; r < PER; ++r) o[r] = o[r] * c + p * v[r];
-    }
+// A value that is not finite (an overflow of the projection, a slot written over) makes 0 times it a NaN, so in a tile of
+// keys that not all of the rows see it may not reach the product: there such values count as 0 (take_out says whether it
+// met one), and the rows that see them get them added after the last tile (taken). What all rows see goes through the
+// product as it is. Two values at a time and without comparisons, whose masks would fill the scalar registers.
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair) {  // ones in the place of each that has the largest exponent
+    const uint32_t top = ((pair & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    return top | (top - (top >> 15));
 }
-
-// Row rr of (s, kh) again, its keys of [k0, k1) alone, into the place where its tile left it. pos0: the
-// position of the sequence's first new token.
-template <int D>
-__device__ void store_alone(const AttnArgs &a, int s, int kh, int first, int pos0, int rr, int k0, int k1, int chunks,
-                                         int c) {
-    constexpr int PER = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int tok = rr / a.gqa, head = kh * a.gqa + rr - tok * a.gqa, pos = pos0 + tok;
-    const int lo = a.window > 0 ? pos - a.window + 1 : 0;
-    float o[PER], l, m;
-    attend_alone<D>(a, s, kh, a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D, k0 > lo ? k0 : lo < 0 ? 0 : lo,
-                    k1 <= pos ? k1 : pos + 1, o, l, m);
-    const int64_t trow = static_cast<int64_t>(first + tok) * a.heads + head;
-    if (chunks > 1) {
-        float *pr = a.part + (trow * a.nsplit + c) * (D + 4);
+template <int E>
+__device__ __forceinline__ uint32_t take_out(half_t __attribute__((ext_vector_type(E))) &v) {
+    typedef uint32_t pairs __attribute__((ext_vector_type(E / 2)));
+    pairs p = __builtin_bit_cast(pairs, v);
+    uint32_t any = 0;
 #pragma unroll
-        for (int r = 0; r < PER; ++r) pr[lane * PER + r] = o[r];
-        if (lane == 0) {
-            pr[D] = l;
-            pr[D + 1] = m;
-        }
-    } else {
-#pragma unroll
-        for (int r = 0; r < PER; ++r) a.out[trow * D + lane * PER + r] = static_cast<half_t>(l == 0.0f ? 0.0f : o[r] / l);
+    for (int e = 0; e < E / 2; ++e) {
+        const uint32_t out = not_finite(p[e]);
+        any |= out;
+        p[e] &= ~out;
     }
+    v = __builtin_bit_cast(half_t __attribute__((ext_vector_type(E))), p);
+    return any;
+}
+template <int E>
+__device__ __forceinline__ half_t __attribute__((ext_vector_type(E))) taken(half_t __attribute__((ext_vector_type(E))) v) {
+    typedef uint32_t pairs __attribute__((ext_vector_type(E / 2)));
+    pairs p = __builtin_bit_cast(pairs, v);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) p[e] &= not_finite(p[e]);
+    return __builtin_bit_cast(half_t __attribute__((ext_vector_type(E))), p);
 }
 
 // ---------------------------------------------------------------- few rows: 16 a tile
@@ -220,11 +190,15 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     int k0, k1;  // the tile's keys in this chunk
     span.chunk_keys(a, c, k0, k1);
     const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
+    // one of the tile's rows at least sees the keys from `bottom` to k1, all of them those from `from` to `upto`
+    const int upto = ctx - n_new + first_tok, bottom = a.window > 0 ? upto - a.window + 1 : 0;
+    const int from = a.window > 0 ? bottom + last_tok - first_tok : 0;
     {
-        const int top = ctx - n_new + last_tok + 1, bottom = a.window > 0 ? ctx - n_new + first_tok - a.window + 1 : 0;
+        const int top = ctx - n_new + last_tok + 1;
         if (k1 > top) k1 = top;
         if (k0 < bottom) k0 = bottom & ~31;
     }
+    auto cut = [&](int kb) { return first_tok != last_tok && (kb < from || kb + 31 > upto); };  // a tile that some rows see a part of
     half8_t qf[C];
     {
         const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
@@ -256,6 +230,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             t.v[j] = *reinterpret_cast<const typename KvTile<D>::ve *>(a.v + base[j >> 2] + (4 * g + (j & 3)) * D + E * l16);
     };
     float m = -INFINITY, l = 0.0f;
+    uint32_t spoilt = 0;
     float4_t o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -298,12 +273,16 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
                 p[4 * u + i] = static_cast<half_t>(x);
             }
         l += sum;
-        // slots past the last key and of missing pages hold anything: 0 times it may be NaN
-        if (kb + 32 > k1 || t.ok != 3) {
+        // what no row sees holds anything: 0 times it may be NaN
+        if (kb + 32 > k1 || kb < bottom || t.ok != 3 || cut(kb)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
-                if (key >= k1 || !(t.ok >> (j >> 2) & 1)) t.v[j] = typename KvTile<D>::ve{};
+                if (key >= k1 || key < bottom || !(t.ok >> (j >> 2) & 1)) t.v[j] = typename KvTile<D>::ve{};
+            }
+            if (cut(kb)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) spoilt |= take_out<E>(t.v[j]);
             }
         }
 #pragma unroll
@@ -318,6 +297,22 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) {
         load(kb, t);
         compute(kb, t);
+    }
+    if (__builtin_expect(__any(spoilt != 0), 0)) {
+        for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) {
+            if (!cut(kb)) continue;
+            for (int key = kb; key < kb + 32 && key < k1; ++key) {
+                const int page = a.batch.page(s, key >> a.batch.page_shift);
+                if (page < 0 || key > pos || key < row_lo) continue;
+                const half_t *vr = a.v + page * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D + 4 * E * g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const auto v = taken<E>(*reinterpret_cast<const typename KvTile<D>::ve *>(vr + E * i));
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e][i] += static_cast<float>(v[e]);
+                }
+            }
+        }
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -347,11 +342,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     }
     const int rr = at * ROWS + (r < n_rows ? r : n_rows - 1), rtok = rr / a.gqa, rhead = kh * a.gqa + rr - rtok * a.gqa;
     const int64_t trow = static_cast<int64_t>(first + rtok) * a.heads + rhead;
-    bool nan = false;
-#pragma unroll
-    for (int e = 0; e < E; ++e) nan |= num[e] != num[e];
-    const uint64_t redo = __ballot(nan && r < n_rows);
-    if (r < n_rows && (redo >> (lane & 48) & 0xffff) == 0) {
+    if (r < n_rows) {
         if (span.n > 1) {
             float *pr = a.part + (trow * a.nsplit + c) * (D + 4);
 #pragma unroll
@@ -369,9 +360,6 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             *reinterpret_cast<typename KvTile<D>::ve *>(a.out + trow * D + E * l16) = y;
         }
     }
-    if (redo == 0) return;
-    for (int i = 0; i < 4; ++i)
-        if (redo >> (16 * i) & 0xffff) store_alone<D>(a, s, kh, first, ctx - n_new, at * ROWS + 4 * w + i, k0, k1, span.n, c);
 }
 
 // ---------------------------------------------------------------- chunks: 128 rows a tile
@@ -392,7 +380,7 @@ template <int D>
 struct ChunkLds {
     static constexpr int KT = 64, KP = D + 8;  // keys a tile; elements from key row to key row
     half_t k[2][KT * KP], v[2][D * KT];
-    int ok[2][4];
+    int ok[2][4], spoilt[4];
 };
 
 template <int D>
@@ -414,8 +402,10 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     const int r0 = at * ROWS, n_rows = n_new * a.gqa - r0 < ROWS ? n_new * a.gqa - r0 : ROWS;
     int k0, k1;
     span.chunk_keys(a, c, k0, k1);
+    // all of the tile's rows see the keys from `from` to `upto`
+    const int upto = pos0 + r0 / a.gqa, from = a.window > 0 ? pos0 + (r0 + n_rows - 1) / a.gqa - a.window + 1 : 0;
     {
-        const int top = pos0 + (r0 + n_rows - 1) / a.gqa + 1, bottom = a.window > 0 ? pos0 + r0 / a.gqa - a.window + 1 : 0;
+        const int top = pos0 + (r0 + n_rows - 1) / a.gqa + 1, bottom = a.window > 0 ? upto - a.window + 1 : 0;
         if (k1 > top) k1 = top;
         if (k0 < bottom) k0 = bottom & ~(KT - 1);
     }
@@ -440,6 +430,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     half8_t gk[KL];
     ve gv[4];
     bool g_ok = false;
+    uint32_t spoilt = 0;
     const int krow = lane / KCH, kch = lane % KCH, a4 = lane >> 4, db = lane & 15;
     const int32_t *table = a.batch.table + static_cast<int64_t>(s) * a.batch.max_pages;
     auto id_of = [&](int kb) {
@@ -464,10 +455,12 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
             const int r = 16 * w + krow + i * (64 / KCH);
             *reinterpret_cast<half8_t *>(&sk[buf][r * KP + kch * 8]) = gk[i];
         }
-        if (!g_ok || kb + 16 * w + 16 > k1) {  // slots that hold no position: 0 times what is there may be NaN
+        if (!g_ok || kb + KT > k1 || kb < from || kb + KT - 1 > upto) {  // slots that hold no position: 0 times what is there may be NaN
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (!g_ok || kb + 16 * w + 4 * a4 + j >= k1) gv[j] = ve{};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) spoilt |= take_out<E>(gv[j]);
         }
         const int kk = 16 * w + ((a4 & 1) << 3 | (a4 >> 1) << 2);
 #pragma unroll
@@ -583,17 +576,31 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
             if (kb < k1) turn(std::integral_constant<int, 1>{});
         }
     }
+    const int met = __any(spoilt != 0);
+    if (lane == 0) lds.spoilt[w] = met;
+    __syncthreads();
     if (wrows <= 0) return;
+    if (__builtin_expect(lds.spoilt[0] | lds.spoilt[1] | lds.spoilt[2] | lds.spoilt[3], 0)) {
+        for (int t0 = k0 & ~(KT - 1); t0 < k1; t0 += KT) {
+            if (t0 + KT <= k1 && t0 >= from && t0 + KT - 1 <= upto) continue;
+            for (int key = t0; key < t0 + KT && key < k1; ++key) {
+                const int page = a.batch.page(s, key >> a.batch.page_shift);
+                if (page < 0 || key > pos || key < row_lo) continue;
+                const half_t *vr = a.v + page * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D + 4 * g;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const half4_t v = taken<4>(*reinterpret_cast<const half4_t *>(vr + 32 * d + 2 * r));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[d][r + i] += static_cast<float>(v[i]);
+                    }
+            }
+        }
+    }
     l += __shfl_xor(l, 32, 64);
     const int64_t trow = static_cast<int64_t>(first + tok) * a.heads + head;
-    bool nan = false;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) nan |= o[d][r] != o[d][r];
-    const uint64_t bad = __ballot(nan && l32 < wrows);
-    const uint32_t redo = static_cast<uint32_t>(bad | bad >> 32);
-    if (l32 < wrows && !(redo >> l32 & 1)) {
+    if (l32 < wrows) {
         if (span.n > 1) {
             float *pr = a.part + (trow * a.nsplit + c) * (D + 4);
 #pragma unroll
@@ -618,9 +625,6 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
                 }
         }
     }
-    if (redo == 0) return;
-    for (int i = 0; i < wrows; ++i)
-        if (redo >> i & 1) store_alone<D>(a, s, kh, first, pos0, r0 + 32 * w + i, k0, k1, span.n, c);
 }
 
 // ---------------------------------------------------------------- the kernels
