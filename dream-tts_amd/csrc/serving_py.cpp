@@ -72,11 +72,17 @@ T *data(const Tensor *t) {
     return t ? static_cast<T *>(t->data_ptr()) : nullptr;
 }
 
-// [rows, heads, D] with contiguous rows: the elements between rows.
+// [rows, heads, D] with contiguous rows: the elements between rows. (Torch leaves any number as the stride of a size of 1.)
 int64_t rows_of(Args &a, const Tensor *t) {
-    if (!t || t->dim() != 3 || t->stride(2) != 1 || t->stride(1) != t->size(2)) return a.fail(), 0;
-    const int64_t row = t->size(1) * t->size(2);
-    return t->size(0) > 1 ? t->stride(0) : std::max(t->stride(0), row);
+    if (!t || t->dim() != 3 || t->stride(2) != 1 || (t->stride(1) != t->size(2) && t->size(1) != 1)) return a.fail(), 0;
+    return t->size(0) > 1 ? t->stride(0) : t->size(1) * t->size(2);
+}
+
+// [n_pages, n_kv, page, D] with contiguous pages: the elements between them.
+int64_t page_stride_of(Args &a, const Tensor *t) {
+    const int64_t rows = t->size(2) * t->size(3);
+    if (t->stride(3) != 1 || t->stride(2) != t->size(3) || (t->stride(1) != rows && t->size(1) != 1)) return a.fail(), 0;
+    return t->size(0) > 1 ? t->stride(0) : t->size(1) * rows;
 }
 
 struct Paged {
@@ -86,12 +92,12 @@ struct Paged {
         : k(a.tensor(i)), v(a.tensor(i + 1)), start(a.tensor(i + 2, at::kInt)), context(a.tensor(i + 3, at::kInt)),
           table(a.tensor(i + 4, at::kInt)) {
         a.need(a.ok && k->dim() == 4 && k->scalar_type() == at::kHalf && v->scalar_type() == at::kHalf && k->sizes() == v->sizes() &&
-               k->strides() == v->strides() && table->dim() == 2);
+               table->dim() == 2);
         if (!a.ok) return;
         n_pages = k->size(0), n_kv = k->size(1), page = k->size(2), hd = k->size(3);
         b = table->size(0), max_pages = table->size(1);
-        a.need(k->stride(3) == 1 && k->stride(2) == hd && k->stride(1) == page * hd && context->numel() == b && start->numel() == b + 1);
-        stride = n_pages > 1 ? k->stride(0) : std::max(k->stride(0), n_kv * page * hd);
+        stride = page_stride_of(a, k);
+        a.need(page_stride_of(a, v) == stride && context->numel() == b && start->numel() == b + 1);
     }
 };
 

@@ -87,11 +87,12 @@ def _tables(name, device, cos, sin):
 
 
 def _rows(name, t, what):
-    """[rows, heads, D] with contiguous rows: its sizes, and the elements between rows."""
+    """[rows, heads, D] with contiguous rows: its sizes, and the elements between rows. The stride of a size of 1 is no
+    one's: torch leaves any number there, also after contiguous()."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or stride[2] != 1 or stride[1] != shape[2]:
+    if len(shape) != 3 or stride[2] != 1 or (stride[1] != shape[2] and shape[1] != 1):
         raise DttsError(f"{name}: {what} must be [rows, heads, D] with contiguous rows, got {tuple(shape)} {stride}")
-    return shape, stride[0] if shape[0] > 1 else max(stride[0], shape[1] * shape[2])
+    return shape, stride[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
 def rotary(x, cos, sin, pos, interleaved=False, out=None):
@@ -129,6 +130,14 @@ def rotary(x, cos, sin, pos, interleaved=False, out=None):
 
 # ---------------------------------------------------------------- the paged cache
 
+def _page_stride(name, t):
+    """The elements between the pages of [n_pages, n_kv, page, D], each of them contiguous."""
+    (n_pages, n_kv, page, hd), st = t.shape, t.stride()
+    if st[3] != 1 or st[2] != hd or (st[1] != page * hd and n_kv != 1):
+        raise DttsError(f"{name}: a page must be contiguous, got strides {st}")
+    return st[0] if n_pages > 1 else n_kv * page * hd
+
+
 def _paged(name, device, k_pages, v_pages, q_start, context, pages):
     """Checks the cache [n_pages, n_kv, page, D] (each page contiguous) and the batch's arrays: b, n_kv, D,
     page, n_pages, max_pages and the elements between pages."""
@@ -143,16 +152,17 @@ def _paged(name, device, k_pages, v_pages, q_start, context, pages):
     if tensors is not None:
         for t, what, dtype in zip(tensors, ("k_pages", "v_pages", "q_start", "context", "pages"), (_F16, _F16, _I32, _I32, _I32)):
             _need(name, device, what, t, (dtype,), contiguous=dtype is _I32)
-    shape, st = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or shape != v_pages.shape or st != v_pages.stride():
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape:
         raise DttsError(f"{name}: k pages {tuple(shape)} and v pages {tuple(v_pages.shape)}")
+    stride = _page_stride(name, k_pages)
+    if stride != _page_stride(name, v_pages):
+        raise DttsError(f"{name}: k pages {k_pages.stride()} and v pages {v_pages.stride()} apart")
     n_pages, n_kv, page, hd = shape
-    if st[3] != 1 or st[2] != hd or st[1] != page * hd:
-        raise DttsError(f"{name}: a page must be contiguous, got strides {st}")
     table = pages.shape
     if len(table) != 2 or table[0] != context.numel() or q_start.numel() != table[0] + 1:
         raise DttsError(f"{name}: page table {tuple(table)}, {context.numel()} contexts, {q_start.numel()} starts")
-    return table[0], n_kv, hd, page, n_pages, table[1], st[0] if n_pages > 1 else max(st[0], n_kv * page * hd)
+    return table[0], n_kv, hd, page, n_pages, table[1], stride
 
 
 def _out(name, device, out, like, tokens, heads, hd):

@@ -1,0 +1,72 @@
+"""Calls of dtts.serving that the documentation allows and a tensor's form makes unusual; through the binding and through
+Python alone."""
+import pytest
+import torch
+
+from dtts import serving
+
+import _serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["binding", "python"])
+def path(request, monkeypatch):
+    if request.param == "python":
+        for name in ("rotary", "qk_rope_append_paged", "paged_attention", "sample"):
+            monkeypatch.setattr(serving._serving, name, lambda *args: None)
+
+
+def _odd_strides(t, dim):
+    """t with another number as the stride of its size of 1 at `dim`, as transposes and slices leave it."""
+    stride = list(t.stride())
+    stride[dim] = 24
+    y = t.as_strided(t.shape, stride)
+    assert y.is_contiguous() and y.stride() != t.stride()
+    return y
+
+
+def test_the_stride_of_a_size_of_one_is_no_ones(dev, path):
+    """One head, one kv head, one row, one page: contiguous tensors, whatever torch has as that stride."""
+    g = torch.Generator().manual_seed(2)
+    b = ref.Batch([3, 1], [40, 90], 1, 64, 16, dev)
+    k, v, *rest = b.device()
+    q = torch.randn((b.tokens, 1, 64), generator=g).half().to(dev)
+    want = serving.paged_attention(q, k, v, *rest, 3, 90, 0.1)
+    assert torch.equal(serving.paged_attention(_odd_strides(q, 1), _odd_strides(k, 1), _odd_strides(v, 1), *rest, 3, 90, 0.1), want)
+    assert torch.equal(serving.paged_attention(q, _odd_strides(k, 1), v, *rest, 3, 90, 0.1), want)  # k's and v's need not agree
+    one = ref.Batch([1], [10], 2, 64, 16, dev, spare=0)
+    k, v, *rest = one.device()
+    q = torch.randn((1, 4, 64), generator=g).half().to(dev)
+    want = serving.paged_attention(q, k, v, *rest, 1, 10, 0.1)
+    assert k.shape[0] == 1 and torch.equal(serving.paged_attention(_odd_strides(q, 0), _odd_strides(k, 0), v, *rest, 1, 10, 0.1), want)
+
+    cos, sin = (torch.from_numpy(t).to(dev) for t in serving.rope_table_scaled(128, 64, 1e4))
+    for shape, dim in (((5, 1, 64), 1), ((1, 4, 64), 0)):
+        x, pos = torch.randn(shape, generator=g).to(dev), torch.arange(shape[0], dtype=torch.int32, device=dev) + 7
+        want = serving.rotary(x, cos, sin, pos)
+        assert torch.equal(serving.rotary(_odd_strides(x, dim), cos, sin, pos), want)
+        out = _odd_strides(torch.zeros_like(x), dim)
+        assert torch.equal(serving.rotary(x, cos, sin, pos, out=out), want)
+        y = _odd_strides(x.clone(), dim)
+        assert torch.equal(serving.rotary(y, cos, sin, pos, out=y), want)
+
+    qkv = torch.randn((b.tokens, 3 * 64), generator=g).to(dev)
+    caches = []
+    for odd in (False, True):
+        k, v, *rest = b.device()
+        q = serving.qk_rope_append_paged(qkv, cos, sin, *((_odd_strides(t, 1) if odd else t) for t in (k, v)), *rest, 1)
+        caches.append((q, k.nan_to_num(9.0), v.nan_to_num(9.0)))
+    assert all(torch.equal(x, y) for x, y in zip(*caches))
+
+
+def test_a_cache_laid_out_position_by_position_of_one_kv_head(dev, path):
+    """[n_pages, page, n_kv, D] turned into the pages' order: with one kv head contiguous() leaves it as it is."""
+    b = ref.Batch([1, 2], [40, 70], 1, 128, 32, dev)
+    k, v, *rest = b.device()
+    q = torch.randn((b.tokens, 2, 128), generator=torch.Generator().manual_seed(1)).half().to(dev)
+    want = serving.paged_attention(q, k, v, *rest, 2, 70, 0.1)
+    turned = [torch.empty((t.shape[0], 32, 1, 128), dtype=t.dtype, device=dev).copy_(t.transpose(1, 2)).transpose(1, 2).contiguous()
+              for t in (k, v)]
+    assert turned[0].stride() != k.stride()
+    assert torch.equal(serving.paged_attention(q, *turned, *rest, 2, 70, 0.1), want)
