@@ -26,10 +26,10 @@ struct AttnArgs {
     PagedBatch batch;
     const half_t *q, *k, *v;
     half_t *out;
-    float *part;       // per (row, chunk): D weighted sums, the weight sum, the maximum (log2)
+    float *part;       // per (row, chunk): D weighted sums, the weight sum, the maximum of q . k
     int64_t q_stride;  // elements between tokens
     int heads, n_kv, gqa, window;
-    float scale2;      // |scale| * log2(e), above 0: the softmax runs in base 2
+    float scale2;      // |scale| * log2(e), above 0: the softmax runs in base 2, its maxima are those of q . k
     bool negate;       // scale < 0: the queries change sign
     int chunk, nsplit; // keys per chunk, chunks at most (the last takes what is left)
     int64_t few;       // sequences of at most this many rows go to the 16-row tiles
@@ -106,6 +106,16 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // 2^kSlack times 2^kChunkBias (their maximum may lag behind by that): both under f16's 65504. kSlack 1 / 4 / 8 (and a
 // bias that goes with it): 2048 tokens after 7952 335 / 333 / 335 us.
 constexpr float kBias = 15.0f, kSlack = 4.0f, kChunkBias = 11.0f;
+// A weight's exponent is fma(q . k, scale2, -m2), m2 the rounded product of the maximum: off by half of m2's last place,
+// alike for all keys of a row, so that it cancels as a bias does. At 2^20 that is 1/16; scores past it are taken relative to
+// their maximum first (another instruction a score), which no size of theirs overflows.
+constexpr float kFar = 1048576.0f;
+// m2 for a new maximum m, less the bias; far: sticky, whether any lane's scores are that large.
+__device__ __forceinline__ float relative_to(float m, float scale2, float bias, bool &far) {
+    const float m2 = m == -INFINITY ? 0.0f : m * scale2;
+    far = far || __any(fabsf(m2) >= kFar);
+    return (far ? 0.0f : m2) - bias;
+}
 
 // A value that is not finite (an overflow of the projection, a slot written over) makes 0 times it a NaN, so in a tile of
 // keys that not all of the rows see it may not reach the product: there such values count as 0 (take_out says whether it
@@ -229,7 +239,8 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
         for (int j = 0; j < 8; ++j)
             t.v[j] = *reinterpret_cast<const typename KvTile<D>::ve *>(a.v + base[j >> 2] + (4 * g + (j & 3)) * D + E * l16);
     };
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, m2 = 0.0f, l = 0.0f;  // m2: what the weights are relative to in log2, anything while there is no m
+    bool far = false;
     uint32_t spoilt = 0;
     float4_t o[E];
 #pragma unroll
@@ -249,18 +260,23 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             for (int i = 0; i < 4; ++i) {
                 const int key = kb + 16 * u + 4 * g + i;
                 const bool seen = key <= pos && key >= row_lo && key < k1 && (t.ok >> u & 1);
-                sc[u][i] = seen ? sc[u][i] * a.scale2 : -INFINITY;
+                sc[u][i] = seen ? sc[u][i] : -INFINITY;
                 mx = fmaxf(mx, sc[u][i]);
             }
         // the row's other keys are 16 and 32 lanes away
         mx = max_16_32_apart(mx);
-        const float mu = mx == -INFINITY ? 0.0f : mx;
         if (__any(mx > m)) {
-            const float f = exp2_fast(m - mu);
+            const float f = exp2_fast(mx == -INFINITY ? 0.0f : (m - mx) * a.scale2);
             l *= f;
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] *= f;
             m = mx;
+            m2 = relative_to(m, a.scale2, kBias, far);
+        }
+        if (far) {
+            const float from_m = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sc[u] -= from_m;
         }
         half8_t p;
         float sum = 0.0f;
@@ -268,7 +284,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float x = exp2_fast(sc[u][i] - mu + kBias);
+                const float x = exp2_fast(__builtin_fmaf(sc[u][i], a.scale2, -m2));
                 sum += x;
                 p[4 * u + i] = static_cast<half_t>(x);
             }
@@ -335,7 +351,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     const float mu = mt == -INFINITY ? 0.0f : mt;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const float f = exp2_fast(sm_m[u][r] - mu);
+        const float f = exp2_fast((sm_m[u][r] - mu) * a.scale2);
         den += sm_l[u][r] * f;
 #pragma unroll
         for (int e = 0; e < E; ++e) num[e] += sm_o[u][r][E * l16 + e] * f;
@@ -350,7 +366,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
                 *reinterpret_cast<float4_t *>(pr + E * l16 + e) = float4_t{num[e], num[e + 1], num[e + 2], num[e + 3]};
             if (l16 == 0) {
                 pr[D] = den;
-                pr[D + 1] = mt - kBias;  // a state's weights are relative to what it holds as its maximum
+                pr[D + 1] = mt;
             }
         } else {
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // a row that sees no key is zero
@@ -472,6 +488,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
         if (lane == 0) s_ok[buf][w] = g_ok;
     };
     float m = -INFINITY, m2 = 0.0f, l = 0.0f;  // m2: what the weights are relative to in log2, anything while there is no m
+    bool far = false;
     float16_t o[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -531,7 +548,14 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= f;
             m = mx;
-            m2 = (m == -INFINITY ? 0.0f : m * a.scale2) - kChunkBias;
+            m2 = relative_to(m, a.scale2, kChunkBias, far);
+        }
+        if (far) {
+            const float from_m = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[u][r] -= from_m;
         }
         half8_t pf[4];
         // the other workgroup's wave on this SIMD yields here, so that the two take turns between products and
@@ -610,7 +634,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
                     *reinterpret_cast<float4_t *>(pr + 32 * d + 2 * r + 4 * g) = float4_t{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
             if (g == 0) {
                 pr[D] = l;
-                pr[D + 1] = m == -INFINITY ? m : m2;
+                pr[D + 1] = m;
             }
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees no key is zero
@@ -652,7 +676,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_mixed(AttnArgs a, int large
 
 // ---------------------------------------------------------------- the chunks' states
 
-// Join a row's chunks: out = sum_c num_c 2^(m_c - M) / sum_c den_c 2^(m_c - M), M the largest m_c.
+// Join a row's chunks: out = sum_c num_c w_c / sum_c den_c w_c, w_c = 2^((m_c - M) scale2), M the largest m_c.
 constexpr int kFewChunks = 8;
 
 // Up to kFewChunks: a wave for R heads of a token, which share its lookups, everything requested at once. 862 tokens of
@@ -694,7 +718,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
 #pragma unroll
         for (int c = 0; c < kFewChunks; ++c)
             if (c < n) {
-                const float f = exp2_fast(mc[r][c] - mu);
+                const float f = exp2_fast((mc[r][c] - mu) * a.scale2);
                 den += lc[r][c] * f;
 #pragma unroll
                 for (int e = 0; e < PER; ++e) num[e] += v[r][c][e] * f;
@@ -731,7 +755,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
         mx = fmaxf(mx, m);
-        const float mu = mx == -INFINITY ? 0.0f : mx, back = exp2_fast(m - mu), f = exp2_fast(mc - mu);
+        const float mu = mx == -INFINITY ? 0.0f : mx, back = exp2_fast((m - mu) * a.scale2), f = exp2_fast((mc - mu) * a.scale2);
         float dl = lc * f;
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) dl += __shfl_xor(dl, off, 64);
@@ -768,13 +792,13 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     float mx = m;
 #pragma unroll
     for (int u = 1; u < W; ++u) mx = fmaxf(mx, sm[u][D + 1]);
-    const float mu = mx == -INFINITY ? 0.0f : mx, f0 = exp2_fast(m - mu);
+    const float mu = mx == -INFINITY ? 0.0f : mx, f0 = exp2_fast((m - mu) * a.scale2);
     den *= f0;
 #pragma unroll
     for (int e = 0; e < PER; ++e) num[e] *= f0;
 #pragma unroll
     for (int u = 1; u < W; ++u) {
-        const float f = exp2_fast(sm[u][D + 1] - mu);
+        const float f = exp2_fast((sm[u][D + 1] - mu) * a.scale2);
         den += sm[u][D] * f;
 #pragma unroll
         for (int e = 0; e < PER; ++e) num[e] += sm[u][lane * PER + e] * f;

@@ -87,3 +87,38 @@ def test_a_row_of_hundreds_of_chunks(dev, n, hd, heads):
             scores[at] = 12.0
             got, want, mag = _run(dev, scores, values, 1, heads, 1, hd, True)
             _check(got, want, mag, n, SMALL[True])
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("q_len,heads,n_kv,hd,n", [(1, 2, 1, 128, 300), (7, 4, 2, 64, 900), (100, 2, 1, 128, 300), (200, 2, 2, 64, 1200)])
+@pytest.mark.parametrize("scale", [0.3, 1.0, 30.0, -30.0, 1e3, 1e9, 1e20, -1e32, 2e38])
+def test_scores_of_any_size(dev, scale, q_len, heads, n_kv, hd, n, workspace):
+    """Scores of whole numbers times 2^9 times the scale, up to past f32's range: a token has the value of its largest one, or
+    the mean of those that share it."""
+    rng = np.random.RandomState(7)
+    pages = -(-n // PAGE)
+    # q . k = 2^9 (64 a + b), a and b whole: exact in f32, and any two are equal or 2^9 apart at least
+    a, b = rng.randint(-500, 501, (pages * PAGE, n_kv)), rng.randint(-200, 201, (pages * PAGE, n_kv))
+    if n == 900:
+        b[:] = 0  # many keys share a score
+        a = a // 100 * 100
+    k = torch.zeros((pages * PAGE, n_kv, hd), dtype=torch.float16)
+    k[:, :, 5], k[:, :, hd - 1] = torch.from_numpy(a).half(), torch.from_numpy(b).half()
+    v = torch.randn((pages * PAGE, n_kv, hd), generator=torch.Generator().manual_seed(5)).half()
+    paged = [t.view(pages, PAGE, n_kv, hd).transpose(1, 2).contiguous().to(dev) for t in (k, v)]
+    q = torch.zeros((q_len, heads, hd), dtype=torch.float16, device=dev)
+    q[..., 5], q[..., hd - 1] = 2.0 ** 15, 2.0 ** 9
+    score = (64 * a + b).astype(np.int64)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    ws = None if workspace else torch.empty(0, dtype=torch.uint8, device=dev)
+    got = serving.paged_attention(q, *paged, i32([0, q_len]), i32([n]), torch.arange(pages, dtype=torch.int32, device=dev)[None].contiguous(),
+                                  q_len, n, scale, workspace=ws).cpu().double()
+    for t in range(q_len):
+        for h in range(heads):
+            s = score[:n - q_len + t + 1, h // (heads // n_kv)] * (1 if scale > 0 else -1)
+            best = torch.from_numpy(np.flatnonzero(s == s.max()))
+            x = v[best, h // (heads // n_kv)].double()
+            # the next score is 2^9 times 0.3 below at least: its weight is under e^-150 of the largest. f16: equal weights round
+            # alike (numerator 2^-11 against the unrounded sum), the output 2^-11; a few f32 steps
+            tol = (2 * 2.0 ** -11 + 2.0 ** -18) * x.abs().mean(0) + 2.0 ** -25
+            assert bool(((got[t, h] - x.mean(0)).abs() <= tol).all()), (t, h, len(best), float((got[t, h] - x.mean(0)).abs().max()))
