@@ -39,6 +39,34 @@ void clear_error();
 
 inline bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// n rows of `width` bytes, `stride` bytes (at least the width) apart.
+struct ByteRows {
+    const void *p;
+    int64_t n, stride, width;
+};
+
+// Whether a row of x and a row of y have a byte in common.
+inline bool share_bytes(const ByteRows &x, const ByteRows &y) {
+    typedef __int128 wide;  // strides may be any numbers
+    const wide d = static_cast<wide>(reinterpret_cast<uintptr_t>(y.p)) - static_cast<wide>(reinterpret_cast<uintptr_t>(x.p));
+    if (x.n < 1 || y.n < 1 || d >= static_cast<wide>(x.n - 1) * x.stride + x.width ||
+        d + static_cast<wide>(y.n - 1) * y.stride + y.width <= 0)
+        return false;
+    if (x.n == 1) return y.n == 1 || share_bytes(y, x);
+    // x's rows t strides on, first <= t <= last, and y.width bytes from `at` on: of the rows that start before those end,
+    // the last reaches furthest
+    const auto meets = [&](wide at, wide first, wide last) {
+        const wide end = at + y.width - 1;
+        wide t = end >= 0 ? end / x.stride : -((x.stride - 1 - end) / x.stride);
+        t = t < last ? t : last;
+        return t >= first && at < t * x.stride + x.width;
+    };
+    if (y.n == 1 || x.stride == y.stride) return meets(d, 1 - y.n, x.n - 1);
+    for (int64_t j = 0; j < y.n; ++j)
+        if (meets(d + static_cast<wide>(j) * y.stride, 0, x.n - 1)) return true;
+    return false;
+}
+
 // ---------------------------------------------------------------- f16
 
 typedef _Float16 half_t;

@@ -172,10 +172,14 @@ int append(const char *name, const T *qkv, const float *norms, const float *cos_
     DTTS_REQUIRE(aligned(qkv, 4 * sizeof(T)) && aligned(cos_t, 16) && aligned(sin_t, 16) && aligned(q_out, 8) && aligned(kp, 8) &&
                      aligned(vp, 8) && aligned(norms, 16) && aligned(q_start, 4) && aligned(context, 4) && aligned(page_table, 4),
                  "%s: misaligned operand", name);
-    DTTS_REQUIRE(static_cast<const void *>(qkv) != q_out, "%s: the queries may not replace qkv", name);
+    const int64_t per = heads + 2 * n_kv, f16 = sizeof(half_t), page_bytes = n_kv * page * hd * f16;
+    DTTS_REQUIRE(!share_bytes({qkv, 1, 0, tokens * per * hd * static_cast<int64_t>(sizeof(T))}, {q_out, 1, 0, tokens * heads * hd * f16}),
+                 "%s: the queries may not replace qkv, nor a part of it", name);
+    DTTS_REQUIRE(!share_bytes({kp, n_pages, page_stride * f16, page_bytes}, {vp, n_pages, page_stride * f16, page_bytes}),
+                 "%s: pages of keys and of values share memory", name);
     // Steps of RW head rows a token has, shared by enough waves to fill the chip (kFillWaves, 16 a CU): few tokens
     // spread over many, each with one step; many tokens have a wave each.
-    const int64_t per = heads + 2 * n_kv, rw = 64 / (hd / 8), steps = (per + rw - 1) / rw;
+    const int64_t rw = 64 / (hd / 8), steps = (per + rw - 1) / rw;
     int64_t parts = (kFillWaves + tokens - 1) / tokens;
     if (parts > steps) parts = steps;
     DTTS_REQUIRE(tokens * parts < (int64_t(1) << 31), "%s: too many rows", name);

@@ -920,10 +920,13 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
     DTTS_REQUIRE(aligned(q, 16) && aligned(kpages, 16) && aligned(vpages, 16) && aligned(out, 16) && aligned(q_start, 4) &&
                      aligned(context, 4) && aligned(page_table, 4),
                  "%s: misaligned operand", name);
-    DTTS_REQUIRE(out != q, "%s: the output may not be the queries", name);
     DTTS_REQUIRE(std::isfinite(scale * kLog2e), "%s: scale %g", name, static_cast<double>(scale));
     Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window);
     DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large) * n_kv < (int64_t(1) << 24), "%s: too many rows", name);
+    const int64_t row = heads * head_dim * static_cast<int64_t>(sizeof(half_t));
+    DTTS_REQUIRE(q_stride < (int64_t(1) << 62), "%s: q_stride %lld", name, (long long)q_stride);
+    DTTS_REQUIRE(!share_bytes({q, tokens, q_stride * static_cast<int64_t>(sizeof(half_t)), row}, {out, 1, 0, tokens * row}),
+                 "%s: the output may not be the queries, nor a part of their memory", name);
     AttnArgs a;
     a.batch = PagedBatch{q_start, context, page_table, static_cast<int>(tokens), static_cast<int>(b), log2_of(page),
                          static_cast<int>(n_pages), static_cast<int>(max_pages), page_stride};

@@ -114,6 +114,10 @@ int rotary(const char *name, const T *x, const float *cos_t, const float *sin_t,
     DTTS_REQUIRE(rows < (int64_t(1) << 31) && heads * per_head < (int64_t(1) << 31), "%s: too many rows", name);
     const int64_t units = rows * heads * per_head;
     DTTS_REQUIRE(units < (int64_t(1) << 31), "%s: too many rows", name);
+    DTTS_REQUIRE(xs < (int64_t(1) << 60) && ys < (int64_t(1) << 60), "%s: row strides %lld, %lld", name, (long long)xs, (long long)ys);
+    const int64_t of = sizeof(T);
+    DTTS_REQUIRE(x == y || !share_bytes({x, rows, xs * of, heads * hd * of}, {y, rows, ys * of, heads * hd * of}),
+                 "%s: the output shares memory with x without being x", name);
     RotaryArgs a;
     a.cos_t = cos_t;
     a.sin_t = sin_t;

@@ -99,7 +99,7 @@ def rotary(x, cos, sin, pos, interleaved=False, out=None):
     """x [rows, heads, D] (f32 or f16; rows may be strided, as a slice of qkv is) with the first
     2 * cos.shape[1] dimensions of each head turned by its row's position pos [rows] int32 (device). A
     position outside the tables is padding: that row of `out` is left as it was (of a new one: unset).
-    out may be x."""
+    out may be x, and otherwise shares no memory with it."""
     y = _serving.rotary(x, cos, sin, pos, interleaved, out)
     if y is not None:
         return y
@@ -193,7 +193,7 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
     values: qkv [tokens, (heads + 2 n_kv) D] f32 or f16 -> queries [tokens, heads, D] f16; k_pages and
     v_pages [n_pages, n_kv, page, D] f16 are written in place. q_start [b + 1], context [b] (new tokens
     included) and pages [b, max_pages] are int32; see dtts.h for what each selects. Rows of `out` that
-    belong to no sequence are left as they were."""
+    belong to no sequence are left as they were. `out` is no part of qkv, and the pages share no memory."""
     y = _serving.qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, pages, heads, norms, eps, interleaved, out)
     if y is not None:
         return y
@@ -237,7 +237,7 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
     up to its own, the last `window` of them when set. max_q and max_context (the longest chunk and context)
     size the launch and never change what is computed. `workspace`: a device byte tensor of
     paged_attention_workspace_bytes (allocated when not given). Rows of `out` that belong to no sequence are
-    left as they were; a token that sees no position gets zeros."""
+    left as they were; a token that sees no position gets zeros. `out` shares no memory with q."""
     y = _serving.paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale, window, out, workspace)
     if y is not None:
         return y

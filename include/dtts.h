@@ -461,7 +461,7 @@ int dtts_rope_table_scaled_f32(int64_t len, int64_t rot_dim, double base, int32_
  * outside [0, table_len) is padding: its y is left as it was. cos / sin [table_len, rot_dim / 2].
  * x_stride and y_stride: elements from row to row (>= heads * D), so the queries or keys inside a qkv
  * tensor can be turned where they are; x == y (in place, equal strides) is allowed, any other overlap
- * is not. Any even rot_dim <= D; interleaved pairs need an even D, even strides and pair-aligned
+ * is refused. Any even rot_dim <= D; interleaved pairs need an even D, even strides and pair-aligned
  * addresses. Fastest when D, rot_dim, strides and addresses are multiples of 16 bytes (rot_dim: 32
  * half-split). */
 #define DTTS_ROPE_HALF 0
@@ -486,8 +486,8 @@ int dtts_rotary_f16(const dtts_f16 *x, const float *cos_t, const float *sin_t, c
  *
  * dtts_qk_rope_append_paged_*: QK-norm (norms [2, D] f32, q's weight then k's, or NULL for none),
  * rotary positions and the write of the new keys and values. qkv [tokens, (heads + 2 n_kv) * D] (q
- * heads, then k, then v); q_out [tokens, heads, D] f16, no part of qkv; k and v go to the pages. f32 arithmetic, one
- * rounding to f16. rot_dim a multiple of 8. A token whose position is outside [0, table_len) or has no
+ * heads, then k, then v); q_out [tokens, heads, D] f16, no part of qkv; k and v go to the pages, which
+ * share no memory. f32 arithmetic, one rounding to f16. rot_dim a multiple of 8. A token whose position is outside [0, table_len) or has no
  * page is left out whole: its q_out row and every page stay as they were. */
 int dtts_qk_rope_append_paged_f32(const float *qkv, const float *norms, const float *cos_t, const float *sin_t,
                                   const int32_t *q_start, const int32_t *context, const int32_t *page_table,
@@ -506,7 +506,7 @@ int dtts_qk_rope_append_paged_f16(const dtts_f16 *qkv, const float *norms, const
  *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / (heads / n_kv)]) v[j, ..]
  * over positions max(0, p - window + 1) <= j <= p of the token's sequence, p its position (window 0: all of
  * them). q [tokens, heads, D] f16 with q_stride elements between tokens (a multiple of 8), out
- * [tokens, heads, D] f16, not q. heads is any multiple of n_kv. Scores, softmax state and sums in f32;
+ * [tokens, heads, D] f16, no part of q's rows. heads is any multiple of n_kv. Scores, softmax state and sums in f32;
  * the weights are rounded to f16 for the product with v (each off by 2^-11 of itself, or by 2^-36 of
  * the largest where that is more). A token that sees no position (p < 0, or no page of its window is
  * there) gets zeros. Positions without a page are not attended to, slots past a

@@ -3,7 +3,7 @@ Python alone."""
 import pytest
 import torch
 
-from dtts import serving
+from dtts import DttsError, serving
 
 import _serving_ref as ref
 
@@ -70,3 +70,38 @@ def test_a_cache_laid_out_position_by_position_of_one_kv_head(dev, path):
               for t in (k, v)]
     assert turned[0].stride() != k.stride()
     assert torch.equal(serving.paged_attention(q, *turned, *rest, 2, 70, 0.1), want)
+
+
+def test_outputs_between_the_rows_of_their_inputs(dev, path):
+    """Memory of the same tensor that is none of the input's: queries inside wider rows with the output in the gap, keys
+    turned into the values' place."""
+    b = ref.Batch([1, 1], [40, 70], 2, 64, 16, dev)
+    arrays = b.device()
+    g = torch.Generator().manual_seed(1)
+    wide = torch.randn((2, 12, 64), generator=g).half().to(dev)
+    want = serving.paged_attention(wide[:, :2].contiguous(), *arrays, 1, 70, 0.1)
+    out = wide.view(-1)[2 * 64:6 * 64].view(2, 2, 64)
+    assert torch.equal(serving.paged_attention(wide[:, :2], *arrays, 1, 70, 0.1, out=out), want)
+    cos, sin = (torch.from_numpy(t).to(dev) for t in serving.rope_table_scaled(64, 64, 1e4))
+    pos = torch.arange(2, dtype=torch.int32, device=dev) + 9
+    want = serving.rotary(wide[:, 6:8].contiguous(), cos, sin, pos)
+    assert torch.equal(serving.rotary(wide[:, 6:8], cos, sin, pos, out=wide[:, 10:]), want)
+    with pytest.raises(DttsError, match="shares memory"):
+        serving.rotary(wide[:, 6:8], cos, sin, pos, out=wide[:, 7:9])
+    with pytest.raises(DttsError, match="may not be the queries"):
+        serving.paged_attention(wide[:, :2], *arrays, 1, 70, 0.1, out=wide.view(-1)[64:5 * 64].view(2, 2, 64))
+
+
+def test_keys_and_values_side_by_side_in_one_pool(dev, path):
+    """Pages of keys and of values in turn; the same tensor for both is refused."""
+    b = ref.Batch([2, 1], [40, 70], 2, 64, 16, dev)
+    k, v, *rest = b.device()
+    pool = torch.stack([k, v], 1)
+    cos, sin = (torch.from_numpy(t).to(dev) for t in serving.rope_table_scaled(128, 64, 1e4))
+    qkv = torch.randn((b.tokens, 8 * 64), generator=torch.Generator().manual_seed(1)).half().to(dev)
+    want = serving.qk_rope_append_paged(qkv, cos, sin, k, v, *rest, 4)
+    got = serving.qk_rope_append_paged(qkv, cos, sin, pool[:, 0], pool[:, 1], *rest, 4)
+    assert torch.equal(got, want)
+    assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in ((pool[:, 0], k), (pool[:, 1], v)))
+    with pytest.raises(DttsError, match="share memory"):
+        serving.qk_rope_append_paged(qkv, cos, sin, k, k, *rest, 4)
