@@ -10,12 +10,15 @@ Every tensor of a call is on one device; the work goes to that device's current 
 
 A right call on the current device is checked and enqueued by ``_serving`` (csrc/serving_py.cpp), since
 reading ten tensors' sizes and addresses in Python takes longer than the work. It returns None for any
-other, and the Python below makes the call or says what is wrong with it.
+other, and the Python below makes the call or says what is wrong with it. Where the binding was built
+for another torch, Python makes all of them (and a warning says so).
 """
 from __future__ import annotations
 
 import ctypes
 import functools
+import types
+import warnings
 
 import torch
 
@@ -24,7 +27,10 @@ from ._lib import DttsError, call, lib
 try:
     from . import _serving
 except ImportError as e:
-    raise DttsError(f"dtts/_serving.so is not built for this torch ({e}); run dream-tts_amd/build.py") from e
+    warnings.warn(f"dtts/_serving.so is not built for this torch ({e}): calls of dtts.serving take some microseconds longer; "
+                  "run dream-tts_amd/build.py", RuntimeWarning)
+    _serving = types.SimpleNamespace(**dict.fromkeys(("rotary", "qk_rope_append_paged", "paged_attention", "sample"),
+                                                     lambda *args: None))
 
 _F16, _F32, _I32 = torch.float16, torch.float32, torch.int32
 _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}

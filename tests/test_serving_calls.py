@@ -1,5 +1,8 @@
 """What dtts.serving checks on the host, beyond the refusals of each call."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -60,3 +63,28 @@ def test_rotary_refuses_an_output_partly_inside_x(y, ys):
     p, x = _at(1 << 16), 8192
     xs = 512 if ys != 512 else 2048 if y > 4000 else 512
     _refused("dtts_rotary_f32", "shares memory", _at(x), p, p, p, _at(x + y), 4, 2, 64, 64, 0, xs // 4, ys // 4, 16, None)
+
+
+def test_the_module_works_without_its_binding():
+    """A torch that the binding was not built for: a warning, and every call through Python."""
+    code = """
+import sys, warnings
+sys.modules["dtts._serving"] = None  # an import of it fails
+with warnings.catch_warnings(record=True) as met:
+    warnings.simplefilter("always")
+    from dtts import DttsError, serving
+assert len(met) == 1 and "_serving.so" in str(met[0].message), met
+import torch
+x, i = torch.zeros((2, 2, 64)), torch.zeros(2, dtype=torch.int32)
+for call in (lambda: serving.rotary(x, x[0], x[0], i), lambda: serving.sample(x[0], x[0, 0]),
+             lambda: serving.paged_attention(x.half(), x, x, i, i, i, 1, 1),
+             lambda: serving.qk_rope_append_paged(x[0], x[0], x[0], x, x, i, i, i, 1)):
+    try:
+        call()
+    except DttsError as e:
+        assert "on the device" in str(e), e
+    else:
+        raise AssertionError("taken")
+assert serving.rope_table_scaled(4, 8, 1e4)[0].shape == (4, 4)
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(serving.__file__)))
