@@ -1,9 +1,9 @@
 """Build libdtts.so (gfx950) in-tree with hipcc.
 
 Every ``csrc/*.hip`` compiles to an object under ``_build/`` (in parallel), then one shared
-library links at ``dream-tts_amd/libdtts.so``, and ``csrc/serving_py.cpp`` (host code against torch's
-and Python's headers) at ``dream-tts_amd/dtts/_serving.so``, which loads it. Run as ``python dream-tts_amd/build.py``; the
-repository's ``__graft_entry__.build()`` calls :func:`build`.
+library links at ``dream-tts_amd/libdtts.so``. Where torch, its headers, Python's and g++ are there, ``csrc/serving_py.cpp``
+is built against them at ``dream-tts_amd/dtts/_serving.so``, which loads the library; elsewhere ``dtts.serving`` does without.
+Run as ``python dream-tts_amd/build.py``; the repository's ``__graft_entry__.build()`` calls :func:`build`.
 """
 from __future__ import annotations
 
@@ -67,12 +67,29 @@ def build(jobs: int | None = None) -> str:
     return LIB
 
 
-def build_binding() -> str:
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+def _rocm_include() -> str:
+    """The headers beside the hipcc in use."""
+    return os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(shutil.which(HIPCC) or HIPCC))), "include")
+
+
+def build_binding() -> str | None:
+    """``dtts/_serving.so``, or None (and a line that says what is missing) where it cannot be built; a binding of another
+    build is not left in its place."""
+    spec, gxx = importlib.util.find_spec("torch"), shutil.which("g++")
+    python = sysconfig.get_paths()["include"]
+    torch = spec.submodule_search_locations[0] if spec else ""
+    missing = [what for what, there in (
+        ("torch", spec), ("a ROCm torch's headers", os.path.exists(os.path.join(torch, "include", "c10", "hip", "HIPFunctions.h"))),
+        ("Python.h", os.path.exists(os.path.join(python, "Python.h"))), ("g++", gxx)) if not there]
+    if missing:
+        if os.path.exists(BINDING):
+            os.remove(BINDING)
+        print(f"dtts/_serving.so is not built ({', '.join(missing)} not found): dtts.serving makes its calls from Python", file=sys.stderr)
+        return None
     tmp = BINDING + ".tmp"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",  # as torch was built
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",  # as torch was built
            "-isystem", os.path.join(torch, "include"), "-isystem", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
-           "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], "-I", os.path.join(REPO, "include"),
+           "-isystem", _rocm_include(), "-isystem", python, "-I", os.path.join(REPO, "include"),
            os.path.join(CSRC, "serving_py.cpp"), "-o", tmp,
            "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
            "-L" + HERE, "-l:libdtts.so", "-Wl,-rpath,$ORIGIN/.."]
