@@ -48,24 +48,18 @@ struct PagedBatch {
         return id >= 0 && id < n_pages ? id : -1;
     }
 
-    // The sequence that row t belongs to: how many of them end at or before it (b: none does). The
-    // wave reads 64 ends at a time and counts with ballots, one memory round trip for any b up to 64
-    // and b / 64 overlapping ones past it (a binary search takes log2 b dependent ones). Every lane of
-    // the wave calls it, each group of `group` lanes with its own t.
-    template <int GROUP>
+    // The sequence that the wave's row t belongs to: how many of them end at or before it (b: all of
+    // them). The wave reads 64 ends at a time and counts with ballots, one memory round trip for any b
+    // up to 64 and b / 64 overlapping ones past it (a binary search takes log2 b dependent ones). Every
+    // lane of the wave calls it.
     __device__ __forceinline__ int sequence_of(int t) const {
         const int lane = threadIdx.x & 63;
-        int mine = 0;
+        int ended = 0;
         for (int s0 = 0; s0 < b; s0 += 64) {
             const int end = s0 + lane < b ? q_start[s0 + lane + 1] : 0x7fffffff;
-#pragma unroll
-            for (int g = 0; g < 64 / GROUP; ++g) {
-                const int tg = __builtin_amdgcn_readlane(t, g * GROUP);
-                const int below = __popcll(__ballot(end <= tg));
-                if (lane / GROUP == g) mine += below;
-            }
+            ended += __popcll(__ballot(end <= t));
         }
-        return mine;
+        return ended;
     }
 };
 

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv,
     };
     int r0 = part * RW + lane / L;
     load(r0);
-    const int s = a.batch.sequence_of<64>(t);
+    const int s = a.batch.sequence_of(t);
     if (s >= a.batch.b) return;
     int first, n;
     a.batch.rows(s, first, n);

@@ -688,7 +688,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t trow = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * R, rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
     if (trow >= rows) return;
-    const int t = static_cast<int>(trow / a.heads), s = a.batch.sequence_of<64>(t);
+    const int t = static_cast<int>(trow / a.heads), s = a.batch.sequence_of(t);
     if (s >= a.batch.b) return;
     int first, n_new;
     a.batch.rows(s, first, n_new);
@@ -738,7 +738,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     __shared__ float sm[W][D + 2];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t trow = blockIdx.x;
-    const int t = static_cast<int>(trow / a.heads), s = a.batch.sequence_of<64>(t);
+    const int t = static_cast<int>(trow / a.heads), s = a.batch.sequence_of(t);
     if (s >= a.batch.b) return;
     int first, n_new;
     a.batch.rows(s, first, n_new);
