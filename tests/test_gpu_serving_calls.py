@@ -105,3 +105,34 @@ def test_keys_and_values_side_by_side_in_one_pool(dev, path):
     assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in ((pool[:, 0], k), (pool[:, 1], v)))
     with pytest.raises(DttsError, match="share memory"):
         serving.qk_rope_append_paged(qkv, cos, sin, k, k, *rest, 4)
+
+
+def test_starts_that_select_nothing_write_nothing(dev, path):
+    """Starts that fall, lie outside the batch or are all alike: rows of `out` and slots of the cache that no sequence of
+    theirs has stay as they were, bit for bit."""
+    heads, c = 2, [30, 40, 50]
+    b = ref.Batch([4, 3, 2], c, 2, 64, 16, dev, extra_tokens=2)
+    cos, sin = (torch.from_numpy(t).to(dev) for t in serving.rope_table_scaled(64, 64, 1e4))
+    qkv = torch.randn((b.tokens, (heads + 4) * 64), generator=torch.Generator().manual_seed(4)).half().to(dev)
+    for starts, rows in (([9, 4, 2, 0], []), ([5, 3, -9, -9], []), ([100, 200, 300, 400], []), ([-8, -8, -8, 0], []),
+                         ([11, 11, 11, 2 ** 31 - 1], []), ([6, 2, 2, 5], [2, 3, 4]), ([0, 0, 0, 3], [0, 1, 2]), ([3, 1, 4, 4], [1, 2, 3])):
+        k, v, _, ctx, table = b.device()
+        start = torch.tensor(starts, dtype=torch.int32, device=dev)
+        k0, v0 = k.clone(), v.clone()
+        out = torch.full((b.tokens, heads, 64), 9.0, dtype=torch.float16, device=dev)
+        serving.qk_rope_append_paged(qkv, cos, sin, k, v, start, ctx, table, heads, out=out)
+        assert bool((out[[t for t in range(b.tokens) if t not in rows]] == 9.0).all()), starts
+        # positions that the selected rows have: sequence s's last n, where its starts rise
+        slots = {(int(b.table[s, p // 16]), p % 16) for s in range(3) for p in range(max(0, c[s] - (starts[s + 1] - starts[s])), c[s])
+                 if 0 <= starts[s] < starts[s + 1] <= b.tokens}
+        kept = torch.ones(k.shape[0], 16, dtype=torch.bool)
+        for at in slots:
+            kept[at] = False
+        for x, y in ((k, k0), (v, v0)):
+            x, y = (t.transpose(1, 2)[kept.to(dev)] for t in (x, y))
+            assert torch.equal(x.view(torch.int16), y.view(torch.int16)), starts
+        out.fill_(9.0)
+        for max_q, workspace in ((4, None), (200, torch.empty(0, dtype=torch.uint8, device=dev))):
+            serving.paged_attention(qkv.view(b.tokens, heads + 4, 64)[:, :heads], k, v, start, ctx, table, max_q, 50, 0.1, out=out,
+                                    workspace=workspace)
+            assert bool((out[[t for t in range(b.tokens) if t not in rows]] == 9.0).all()), starts
