@@ -107,9 +107,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // bias that goes with it): 2048 tokens after 7952 335 / 333 / 335 us.
 constexpr float kBias = 15.0f, kSlack = 4.0f, kChunkBias = 11.0f;
 // A weight's exponent is fma(q . k, scale2, -m2), m2 the rounded product of the maximum: off by half of m2's last place,
-// alike for all keys of a row, so that it cancels as a bias does. At 2^20 that is 1/16; scores past it are taken relative to
-// their maximum first (another instruction a score), which no size of theirs overflows.
-constexpr float kFar = 1048576.0f;
+// alike for all keys that a wave takes relative to one maximum, so that it cancels among them as a bias does, but not
+// against what was summed relative to another. At 2^12 that is 2^-13, under the weights' own rounding; scores past it are
+// taken relative to their maximum first (another instruction a score), which no size of theirs overflows.
+constexpr float kFar = 4096.0f;
 // m2 for a new maximum m, less the bias; far: sticky, whether any lane's scores are that large.
 __device__ __forceinline__ float relative_to(float m, float scale2, float bias, bool &far) {
     const float m2 = m == -INFINITY ? 0.0f : m * scale2;
@@ -825,8 +826,9 @@ constexpr int64_t kFew = 32;
 // 1024 / 2048 / 4096: 48 tokens over up to 1536 keys each 40 / 35 / 36 / 37 us, 5 over 65000 82 / 79 / 79 / 84;
 // kFillLarge 256 / 384 / 512: a batch of two chunks and 30 tokens 28.7 / 28.4 / 29.8. kMinChunk 128 / 256 / 512: one
 // token over 1024 keys 8.1 / 9.1 / 11.6. Contexts of up to kWhole keys are not cut, whose second launch costs more than it
-// saves (one token over 256 / 384 / 512 keys: 6.7 / 8.0 / 9.2 us whole, 7.6 / 7.6 / 7.7 cut); from 128 tiles on, twice
-// that (16 tokens of 8 kv heads over 512 / 768 / 1024: 10.5 / 14.9 / 18.3 whole, 13.0 / 16.1 / 18.4 cut).
+// saves. In a captured graph, one token of 8 kv heads over 256 / 384 / 448 / 512 keys: 6.8 / 8.1 / 8.8 / 9.1 us whole,
+// 8.0 / 8.2 / 8.2 / 8.3 cut (4 of D = 64: 5.6 / 6.6 / 7.2 / 7.3 and 7.2 / 7.4 / 7.5 / 7.5). From 128 tiles on, twice that
+// (16 tokens of 8 kv heads over 512 / 768 / 1024: 10.9 / 15.7 / 19.2 whole, 13.1 / 15.7 / 19.0 cut).
 constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kMinChunk = 128, kWhole = 384;
 
 inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window) {

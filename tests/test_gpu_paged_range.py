@@ -122,3 +122,35 @@ def test_scores_of_any_size(dev, scale, q_len, heads, n_kv, hd, n, workspace):
             # alike (numerator 2^-11 against the unrounded sum), the output 2^-11; a few f32 steps
             tol = (2 * 2.0 ** -11 + 2.0 ** -18) * x.abs().mean(0) + 2.0 ** -25
             assert bool(((got[t, h] - x.mean(0)).abs() <= tol).all()), (t, h, len(best), float((got[t, h] - x.mean(0)).abs().max()))
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("q_len,heads,n_kv,hd,n", [(1, 2, 1, 128, 200), (1, 8, 2, 64, 3000), (8, 4, 2, 64, 900), (100, 2, 2, 128, 300), (200, 4, 1, 64, 1500)])
+@pytest.mark.parametrize("base", [2.0 ** 10, 2.0 ** 13, 2.0 ** 18, 2.0 ** 20, -2.0 ** 20])
+def test_large_scores_that_differ_by_little(dev, base, q_len, heads, n_kv, hd, n, workspace):
+    """Scores of `base` and up to 8 more, in quarters (exact in f32): their differences count in full, also between the keys
+    of several waves, tiles and chunks."""
+    rng = np.random.RandomState(int(abs(base)) % 97 + n)
+    pages = -(-n // PAGE)
+    more = rng.randint(0, 33, (pages * PAGE, n_kv)) / 4.0
+    k = torch.zeros((pages * PAGE, n_kv, hd), dtype=torch.float16)
+    k[:, :, 5], k[:, :, hd - 1] = base / 2.0 ** 10, torch.from_numpy(more).half()
+    v = torch.randn((pages * PAGE, n_kv, hd), generator=torch.Generator().manual_seed(5)).half()
+    paged = [t.view(pages, PAGE, n_kv, hd).transpose(1, 2).contiguous().to(dev) for t in (k, v)]
+    q = torch.zeros((q_len, heads, hd), dtype=torch.float16, device=dev)
+    q[..., 5], q[..., hd - 1] = 2.0 ** 10, 1.0
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    ws = None if workspace else torch.empty(0, dtype=torch.uint8, device=dev)
+    got = serving.paged_attention(q, *paged, i32([0, q_len]), i32([n]), torch.arange(pages, dtype=torch.int32, device=dev)[None].contiguous(),
+                                  q_len, n, 1.0, workspace=ws).cpu().double()
+    w = torch.from_numpy(np.exp(more - 8.0))[:, :, None]
+    x = v.double()
+    num, den, mag = ((w * x).cumsum(0), w.cumsum(0), (w * x.abs()).cumsum(0))
+    rows = slice(n - q_len, n)
+    want, mag = (num[rows] / den[rows]), (mag[rows] / den[rows])
+    got = got.view(q_len, n_kv, heads // n_kv, hd)
+    # f16: 2^-11 of each weight and of the output; a maximum's rounded product: 2^-13 in base 2 where it is under 2^12, twice
+    # (what was summed and what it joins); f32: the sums, the scale's own rounding (2^-24 of a difference up to 8 * 1.45)
+    tol = (2 * 2.0 ** -11 + 2 * 2.0 ** -13 * 0.7 + (2 * n / 16 + 64) * 2.0 ** -24 + 2.0 ** -19) * mag + 2.0 ** -25
+    err = (got - want[:, :, None]).abs()
+    assert bool((err <= tol[:, :, None]).all()), float((err / tol[:, :, None]).max())
