@@ -162,7 +162,7 @@ __device__ __forceinline__ half_t __attribute__((ext_vector_type(E))) taken(half
 //
 // Bound by memory: 5 tokens of 32 heads over 4 and up to 65000 keys 74 us, 4.9 TB/s; 48 over 16000 each 5.6 TB/s. A few
 // hundred keys are a chain of trips to memory (starts, page ids, keys, 32 keys a wave and step): one token over 300
-// 7.9 us. Two tiles in flight a wave halve the waves a SIMD holds (74 -> 81); page ids a tile ahead win half a
+// 7.7 us. Two tiles in flight a wave halve the waves a SIMD holds (74 -> 81); page ids a tile ahead win half a
 // microsecond under 1000 keys and lose 1 % of the long ones.
 template <int D>
 struct KvTile {
@@ -391,8 +391,8 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
 //
 // Two buffers: the next keys' rows are requested a tile ahead and stored after the tile's products, one barrier a
 // tile. Bound by issue: two waves a SIMD take turns between the matrix cores and the softmax's 32 exponentials,
-// products with the scale and conversions a lane (matrix cores busy 41 % of the cycles, vector instructions 38 %,
-// LDS 37 %). 2048 tokens after 7952, 32 heads over 8, D = 128: 333 us, 900 TFLOP/s of the unmasked products.
+// products with the scale and conversions a lane (matrix cores busy 49 % of the cycles, vector instructions 46 %,
+// LDS 44 %). 2048 tokens after 7952, 32 heads over 8, D = 128: 333 us, 900 TFLOP/s of the unmasked products.
 template <int D>
 struct ChunkLds {
     static constexpr int KT = 64, KP = D + 8;  // keys a tile; elements from key row to key row

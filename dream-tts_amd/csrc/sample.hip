@@ -19,9 +19,15 @@
 // A short row is one workgroup with its logits and weights in registers. A long one is shared by
 // workgroups in four launches (its largest logit; the histogram; the crossing bins' members; the token),
 // every pass over the logits after the first from L2 or the MALL. What bounds them: a short row the chain
-// of block-wide steps (48 rows of 2048: 10 us, of which the bytes are 0.1), a long one the vector instructions of the
-// f64 exponentials and the launches' chains of small steps (64 x 131072 by top-p: 9 + 17 + 22 + 13 us, two passes of
-// 8.4M exponentials; one row 24).
+// of block-wide steps (48 rows of 2048: 10 us, of which the bytes are 0.1), a long one the f64 exponentials (two
+// passes of 8.4M at 64 x 131072; vector instructions 0.5 and 0.65 of those launches' cycles) and the launches' chains of
+// small steps. 64 x 131072 with all rows by top-p 0.9: 62 us; with rows of every kind (about a seventh each greedy,
+// unfiltered, by top-k, top-p or min-p alone, by two and by all three): 51, the launches 8.5 + 15 + 15.4 + 13.6. One row by
+// top-p: 30.
+//
+// A row whose crossing bins have more than 1024 members (equal logits, a narrow spread, a wide vocabulary at a high
+// temperature) falls to one workgroup and eight passes. 131072 logits by top-p: all equal 1.9 ms, within 1e-3 0.8, spread by
+// 2.5 at a temperature of 5 0.5; 64 such rows take as long as one; 2^20 equal ones 14 ms.
 #include <cmath>
 #include <type_traits>
 
@@ -1082,10 +1088,12 @@ struct Parts {
     int part, parts;
 };
 
-// Rows of up to kWholeVocab logits, which 1024 threads hold in registers, are one workgroup each (16384 logits,
-// 1 / 64 / 256 rows: 20 / 22 / 25 us, shared 22 / 33 / 40; the next size, 32 logits a thread, spills: 58 us for a row
-// of 32768, shared 23). Longer ones are shared by as many as the chip runs at once (kPartFill: two of 65 KB LDS a CU)
-// and none has under 2048 logits; from 257 rows on that is one (400 rows of 131072: 298 us, in two parts 336).
+// Rows of up to kWholeVocab logits are one workgroup each: 1024 threads hold them in registers, past 8192 (16 a thread)
+// with 84 registers a lane in scratch. 16384 logits by top-p, 1 / 16 / 64 / 256 rows: 27 / 28 / 30 / 43 us, shared 24 / 27
+// / 33 / 43; 10240: 24 / 25 / 27 / 35, shared 24 / 26 / 30 / 38; 32 a thread spill more (58 us for a row of 32768, shared
+// 23). Longer ones are shared by as many as the chip runs at once (kPartFill: two a CU of 512 threads and 104 registers; 64
+// x 131072 with 512 / 768: 62 / 69) and none has under 2048 logits; from 257 rows on that is one (400 rows of 131072: 298
+// us, in two parts 336).
 constexpr int64_t kWholeVocab = 16384, kPartFill = 512;
 
 inline Parts parts_of(int64_t rows, int64_t vocab) {
