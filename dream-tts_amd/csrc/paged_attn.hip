@@ -201,15 +201,17 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     int k0, k1;  // the tile's keys in this chunk
     span.chunk_keys(a, c, k0, k1);
     const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
-    // one of the tile's rows at least sees the keys from `bottom` to k1, all of them those from `from` to `upto`
-    const int upto = ctx - n_new + first_tok, bottom = a.window > 0 ? upto - a.window + 1 : 0;
+    // one of the tile's rows at least sees the keys [bottom, k1), all of them [from, end)
+    const bool one_token = first_tok == last_tok;
+    const int bottom = a.window > 0 ? ctx - n_new + first_tok - a.window + 1 : 0;
     const int from = a.window > 0 ? bottom + last_tok - first_tok : 0;
+    int end = ctx - n_new + first_tok + 1;
     {
         const int top = ctx - n_new + last_tok + 1;
         if (k1 > top) k1 = top;
         if (k0 < bottom) k0 = bottom & ~31;
+        if (end > k1) end = k1;
     }
-    auto cut = [&](int kb) { return first_tok != last_tok && (kb < from || kb + 31 > upto); };  // a tile that some rows see a part of
     half8_t qf[C];
     {
         const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
@@ -291,13 +293,13 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             }
         l += sum;
         // what no row sees holds anything: 0 times it may be NaN
-        if (kb + 32 > k1 || kb < bottom || t.ok != 3 || cut(kb)) {
+        if (kb < from || kb + 32 > end || t.ok != 3) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
                 if (key >= k1 || key < bottom || !(t.ok >> (j >> 2) & 1)) t.v[j] = typename KvTile<D>::ve{};
             }
-            if (cut(kb)) {
+            if (!one_token && (kb < from || kb + 32 > end)) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) spoilt |= take_out<E>(t.v[j]);
             }
@@ -317,7 +319,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     }
     if (__builtin_expect(__any(spoilt != 0), 0)) {
         for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) {
-            if (!cut(kb)) continue;
+            if (kb >= from && kb + 32 <= end) continue;
             for (int key = kb; key < kb + 32 && key < k1; ++key) {
                 const int page = a.batch.page(s, key >> a.batch.page_shift);
                 if (page < 0 || key > pos || key < row_lo) continue;
