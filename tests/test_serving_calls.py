@@ -46,14 +46,14 @@ def test_attention_refuses_an_output_inside_the_queries(q, q_stride, out):
 
 
 @pytest.mark.parametrize("q_out,k,v,match", [
-    (512, 1 << 16, 1 << 17, "may not replace qkv"), (3072 - 16, 1 << 16, 1 << 17, "may not replace qkv"),
+    (512, 1 << 16, 1 << 17, "may not replace qkv"), (2048 - 16, 1 << 16, 1 << 17, "may not replace qkv"),
     (8192, 1 << 16, 1 << 16, "share memory"), (8192, 1 << 16, (1 << 16) + 4096 - 16, "share memory"),
     (8192, (1 << 16) + 3 * 8192 + 4080, 1 << 16, "share memory"), (8192, 1 << 16, (1 << 16) + 8192 - 16, "share memory"),
 ])
 def test_append_refuses_operands_that_share_memory(q_out, k, v, match):
-    """Three f16 tokens of 4 + 2 * 2 heads of 64 (3072 bytes); pages of 4096 bytes, 8192 apart."""
+    """Two f16 tokens of 4 + 2 * 2 heads of 64 (2048 bytes); pages of 4096 bytes, 8192 apart."""
     p = _at(1 << 19)
-    _refused("dtts_qk_rope_append_paged_f16", match, _at(0), None, p, p, p, p, p, _at(q_out), _at(k), _at(v), 3, 2, 4, 2, 64, 64, 0,
+    _refused("dtts_qk_rope_append_paged_f16", match, _at(0), None, p, p, p, p, p, _at(q_out), _at(k), _at(v), 2, 2, 4, 2, 64, 64, 0,
              16, 8, 4, 4096, 64, 1e-6, None)
 
 
