@@ -63,7 +63,8 @@ struct PagedBatch {
     }
 };
 
-#define DTTS_REQUIRE_PAGED(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride)                               \
+// row_units: elements of a row of f16 pages, bytes of a row of 4-bit ones; page_stride and its multiple are in the same.
+#define DTTS_REQUIRE_PAGED_ROWS(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride, row_units, multiple)      \
     do {                                                                                                                          \
         DTTS_REQUIRE((tokens) >= 0 && (b) >= 0 && (n_kv) > 0 && (n_pages) > 0 && (max_pages) > 0,                                 \
                      "%s: bad shape (tokens %lld, b %lld, n_kv %lld, n_pages %lld, max_pages %lld)", name, (long long)(tokens),   \
@@ -75,11 +76,19 @@ struct PagedBatch {
         DTTS_REQUIRE((tokens) < (int64_t(1) << 24) && (b) <= kMaxSeqs && (n_kv) <= 4096 && (n_pages) < (int64_t(1) << 31) &&      \
                          (max_pages) <= (int64_t(1) << 30) / (page),                                                              \
                      "%s: too many rows, sequences, heads or positions", name);                                                   \
-        DTTS_REQUIRE((page_stride) >= (n_kv) * (page) * (head_dim) && (page_stride) % 8 == 0 &&                                   \
+        DTTS_REQUIRE((page_stride) >= (n_kv) * (page) * (row_units) && (page_stride) % (multiple) == 0 &&                         \
                          (page_stride) < (int64_t(1) << 32),                                                                      \
-                     "%s: page_stride %lld (a multiple of 8 under 2^32, at least n_kv * page * head_dim)", name,                  \
-                     (long long)(page_stride));                                                                                   \
+                     "%s: page_stride %lld (a multiple of %d under 2^32, at least a page)", name, (long long)(page_stride),       \
+                     static_cast<int>(multiple));                                                                                 \
     } while (0)
+
+#define DTTS_REQUIRE_PAGED(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride)                               \
+    DTTS_REQUIRE_PAGED_ROWS(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride, head_dim, 8)
+
+#define DTTS_REQUIRE_PAGE(name, page, max_pages)                                                                                 \
+    DTTS_REQUIRE((page) >= 16 && (page) <= 65536 && ((page) & ((page) - 1)) == 0 && (max_pages) <= (int64_t(1) << 30) / (page),  \
+                 "%s: pages of %lld positions, %lld a sequence (a power of two from 16 to 65536, 2^30 positions at most)", name, \
+                 (long long)(page), (long long)(max_pages))
 
 inline int log2_of(int64_t page) {
     int s = 0;

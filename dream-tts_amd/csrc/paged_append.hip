@@ -7,6 +7,12 @@
 // Everything is f32 until the one rounding of the store: the cache is f16, and the queries are f16
 // because the attention that reads them multiplies on the f16 matrix cores.
 //
+// 4-bit pages (q4.hpp) take k = turn(x') and v in groups of 32 instead:
+//   d = f16((max - min) / 15), b = f16(min - 64 d), n = rint((x - (64 d + b)) / d) from 0 to 15
+// 64 d + b is exact in f32 (two f16 numbers that nearly cancel) and b is rounded before the codes are chosen, so the
+// steps lie where the values read back do. A lane needs eight neighbours of a row, a group being four lanes: half-split
+// rows, whose lanes hold two groups of four apart, meet in LDS, a wave's rows in its own.
+//
 // HBM-bound: qkv in, q, k and v out, once. D/8 lanes own a head row, two groups of four elements each:
 // half-split, four pairs' first and second members; interleaved, eight neighbours (four pairs), so
 // both layouts turn in registers and the norm is a shuffle sum over D/8 lanes. At a decode step's
@@ -16,6 +22,7 @@
 
 #include "norm_rope.hpp"
 #include "paged.hpp"
+#include "q4.hpp"
 
 #pragma clang fp contract(off)
 
@@ -52,10 +59,41 @@ struct Four<half_t> {
     }
 };
 
+// Eight neighbours of a row, of a group that four lanes share: their word, and the group's pair. A group with a value that is
+// not finite, or whose values pass f16's range, is NaN, all of it.
+__device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair) {
+    float lo = z[0], hi = z[0];
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        lo = fminf(lo, z[i]);
+        hi = fmaxf(hi, z[i]);
+        finite = finite && fabsf(z[i]) < INFINITY;
+    }
+    if (!finite) hi = INFINITY;
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) {
+        lo = fminf(lo, __shfl_xor(lo, off, 64));
+        hi = fmaxf(hi, __shfl_xor(hi, off, 64));
+    }
+    half_t d = static_cast<half_t>((hi - lo) / 15.0f), b = static_cast<half_t>(lo - kQ4First * static_cast<float>(d));
+    const float step = static_cast<float>(d), first = __builtin_fmaf(kQ4First, step, static_cast<float>(b));
+    const float last = __builtin_fmaf(kQ4Last, step, static_cast<float>(b));
+    constexpr float kOver = 65520.0f;  // what f16 rounds to infinity
+    if (!(fabsf(first) < kOver && fabsf(last) < kOver)) d = b = static_cast<half_t>(NAN);
+    pair = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, d)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
+    const float per = step > 0.0f ? 1.0f / step : 0.0f;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        word |= static_cast<uint32_t>(fminf(fmaxf(rintf((z[i] - first) * per), 0.0f), 15.0f)) << (4 * (i >> 1) + 16 * (i & 1));
+    return word;
+}
+
 // A wave takes one token, or one of its `parts`: rows part * RW + its lane group's, then parts * RW further.
 // What a token's rows share (its sequence, position and page, and a lane's cos and sin, whatever the row) is
 // read once for all of them.
-template <typename T, int D, bool INTERLEAVED>
+template <typename T, int D, bool INTERLEAVED, bool Q4>
 __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv, AppendArgs a) {
     constexpr int L = D / 8, RW = 64 / L, U = 4;  // lanes per head row, head rows per wave step, steps requested together
     const uint32_t wid = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -92,7 +130,10 @@ __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv,
         Four<float>::load(a.cos_t + static_cast<int64_t>(pos) * a.half + 4 * j, c);
         Four<float>::load(a.sin_t + static_cast<int64_t>(pos) * a.half + 4 * j, sn);
     }
-    const int64_t slot = page * a.batch.page_stride + static_cast<int64_t>(pos & ((1 << a.batch.page_shift) - 1)) * D;
+    const int in_page = pos & ((1 << a.batch.page_shift) - 1);
+    const int64_t slot = page * a.batch.page_stride + static_cast<int64_t>(in_page) * D;
+    constexpr bool APART = Q4 && !INTERLEAVED;
+    __shared__ __attribute__((aligned(16))) float exchange[APART ? 4 : 1][APART ? RW : 1][APART ? D + 4 : 1];
     for (;;) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -130,6 +171,36 @@ __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv,
                     }
                 }
             }
+            if constexpr (Q4) {
+                if (!is_q) {
+                    float z[8];
+                    if constexpr (INTERLEAVED) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            z[i] = x[u][i];
+                            z[4 + i] = y[u][i];
+                        }
+                    } else {
+                        float *row = exchange[threadIdx.x >> 6][lane / L];
+                        *reinterpret_cast<float4_t *>(row + o1) = float4_t{x[u][0], x[u][1], x[u][2], x[u][3]};
+                        *reinterpret_cast<float4_t *>(row + o2) = float4_t{y[u][0], y[u][1], y[u][2], y[u][3]};
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+                        Four<float>::load(row + 8 * j, *reinterpret_cast<float (*)[4]>(z));
+                        Four<float>::load(row + 8 * j + 4, *reinterpret_cast<float (*)[4]>(z + 4));
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+                    }
+                    uint32_t pair;
+                    const uint32_t word = quantise(z, pair);
+                    const int kv = r - a.heads - (is_v ? a.n_kv : 0);
+                    uint8_t *dst = reinterpret_cast<uint8_t *>(is_v ? a.vp : a.kp) + page * a.batch.page_stride +
+                                   (static_cast<int64_t>(kv) << a.batch.page_shift) * Q4Row<D>::kBytes;
+                    *reinterpret_cast<uint32_t *>(dst + (is_v ? Q4Row<D>::value_word(in_page, j) : Q4Row<D>::key_word(in_page, j))) = word;
+                    if ((j & 3) == 0) *reinterpret_cast<uint32_t *>(dst + Q4Row<D>::pair(1 << a.batch.page_shift, in_page, j >> 2)) = pair;
+                    continue;
+                }
+            }
             half_t *dst;
             if (is_q)
                 dst = a.q_out + (static_cast<int64_t>(t) * a.heads + r) * D;
@@ -155,13 +226,14 @@ __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv,
 // repeats the token's lookups; a row a lane group and no sharing 18.7); 48 f32 tokens of 32 rows of 128 the same.
 constexpr int64_t kFillWaves = 4096;
 
-template <typename T>
+template <bool Q4, typename T>
 int append(const char *name, const T *qkv, const float *norms, const float *cos_t, const float *sin_t,
-           const int32_t *q_start, const int32_t *context, const int32_t *page_table, dtts_f16 *q_out, dtts_f16 *kp,
-           dtts_f16 *vp, int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t hd, int64_t rot, int32_t layout,
+           const int32_t *q_start, const int32_t *context, const int32_t *page_table, dtts_f16 *q_out, void *kp,
+           void *vp, int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t hd, int64_t rot, int32_t layout,
            int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride, int64_t table_len, float eps,
            hipStream_t stream) {
-    DTTS_REQUIRE_PAGED(name, tokens, b, n_kv, hd, page, n_pages, max_pages, page_stride);
+    const int64_t row_units = Q4 ? 5 * hd / 8 : hd, unit = Q4 ? 1 : sizeof(half_t);
+    DTTS_REQUIRE_PAGED_ROWS(name, tokens, b, n_kv, hd, page, n_pages, max_pages, page_stride, row_units, Q4 ? 16 : 8);
     DTTS_REQUIRE(heads > 0 && heads <= 65536, "%s: %lld heads", name, (long long)heads);
     DTTS_REQUIRE(rot > 0 && rot % 8 == 0 && rot <= hd, "%s: %lld rotated dimensions of %lld (a multiple of 8)", name,
                  (long long)rot, (long long)hd);
@@ -169,13 +241,13 @@ int append(const char *name, const T *qkv, const float *norms, const float *cos_
     DTTS_REQUIRE(table_len > 0 && table_len < (int64_t(1) << 31), "%s: a table of %lld positions", name, (long long)table_len);
     if (tokens == 0 || b == 0) return DTTS_OK;
     DTTS_REQUIRE(qkv && cos_t && sin_t && q_start && context && page_table && q_out && kp && vp, "%s: null pointer", name);
-    DTTS_REQUIRE(aligned(qkv, 4 * sizeof(T)) && aligned(cos_t, 16) && aligned(sin_t, 16) && aligned(q_out, 8) && aligned(kp, 8) &&
-                     aligned(vp, 8) && aligned(norms, 16) && aligned(q_start, 4) && aligned(context, 4) && aligned(page_table, 4),
+    DTTS_REQUIRE(aligned(qkv, 4 * sizeof(T)) && aligned(cos_t, 16) && aligned(sin_t, 16) && aligned(q_out, 8) && aligned(kp, Q4 ? 16 : 8) &&
+                     aligned(vp, Q4 ? 16 : 8) && aligned(norms, 16) && aligned(q_start, 4) && aligned(context, 4) && aligned(page_table, 4),
                  "%s: misaligned operand", name);
-    const int64_t per = heads + 2 * n_kv, f16 = sizeof(half_t), page_bytes = n_kv * page * hd * f16;
+    const int64_t per = heads + 2 * n_kv, f16 = sizeof(half_t), page_bytes = n_kv * page * row_units * unit;
     DTTS_REQUIRE(!share_bytes({qkv, 1, 0, tokens * per * hd * static_cast<int64_t>(sizeof(T))}, {q_out, 1, 0, tokens * heads * hd * f16}),
                  "%s: the queries may not replace qkv, nor a part of it", name);
-    DTTS_REQUIRE(!share_bytes({kp, n_pages, page_stride * f16, page_bytes}, {vp, n_pages, page_stride * f16, page_bytes}),
+    DTTS_REQUIRE(!share_bytes({kp, n_pages, page_stride * unit, page_bytes}, {vp, n_pages, page_stride * unit, page_bytes}),
                  "%s: pages of keys and of values share memory", name);
     // Steps of RW head rows a token has, shared by enough waves to fill the chip (kFillWaves, 16 a CU): few tokens
     // spread over many, each with one step; many tokens have a wave each.
@@ -190,8 +262,8 @@ int append(const char *name, const T *qkv, const float *norms, const float *cos_
     a.cos_t = cos_t;
     a.sin_t = sin_t;
     a.q_out = reinterpret_cast<half_t *>(q_out);
-    a.kp = reinterpret_cast<half_t *>(kp);
-    a.vp = reinterpret_cast<half_t *>(vp);
+    a.kp = static_cast<half_t *>(kp);
+    a.vp = static_cast<half_t *>(vp);
     a.heads = static_cast<int>(heads);
     a.n_kv = static_cast<int>(n_kv);
     a.half = static_cast<int>(rot / 2);
@@ -201,13 +273,13 @@ int append(const char *name, const T *qkv, const float *norms, const float *cos_
     const unsigned blocks = static_cast<unsigned>((tokens * parts + 3) / 4);
     const bool inter = layout == DTTS_ROPE_INTERLEAVED;
     if (hd == 128 && inter)
-        qk_rope_append_paged_kernel<T, 128, true><<<blocks, 256, 0, stream>>>(qkv, a);
+        qk_rope_append_paged_kernel<T, 128, true, Q4><<<blocks, 256, 0, stream>>>(qkv, a);
     else if (hd == 128)
-        qk_rope_append_paged_kernel<T, 128, false><<<blocks, 256, 0, stream>>>(qkv, a);
+        qk_rope_append_paged_kernel<T, 128, false, Q4><<<blocks, 256, 0, stream>>>(qkv, a);
     else if (inter)
-        qk_rope_append_paged_kernel<T, 64, true><<<blocks, 256, 0, stream>>>(qkv, a);
+        qk_rope_append_paged_kernel<T, 64, true, Q4><<<blocks, 256, 0, stream>>>(qkv, a);
     else
-        qk_rope_append_paged_kernel<T, 64, false><<<blocks, 256, 0, stream>>>(qkv, a);
+        qk_rope_append_paged_kernel<T, 64, false, Q4><<<blocks, 256, 0, stream>>>(qkv, a);
     DTTS_LAUNCH_CHECK(name);
     return DTTS_OK;
 }
@@ -221,7 +293,7 @@ extern "C" int dtts_qk_rope_append_paged_f32(const float *qkv, const float *norm
                                              int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
                                              int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
                                              int64_t table_len, float eps, hipStream_t stream) {
-    return dtts::append<float>("dtts_qk_rope_append_paged_f32", qkv, norms, cos_t, sin_t, q_start, context, page_table, q_out,
+    return dtts::append<false>("dtts_qk_rope_append_paged_f32", qkv, norms, cos_t, sin_t, q_start, context, page_table, q_out,
                                kpages, vpages, tokens, b, heads, n_kv, head_dim, rot_dim, layout, page, n_pages, max_pages,
                                page_stride, table_len, eps, stream);
 }
@@ -232,7 +304,30 @@ extern "C" int dtts_qk_rope_append_paged_f16(const dtts_f16 *qkv, const float *n
                                              int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
                                              int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
                                              int64_t table_len, float eps, hipStream_t stream) {
-    return dtts::append<dtts::half_t>("dtts_qk_rope_append_paged_f16", reinterpret_cast<const dtts::half_t *>(qkv), norms,
+    return dtts::append<false>("dtts_qk_rope_append_paged_f16", reinterpret_cast<const dtts::half_t *>(qkv), norms,
+                                      cos_t, sin_t, q_start, context, page_table, q_out, kpages, vpages, tokens, b, heads,
+                                      n_kv, head_dim, rot_dim, layout, page, n_pages, max_pages, page_stride, table_len, eps,
+                                      stream);
+}
+
+extern "C" int dtts_qk_rope_append_paged_q4_f32(const float *qkv, const float *norms, const float *cos_t, const float *sin_t,
+                                             const int32_t *q_start, const int32_t *context, const int32_t *page_table,
+                                             dtts_f16 *q_out, void *kpages, void *vpages, int64_t tokens, int64_t b,
+                                             int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
+                                             int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
+                                             int64_t table_len, float eps, hipStream_t stream) {
+    return dtts::append<true>("dtts_qk_rope_append_paged_q4_f32", qkv, norms, cos_t, sin_t, q_start, context, page_table, q_out,
+                               kpages, vpages, tokens, b, heads, n_kv, head_dim, rot_dim, layout, page, n_pages, max_pages,
+                               page_stride, table_len, eps, stream);
+}
+
+extern "C" int dtts_qk_rope_append_paged_q4_f16(const dtts_f16 *qkv, const float *norms, const float *cos_t, const float *sin_t,
+                                             const int32_t *q_start, const int32_t *context, const int32_t *page_table,
+                                             dtts_f16 *q_out, void *kpages, void *vpages, int64_t tokens, int64_t b,
+                                             int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
+                                             int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
+                                             int64_t table_len, float eps, hipStream_t stream) {
+    return dtts::append<true>("dtts_qk_rope_append_paged_q4_f16", reinterpret_cast<const dtts::half_t *>(qkv), norms,
                                       cos_t, sin_t, q_start, context, page_table, q_out, kpages, vpages, tokens, b, heads,
                                       n_kv, head_dim, rot_dim, layout, page, n_pages, max_pages, page_stride, table_len, eps,
                                       stream);

@@ -1,5 +1,5 @@
-// Attention of each sequence's new tokens over its paged f16 cache: out_i = sum_j softmax_j(scale
-// q_i . k_j) v_j over p_i - window < j <= p_i, a ragged batch of chunks and single tokens.
+// Attention of each sequence's new tokens over its paged cache, f16 or in 4 bits (q4.hpp): out_i = sum_j softmax_j(scale
+// q_i . k_j) v_j over p_i - window < j <= p_i and j < sinks, a ragged batch of chunks and single tokens.
 //
 // A row is one (new token, query head). The heads / n_kv query heads of a kv head read the same keys,
 // so rows are numbered token * gqa + head within (sequence, kv head), and a tile of consecutive rows goes to one
@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "paged.hpp"
+#include "q4.hpp"
 
 namespace dtts {
 namespace {
@@ -24,11 +25,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 struct AttnArgs {
     PagedBatch batch;
-    const half_t *q, *k, *v;
+    const half_t *q, *k, *v;  // k and v: of 4-bit pages their bytes, and the batch's page stride counts those
     half_t *out;
     float *part;       // per (row, chunk): D weighted sums, the weight sum, the maximum of q . k
     int64_t q_stride;  // elements between tokens
-    int heads, n_kv, gqa, window;
+    int heads, n_kv, gqa, window, sinks;  // sinks: positions that every later token sees, 0 without a window
     float scale2;      // |scale| * log2(e), above 0: the softmax runs in base 2, its maxima are those of q . k
     bool negate;       // scale < 0: the queries change sign
     int chunk, nsplit; // keys per chunk, chunks at most (the last takes what is left)
@@ -36,20 +37,41 @@ struct AttnArgs {
 };
 
 // The keys that sequence s's rows see, in chunks: [lo, hi), lo a multiple of 64, `n` chunks. hi stops
-// at the table's end, whatever the context says.
+// at the table's end, whatever the context says. With sinks the keys are [0, head) and [head + gap, hi), head and gap
+// multiples of 64 (no gap where the windows reach the head, which may pass hi), and chunks cut the axis that leaves the gap
+// out: a key past the head is `gap` less there.
 struct Span {
-    int lo, hi, n;
+    int lo, hi, n, head, gap;
     __device__ __forceinline__ Span(const AttnArgs &a, int s, int n_new, int ctx) {
         const int64_t cap = static_cast<int64_t>(a.batch.max_pages) << a.batch.page_shift;
         hi = ctx < 0 ? 0 : ctx < cap ? ctx : static_cast<int>(cap);
         lo = a.window > 0 && ctx - n_new - a.window + 1 > 0 ? (ctx - n_new - a.window + 1) & ~63 : 0;
         if (lo > hi) lo = hi & ~63;
-        n = static_cast<int>((static_cast<int64_t>(hi) - lo + a.chunk - 1) / a.chunk);
+        head = gap = 0;
+        if (a.sinks > 0) {
+            head = (a.sinks + 63) & ~63;
+            gap = lo > head ? lo - head : 0;
+            lo = 0;
+        }
+        n = static_cast<int>((static_cast<int64_t>(hi) - gap - lo + a.chunk - 1) / a.chunk);
         n = n < 1 ? 1 : n > a.nsplit ? a.nsplit : n;
     }
     __device__ __forceinline__ void chunk_keys(const AttnArgs &a, int c, int &k0, int &k1) const {
         k0 = lo + c * a.chunk;
-        k1 = c == n - 1 ? hi : k0 + a.chunk;
+        k1 = c == n - 1 ? hi - gap : k0 + a.chunk;
+    }
+};
+
+// A chunk's key tiles of K keys with sinks: those of the head, [k0, mid), then from `next` on up to k1 (all real keys).
+// `bottom`: the first key of the tile's rows' windows.
+struct SinkTiles {
+    int mid, next;
+    __device__ __forceinline__ SinkTiles(const Span &span, int bottom, int K, int &k0, int &k1) {
+        mid = k0 < span.head ? (k1 < span.head ? k1 : span.head) : k0;
+        next = (k0 < span.head ? span.head : k0) + span.gap;
+        if (next < (bottom & -K)) next = bottom & -K;
+        if (k1 > span.head) k1 += span.gap;
+        if (k0 >= span.head) k0 = mid = next;
     }
 };
 
@@ -164,21 +186,116 @@ __device__ __forceinline__ half_t __attribute__((ext_vector_type(E))) taken(half
 // hundred keys are a chain of trips to memory (starts, page ids, keys, 32 keys a wave and step): one token over 300
 // 7.7 us. Two tiles in flight a wave halve the waves a SIMD holds (74 -> 81); page ids a tile ahead win half a
 // microsecond under 1000 keys and lose 1 % of the long ones.
-template <int D>
+template <int D, bool Q4>
 struct KvTile {
     static constexpr int E = D / 16;  // dimensions a lane holds of each of its 8 value rows
     typedef half_t ve __attribute__((ext_vector_type(E)));
     half8_t k[2][D / 32];
     ve v[8];
     int ok;  // bit u: keys 16u .. 16u + 15 have a page
+
+    // Of the score product's step i, a lane of group g has the dimensions from here on.
+    __device__ __forceinline__ static int dim(int i, int g) { return 32 * i + 8 * g; }
+    // base: of the page's kv head; slot: keys 16u's place there; l16, g: the lane's
+    __device__ __forceinline__ void load(const AttnArgs &a, int u, int64_t base, int slot, int l16, int g) {
+        base += static_cast<int64_t>(slot) * D;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) k[u][i] = *reinterpret_cast<const half8_t *>(a.k + base + l16 * D + dim(i, g));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * u + j] = *reinterpret_cast<const ve *>(a.v + base + (4 * g + j) * D + E * l16);
+    }
+    __device__ __forceinline__ half8_t key(int u, int i) const { return k[u][i]; }
+    __device__ __forceinline__ void drop(int j) { v[j] = ve{}; }
+    __device__ __forceinline__ void turn(int) {}
+    __device__ __forceinline__ half8_t value(int e) const {
+        half8_t f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = v[j][e];
+        return f;
+    }
 };
+
+// Of 4-bit pages a lane has 16 or 32 neighbouring dimensions of its key (one load and their pair), and of the values a word
+// of four keys at once (one load) with their pairs (another). The words are turned before they become numbers: halves of two
+// keys' words make pairs of keys, which is what the product's operand holds.
+template <int D>
+struct KvTile<D, true> {
+    static constexpr int E = D / 16, W = D / 32;  // W: key words a lane holds
+    typedef half_t ve __attribute__((ext_vector_type(E)));
+    typedef uint32_t kw __attribute__((ext_vector_type(W)));
+    kw k[2];
+    uint32_t ks[2];
+    u32x4 v[2], vs[2];
+    uint32_t lo[4], hi[4];  // of the values' key pairs, after turn
+    half2_t d[4], b[4];
+    int ok;
+
+    __device__ __forceinline__ static int dim(int i, int g) { return 8 * (W * g + i); }
+    __device__ __forceinline__ void load(const AttnArgs &a, int u, int64_t base, int slot, int l16, int g) {
+        const int page = 1 << a.batch.page_shift;
+        const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.k) + base, *vp = reinterpret_cast<const uint8_t *>(a.v) + base;
+        k[u] = *reinterpret_cast<const kw *>(kp + Q4Row<D>::key_word(slot + l16, W * g));
+        ks[u] = *reinterpret_cast<const uint32_t *>(kp + Q4Row<D>::pair(page, slot + l16, W * g / 4));
+        v[u] = *reinterpret_cast<const u32x4 *>(vp + Q4Row<D>::value_word(slot + 4 * g, E * l16 / 8));
+        vs[u] = *reinterpret_cast<const u32x4 *>(vp + Q4Row<D>::pair(page, slot + 4 * g, E * l16 / 32));
+    }
+    __device__ __forceinline__ half8_t key(int u, int i) const { return q4_values(k[u][i], ks[u]); }
+    __device__ __forceinline__ void drop(int j) { vs[j >> 2][j & 3] = 0; }  // 64 + n times 0
+    __device__ __forceinline__ void turn(int l16) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int u = t >> 1, j = 2 * (t & 1);
+            lo[t] = low_halves(v[u][j], v[u][j + 1]);
+            hi[t] = high_halves(v[u][j], v[u][j + 1]);
+            if (E == 4 && (l16 & 1)) {  // the word's second four dimensions
+                lo[t] >>= 8;
+                hi[t] >>= 8;
+            }
+            d[t] = __builtin_bit_cast(half2_t, low_halves(vs[u][j], vs[u][j + 1]));
+            b[t] = __builtin_bit_cast(half2_t, high_halves(vs[u][j], vs[u][j + 1]));
+        }
+    }
+    __device__ __forceinline__ half8_t value(int e) const {
+        half8_t f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const half2_t x = __builtin_elementwise_fma(q4_codes(e & 1 ? hi[t] : lo[t], e >> 1), d[t], b[t]);
+            f[2 * t] = x[0];
+            f[2 * t + 1] = x[1];
+        }
+        return f;
+    }
+};
+
+// Four or eight neighbouring dimensions (a multiple of as many) of a key's value row. base: of the page's kv head.
+template <int D, bool Q4, int E>
+__device__ __forceinline__ half_t __attribute__((ext_vector_type(E))) value_run(const AttnArgs &a, int64_t base, int slot, int dim) {
+    typedef half_t ve __attribute__((ext_vector_type(E)));
+    if constexpr (Q4) {
+        const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.v) + base;
+        const uint32_t word = *reinterpret_cast<const uint32_t *>(vp + Q4Row<D>::value_word(slot, dim / 8));
+        const half8_t x = q4_values(word, *reinterpret_cast<const uint32_t *>(vp + Q4Row<D>::pair(1 << a.batch.page_shift, slot, dim / 32)));
+        ve y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = E == 4 && (dim & 4) ? x[4 + e] : x[e];
+        return y;
+    } else {
+        return *reinterpret_cast<const ve *>(a.v + base + static_cast<int64_t>(slot) * D + dim);
+    }
+}
+
+// Where a page's kv head begins in it.
+template <int D, bool Q4>
+__device__ __forceinline__ int64_t head_offset(const AttnArgs &a, int kh) {
+    return (static_cast<int64_t>(kh) << a.batch.page_shift) * (Q4 ? Q4Row<D>::kBytes : D);
+}
 
 template <int D>
 struct RowsLds {
     float o[4][16][D + 4], m[4][16], l[4][16];
 };
 
-template <int D>
+template <int D, bool Q4, bool SINKS>
 __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, int block) {
     constexpr int C = D / 32, E = D / 16, ROWS = 16;
     auto &sm_o = lds.o;
@@ -205,42 +322,39 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     const bool one_token = first_tok == last_tok;
     const int bottom = a.window > 0 ? ctx - n_new + first_tok - a.window + 1 : 0;
     const int from = a.window > 0 ? bottom + last_tok - first_tok : 0;
-    int end = ctx - n_new + first_tok + 1;
+    int end = ctx - n_new + first_tok + 1, mid = 0, next = 0;
+    if constexpr (SINKS) {
+        const SinkTiles tiles(span, bottom, 32, k0, k1);
+        mid = tiles.mid;
+        next = tiles.next;
+    }
     {
         const int top = ctx - n_new + last_tok + 1;
         if (k1 > top) k1 = top;
-        if (k0 < bottom) k0 = bottom & ~31;
+        if (!SINKS && k0 < bottom) k0 = bottom & ~31;
         if (end > k1) end = k1;
     }
+    const int shown = SINKS ? (a.sinks < end ? a.sinks : end) : 0;  // and all of them [0, shown)
     half8_t qf[C];
     {
         const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            qf[i] = *reinterpret_cast<const half8_t *>(qr + 32 * i + 8 * g);
+            qf[i] = *reinterpret_cast<const half8_t *>(qr + KvTile<D, Q4>::dim(i, g));
             if (a.negate) qf[i] = -qf[i];
         }
     }
     const int in_page = (1 << a.batch.page_shift) - 1;
-    const int64_t head_at = (static_cast<int64_t>(kh) << a.batch.page_shift) * D;
-    auto load = [&](int kb, KvTile<D> &t) {
+    const int64_t head_at = head_offset<D, Q4>(a, kh);
+    auto load = [&](int kb, KvTile<D, Q4> &t) {
         t.ok = 0;
-        int64_t base[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int key = kb + 16 * u;
             const int page = key < k1 ? a.batch.page(s, key >> a.batch.page_shift) : -1;
             if (page >= 0) t.ok |= 1 << u;
-            base[u] = (page < 0 ? 0 : page) * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D;
+            t.load(a, u, (page < 0 ? 0 : page) * a.batch.page_stride + head_at, key & in_page, l16, g);
         }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < C; ++i)
-                t.k[u][i] = *reinterpret_cast<const half8_t *>(a.k + base[u] + l16 * D + 32 * i + 8 * g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            t.v[j] = *reinterpret_cast<const typename KvTile<D>::ve *>(a.v + base[j >> 2] + (4 * g + (j & 3)) * D + E * l16);
     };
     float m = -INFINITY, m2 = 0.0f, l = 0.0f;  // m2: what the weights are relative to in log2, anything while there is no m
     bool far = false;
@@ -248,13 +362,13 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     float4_t o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
-    auto compute = [&](int kb, KvTile<D> &t) {
+    auto compute = [&](int kb, KvTile<D, Q4> &t) {
         float4_t sc[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             sc[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < C; ++i) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[u][i], qf[i], sc[u], 0, 0, 0);
+            for (int i = 0; i < C; ++i) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.key(u, i), qf[i], sc[u], 0, 0, 0);
         }
         float mx = m;
 #pragma unroll
@@ -262,7 +376,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = kb + 16 * u + 4 * g + i;
-                const bool seen = key <= pos && key >= row_lo && key < k1 && (t.ok >> u & 1);
+                const bool seen = key <= pos && (key >= row_lo || (SINKS && key < a.sinks)) && key < k1 && (t.ok >> u & 1);
                 sc[u][i] = seen ? sc[u][i] : -INFINITY;
                 mx = fmaxf(mx, sc[u][i]);
             }
@@ -293,45 +407,53 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             }
         l += sum;
         // what no row sees holds anything: 0 times it may be NaN
-        if (kb < from || kb + 32 > end || t.ok != 3) {
+        const bool partly = (kb < from && !(SINKS && kb + 32 <= shown)) || kb + 32 > end;
+        if (partly || t.ok != 3) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
-                if (key >= k1 || key < bottom || !(t.ok >> (j >> 2) & 1)) t.v[j] = typename KvTile<D>::ve{};
-            }
-            if (!one_token && (kb < from || kb + 32 > end)) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) spoilt |= take_out<E>(t.v[j]);
+                if (key >= k1 || (key < bottom && !(SINKS && key < a.sinks)) || !(t.ok >> (j >> 2) & 1)) t.drop(j);
             }
         }
+        t.turn(l16);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            half8_t f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = t.v[j][e];
+            half8_t f = t.value(e);
+            if (partly && !one_token) spoilt |= take_out<8>(f);
             o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[e], 0, 0, 0);
         }
     };
-    KvTile<D> t;
-    for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) {
+    // the wave's key tiles, every fourth: f(first key)
+    auto for_tiles = [&](auto f) {
+        if constexpr (SINKS) {
+            const int heads_tiles = (mid - k0 + 31) >> 5, rest = next < k1 ? (k1 - next + 31) >> 5 : 0;
+            for (int i = w; i < heads_tiles + rest; i += 4) {
+                const int kb = i < heads_tiles ? k0 + 32 * i : next + 32 * (i - heads_tiles);
+                if (kb < k1) f(kb);
+            }
+        } else {
+            for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) f(kb);
+        }
+    };
+    KvTile<D, Q4> t;
+    for_tiles([&](int kb) {
         load(kb, t);
         compute(kb, t);
-    }
+    });
     if (__builtin_expect(__any(spoilt != 0), 0)) {
-        for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) {
-            if (kb >= from && kb + 32 <= end) continue;
+        for_tiles([&](int kb) {
+            if ((kb >= from || (SINKS && kb + 32 <= shown)) && kb + 32 <= end) return;
             for (int key = kb; key < kb + 32 && key < k1; ++key) {
                 const int page = a.batch.page(s, key >> a.batch.page_shift);
-                if (page < 0 || key > pos || key < row_lo) continue;
-                const half_t *vr = a.v + page * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D + 4 * E * g;
+                if (page < 0 || key > pos || (key < row_lo && !(SINKS && key < a.sinks))) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const auto v = taken<E>(*reinterpret_cast<const typename KvTile<D>::ve *>(vr + E * i));
+                    const auto v = taken<E>(value_run<D, Q4, E>(a, page * a.batch.page_stride + head_at, key & in_page, 4 * E * g + E * i));
 #pragma unroll
                     for (int e = 0; e < E; ++e) o[e][i] += static_cast<float>(v[e]);
                 }
             }
-        }
+        });
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -373,10 +495,10 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             }
         } else {
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // a row that sees no key is zero
-            typename KvTile<D>::ve y;
+            typename KvTile<D, Q4>::ve y;
 #pragma unroll
             for (int e = 0; e < E; ++e) y[e] = static_cast<half_t>(num[e] * inv);
-            *reinterpret_cast<typename KvTile<D>::ve *>(a.out + trow * D + E * l16) = y;
+            *reinterpret_cast<typename KvTile<D, Q4>::ve *>(a.out + trow * D + E * l16) = y;
         }
     }
 }
@@ -402,7 +524,7 @@ struct ChunkLds {
     int ok[2][4], spoilt[4];
 };
 
-template <int D>
+template <int D, bool Q4, bool SINKS>
 __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, int block_no) {
     constexpr int ROWS = 128, KT = 64, E = D / 16, C = D / 16, KL = D / 32;  // C: k steps, KL: 16-byte key loads a thread
     constexpr int KCH = D / 8, KP = ChunkLds<D>::KP;                         // KCH: 16-byte pieces of a key row
@@ -423,11 +545,22 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     span.chunk_keys(a, c, k0, k1);
     // all of the tile's rows see the keys from `from` to `upto`
     const int upto = pos0 + r0 / a.gqa, from = a.window > 0 ? pos0 + (r0 + n_rows - 1) / a.gqa - a.window + 1 : 0;
+    int mid = 0, next = 0;
     {
         const int top = pos0 + (r0 + n_rows - 1) / a.gqa + 1, bottom = a.window > 0 ? upto - a.window + 1 : 0;
+        if constexpr (SINKS) {
+            const SinkTiles tiles(span, bottom, KT, k0, k1);
+            mid = tiles.mid;
+            next = tiles.next;
+        }
         if (k1 > top) k1 = top;
-        if (k0 < bottom) k0 = bottom & ~(KT - 1);
+        if (!SINKS && k0 < bottom) k0 = bottom & ~(KT - 1);
     }
+    const int shown = SINKS ? a.sinks : 0;  // and those before `shown`, up to `upto`
+    auto after = [&](int kb) {  // the key tile that follows
+        kb += KT;
+        return SINKS && kb >= mid && kb < next ? next : kb;
+    };
     // the wave's rows and the lane's
     const int wrows = n_rows - 32 * w < 32 ? n_rows - 32 * w : 32;
     const int row = r0 + 32 * w + (l32 < wrows ? l32 : wrows > 0 ? wrows - 1 : -32 * w);
@@ -444,10 +577,15 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
         }
     }
     const int in_page = (1 << a.batch.page_shift) - 1;
-    const int64_t head_at = (static_cast<int64_t>(kh) << a.batch.page_shift) * D;
-    // staging: wave w takes keys 16w .. 16w + 15 of a tile, one page
+    const int64_t head_at = head_offset<D, Q4>(a, kh);
+    // staging: wave w takes keys 16w .. 16w + 15 of a tile, one page; of 4-bit pages as words, a quarter of a key's row and
+    // of the values what four keys have of E dimensions
+    typedef uint32_t kw __attribute__((ext_vector_type(KL)));
     half8_t gk[KL];
     ve gv[4];
+    kw gkw;
+    uint32_t gks;
+    u32x4 gvw, gvs;
     bool g_ok = false;
     uint32_t spoilt = 0;
     const int krow = lane / KCH, kch = lane % KCH, a4 = lane >> 4, db = lane & 15;
@@ -459,8 +597,18 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     int next_id = id_of(k0 & ~(KT - 1));  // of the tile to be requested next
     auto load = [&](int kb) {  // past the last key: somewhere in page 0, for nothing, so that no branch holds a request
         const int key = kb + 16 * w, id = next_id;
-        next_id = id_of(kb + KT);
+        next_id = id_of(after(kb));
         g_ok = key < k1 && id >= 0 && id < a.batch.n_pages;
+        if constexpr (Q4) {
+            const int64_t base = (g_ok ? id : 0) * a.batch.page_stride + head_at;
+            const int page = in_page + 1, slot = key & in_page;
+            const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.k) + base, *vp = reinterpret_cast<const uint8_t *>(a.v) + base;
+            gkw = *reinterpret_cast<const kw *>(kp + Q4Row<D>::key_word(slot + (lane >> 2), KL * (lane & 3)));
+            gks = *reinterpret_cast<const uint32_t *>(kp + Q4Row<D>::pair(page, slot + (lane >> 2), KL * (lane & 3) / 4));
+            gvw = *reinterpret_cast<const u32x4 *>(vp + Q4Row<D>::value_word(slot + 4 * a4, E * db / 8));
+            gvs = *reinterpret_cast<const u32x4 *>(vp + Q4Row<D>::pair(page, slot + 4 * a4, E * db / 32));
+            return;
+        }
         const int64_t base = (g_ok ? id : 0) * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D;
 #pragma unroll
         for (int i = 0; i < KL; ++i)
@@ -469,24 +617,62 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
         for (int j = 0; j < 4; ++j) gv[j] = *reinterpret_cast<const ve *>(a.v + base + (4 * a4 + j) * D + E * db);
     };
     auto store = [&](int kb, int buf) {
-#pragma unroll
-        for (int i = 0; i < KL; ++i) {
-            const int r = 16 * w + krow + i * (64 / KCH);
-            *reinterpret_cast<half8_t *>(&sk[buf][r * KP + kch * 8]) = gk[i];
-        }
-        if (!g_ok || kb + KT > k1 || kb < from || kb + KT - 1 > upto) {  // slots that hold no position: 0 times what is there may be NaN
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (!g_ok || kb + 16 * w + 4 * a4 + j >= k1) gv[j] = ve{};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) spoilt |= take_out<E>(gv[j]);
-        }
+        // slots that hold no position: 0 times what is there may be NaN
+        const bool partly = !g_ok || kb + KT > k1 || (kb < from && !(SINKS && kb + KT <= shown)) || kb + KT - 1 > upto;
         const int kk = 16 * w + ((a4 & 1) << 3 | (a4 >> 1) << 2);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
+        auto put = [&](int e, half4_t x) {
             const int d = E * db + e;
-            *reinterpret_cast<half4_t *>(&sv[buf][d * KT + (((kk >> 3) ^ d ^ (d >> 3)) & 7) * 8 + (kk & 4)]) =
-                half4_t{gv[0][e], gv[1][e], gv[2][e], gv[3][e]};
+            *reinterpret_cast<half4_t *>(&sv[buf][d * KT + (((kk >> 3) ^ d ^ (d >> 3)) & 7) * 8 + (kk & 4)]) = x;
+        };
+        if constexpr (Q4) {
+#pragma unroll
+            for (int i = 0; i < KL; ++i)
+                *reinterpret_cast<half8_t *>(&sk[buf][(16 * w + (lane >> 2)) * KP + 8 * (KL * (lane & 3) + i)]) = q4_values(gkw[i], gks);
+            if (partly) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!g_ok || kb + 16 * w + 4 * a4 + j >= k1) gvs[j] = 0;
+            }
+            uint32_t lo[2], hi[2];
+            half2_t sd[2], sb[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                lo[t] = low_halves(gvw[2 * t], gvw[2 * t + 1]);
+                hi[t] = high_halves(gvw[2 * t], gvw[2 * t + 1]);
+                if (E == 4 && (db & 1)) {
+                    lo[t] >>= 8;
+                    hi[t] >>= 8;
+                }
+                sd[t] = __builtin_bit_cast(half2_t, low_halves(gvs[2 * t], gvs[2 * t + 1]));
+                sb[t] = __builtin_bit_cast(half2_t, high_halves(gvs[2 * t], gvs[2 * t + 1]));
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                half4_t x;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const half2_t y = __builtin_elementwise_fma(q4_codes(e & 1 ? hi[t] : lo[t], e >> 1), sd[t], sb[t]);
+                    x[2 * t] = y[0];
+                    x[2 * t + 1] = y[1];
+                }
+                if (partly) spoilt |= take_out<4>(x);
+                put(e, x);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < KL; ++i) {
+                const int r = 16 * w + krow + i * (64 / KCH);
+                *reinterpret_cast<half8_t *>(&sk[buf][r * KP + kch * 8]) = gk[i];
+            }
+            if (partly) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!g_ok || kb + 16 * w + 4 * a4 + j >= k1) gv[j] = ve{};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) spoilt |= take_out<E>(gv[j]);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) put(e, half4_t{gv[0][e], gv[1][e], gv[2][e], gv[3][e]});
         }
         if (lane == 0) s_ok[buf][w] = g_ok;
     };
@@ -524,16 +710,18 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        const bool whole = kb + KT - 1 <= wfirst && kb + KT <= k1 && (a.window == 0 || kb > wlast - a.window) &&
+        const bool whole = kb + KT - 1 <= wfirst && kb + KT <= k1 &&
+                           (a.window == 0 || kb > wlast - a.window || (SINKS && kb + KT <= a.sinks)) &&
                            (ok[0] & ok[1] & ok[2] & ok[3]);
         if (!whole) {
             const int hi = (pos < k1 ? pos : k1 - 1) - kb - 4 * g, lo = row_lo - kb - 4 * g;  // of the key's place in the tile
+            const int sink = a.sinks - kb - 4 * g;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int at_key = 32 * u + 8 * (r >> 2) + (r & 3);
-                    if (at_key > hi || at_key < lo || !ok[2 * u + (r >> 3)]) sc[u][r] = -INFINITY;
+                    if (at_key > hi || (at_key < lo && !(SINKS && at_key < sink)) || !ok[2 * u + (r >> 3)]) sc[u][r] = -INFINITY;
                 }
         }
         float mx = fmaxf(sc[0][0], sc[1][0]);
@@ -584,19 +772,21 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
             }
         __builtin_amdgcn_s_setprio(0);
     };
-    int kb = k0 & ~(KT - 1);
+    int kb = k0 & ~(KT - 1), then = after(kb);  // the tile, and the one after it
     auto turn = [&](auto which) {
         constexpr int buf = decltype(which)::value;
-        if (wrows > 0 && kb <= wlast && (a.window == 0 || kb + KT > wfirst - a.window + 1)) compute(kb, which);
-        store(kb + KT, buf ^ 1);
-        load(kb + 2 * KT);
+        if (wrows > 0 && kb <= wlast && (a.window == 0 || kb + KT > wfirst - a.window + 1 || (SINKS && kb < a.sinks))) compute(kb, which);
+        store(then, buf ^ 1);
+        const int last = after(then);
+        load(last);
         __syncthreads();
-        kb += KT;
+        kb = then;
+        then = last;
     };
     if (kb < k1) {
         load(kb);
         store(kb, 0);
-        load(kb + KT);
+        load(then);
         __syncthreads();
         while (kb < k1) {
             turn(std::integral_constant<int, 0>{});
@@ -608,17 +798,16 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     __syncthreads();
     if (wrows <= 0) return;
     if (__builtin_expect(lds.spoilt[0] | lds.spoilt[1] | lds.spoilt[2] | lds.spoilt[3], 0)) {
-        for (int t0 = k0 & ~(KT - 1); t0 < k1; t0 += KT) {
-            if (t0 + KT <= k1 && t0 >= from && t0 + KT - 1 <= upto) continue;
+        for (int t0 = k0 & ~(KT - 1); t0 < k1; t0 = after(t0)) {
+            if (t0 + KT <= k1 && (t0 >= from || (SINKS && t0 + KT <= shown)) && t0 + KT - 1 <= upto) continue;
             for (int key = t0; key < t0 + KT && key < k1; ++key) {
                 const int page = a.batch.page(s, key >> a.batch.page_shift);
-                if (page < 0 || key > pos || key < row_lo) continue;
-                const half_t *vr = a.v + page * a.batch.page_stride + head_at + static_cast<int64_t>(key & in_page) * D + 4 * g;
+                if (page < 0 || key > pos || (key < row_lo && !(SINKS && key < a.sinks))) continue;
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; r += 4) {
-                        const half4_t v = taken<4>(*reinterpret_cast<const half4_t *>(vr + 32 * d + 2 * r));
+                        const half4_t v = taken<4>(value_run<D, Q4, 4>(a, page * a.batch.page_stride + head_at, key & in_page, 32 * d + 2 * r + 4 * g));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[d][r + i] += static_cast<float>(v[i]);
                     }
@@ -656,25 +845,25 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
 
 // ---------------------------------------------------------------- the kernels
 
-template <int D>
+template <int D, bool Q4, bool SINKS>
 __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
-    rows_tile<D>(a, lds, blockIdx.x);
+    rows_tile<D, Q4, SINKS>(a, lds, blockIdx.x);
 }
 
 // Batches with long chunks: the first `large` blocks are 128-row tiles, the rest the short chunks' 16-row
 // ones, which fill the CUs that the long ones leave (a launch of its own after them: 37 us for the two chunks
 // of 501 and 332 tokens beside 29 single ones, 28 so).
-template <int D>
+template <int D, bool Q4, bool SINKS>
 __global__ __launch_bounds__(256, 2) void paged_attn_mixed(AttnArgs a, int large) {
     __shared__ __attribute__((aligned(16))) union {
         RowsLds<D> rows;
         ChunkLds<D> chunk;
     } lds;
     if (static_cast<int>(blockIdx.x) < large)
-        chunk_tile<D>(a, lds.chunk, blockIdx.x);
+        chunk_tile<D, Q4, SINKS>(a, lds.chunk, blockIdx.x);
     else
-        rows_tile<D>(a, lds.rows, static_cast<int>(blockIdx.x) - large);
+        rows_tile<D, Q4, SINKS>(a, lds.rows, static_cast<int>(blockIdx.x) - large);
 }
 
 // ---------------------------------------------------------------- the chunks' states
@@ -833,7 +1022,8 @@ constexpr int64_t kFew = 32;
 // (16 tokens of 8 kv heads over 512 / 768 / 1024: 10.9 / 15.7 / 19.2 whole, 13.1 / 15.7 / 19.0 cut).
 constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kMinChunk = 128, kWhole = 384;
 
-inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window) {
+inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window,
+                    int64_t sinks) {
     Plan p;
     const int64_t rows = tokens * gqa, live = b < tokens ? b : tokens;
     if (max_q * gqa <= kFew) {
@@ -850,7 +1040,8 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
         const int64_t most = rows / (kFew + 1) < live ? rows / (kFew + 1) : live;  // sequences of that many rows
         p.large = (rows + 127 * most) / 128;
     }
-    int64_t span = window > 0 && window + max_q + 63 < max_context ? window + max_q + 63 : max_context;
+    const int64_t seen = window + max_q + 63 + (sinks > 0 ? sinks + 63 : 0);
+    int64_t span = window > 0 && seen < max_context ? seen : max_context;
     if (span < 1) span = 1;
     if (span > int64_t(1) << 30) span = int64_t(1) << 30;  // no table holds more
     // the launch is sized for the most tiles there can be; the chunks go by what a batch of long chunks has
@@ -867,13 +1058,13 @@ inline size_t part_bytes(const Plan &p, int64_t tokens, int64_t heads, int64_t h
     return p.nsplit > 1 ? static_cast<size_t>(tokens * heads * p.nsplit * (hd + 4)) * sizeof(float) : 0;
 }
 
-template <int D>
+template <int D, bool Q4, bool SINKS>
 hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
     if (p.large > 0)
-        paged_attn_mixed<D><<<dim3(static_cast<unsigned>((p.large + p.small) * a.n_kv), a.nsplit), 256, 0, stream>>>(
+        paged_attn_mixed<D, Q4, SINKS><<<dim3(static_cast<unsigned>((p.large + p.small) * a.n_kv), a.nsplit), 256, 0, stream>>>(
             a, static_cast<int>(p.large * a.n_kv));
     else
-        paged_attn_rows<D><<<dim3(static_cast<unsigned>(p.small * a.n_kv), a.nsplit), 256, 0, stream>>>(a);
+        paged_attn_rows<D, Q4, SINKS><<<dim3(static_cast<unsigned>(p.small * a.n_kv), a.nsplit), 256, 0, stream>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
@@ -887,36 +1078,30 @@ hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
 }
 
 inline bool plannable(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t hd, int64_t max_q, int64_t max_context,
-                      int64_t window) {
-    return tokens > 0 && b > 0 && n_kv > 0 && heads > 0 && heads % n_kv == 0 && hd > 0 && max_q > 0 && max_context > 0 && window >= 0 &&
+                      int64_t window, int64_t sinks) {
+    return sinks >= 0 && sinks < (int64_t(1) << 31) && tokens > 0 && b > 0 && n_kv > 0 && heads > 0 && heads % n_kv == 0 && hd > 0 && max_q > 0 && max_context > 0 && window >= 0 &&
            tokens < (int64_t(1) << 24) && b <= kMaxSeqs && heads <= 65536 && hd <= 128 && max_q < (int64_t(1) << 31) &&
            max_context < (int64_t(1) << 31) && window < (int64_t(1) << 31);
 }
 
-}  // namespace
-}  // namespace dtts
-
-extern "C" size_t dtts_paged_attention_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
-                                                       int64_t max_q, int64_t max_context, int64_t window) {
-    using namespace dtts;
-    if (!plannable(tokens, b, heads, n_kv, head_dim, max_q, max_context, window)) return 0;
-    return part_bytes(plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window), tokens, heads, head_dim);
+template <bool Q4, bool SINKS>
+hipError_t launch_for(int64_t head_dim, const AttnArgs &a, const Plan &p, hipStream_t stream) {
+    return head_dim == 128 ? launch<128, Q4, SINKS>(a, p, stream) : launch<64, Q4, SINKS>(a, p, stream);
 }
 
-extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dtts_f16 *vpages, const int32_t *q_start,
-                                        const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens,
-                                        int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages,
-                                        int64_t max_pages, int64_t page_stride, int64_t q_stride, int64_t max_q,
-                                        int64_t max_context, int64_t window, float scale, void *workspace, size_t ws_bytes,
-                                        hipStream_t stream) {
-    using namespace dtts;
-    const char *name = "dtts_paged_attention_f16";
-    DTTS_REQUIRE_PAGED(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride);
+int attention(const char *name, int bits, const dtts_f16 *q, const void *kpages, const void *vpages, const int32_t *q_start,
+              const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens, int64_t b, int64_t heads, int64_t n_kv,
+              int64_t head_dim, int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride, int64_t q_stride, int64_t max_q,
+              int64_t max_context, int64_t window, int64_t sinks, float scale, void *workspace, size_t ws_bytes, hipStream_t stream) {
+    DTTS_REQUIRE(bits == 16 || bits == 4, "%s: pages of %d bits (16 or 4)", name, bits);
+    const int64_t units = bits == 16 ? head_dim : 5 * head_dim / 8;
+    DTTS_REQUIRE_PAGED_ROWS(name, tokens, b, n_kv, head_dim, page, n_pages, max_pages, page_stride, units, bits == 16 ? 8 : 16);
     DTTS_REQUIRE(heads > 0 && heads <= 65536 && heads % n_kv == 0, "%s: %lld heads over %lld kv heads", name, (long long)heads,
                  (long long)n_kv);
     DTTS_REQUIRE(q_stride >= heads * head_dim && q_stride % 8 == 0, "%s: q_stride %lld (a multiple of 8, at least heads * head_dim)",
                  name, (long long)q_stride);
     DTTS_REQUIRE(window >= 0 && window < (int64_t(1) << 31), "%s: window %lld", name, (long long)window);
+    DTTS_REQUIRE(sinks >= 0 && sinks < (int64_t(1) << 31), "%s: sinks %lld", name, (long long)sinks);
     if (tokens == 0 || b == 0) return DTTS_OK;
     DTTS_REQUIRE(max_q > 0 && max_context > 0 && max_q < (int64_t(1) << 31) && max_context < (int64_t(1) << 31),
                  "%s: max_q %lld, max_context %lld", name, (long long)max_q, (long long)max_context);
@@ -925,7 +1110,8 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
                      aligned(context, 4) && aligned(page_table, 4),
                  "%s: misaligned operand", name);
     DTTS_REQUIRE(std::isfinite(scale * kLog2e), "%s: scale %g", name, static_cast<double>(scale));
-    Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window);
+    if (window == 0) sinks = 0;  // every token sees them
+    Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks);
     DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large) * n_kv < (int64_t(1) << 24), "%s: too many rows", name);
     const int64_t row = heads * head_dim * static_cast<int64_t>(sizeof(half_t));
     DTTS_REQUIRE(q_stride < (int64_t(1) << 62), "%s: q_stride %lld", name, (long long)q_stride);
@@ -935,8 +1121,8 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
     a.batch = PagedBatch{q_start, context, page_table, static_cast<int>(tokens), static_cast<int>(b), log2_of(page),
                          static_cast<int>(n_pages), static_cast<int>(max_pages), page_stride};
     a.q = reinterpret_cast<const half_t *>(q);
-    a.k = reinterpret_cast<const half_t *>(kpages);
-    a.v = reinterpret_cast<const half_t *>(vpages);
+    a.k = static_cast<const half_t *>(kpages);
+    a.v = static_cast<const half_t *>(vpages);
     a.out = reinterpret_cast<half_t *>(out);
     a.q_stride = q_stride;
     a.heads = static_cast<int>(heads);
@@ -944,6 +1130,7 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
     a.gqa = static_cast<int>(heads / n_kv);
     // one of 2^30 reaches past every position that a table holds, and the differences below stay ints
     a.window = window >= int64_t(1) << 30 ? 0 : static_cast<int>(window);
+    a.sinks = a.window == 0 ? 0 : sinks >= int64_t(1) << 30 ? 1 << 30 : static_cast<int>(sinks);
     // a scale of 0 is the smallest number: every score then is 0, and a masked one still -inf
     a.scale2 = fmaxf(fabsf(scale) * kLog2e, FLT_MIN);
     a.negate = scale < 0.0f;
@@ -957,6 +1144,44 @@ extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpage
     }
     a.chunk = p.chunk;
     a.nsplit = p.nsplit;
-    DTTS_HIP_CHECK(head_dim == 128 ? launch<128>(a, p, stream) : launch<64>(a, p, stream), name);
+    const auto fn = bits == 16 ? (a.sinks > 0 ? launch_for<false, true> : launch_for<false, false>)
+                               : (a.sinks > 0 ? launch_for<true, true> : launch_for<true, false>);
+    DTTS_HIP_CHECK(fn(head_dim, a, p, stream), name);
     return DTTS_OK;
+}
+
+}  // namespace
+}  // namespace dtts
+
+extern "C" size_t dtts_paged_attention_sinks_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim, int64_t max_q,
+                                             int64_t max_context, int64_t window, int64_t sinks) {
+    using namespace dtts;
+    if (!plannable(tokens, b, heads, n_kv, head_dim, max_q, max_context, window, sinks)) return 0;
+    return part_bytes(plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, window ? sinks : 0), tokens, heads, head_dim);
+}
+
+extern "C" size_t dtts_paged_attention_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
+                                                       int64_t max_q, int64_t max_context, int64_t window) {
+    return dtts_paged_attention_sinks_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window, 0);
+}
+
+extern "C" int dtts_paged_attention(int32_t bits, const dtts_f16 *q, const void *kpages, const void *vpages, const int32_t *q_start,
+                                    const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens, int64_t b,
+                                    int64_t heads, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages, int64_t max_pages,
+                                    int64_t page_stride, int64_t q_stride, int64_t max_q, int64_t max_context, int64_t window,
+                                    int64_t sinks, float scale, void *workspace, size_t ws_bytes, hipStream_t stream) {
+    return dtts::attention("dtts_paged_attention", bits, q, kpages, vpages, q_start, context, page_table, out, tokens, b, heads, n_kv,
+                           head_dim, page, n_pages, max_pages, page_stride, q_stride, max_q, max_context, window, sinks, scale, workspace,
+                           ws_bytes, stream);
+}
+
+extern "C" int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dtts_f16 *vpages, const int32_t *q_start,
+                                        const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens,
+                                        int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages,
+                                        int64_t max_pages, int64_t page_stride, int64_t q_stride, int64_t max_q,
+                                        int64_t max_context, int64_t window, float scale, void *workspace, size_t ws_bytes,
+                                        hipStream_t stream) {
+    return dtts::attention("dtts_paged_attention_f16", 16, q, kpages, vpages, q_start, context, page_table, out, tokens, b, heads, n_kv,
+                           head_dim, page, n_pages, max_pages, page_stride, q_stride, max_q, max_context, window, 0, scale, workspace,
+                           ws_bytes, stream);
 }

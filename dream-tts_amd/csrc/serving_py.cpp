@@ -11,6 +11,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <vector>
+
 #include "dtts.h"
 
 namespace {
@@ -85,19 +87,42 @@ int64_t page_stride_of(Args &a, const Tensor *t) {
     return t->size(0) > 1 ? t->stride(0) : t->size(1) * rows;
 }
 
-struct Paged {
-    const Tensor *k, *v, *start, *context, *table;
-    int64_t b, n_kv, hd, page, n_pages, max_pages, stride;
-    Paged(Args &a, int i)
-        : k(a.tensor(i)), v(a.tensor(i + 1)), start(a.tensor(i + 2, at::kInt)), context(a.tensor(i + 3, at::kInt)),
-          table(a.tensor(i + 4, at::kInt)) {
-        a.need(a.ok && k->dim() == 4 && k->scalar_type() == at::kHalf && v->scalar_type() == at::kHalf && k->sizes() == v->sizes() &&
-               table->dim() == 2);
+// Pages of f16 values, or of bytes that hold 4-bit ones (5 D / 8 a row).
+struct Cache {
+    const Tensor *k, *v;
+    int64_t n_kv = 0, hd = 0, page = 0, n_pages = 0, stride = 0;
+    bool q4 = false;
+    Cache(Args &a, int i) : k(a.tensor(i)), v(a.tensor(i + 1)) {
+        a.need(a.ok && k->dim() == 4 && k->scalar_type() == v->scalar_type() && k->sizes() == v->sizes());
         if (!a.ok) return;
-        n_pages = k->size(0), n_kv = k->size(1), page = k->size(2), hd = k->size(3);
-        b = table->size(0), max_pages = table->size(1);
+        q4 = k->scalar_type() == at::kByte;
+        n_pages = k->size(0), n_kv = k->size(1), page = k->size(2), hd = q4 ? k->size(3) / 5 * 8 : k->size(3);
+        a.need((q4 && k->size(3) % 5 == 0) || k->scalar_type() == at::kHalf);
         stride = page_stride_of(a, k);
-        a.need(page_stride_of(a, v) == stride && context->numel() == b && start->numel() == b + 1);
+        a.need(page_stride_of(a, v) == stride);
+    }
+};
+
+struct Paged : Cache {
+    const Tensor *start, *context, *table;
+    int64_t b = 0, max_pages = 0;
+    Paged(Args &a, int i)
+        : Cache(a, i), start(a.tensor(i + 2, at::kInt)), context(a.tensor(i + 3, at::kInt)), table(a.tensor(i + 4, at::kInt)) {
+        a.need(a.ok && table->dim() == 2);
+        if (!a.ok) return;
+        b = table->size(0), max_pages = table->size(1);
+        a.need(context->numel() == b && start->numel() == b + 1);
+    }
+};
+
+// A page table and its pages' counts.
+struct Table {
+    const Tensor *pages, *refs;
+    int64_t b = 0, max_pages = 0, n_pages = 0;
+    explicit Table(Args &a) : pages(a.tensor(0, at::kInt)), refs(a.tensor(1, at::kInt)) {
+        a.need(a.ok && pages->dim() == 2 && refs->dim() == 1);
+        if (!a.ok) return;
+        b = pages->size(0), max_pages = pages->size(1), n_pages = refs->numel();
     }
 };
 
@@ -117,6 +142,16 @@ Tensor workspace_of(Args &a, int i, size_t need, const Tensor &like) {
         return t ? *t : Tensor();
     }
     return a.ok && need ? at::empty({static_cast<int64_t>(need)}, like.options().dtype(at::kByte).requires_grad(false)) : Tensor();
+}
+
+Tensor ints(const Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kInt).requires_grad(false)); }
+
+PyObject *tuple_of(std::initializer_list<Tensor> all) {
+    PyObject *t = PyTuple_New(static_cast<Py_ssize_t>(all.size()));
+    if (!t) return nullptr;
+    Py_ssize_t i = 0;
+    for (const Tensor &x : all) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(x));
+    return t;
 }
 
 PyObject *none() { Py_RETURN_NONE; }
@@ -167,35 +202,39 @@ PyObject *append(PyObject *const *args) {
     const int64_t tokens = qkv->size(0);
     const Tensor out = out_of(a, 12, *qkv, tokens, heads, p.hd);
     if (!a.ok) return none();
-    const auto call = [&](auto fn, auto x) {
+    const auto call_on = [&](auto fn, auto x, auto k, auto v) {
         return fn(x, data<float>(norms), data<float>(cos), data<float>(sin), data<int32_t>(p.start), data<int32_t>(p.context),
-                  data<int32_t>(p.table), data<dtts_f16>(&out), data<dtts_f16>(p.k), data<dtts_f16>(p.v), tokens, p.b, heads, p.n_kv,
+                  data<int32_t>(p.table), data<dtts_f16>(&out), k, v, tokens, p.b, heads, p.n_kv,
                   p.hd, 2 * cos->size(1), layout, p.page, p.n_pages, p.max_pages, p.stride, cos->size(0), eps, a.stream());
     };
-    const int status = f32 ? call(dtts_qk_rope_append_paged_f32, data<const float>(qkv))
-                           : call(dtts_qk_rope_append_paged_f16, data<const dtts_f16>(qkv));
+    const auto call = [&](auto f16_pages, auto q4_pages, auto x) {
+        return p.q4 ? call_on(q4_pages, x, p.k->data_ptr(), p.v->data_ptr()) : call_on(f16_pages, x, data<dtts_f16>(p.k), data<dtts_f16>(p.v));
+    };
+    const int status = f32 ? call(dtts_qk_rope_append_paged_f32, dtts_qk_rope_append_paged_q4_f32, data<const float>(qkv))
+                           : call(dtts_qk_rope_append_paged_f16, dtts_qk_rope_append_paged_q4_f16, data<const dtts_f16>(qkv));
     return status == DTTS_OK ? THPVariable_Wrap(out) : none();
 }
 
-// (q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale, window, out, workspace) -> out
+// (q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale, window, out, workspace, sinks) -> out
 PyObject *attention(PyObject *const *args) {
     Args a(args);
     const Tensor *q = a.tensor(0);
     const int64_t qs = rows_of(a, q);
     const Paged p(a, 1);
-    const int64_t max_q = a.integer(6), max_context = a.integer(7), window = a.integer(9);
+    const int64_t max_q = a.integer(6), max_context = a.integer(7), window = a.integer(9), sinks = args[12] == Py_None ? 0 : a.integer(12);
     const float scale = a.real(8);
     a.need(a.ok && q->scalar_type() == at::kHalf && q->size(2) == p.hd);
     if (!a.ok) return none();
     const int64_t tokens = q->size(0), heads = q->size(1);
     const Tensor out = out_of(a, 10, *q, tokens, heads, p.hd);
-    const size_t need = args[11] == Py_None ? dtts_paged_attention_workspace_bytes(tokens, p.b, heads, p.n_kv, p.hd, max_q, max_context, window) : 0;
+    const size_t need = args[11] == Py_None ? dtts_paged_attention_sinks_workspace_bytes(tokens, p.b, heads, p.n_kv, p.hd, max_q,
+                                                                                         max_context, window, sinks) : 0;
     const Tensor ws = workspace_of(a, 11, need, *q);
     if (!a.ok) return none();
-    const int status = dtts_paged_attention_f16(
-        data<dtts_f16>(q), data<dtts_f16>(p.k), data<dtts_f16>(p.v), data<int32_t>(p.start), data<int32_t>(p.context),
+    const int status = dtts_paged_attention(
+        p.q4 ? 4 : 16, data<dtts_f16>(q), p.k->data_ptr(), p.v->data_ptr(), data<int32_t>(p.start), data<int32_t>(p.context),
         data<int32_t>(p.table), data<dtts_f16>(&out), tokens, p.b, heads, p.n_kv, p.hd, p.page, p.n_pages, p.max_pages, p.stride, qs,
-        max_q, max_context, window, scale, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, a.stream());
+        max_q, max_context, window, sinks, scale, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, a.stream());
     return status == DTTS_OK ? THPVariable_Wrap(out) : none();
 }
 
@@ -223,35 +262,149 @@ PyObject *sample(PyObject *const *args) {
     };
     const int status = f32 ? call(dtts_sample_f32, data<const float>(x)) : call(dtts_sample_f16, data<const dtts_f16>(x));
     if (status != DTTS_OK) return none();
-    PyObject *both = PyTuple_New(2);
-    if (!both) return nullptr;
-    PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(token));
-    PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(logprob));
-    return both;
+    return tuple_of({token, logprob});
+}
+
+// (k_pages, v_pages, ids) -> (k, v)
+PyObject *unpack(PyObject *const *args) {
+    Args a(args);
+    const Cache c(a, 0);
+    const Tensor *ids = a.maybe(2, at::kInt);
+    a.need(a.ok && c.q4);
+    if (!a.ok) return none();
+    const int64_t n = ids ? ids->numel() : c.n_pages;
+    const auto like = c.k->options().dtype(at::kHalf).requires_grad(false);
+    const Tensor k = at::empty({n, c.n_kv, c.page, c.hd}, like), v = at::empty({n, c.n_kv, c.page, c.hd}, like);
+    const int status = dtts_unpack_pages_q4(c.k->data_ptr(), c.v->data_ptr(), data<int32_t>(ids), data<dtts_f16>(&k), data<dtts_f16>(&v), n,
+                                            c.n_kv, c.hd, c.page, c.n_pages, c.stride, a.stream());
+    return status == DTTS_OK ? tuple_of({k, v}) : none();
+}
+
+// (pages, refs, parent, out, workspace) -> out
+PyObject *fork(PyObject *const *args) {
+    Args a(args);
+    const Table t(a);
+    const Tensor *parent = a.tensor(2, at::kInt);
+    if (!a.ok) return none();
+    const int64_t n = parent->numel();
+    Tensor out;
+    if (args[3] != Py_None) {
+        const Tensor *o = a.tensor(3, at::kInt);
+        a.need(o && o->dim() == 2 && o->size(0) == n && o->size(1) == t.max_pages);
+        if (a.ok) out = *o;
+    } else {
+        out = at::empty({n, t.max_pages}, t.pages->options().requires_grad(false));
+    }
+    if (!a.ok) return none();
+    const bool in_place = out.data_ptr() == t.pages->data_ptr();
+    const Tensor ws = workspace_of(a, 4, in_place ? 4 * t.b * t.max_pages : 0, *t.pages);
+    if (!a.ok) return none();
+    const int status = dtts_fork_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(parent), data<int32_t>(&out), t.b, n,
+                                       t.max_pages, t.n_pages, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0,
+                                       a.stream());
+    return status == DTTS_OK ? THPVariable_Wrap(out) : none();
+}
+
+// (pages, refs, q_start, context, page, workspace) -> (src, dst, lacking)
+PyObject *claim(PyObject *const *args) {
+    Args a(args);
+    const Table t(a);
+    const Tensor *start = a.tensor(2, at::kInt), *context = a.tensor(3, at::kInt);
+    const int64_t page = a.integer(4);
+    a.need(a.ok && start->numel() == t.b + 1 && context->numel() == t.b);
+    if (!a.ok) return none();
+    const Tensor ws = workspace_of(a, 5, args[5] == Py_None ? dtts_claim_pages_workspace_bytes(t.b, t.max_pages, t.n_pages) : 0, *t.pages);
+    if (!a.ok) return none();
+    const Tensor src = ints(*t.pages, t.b), dst = ints(*t.pages, t.b), lacking = ints(*t.pages, 1);
+    const int status = dtts_claim_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(start), data<int32_t>(context),
+                                        data<int32_t>(&src), data<int32_t>(&dst), data<int32_t>(&lacking), t.b, page, t.max_pages,
+                                        t.n_pages, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, a.stream());
+    return status == DTTS_OK ? tuple_of({src, dst, lacking}) : none();
+}
+
+// (pages, refs, context, page, window, sinks) -> True
+PyObject *trim(PyObject *const *args) {
+    Args a(args);
+    const Table t(a);
+    const Tensor *context = a.tensor(2, at::kInt);
+    const int64_t page = a.integer(3), window = a.integer(4), sinks = a.integer(5);
+    a.need(a.ok && context->numel() == t.b);
+    if (!a.ok) return none();
+    const int status = dtts_trim_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(context), t.b, page, t.max_pages,
+                                       t.n_pages, window, sinks, a.stream());
+    if (status != DTTS_OK) return none();
+    Py_RETURN_TRUE;
+}
+
+// (pages, refs, workspace) -> (src, dst, used)
+PyObject *compact(PyObject *const *args) {
+    Args a(args);
+    const Table t(a);
+    const Tensor ws = a.ok ? workspace_of(a, 2, dtts_compact_pages_workspace_bytes(t.n_pages), *t.pages) : Tensor();
+    if (!a.ok) return none();
+    const Tensor src = ints(*t.pages, t.n_pages), dst = ints(*t.pages, t.n_pages), used = ints(*t.pages, 1);
+    const int status = dtts_compact_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(&src), data<int32_t>(&dst),
+                                          data<int32_t>(&used), t.b, t.max_pages, t.n_pages, ws.defined() ? ws.data_ptr() : nullptr,
+                                          ws.defined() ? ws.numel() : 0, a.stream());
+    return status == DTTS_OK ? tuple_of({src, dst, used}) : none();
+}
+
+// (caches, src, dst) -> True; caches a list or a tuple
+PyObject *copy(PyObject *const *args) {
+    Args a(args);
+    const Tensor *src = a.tensor(1, at::kInt), *dst = a.tensor(2, at::kInt);
+    a.need(a.ok && src->numel() == dst->numel() && (PyList_Check(args[0]) || PyTuple_Check(args[0])));
+    if (!a.ok) return none();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(args[0]);
+    Args of(PySequence_Fast_ITEMS(args[0]));
+    of.device = a.device;
+    std::vector<void *> at(n);
+    std::vector<int64_t> size(n), stride(n);
+    int64_t n_pages = 0;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor *t = of.tensor(static_cast<int>(i));
+        if (!t || t->dim() < 2 || t->numel() == 0 || (i && t->size(0) != n_pages)) return none();
+        n_pages = t->size(0);
+        int64_t row = 1;  // contiguous pages; the stride of a size of 1 is no one's
+        for (int64_t d = t->dim() - 1; d > 0; row *= t->size(d), --d)
+            if (t->size(d) != 1 && t->stride(d) != row) return none();
+        at[i] = t->data_ptr();
+        size[i] = row * t->element_size();
+        stride[i] = n_pages > 1 ? t->stride(0) * static_cast<int64_t>(t->element_size()) : size[i];
+    }
+    if (n > 0 && dtts_copy_pages(at.data(), size.data(), stride.data(), n, data<int32_t>(src), data<int32_t>(dst), src->numel(), n_pages,
+                                 a.stream()) != DTTS_OK)
+        return none();
+    Py_RETURN_TRUE;
 }
 
 // No C++ exception leaves: where torch refuses an allocation, nothing is enqueued yet, and the Python path meets the
 // same refusal.
-template <PyObject *(*F)(PyObject *const *), int N>
+template <PyObject *(*F)(PyObject *const *), int N, int OPTIONAL>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    if (n != N) {
+    if (n > N || n < N - OPTIONAL) {
         PyErr_Format(PyExc_TypeError, "%d arguments expected, got %zd", N, n);
         return nullptr;
     }
+    PyObject *all[N];
+    for (int i = 0; i < N; ++i) all[i] = i < n ? args[i] : Py_None;
     try {
-        return F(args);
+        return F(all);
     } catch (...) {
         return none();
     }
 }
 
-template <PyObject *(*F)(PyObject *const *), int N>
+template <PyObject *(*F)(PyObject *const *), int N, int OPTIONAL = 0>
 PyMethodDef method(const char *name) {
-    return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<F, N>)), METH_FASTCALL, nullptr};
+    return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<F, N, OPTIONAL>)), METH_FASTCALL, nullptr};
 }
 
 PyMethodDef kMethods[] = {method<rotary, 6>("rotary"), method<append, 13>("qk_rope_append_paged"),
-                          method<attention, 12>("paged_attention"), method<sample, 7>("sample"), {nullptr, nullptr, 0, nullptr}};
+                          method<attention, 13, 1>("paged_attention"), method<sample, 7>("sample"),
+                          method<unpack, 3>("unpack_pages"), method<fork, 5>("fork_pages"), method<claim, 6>("claim_pages"),
+                          method<trim, 6>("trim_pages"), method<compact, 3>("compact_pages"), method<copy, 3>("copy_pages"),
+                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -74,6 +74,18 @@ SIGNATURES = {
     "dtts_qk_rope_append_paged_f16": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],
     "dtts_paged_attention_workspace_bytes": [_I64] * 8,
     "dtts_paged_attention_f16": [_P] * 7 + [_I64] * 13 + [_F32, _P, _SZ, _P],
+    "dtts_paged_attention_sinks_workspace_bytes": [_I64] * 9,
+    "dtts_paged_attention": [_I32] + [_P] * 7 + [_I64] * 14 + [_F32, _P, _SZ, _P],
+    "dtts_qk_rope_append_paged_q4_f32": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],
+    "dtts_qk_rope_append_paged_q4_f16": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],
+    "dtts_unpack_pages_q4": [_P] * 5 + [_I64] * 6 + [_P],
+    "dtts_fork_pages": [_P] * 4 + [_I64] * 4 + [_P, _SZ, _P],
+    "dtts_claim_pages_workspace_bytes": [_I64] * 3,
+    "dtts_claim_pages": [_P] * 7 + [_I64] * 4 + [_P, _SZ, _P],
+    "dtts_trim_pages": [_P] * 3 + [_I64] * 6 + [_P],
+    "dtts_compact_pages_workspace_bytes": [_I64],
+    "dtts_compact_pages": [_P] * 5 + [_I64] * 3 + [_P, _SZ, _P],
+    "dtts_copy_pages": [_P] * 3 + [_I64] + [_P] * 2 + [_I64] * 2 + [_P],
     "dtts_sample_workspace_bytes": [_I64, _I64],
     "dtts_sample_f32": [_P] * 8 + [_I64] * 3 + [_P, _SZ, _P],
     "dtts_sample_f16": [_P] * 8 + [_I64] * 3 + [_P, _SZ, _P],
@@ -153,6 +165,8 @@ _RESTYPES = {"dtts_last_error": ctypes.c_char_p, "dtts_codec_destroy": None,
              "dtts_codec_hop": ctypes.c_int64, "dtts_codec_workspace_bytes": ctypes.c_size_t,
              "dtts_decode_attention_workspace_bytes": ctypes.c_size_t,
              "dtts_paged_attention_workspace_bytes": ctypes.c_size_t, "dtts_sample_workspace_bytes": ctypes.c_size_t,
+             "dtts_paged_attention_sinks_workspace_bytes": ctypes.c_size_t, "dtts_claim_pages_workspace_bytes": ctypes.c_size_t,
+             "dtts_compact_pages_workspace_bytes": ctypes.c_size_t,
              "dtts_gemm_f16_workspace_bytes": ctypes.c_size_t, "dtts_stack_destroy": None,
              "dtts_stack_workspace_bytes": ctypes.c_size_t, "dtts_gemm_f32_nt_workspace_bytes": ctypes.c_size_t, "dtts_stack_prefill_workspace_bytes": ctypes.c_size_t, "dtts_codec_front_destroy": None,
              "dtts_codec_front_workspace_bytes": ctypes.c_size_t,

@@ -1,9 +1,10 @@
 """What a server of many requests calls beside the ops of ``dtts.ops``: rotary positions of every
-layout and scaling, a paged KV cache's write and attention over ragged batches, and sampling.
+layout and scaling, a paged KV cache's write and attention over ragged batches (f16 or in 4 bits), its
+pages' forks, claims, trims, moves and copies, and sampling.
 
 A step of a batch is: project to qkv, ``qk_rope_append_paged`` (queries turned, keys and values into
 their pages), ``paged_attention``, the output projection, and after the last layer logits to
-``sample``. Lengths, positions, page tables and sampling settings are device tensors, so a step
+``sample``. Before a step, ``claim_pages`` gives each sequence the pages that its new tokens go to. Lengths, positions, page tables and sampling settings are device tensors, so a step
 captured into a graph is replayed while they change. Outputs are allocated unless given.
 
 Every tensor of a call is on one device; the work goes to that device's current stream.
@@ -29,10 +30,11 @@ try:
 except ImportError as e:
     warnings.warn(f"dtts/_serving.so is not built for this torch ({e}): calls of dtts.serving take some microseconds longer; "
                   "run dream-tts_amd/build.py", RuntimeWarning)
-    _serving = types.SimpleNamespace(**dict.fromkeys(("rotary", "qk_rope_append_paged", "paged_attention", "sample"),
-                                                     lambda *args: None))
+    _serving = types.SimpleNamespace(**dict.fromkeys(
+        ("rotary", "qk_rope_append_paged", "paged_attention", "sample", "unpack_pages", "fork_pages", "claim_pages", "trim_pages",
+         "compact_pages", "copy_pages"), lambda *args: None))
 
-_F16, _F32, _I32 = torch.float16, torch.float32, torch.int32
+_F16, _F32, _I32, _U8 = torch.float16, torch.float32, torch.int32, torch.uint8
 _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 _Tensor = torch.Tensor
 
@@ -144,31 +146,37 @@ def _page_stride(name, t):
     return st[0] if n_pages > 1 else n_kv * page * hd
 
 
-def _paged(name, device, k_pages, v_pages, q_start, context, pages):
-    """Checks the cache [n_pages, n_kv, page, D] (each page contiguous) and the batch's arrays: b, n_kv, D,
-    page, n_pages, max_pages and the elements between pages."""
-    tensors = (k_pages, v_pages, q_start, context, pages)
-    for t in tensors:
-        if not isinstance(t, _Tensor) or t.get_device() != device:
-            break
-    else:
-        if (k_pages.dtype is _F16 and v_pages.dtype is _F16 and q_start.dtype is _I32 and context.dtype is _I32
-                and pages.dtype is _I32 and q_start.is_contiguous() and context.is_contiguous() and pages.is_contiguous()):
-            tensors = None
-    if tensors is not None:
-        for t, what, dtype in zip(tensors, ("k_pages", "v_pages", "q_start", "context", "pages"), (_F16, _F16, _I32, _I32, _I32)):
-            _need(name, device, what, t, (dtype,), contiguous=dtype is _I32)
+def _cache(name, device, k_pages, v_pages):
+    """Checks the cache's pages [n_pages, n_kv, page, D] f16 or [n_pages, n_kv, page, 5 D / 8] uint8 (each contiguous): n_kv, D,
+    page, n_pages, the elements (bytes) between pages, and the bits of a value."""
+    for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if not isinstance(t, _Tensor) or t.get_device() != device or (t.dtype is not _F16 and t.dtype is not _U8):
+            _need(name, device, what, t, (_F16, _U8), contiguous=False)
     shape = k_pages.shape
-    if len(shape) != 4 or shape != v_pages.shape:
-        raise DttsError(f"{name}: k pages {tuple(shape)} and v pages {tuple(v_pages.shape)}")
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype:
+        raise DttsError(f"{name}: k pages {tuple(shape)} {k_pages.dtype} and v pages {tuple(v_pages.shape)} {v_pages.dtype}")
     stride = _page_stride(name, k_pages)
     if stride != _page_stride(name, v_pages):
         raise DttsError(f"{name}: k pages {k_pages.stride()} and v pages {v_pages.stride()} apart")
-    n_pages, n_kv, page, hd = shape
+    n_pages, n_kv, page, row = shape
+    if k_pages.dtype is _F16:
+        return n_kv, row, page, n_pages, stride, 16
+    if row % 5:
+        raise DttsError(f"{name}: rows of {row} bytes are not 5 D / 8")
+    return n_kv, row * 8 // 5, page, n_pages, stride, 4
+
+
+def _paged(name, device, k_pages, v_pages, q_start, context, pages):
+    """Checks the cache and the batch's arrays: b, n_kv, D, page, n_pages, max_pages, the elements between pages and the bits of
+    a value."""
+    n_kv, hd, page, n_pages, stride, bits = _cache(name, device, k_pages, v_pages)
+    for t, what in ((q_start, "q_start"), (context, "context"), (pages, "pages")):
+        if not (isinstance(t, _Tensor) and t.dtype is _I32 and t.get_device() == device and t.is_contiguous()):
+            _need(name, device, what, t, (_I32,))
     table = pages.shape
     if len(table) != 2 or table[0] != context.numel() or q_start.numel() != table[0] + 1:
         raise DttsError(f"{name}: page table {tuple(table)}, {context.numel()} contexts, {q_start.numel()} starts")
-    return table[0], n_kv, hd, page, n_pages, table[1], stride
+    return table[0], n_kv, hd, page, n_pages, table[1], stride, bits
 
 
 def _out(name, device, out, like, tokens, heads, hd):
@@ -197,7 +205,7 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
                          interleaved=False, out=None):
     """QK-norm (norms [2, D] f32, or None), rotary positions and the write of a ragged batch's new keys and
     values: qkv [tokens, (heads + 2 n_kv) D] f32 or f16 -> queries [tokens, heads, D] f16; k_pages and
-    v_pages [n_pages, n_kv, page, D] f16 are written in place. q_start [b + 1], context [b] (new tokens
+    v_pages, [n_pages, n_kv, page, D] f16 or 4-bit pages [n_pages, n_kv, page, 5 D / 8] uint8, are written in place. q_start [b + 1], context [b] (new tokens
     included) and pages [b, max_pages] are int32; see dtts.h for what each selects. Rows of `out` that
     belong to no sequence are left as they were. `out` is no part of qkv, and the pages share no memory."""
     y = _serving.qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, pages, heads, norms, eps, interleaved, out)
@@ -210,7 +218,7 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
     f32 = qkv.dtype is _F32
     if dev < 0 or not (f32 or qkv.dtype is _F16) or not qkv.is_contiguous():
         _need(name, dev, "qkv", qkv, (_F32, _F16))
-    b, n_kv, hd, page, n_pages, max_pages, stride = _paged(name, dev, k_pages, v_pages, q_start, context, pages)
+    b, n_kv, hd, page, n_pages, max_pages, stride, bits = _paged(name, dev, k_pages, v_pages, q_start, context, pages)
     n, half = _tables(name, dev, cos, sin)
     size = qkv.shape
     if len(size) != 2 or size[1] != (heads + 2 * n_kv) * hd:
@@ -222,7 +230,7 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
             raise DttsError(f"{name}: norms {tuple(norms.shape)} is not [2, {hd}]")
     tokens = size[0]
     out = _out(name, dev, out, qkv, tokens, heads, hd)
-    _enqueue("dtts_qk_rope_append_paged_f32" if f32 else "dtts_qk_rope_append_paged_f16", dev, qkv.data_ptr(),
+    _enqueue(f"dtts_qk_rope_append_paged_{'q4_' if bits == 4 else ''}{'f32' if f32 else 'f16'}", dev, qkv.data_ptr(),
              None if norms is None else norms.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_start.data_ptr(),
              context.data_ptr(), pages.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tokens, b, heads,
              n_kv, hd, 2 * half, 1 if interleaved else 0, page, n_pages, max_pages, stride, n, float(eps))
@@ -230,21 +238,23 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
 
 
 @functools.lru_cache(maxsize=4096)
-def paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window=0):
+def paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window=0, sinks=0):
     """Workspace bytes paged_attention splits contexts over workgroups with."""
-    return int(lib().dtts_paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, int(max_q), int(max_context),
-                                                          int(window)))
+    return int(lib().dtts_paged_attention_sinks_workspace_bytes(tokens, b, heads, n_kv, head_dim, int(max_q), int(max_context),
+                                                                int(window), int(sinks)))
 
 
 def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale=1.0, window=0, out=None,
-                    workspace=None):
-    """Attention of a ragged batch's new tokens over their pages, their own keys included: q [tokens, heads,
-    D] f16 (rows may be strided) -> [tokens, heads, D] f16. Each token attends to its sequence's positions
-    up to its own, the last `window` of them when set. max_q and max_context (the longest chunk and context)
+                    workspace=None, sinks=0):
+    """Attention of a ragged batch's new tokens over their pages (f16, or 4-bit ones as qk_rope_append_paged
+    writes them), their own keys included: q [tokens, heads, D] f16 (rows may be strided) -> [tokens, heads,
+    D] f16. Each token attends to its sequence's positions up to its own, when `window` is set to the last
+    `window` of them and to the sequence's first `sinks`. max_q and max_context (the longest chunk and context)
     size the launch and never change what is computed. `workspace`: a device byte tensor of
     paged_attention_workspace_bytes (allocated when not given). Rows of `out` that belong to no sequence are
     left as they were; a token that sees no position gets zeros. `out` shares no memory with q."""
-    y = _serving.paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale, window, out, workspace)
+    y = _serving.paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale, window, out, workspace,
+                                 sinks)
     if y is not None:
         return y
     name = "paged_attention"
@@ -254,19 +264,174 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
     if dev < 0:
         _need(name, dev, "q", q, (_F16,), contiguous=False)
     (tokens, heads, qd), qs = _rows(name, q, "q")
-    b, n_kv, hd, page, n_pages, max_pages, stride = _paged(name, dev, k_pages, v_pages, q_start, context, pages)
+    b, n_kv, hd, page, n_pages, max_pages, stride, bits = _paged(name, dev, k_pages, v_pages, q_start, context, pages)
     if qd != hd:
         raise DttsError(f"{name}: q {tuple(q.shape)} over pages of head_dim {hd}")
     out = _out(name, dev, out, q, tokens, heads, hd)
-    need = 0 if workspace is not None else paged_attention_workspace_bytes(tokens, b, heads, n_kv, hd, max_q, max_context, window)
+    need = 0 if workspace is not None else paged_attention_workspace_bytes(tokens, b, heads, n_kv, hd, max_q, max_context, window,
+                                                                                      sinks)
     keep = ws = None
     ws_bytes = 0
     if need or workspace is not None:
         keep, ws, ws_bytes = _bytes(name, dev, workspace, need, q)
-    _enqueue("dtts_paged_attention_f16", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_start.data_ptr(),
+    _enqueue("dtts_paged_attention", dev, bits, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_start.data_ptr(),
              context.data_ptr(), pages.data_ptr(), out.data_ptr(), tokens, b, heads, n_kv, hd, page, n_pages, max_pages, stride,
-             qs, int(max_q), int(max_context), int(window), float(scale), ws, ws_bytes)
+             qs, int(max_q), int(max_context), int(window), int(sinks), float(scale), ws, ws_bytes)
     return out
+
+
+def unpack_pages(k_pages, v_pages, ids=None):
+    """The values (k, v) [n, n_kv, page, D] f16 of 4-bit pages [n_pages, n_kv, page, 5 D / 8] uint8: of all of
+    them, or of the pages ids [n] int32 (a row of a page table, say; an id outside the pool leaves its part unset).
+    Slots that hold no position stand for whatever is there."""
+    y = _serving.unpack_pages(k_pages, v_pages, ids)
+    if y is not None:
+        return y
+    name = "unpack_pages"
+    if not isinstance(k_pages, _Tensor):
+        raise DttsError(f"{name}: k_pages must be a tensor")
+    dev = k_pages.get_device()
+    n_kv, hd, page, n_pages, stride, bits = _cache(name, dev, k_pages, v_pages)
+    if bits != 4:
+        raise DttsError(f"{name}: k_pages dtype {k_pages.dtype} not in ({_U8},)")
+    if ids is not None:
+        _need(name, dev, "ids", ids, (_I32,))
+    n = n_pages if ids is None else ids.numel()
+    k, v = (torch.empty((n, n_kv, page, hd), dtype=_F16, device=k_pages.device) for _ in range(2))
+    _enqueue("dtts_unpack_pages_q4", dev, k_pages.data_ptr(), v_pages.data_ptr(), None if ids is None else ids.data_ptr(),
+             k.data_ptr(), v.data_ptr(), n, n_kv, hd, page, n_pages, stride)
+    return k, v
+
+
+# ---------------------------------------------------------------- the cache's pages between steps
+
+def _table(name, pages, refs, *more):
+    """Checks a page table, its pages' counts and further int32 arrays (tensor, name, elements): the device."""
+    if not isinstance(pages, _Tensor):
+        raise DttsError(f"{name}: pages must be a tensor")
+    dev = pages.get_device()
+    for t, what in ((pages, "pages"), (refs, "refs"), *((t, what) for t, what, _ in more)):
+        if not (isinstance(t, _Tensor) and t.dtype is _I32 and t.get_device() == dev and t.is_contiguous()) or dev < 0:
+            _need(name, dev, what, t, (_I32,))
+    if pages.dim() != 2 or refs.dim() != 1:
+        raise DttsError(f"{name}: pages {tuple(pages.shape)} and refs {tuple(refs.shape)} must be [b, max_pages] and [n_pages]")
+    for t, what, n in more:
+        if n is not None and t.numel() != n:
+            raise DttsError(f"{name}: {t.numel()} of {what} for a page table {tuple(pages.shape)}")
+    return dev
+
+
+def _empty_i32(n, like):
+    return torch.empty(n, dtype=_I32, device=like.device)
+
+
+def fork_pages(pages, refs, parent, out=None, workspace=None):
+    """A table whose row i has the pages of row parent[i] (int32 [n]; none for a parent outside the table), and refs
+    (int32 [n_pages], how many entries hold each page) brought up to it in place: forks and reorders sequences and
+    frees those that no row takes over. `out`: None for a new table [n, max_pages], or `pages` itself for the
+    change in place (through a workspace of as many bytes, allocated when not given)."""
+    y = _serving.fork_pages(pages, refs, parent, out, workspace)
+    if y is not None:
+        return y
+    name = "fork_pages"
+    dev = _table(name, pages, refs, (parent, "parent", None))
+    (b, m), n = pages.shape, parent.numel()
+    if out is None:
+        out = torch.empty((n, m), dtype=_I32, device=pages.device)
+    else:
+        _need(name, dev, "out", out, (_I32,))
+        if out.shape != (n, m):
+            raise DttsError(f"{name}: out {tuple(out.shape)} is not [{n}, {m}]")
+    keep, ws, ws_bytes = _bytes(name, dev, workspace, 4 * b * m if out.data_ptr() == pages.data_ptr() else 0, pages)
+    _enqueue("dtts_fork_pages", dev, pages.data_ptr(), refs.data_ptr(), parent.data_ptr(), out.data_ptr(), b, n, m, refs.numel(), ws,
+             ws_bytes)
+    return out
+
+
+def claim_pages_workspace_bytes(b, max_pages, n_pages):
+    return int(lib().dtts_claim_pages_workspace_bytes(b, max_pages, n_pages))
+
+
+def claim_pages(pages, refs, q_start, context, page, workspace=None):
+    """Before a step writes: a page of its own for every block of `page` positions that a sequence's new tokens go to. Missing
+    ones come from the free pages (refs under 1), lowest first, and a page that other sequences hold too is replaced.
+    pages [b, max_pages] and refs [n_pages] change in place; returns (src, dst, lacking) int32 [b], [b], [1]: copy_pages carries
+    src and dst out in every layer's pools, and where lacking is above 0 there were that many free pages too few and nothing was
+    changed: the step must wait."""
+    y = _serving.claim_pages(pages, refs, q_start, context, page, workspace)
+    if y is not None:
+        return y
+    name = "claim_pages"
+    b = pages.shape[0] if isinstance(pages, _Tensor) and pages.dim() == 2 else 0
+    dev = _table(name, pages, refs, (q_start, "q_start", b + 1), (context, "context", b))
+    src, dst, lacking = _empty_i32(b, pages), _empty_i32(b, pages), _empty_i32(1, pages)
+    keep, ws, ws_bytes = _bytes(name, dev, workspace, claim_pages_workspace_bytes(b, pages.shape[1], refs.numel()), pages)
+    _enqueue("dtts_claim_pages", dev, pages.data_ptr(), refs.data_ptr(), q_start.data_ptr(), context.data_ptr(), src.data_ptr(),
+             dst.data_ptr(), lacking.data_ptr(), b, int(page), pages.shape[1], refs.numel(), ws, ws_bytes)
+    return src, dst, lacking
+
+
+def trim_pages(pages, refs, context, page, window, sinks=0):
+    """Frees, in place, the pages that tokens from position context[s] on see nothing of under `window` and `sinks`."""
+    if _serving.trim_pages(pages, refs, context, page, window, sinks) is not None:
+        return
+    name = "trim_pages"
+    b = pages.shape[0] if isinstance(pages, _Tensor) and pages.dim() == 2 else 0
+    dev = _table(name, pages, refs, (context, "context", b))
+    _enqueue("dtts_trim_pages", dev, pages.data_ptr(), refs.data_ptr(), context.data_ptr(), b, int(page), pages.shape[1], refs.numel(),
+             int(window), int(sinks))
+
+
+def compact_pages_workspace_bytes(n_pages):
+    return int(lib().dtts_compact_pages_workspace_bytes(n_pages))
+
+
+def compact_pages(pages, refs, workspace=None):
+    """Gives the pages in use the first ids, so that a pool can end after them: pages and refs change in place; returns (src, dst,
+    used) int32 [n_pages], [n_pages], [1]: the moves that copy_pages carries out in every layer's pools, and how many pages are
+    in use. Other tables over the same pools hold none of these ids any more."""
+    y = _serving.compact_pages(pages, refs, workspace)
+    if y is not None:
+        return y
+    name = "compact_pages"
+    dev = _table(name, pages, refs)
+    n = refs.numel()
+    src, dst, used = _empty_i32(n, pages), _empty_i32(n, pages), _empty_i32(1, pages)
+    keep, ws, ws_bytes = _bytes(name, dev, workspace, compact_pages_workspace_bytes(n), pages)
+    _enqueue("dtts_compact_pages", dev, pages.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), used.data_ptr(),
+             pages.shape[0], pages.shape[1], n, ws, ws_bytes)
+    return src, dst, used
+
+
+def copy_pages(caches, src, dst):
+    """Page src[i] to page dst[i] (int32) in each of `caches`, tensors [n_pages, ...] whose pages are contiguous and some
+    multiple of 16 bytes: f16 and 4-bit pages of any number of layers at once. Pairs with an id outside the pool (the -1 of
+    claim_pages and compact_pages) copy nothing. A page is the destination of one pair at most, and then no source."""
+    if isinstance(caches, _Tensor):
+        caches = (caches,)
+    if _serving.copy_pages(caches, src, dst) is not None:
+        return
+    name = "copy_pages"
+    if not isinstance(src, _Tensor):
+        raise DttsError(f"{name}: src must be a tensor")
+    dev = src.get_device()
+    _need(name, dev, "src", src, (_I32,))
+    _need(name, dev, "dst", dst, (_I32,))
+    if src.numel() != dst.numel():
+        raise DttsError(f"{name}: {src.numel()} sources and {dst.numel()} destinations")
+    caches = list(caches)
+    at, size, stride = ((t * len(caches))() for t in (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64))
+    for i, t in enumerate(caches):
+        if not isinstance(t, _Tensor):
+            raise DttsError(f"{name}: cache {i} must be a tensor")
+        _need(name, dev, f"cache {i}", t, (t.dtype,), contiguous=False)
+        if t.dim() < 2 or t.shape[0] != caches[0].shape[0] or t.numel() == 0 or not t[0].is_contiguous():
+            raise DttsError(f"{name}: cache {i} {tuple(t.shape)} {t.stride()} is not [{caches[0].shape[0]}, ...] with contiguous pages")
+        at[i] = t.data_ptr()
+        size[i] = t[0].numel() * t.element_size()
+        stride[i] = t.stride(0) * t.element_size() if t.shape[0] > 1 else size[i]
+    if caches:
+        _enqueue("dtts_copy_pages", dev, at, size, stride, len(caches), src.data_ptr(), dst.data_ptr(), src.numel(), caches[0].shape[0])
 
 
 # ---------------------------------------------------------------- sampling

@@ -527,6 +527,88 @@ int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dt
                              int64_t max_pages, int64_t page_stride, int64_t q_stride, int64_t max_q, int64_t max_context,
                              int64_t window, float scale, void *workspace, size_t ws_bytes, hipStream_t stream);
 
+/* The same with `sinks`: beside its window a token sees the sequence's first `sinks` positions (those up to its own), so a stream can
+ * run on past its window over the first tokens that its attention rests on. Pages that hold neither may be freed
+ * (dtts_trim_pages). Without a window sinks count for nothing. And over pages of `bits`: 16, as above, or 4.
+ *
+ * 4-bit pages take 5 D / 8 bytes a row in the place of 2 D. kpages and vpages are bytes, 16-byte aligned; page_stride counts
+ * bytes (a multiple of 16, at least n_kv * page * 5 D / 8, under 2^32). A row's values in groups of 32 share an f16 pair
+ * (d, b); a value is f16(c d + b), one rounding, c = 64 + n with its 4 bits n. A page of a kv head is the rows' codes, D / 8
+ * words of 32 bits a row (element 8 w + 2 i of a row in bits 4 i of its word w, element 8 w + 2 i + 1 in bits 16 + 4 i), keys'
+ * words in the order [row][w], values' in [row / 4][w][row % 4]; then the pairs, d in the low half, [D / 32][row].
+ *
+ * dtts_qk_rope_append_paged_q4_*: dtts_qk_rope_append_paged_* into 4-bit pages. Of a group's f32 values
+ * d = f16((max - min) / 15), b = f16(min - 64 d), n = (x - (64 d + b)) / d rounded to the nearest (ties to even) from 0 to 15
+ * (0 where d is 0). A group with a value that is not finite, or whose values pass f16's range in this form (its least minus
+ * 4.27 times its width, where the width is its largest less its least), is NaN, all 32.
+ * dtts_unpack_pages_q4: the f16 pages [n, n_kv, page, D] that the pages ids[0 .. n - 1] (DEVICE; NULL: the first n) stand for,
+ * whatever their slots hold; an id outside [0, n_pages) leaves its part as it was. */
+size_t dtts_paged_attention_sinks_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
+                                                  int64_t max_q, int64_t max_context, int64_t window, int64_t sinks);
+int dtts_paged_attention(int32_t bits, const dtts_f16 *q, const void *kpages, const void *vpages, const int32_t *q_start,
+                         const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens, int64_t b,
+                         int64_t heads, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages, int64_t max_pages,
+                         int64_t page_stride, int64_t q_stride, int64_t max_q, int64_t max_context, int64_t window,
+                         int64_t sinks, float scale, void *workspace, size_t ws_bytes, hipStream_t stream);
+int dtts_qk_rope_append_paged_q4_f32(const float *qkv, const float *norms, const float *cos_t, const float *sin_t,
+                                     const int32_t *q_start, const int32_t *context, const int32_t *page_table,
+                                     dtts_f16 *q_out, void *kpages, void *vpages, int64_t tokens, int64_t b,
+                                     int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
+                                     int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
+                                     int64_t table_len, float eps, hipStream_t stream);
+int dtts_qk_rope_append_paged_q4_f16(const dtts_f16 *qkv, const float *norms, const float *cos_t, const float *sin_t,
+                                     const int32_t *q_start, const int32_t *context, const int32_t *page_table,
+                                     dtts_f16 *q_out, void *kpages, void *vpages, int64_t tokens, int64_t b,
+                                     int64_t heads, int64_t n_kv, int64_t head_dim, int64_t rot_dim, int32_t layout,
+                                     int64_t page, int64_t n_pages, int64_t max_pages, int64_t page_stride,
+                                     int64_t table_len, float eps, hipStream_t stream);
+int dtts_unpack_pages_q4(const void *kpages, const void *vpages, const int32_t *ids, dtts_f16 *k_out, dtts_f16 *v_out,
+                         int64_t n, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages, int64_t page_stride,
+                         hipStream_t stream);
+
+/* The pages themselves, between steps. page_table [b, max_pages] as above, refs DEVICE int32[n_pages]: how many of its entries
+ * hold each page; under 1 the page is free. What each call reads and writes is on the device, so all of them can be captured; a
+ * result depends on its arguments alone (free pages are given out from the lowest id on, sequences are served in order). One
+ * table serves every layer's pools: ids are decided once, and dtts_copy_pages carries out what has to be copied in all of them.
+ * n_pages <= 2^24, b <= 65536, b * max_pages < 2^31. Calls on one table or refs are ordered by the caller, and a call's
+ * operands share no memory (refused).
+ *
+ * dtts_fork_pages: row i of `out` [n, max_pages] takes the entries of row parent[i] of page_table [b, max_pages] (outside
+ * [0, b): -1 in all of them), and refs follow: forks, reorders beams and frees rows in one step. out is another table, or
+ * page_table itself with n == b and a workspace of b * max_pages * 4 bytes (without it refused).
+ *
+ * dtts_claim_pages: before a step writes, a page of its own for each block of positions that a sequence's new tokens
+ * (positions context[s] - n to context[s] - 1, n of q_start, within the table) go to. A block without a page that is in use
+ * gets a free one; a page with other owners is replaced by one, so that the writes of one do not reach the others (of c writers
+ * to a page of r owners the first min(c, r - 1) in order). src[s] and dst[s] [b]: where positions before the new ones are in
+ * that page, what to copy, or -1. lacking[0]: how many free pages there are too few; above 0 nothing was changed, src and dst
+ * are -1, and the step must wait. workspace of dtts_claim_pages_workspace_bytes (refused without it).
+ * Cost beside the trips to memory: a writer to a shared page is ranked among the earlier writers, one after another.
+ *
+ * dtts_trim_pages: entries whose positions no later token sees under `window` and `sinks` become -1 (blocks that end at
+ * context[s] - window + 1 or before and start at `sinks` or later), refs follow. window > 0.
+ *
+ * dtts_compact_pages: the pages in use come to be the first ones, used[0] in number: those past them move to the free ids
+ * below, in order. The table's entries and refs are rewritten, src and dst [n_pages] list the moves, -1 past their last; entries that hold no
+ * page in use become -1. workspace of dtts_compact_pages_workspace_bytes (refused without it).
+ *
+ * dtts_copy_pages: in each of n_caches pools (HOST arrays: its address, bytes of a page, bytes from page to page; multiples of
+ * 16) page src[i] to page dst[i], i < n (DEVICE arrays; pairs with an id outside [0, n_pages) copy nothing). No page is the
+ * destination of two pairs, nor of one and the source of another: what such pages hold afterwards is not said. */
+int dtts_fork_pages(const int32_t *page_table, int32_t *refs, const int32_t *parent, int32_t *out, int64_t b, int64_t n,
+                    int64_t max_pages, int64_t n_pages, void *workspace, size_t ws_bytes, hipStream_t stream);
+size_t dtts_claim_pages_workspace_bytes(int64_t b, int64_t max_pages, int64_t n_pages);
+int dtts_claim_pages(int32_t *page_table, int32_t *refs, const int32_t *q_start, const int32_t *context, int32_t *src,
+                     int32_t *dst, int32_t *lacking, int64_t b, int64_t page, int64_t max_pages, int64_t n_pages,
+                     void *workspace, size_t ws_bytes, hipStream_t stream);
+int dtts_trim_pages(int32_t *page_table, int32_t *refs, const int32_t *context, int64_t b, int64_t page, int64_t max_pages,
+                    int64_t n_pages, int64_t window, int64_t sinks, hipStream_t stream);
+size_t dtts_compact_pages_workspace_bytes(int64_t n_pages);
+int dtts_compact_pages(int32_t *page_table, int32_t *refs, int32_t *src, int32_t *dst, int32_t *used, int64_t b,
+                       int64_t max_pages, int64_t n_pages, void *workspace, size_t ws_bytes, hipStream_t stream);
+int dtts_copy_pages(void **caches, const int64_t *page_bytes, const int64_t *page_strides, int64_t n_caches,
+                    const int32_t *src, const int32_t *dst, int64_t n, int64_t n_pages, hipStream_t stream);
+
 /* Sampling: one token per row of logits [rows, vocab] (row_stride elements apart), from a given uniform
  * random number. Per row, with the settings of the DEVICE arrays [rows] (each may be NULL: off):
  *   w_i = exp((l_i - max l) / temperature); tokens in order of logit, equal ones by index;
