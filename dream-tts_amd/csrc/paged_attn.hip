@@ -23,6 +23,9 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// The fewest keys of a chunk: 128 / 256 / 512, one token over 1024 keys 8.1 / 9.1 / 11.6 us.
+constexpr int kMinChunk = 128;
+
 struct AttnArgs {
     PagedBatch batch;
     const half_t *q, *k, *v;  // k and v: of 4-bit pages their bytes, and the batch's page stride counts those
@@ -33,6 +36,9 @@ struct AttnArgs {
     float scale2;      // |scale| * log2(e), above 0: the softmax runs in base 2, its maxima are those of q . k
     bool negate;       // scale < 0: the queries change sign
     int chunk, nsplit; // keys per chunk, chunks at most (the last takes what is left)
+    int target;        // above 0: the chunk is chosen for this many units (tiles' chunks) of a kv head, see shared_blocks
+    float per_target;  // 1 / target
+    FastDiv by_kv, by_gqa;
     int64_t few;       // sequences of at most this many rows go to the 16-row tiles
 };
 
@@ -42,7 +48,7 @@ struct AttnArgs {
 // out: a key past the head is `gap` less there.
 struct Span {
     int lo, hi, n, head, gap;
-    __device__ __forceinline__ Span(const AttnArgs &a, int s, int n_new, int ctx) {
+    __device__ __forceinline__ Span(const AttnArgs &a, int n_new, int ctx, int chunk) {
         const int64_t cap = static_cast<int64_t>(a.batch.max_pages) << a.batch.page_shift;
         hi = ctx < 0 ? 0 : ctx < cap ? ctx : static_cast<int>(cap);
         lo = a.window > 0 && ctx - n_new - a.window + 1 > 0 ? (ctx - n_new - a.window + 1) & ~63 : 0;
@@ -53,12 +59,14 @@ struct Span {
             gap = lo > head ? lo - head : 0;
             lo = 0;
         }
-        n = static_cast<int>((static_cast<int64_t>(hi) - gap - lo + a.chunk - 1) / a.chunk);
-        n = n < 1 ? 1 : n > a.nsplit ? a.nsplit : n;
+        cut(a, static_cast<int>((static_cast<uint32_t>(hi - gap - lo) + chunk - 1) / static_cast<uint32_t>(chunk)));
     }
-    __device__ __forceinline__ void chunk_keys(const AttnArgs &a, int c, int &k0, int &k1) const {
-        k0 = lo + c * a.chunk;
-        k1 = c == n - 1 ? hi - gap : k0 + a.chunk;
+    __device__ __forceinline__ Span(const AttnArgs &a, int n_new, int ctx) : Span(a, n_new, ctx, 64) {}
+    __device__ __forceinline__ void cut(const AttnArgs &a, int chunks) { n = chunks < 1 ? 1 : chunks > a.nsplit ? a.nsplit : chunks; }
+    __device__ __forceinline__ int blocks() const { return (hi - gap - lo + 63) >> 6; }  // of 64 keys
+    __device__ __forceinline__ void chunk_keys(int chunk, int c, int &k0, int &k1) const {
+        k0 = lo + c * chunk;
+        k1 = c == n - 1 ? hi - gap : k0 + chunk;
     }
 };
 
@@ -112,6 +120,101 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs &a, int rows, int64_t a
     return Tile{-1, 0, 0, 0, 0};
 }
 
+// Inclusive sums and maxima over the wave's lanes, by data-parallel moves: no trip through LDS.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T from_before(T old, T x) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+template <typename T>
+__device__ __forceinline__ T sums_to_here(T x) {
+    x += from_before<0x111, 0xf>(T(0), x);
+    x += from_before<0x112, 0xf>(T(0), x);
+    x += from_before<0x114, 0xf>(T(0), x);
+    x += from_before<0x118, 0xf>(T(0), x);
+    x += from_before<0x142, 0xa>(T(0), x);
+    return x + from_before<0x143, 0xc>(T(0), x);
+}
+__device__ __forceinline__ int most_to_here(int x) {
+    const auto most = [](int p, int q) { return p > q ? p : q; };
+    x = most(x, from_before<0x111, 0xf>(x, x));
+    x = most(x, from_before<0x112, 0xf>(x, x));
+    x = most(x, from_before<0x114, 0xf>(x, x));
+    x = most(x, from_before<0x118, 0xf>(x, x));
+    x = most(x, from_before<0x142, 0xa>(x, x));
+    return most(x, from_before<0x143, 0xc>(x, x));
+}
+
+// Sequence s as a lane of the wave sees it: its first row, new tokens, context, 16-row tiles, and blocks of 64 keys.
+struct Lane {
+    int first = 0, n = 0, ctx = 0, tiles = 0, blocks = 0;
+    __device__ __forceinline__ Lane(const AttnArgs &a, int s) {
+        if (s >= a.batch.b) return;
+        ctx = a.batch.length(s);
+        a.batch.rows(s, first, n);
+        if (n == 0) return;
+        tiles = static_cast<int>((static_cast<int64_t>(n) * a.gqa + 15) >> 4);
+        blocks = Span(a, n, ctx).blocks();
+    }
+};
+
+// The chunk, in blocks of 64 keys, that cuts what keys there are (not the longest context's, which the host knows) into about
+// `target` units of a kv head, all of one size but a tile's last. Every wave finds it for itself from the batch's arrays, in
+// the same order of sums.
+__device__ __forceinline__ int shared_blocks(const AttnArgs &a, const Lane &first) {
+    const int lane = threadIdx.x & 63;
+    float total = static_cast<float>(first.tiles) * static_cast<float>(first.blocks);
+    int longest = first.blocks;
+    for (int s0 = 64; s0 < a.batch.b; s0 += 64) {
+        const Lane l(a, s0 + lane);
+        total += static_cast<float>(l.tiles) * static_cast<float>(l.blocks);
+        longest = l.blocks > longest ? l.blocks : longest;
+    }
+    const float all = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sums_to_here(total)), 63));
+    longest = __builtin_amdgcn_readlane(most_to_here(longest), 63);
+    const float even = ceilf(all * a.per_target);
+    const int per = static_cast<int>((static_cast<uint32_t>(longest) + a.nsplit - 1) / static_cast<uint32_t>(a.nsplit));  // room for a tile's
+    int blocks = even < static_cast<float>(1 << 24) ? static_cast<int>(even) : 1 << 24;
+    blocks = blocks < per ? per : blocks;
+    blocks = blocks < kMinChunk / 64 ? kMinChunk / 64 : blocks;
+    return __builtin_amdgcn_readfirstlane(blocks);
+}
+
+__device__ __forceinline__ int chunks_of(int blocks, int per) {
+    return static_cast<int>((static_cast<uint32_t>(blocks) + per - 1) / static_cast<uint32_t>(per));
+}
+
+// A tile, which of its chunks, and how many it has.
+struct Unit {
+    Tile tile;
+    int c, chunks, chunk;
+};
+
+// The unit-th of all sequences' tiles' chunks.
+__device__ __forceinline__ Unit find_unit(const AttnArgs &a, int unit) {
+    const int lane = threadIdx.x & 63;
+    const Lane first(a, lane);
+    const int per = shared_blocks(a, first);
+    for (int s0 = 0; s0 < a.batch.b; s0 += 64) {
+        const Lane l = s0 == 0 ? first : Lane(a, s0 + lane);
+        int n = chunks_of(l.blocks, per);
+        n = n < 1 ? 1 : n;
+        const int units = l.tiles * n, sum = sums_to_here(units);
+        const uint64_t past = __ballot(sum > unit);
+        if (past) {
+            const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            const int of = __builtin_amdgcn_readlane(units, at), k = __builtin_amdgcn_readlane(sum, at) - 1 - unit;
+            if (k < 0 || k >= of) break;  // starts that do not rise can pass any sum
+            const int chunks = __builtin_amdgcn_readlane(n, at);
+            const int tile = chunks == 1 ? k : static_cast<int>(static_cast<uint32_t>(k) / static_cast<uint32_t>(chunks));
+            return Unit{Tile{s0 + at, tile, __builtin_amdgcn_readlane(l.first, at), __builtin_amdgcn_readlane(l.n, at),
+                             __builtin_amdgcn_readlane(l.ctx, at)},
+                        k - tile * chunks, chunks, 64 * per};
+        }
+        unit -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return Unit{Tile{-1, 0, 0, 0, 0}, 0, 1, 64 * per};
+}
+
 // The largest of the lanes 32 apart (and 16 apart), by exchanging halves of registers: no trip through LDS.
 __device__ __forceinline__ float max_32_apart(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -147,6 +250,16 @@ __device__ __forceinline__ float relative_to(float m, float scale2, float bias, 
 __device__ __forceinline__ uint32_t not_finite(uint32_t pair) {  // ones in the place of each that has the largest exponent
     const uint32_t top = ((pair & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
     return top | (top - (top >> 15));
+}
+// The same of the groups of 4-bit values of two pairs: ones in the place of each that holds a value with the largest exponent, or could.
+__device__ __forceinline__ uint32_t q4_not_finite(half2_t d, half2_t b) {
+    const half_t first = static_cast<half_t>(kQ4First), last = static_cast<half_t>(kQ4Last);
+    return not_finite(__builtin_bit_cast(uint32_t, __builtin_elementwise_fma(half2_t{first, first}, d, b))) |
+           not_finite(__builtin_bit_cast(uint32_t, __builtin_elementwise_fma(half2_t{last, last}, d, b)));
+}
+__device__ __forceinline__ bool q4_not_finite(uint32_t pair) {
+    const half2_t p = __builtin_bit_cast(half2_t, pair);
+    return q4_not_finite(half2_t{p[0], p[0]}, half2_t{p[1], p[1]}) != 0;
 }
 template <int E>
 __device__ __forceinline__ uint32_t take_out(half_t __attribute__((ext_vector_type(E))) &v) {
@@ -196,18 +309,29 @@ struct KvTile {
 
     // Of the score product's step i, a lane of group g has the dimensions from here on.
     __device__ __forceinline__ static int dim(int i, int g) { return 32 * i + 8 * g; }
-    // base: of the page's kv head; slot: keys 16u's place there; l16, g: the lane's
-    __device__ __forceinline__ void load(const AttnArgs &a, int u, int64_t base, int slot, int l16, int g) {
+    struct Lane {
+        int l16, g;
+        __device__ __forceinline__ Lane(const AttnArgs &, int lane16, int group) : l16(lane16), g(group) {}
+    };
+    // base: of the page's kv head; slot: keys 16u's place there
+    __device__ __forceinline__ void load_keys(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
         base += static_cast<int64_t>(slot) * D;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) k[u][i] = *reinterpret_cast<const half8_t *>(a.k + base + l16 * D + dim(i, g));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * u + j] = *reinterpret_cast<const ve *>(a.v + base + (4 * g + j) * D + E * l16);
+        for (int i = 0; i < D / 32; ++i) k[u][i] = *reinterpret_cast<const half8_t *>(a.k + base + at.l16 * D + dim(i, at.g));
     }
-    __device__ __forceinline__ half8_t key(int u, int i) const { return k[u][i]; }
+    __device__ __forceinline__ void load_values(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
+        base += static_cast<int64_t>(slot) * D;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * u + j] = *reinterpret_cast<const ve *>(a.v + base + (4 * at.g + j) * D + E * at.l16);
+    }
+    __device__ __forceinline__ half8_t key(int u, int i, const Q4Bits &) const { return k[u][i]; }
     __device__ __forceinline__ void drop(int j) { v[j] = ve{}; }
     __device__ __forceinline__ void turn(int) {}
-    __device__ __forceinline__ half8_t value(int e) const {
+    __device__ __forceinline__ void take_out_values(uint32_t &spoilt) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) spoilt |= take_out<E>(v[j]);
+    }
+    __device__ __forceinline__ half8_t value(int e, const Q4Bits &) const {
         half8_t f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = v[j][e];
@@ -231,15 +355,30 @@ struct KvTile<D, true> {
     int ok;
 
     __device__ __forceinline__ static int dim(int i, int g) { return 8 * (W * g + i); }
-    __device__ __forceinline__ void load(const AttnArgs &a, int u, int64_t base, int slot, int l16, int g) {
-        const int page = 1 << a.batch.page_shift;
-        const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.k) + base, *vp = reinterpret_cast<const uint8_t *>(a.v) + base;
-        k[u] = *reinterpret_cast<const kw *>(kp + Q4Row<D>::key_word(slot + l16, W * g));
-        ks[u] = *reinterpret_cast<const uint32_t *>(kp + Q4Row<D>::pair(page, slot + l16, W * g / 4));
-        v[u] = *reinterpret_cast<const u32x4 *>(vp + Q4Row<D>::value_word(slot + 4 * g, E * l16 / 8));
-        vs[u] = *reinterpret_cast<const u32x4 *>(vp + Q4Row<D>::pair(page, slot + 4 * g, E * l16 / 32));
+    // What a lane reads lies at these bytes from what the wave does.
+    struct Lane {
+        uint32_t k, ks, v, vs;
+        __device__ __forceinline__ Lane(const AttnArgs &a, int l16, int g) {
+            const int page = 1 << a.batch.page_shift;
+            k = Q4Row<D>::key_word(l16, W * g);
+            ks = (W * g / 4 * page + l16) * 4;
+            v = Q4Row<D>::value_word(4 * g, E * l16 / 8);
+            vs = (E * l16 / 32 * page + 4 * g) * 4;
+        }
+    };
+    __device__ __forceinline__ void load_keys(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
+        const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.k) + base;
+        const uint32_t words = slot * (Q4Row<D>::kWords * 4), pairs = Q4Row<D>::pair(1 << a.batch.page_shift, slot, 0);
+        k[u] = *reinterpret_cast<const kw *>(kp + words + at.k);
+        ks[u] = *reinterpret_cast<const uint32_t *>(kp + pairs + at.ks);
     }
-    __device__ __forceinline__ half8_t key(int u, int i) const { return q4_values(k[u][i], ks[u]); }
+    __device__ __forceinline__ void load_values(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
+        const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.v) + base;
+        const uint32_t words = slot * (Q4Row<D>::kWords * 4), pairs = Q4Row<D>::pair(1 << a.batch.page_shift, slot, 0);
+        v[u] = *reinterpret_cast<const u32x4 *>(vp + words + at.v);
+        vs[u] = *reinterpret_cast<const u32x4 *>(vp + pairs + at.vs);
+    }
+    __device__ __forceinline__ half8_t key(int u, int i, const Q4Bits &bits) const { return q4_values(k[u][i], ks[u], bits); }
     __device__ __forceinline__ void drop(int j) { vs[j >> 2][j & 3] = 0; }  // 64 + n times 0
     __device__ __forceinline__ void turn(int l16) {
 #pragma unroll
@@ -255,11 +394,21 @@ struct KvTile<D, true> {
             b[t] = __builtin_bit_cast(half2_t, high_halves(vs[u][j], vs[u][j + 1]));
         }
     }
-    __device__ __forceinline__ half8_t value(int e) const {
+    // A group's values lie between those of its first and last code: one of which either is not finite is left out whole.
+    __device__ __forceinline__ void take_out_values(uint32_t &spoilt) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint32_t out = q4_not_finite(d[t], b[t]);
+            spoilt |= out;
+            d[t] = __builtin_bit_cast(half2_t, __builtin_bit_cast(uint32_t, d[t]) & ~out);
+            b[t] = __builtin_bit_cast(half2_t, __builtin_bit_cast(uint32_t, b[t]) & ~out);
+        }
+    }
+    __device__ __forceinline__ half8_t value(int e, const Q4Bits &bits) const {
         half8_t f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const half2_t x = __builtin_elementwise_fma(q4_codes(e & 1 ? hi[t] : lo[t], e >> 1), d[t], b[t]);
+            const half2_t x = __builtin_elementwise_fma(q4_codes(e & 1 ? hi[t] : lo[t], e >> 1, bits), d[t], b[t]);
             f[2 * t] = x[0];
             f[2 * t + 1] = x[1];
         }
@@ -274,7 +423,7 @@ __device__ __forceinline__ half_t __attribute__((ext_vector_type(E))) value_run(
     if constexpr (Q4) {
         const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.v) + base;
         const uint32_t word = *reinterpret_cast<const uint32_t *>(vp + Q4Row<D>::value_word(slot, dim / 8));
-        const half8_t x = q4_values(word, *reinterpret_cast<const uint32_t *>(vp + Q4Row<D>::pair(1 << a.batch.page_shift, slot, dim / 32)));
+        const half8_t x = q4_values(word, *reinterpret_cast<const uint32_t *>(vp + Q4Row<D>::pair(1 << a.batch.page_shift, slot, dim / 32)), Q4Bits());
         ve y;
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = E == 4 && (dim & 4) ? x[4 + e] : x[e];
@@ -282,6 +431,13 @@ __device__ __forceinline__ half_t __attribute__((ext_vector_type(E))) value_run(
     } else {
         return *reinterpret_cast<const ve *>(a.v + base + static_cast<int64_t>(slot) * D + dim);
     }
+}
+
+// The pair of a key's value group that holds dimension dim.
+template <int D>
+__device__ __forceinline__ uint32_t value_pair(const AttnArgs &a, int64_t base, int slot, int dim) {
+    return *reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint8_t *>(a.v) + base +
+                                               Q4Row<D>::pair(1 << a.batch.page_shift, slot, dim / 32));
 }
 
 // Where a page's kv head begins in it.
@@ -301,22 +457,26 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     auto &sm_o = lds.o;
     auto &sm_m = lds.m;
     auto &sm_l = lds.l;
-    const int kh = block % a.n_kv;
-    const Tile tile = find_tile(a, ROWS, 0, a.few, block / a.n_kv);
+    const bool shared = Q4 && a.target > 0;
+    const int tile_no = static_cast<int>(a.by_kv.div(static_cast<uint32_t>(block))), kh = block - tile_no * a.n_kv;
+    const Unit unit = shared ? find_unit(a, tile_no) : Unit{find_tile(a, ROWS, 0, a.few, tile_no), static_cast<int>(blockIdx.y), 0, a.chunk};
+    const Tile &tile = unit.tile;
     if (tile.s < 0) return;
     const int s = tile.s, at = tile.at, first = tile.first, n_new = tile.n_new, ctx = tile.ctx;
-    const Span span(a, s, n_new, ctx);
-    const int c = blockIdx.y;
+    Span span = shared ? Span(a, n_new, ctx) : Span(a, n_new, ctx, unit.chunk);
+    if (shared) span.cut(a, unit.chunks);
+    const int c = unit.c;
     if (c >= span.n) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     const int n_rows = n_new * a.gqa - at * ROWS < ROWS ? n_new * a.gqa - at * ROWS : ROWS;
     // the lane's row: token `tok` of the sequence, query head kh * gqa + head
     const int row = at * ROWS + (l16 < n_rows ? l16 : n_rows - 1);
-    const int tok = row / a.gqa, head = kh * a.gqa + row - tok * a.gqa;
+    const auto token_of = [&](int r) { return static_cast<int>(a.by_gqa.div(static_cast<uint32_t>(r))); };
+    const int tok = token_of(row), head = kh * a.gqa + row - tok * a.gqa;
     const int pos = ctx - n_new + tok;
-    const int first_tok = at * ROWS / a.gqa, last_tok = (at * ROWS + n_rows - 1) / a.gqa;
+    const int first_tok = token_of(at * ROWS), last_tok = token_of(at * ROWS + n_rows - 1);
     int k0, k1;  // the tile's keys in this chunk
-    span.chunk_keys(a, c, k0, k1);
+    span.chunk_keys(unit.chunk, c, k0, k1);
     const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
     // one of the tile's rows at least sees the keys [bottom, k1), all of them [from, end)
     const bool one_token = first_tok == last_tok;
@@ -346,14 +506,33 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     }
     const int in_page = (1 << a.batch.page_shift) - 1;
     const int64_t head_at = head_offset<D, Q4>(a, kh);
-    auto load = [&](int kb, KvTile<D, Q4> &t) {
+    const typename KvTile<D, Q4>::Lane lane_at(a, l16, g);
+    // the wave's key tiles are every fourth: the i-th begins at key_of(i)
+    const int base = SINKS ? k0 : k0 & ~31;
+    const int heads_tiles = SINKS ? (mid - k0 + 31) >> 5 : 0, rest_at = SINKS ? next : base;
+    const int n_tiles = heads_tiles + (rest_at < k1 ? (k1 - rest_at + 31) >> 5 : 0);
+    auto key_of = [&](int i) { return SINKS && i < heads_tiles ? base + 32 * i : rest_at + 32 * (i - heads_tiles); };
+    // The page ids of the wave's next 32 tiles at once, a lane for each 16 keys: a tile's keys wait for no id of their own.
+    int id_lane = -1;
+    auto ids_from = [&](int i) {
+        const int key = key_of(i + 4 * (lane >> 1)) + 16 * (lane & 1);
+        id_lane = i + 4 * (lane >> 1) < n_tiles && key < k1 ? a.batch.page(s, key >> a.batch.page_shift) : -1;
+    };
+    auto page_of = [&](int i, int u) { return __builtin_amdgcn_readlane(id_lane, ((i - w) >> 1 & 62) + u); };  // i: w and every fourth
+    auto load_keys = [&](int i, KvTile<D, Q4> &t) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int page = page_of(i, u);
+            t.load_keys(a, u, (page < 0 ? 0 : page) * a.batch.page_stride + head_at, (key_of(i) + 16 * u) & in_page, lane_at);
+        }
+    };
+    auto load_values = [&](int i, KvTile<D, Q4> &t) {
         t.ok = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int key = kb + 16 * u;
-            const int page = key < k1 ? a.batch.page(s, key >> a.batch.page_shift) : -1;
+            const int page = page_of(i, u);
             if (page >= 0) t.ok |= 1 << u;
-            t.load(a, u, (page < 0 ? 0 : page) * a.batch.page_stride + head_at, key & in_page, l16, g);
+            t.load_values(a, u, (page < 0 ? 0 : page) * a.batch.page_stride + head_at, (key_of(i) + 16 * u) & in_page, lane_at);
         }
     };
     float m = -INFINITY, m2 = 0.0f, l = 0.0f;  // m2: what the weights are relative to in log2, anything while there is no m
@@ -362,33 +541,45 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     float4_t o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
-    auto compute = [&](int kb, KvTile<D, Q4> &t) {
+    const Q4Bits bits;
+    auto compute = [&](int kb, KvTile<D, Q4> &t, auto after_scores) {
         float4_t sc[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             sc[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < C; ++i) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.key(u, i), qf[i], sc[u], 0, 0, 0);
+            for (int i = 0; i < C; ++i) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.key(u, i, bits), qf[i], sc[u], 0, 0, 0);
+            if (Q4) __builtin_amdgcn_sched_barrier(0);
         }
-        float mx = m;
+        after_scores();
+        // whether some of the rows do not see some of the keys
+        const bool partly = (kb < from && !(SINKS && kb + 32 <= shown)) || kb + 32 > end;
+        if (__builtin_expect(partly || t.ok != 3, 0)) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = kb + 16 * u + 4 * g + i;
                 const bool seen = key <= pos && (key >= row_lo || (SINKS && key < a.sinks)) && key < k1 && (t.ok >> u & 1);
                 sc[u][i] = seen ? sc[u][i] : -INFINITY;
-                mx = fmaxf(mx, sc[u][i]);
             }
+        }
+        float mx = Q4 ? sc[0][0] : m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[u][i]);
         // the row's other keys are 16 and 32 lanes away
         mx = max_16_32_apart(mx);
-        if (__any(mx > m)) {
+        // over 4-bit pages, where issue counts, only a maximum that has grown by 2^kSlack moves the sums
+        if (Q4 ? __any((mx - m) * a.scale2 > kSlack) : __any(mx > m)) {
+            if (Q4) mx = fmaxf(mx, m);
             const float f = exp2_fast(mx == -INFINITY ? 0.0f : (m - mx) * a.scale2);
             l *= f;
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] *= f;
             m = mx;
-            m2 = relative_to(m, a.scale2, kBias, far);
+            m2 = relative_to(m, a.scale2, Q4 ? kChunkBias : kBias, far);
         }
         if (far) {
             const float from_m = m == -INFINITY ? 0.0f : m;
@@ -407,8 +598,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             }
         l += sum;
         // what no row sees holds anything: 0 times it may be NaN
-        const bool partly = (kb < from && !(SINKS && kb + 32 <= shown)) || kb + 32 > end;
-        if (partly || t.ok != 3) {
+        if (__builtin_expect(partly || t.ok != 3, 0)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
@@ -416,36 +606,79 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             }
         }
         t.turn(l16);
+        if (__builtin_expect(partly && !one_token, 0)) t.take_out_values(spoilt);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            half8_t f = t.value(e);
-            if (partly && !one_token) spoilt |= take_out<8>(f);
-            o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, o[e], 0, 0, 0);
-        }
-    };
-    // the wave's key tiles, every fourth: f(first key)
-    auto for_tiles = [&](auto f) {
-        if constexpr (SINKS) {
-            const int heads_tiles = (mid - k0 + 31) >> 5, rest = next < k1 ? (k1 - next + 31) >> 5 : 0;
-            for (int i = w; i < heads_tiles + rest; i += 4) {
-                const int kb = i < heads_tiles ? k0 + 32 * i : next + 32 * (i - heads_tiles);
-                if (kb < k1) f(kb);
-            }
-        } else {
-            for (int kb = (k0 & ~31) + 32 * w; kb < k1; kb += 128) f(kb);
+            o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.value(e, bits), p, o[e], 0, 0, 0);
+            if (Q4 && (e & 1)) __builtin_amdgcn_sched_barrier(0);
         }
     };
     KvTile<D, Q4> t;
-    for_tiles([&](int kb) {
-        load(kb, t);
-        compute(kb, t);
-    });
+    if constexpr (Q4) {
+        // the next tile's keys are requested as soon as this one's have made their scores, in the same registers; past the last
+        // key page 0 is read, for nothing, so that no branch holds a request
+        if (w < n_tiles) {
+            ids_from(w);
+            load_keys(w, t);
+        }
+        for (int i = w; i < n_tiles; i += 4) {
+            load_values(i, t);
+            compute(key_of(i), t, [&] {
+                if (((i - w) & 124) == 124) ids_from(i + 4);
+                load_keys(i + 4, t);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
+    } else {
+        for (int i = w; i < n_tiles; i += 4) {
+            if (((i - w) & 124) == 0) ids_from(i);
+            load_keys(i, t);
+            load_values(i, t);
+            compute(key_of(i), t, [] {});
+        }
+    }
+    // the weight of a key for the lane's row, from the key's row in memory; the four lanes that share the row each take a quarter
+    auto weight_again = [&](int64_t at_head, int slot) {
+        const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.k) + at_head;
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int d = KvTile<D, Q4>::dim(i, g);
+            const half8_t k = q4_values(*reinterpret_cast<const uint32_t *>(kp + Q4Row<D>::key_word(slot, d / 8)),
+                                        *reinterpret_cast<const uint32_t *>(kp + Q4Row<D>::pair(in_page + 1, slot, d / 32)), bits);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x = __builtin_fmaf(static_cast<float>(k[e]), static_cast<float>(qf[i][e]), x);
+        }
+        x += __shfl_xor(x, 16, 64);
+        x += __shfl_xor(x, 32, 64);
+        return exp2_fast((x - m) * a.scale2 + kChunkBias);
+    };
     if (__builtin_expect(__any(spoilt != 0), 0)) {
-        for_tiles([&](int kb) {
-            if ((kb >= from || (SINKS && kb + 32 <= shown)) && kb + 32 <= end) return;
+        for (int i = w; i < n_tiles; i += 4) {
+            const int kb = key_of(i);
+            if ((kb >= from || (SINKS && kb + 32 <= shown)) && kb + 32 <= end) continue;
             for (int key = kb; key < kb + 32 && key < k1; ++key) {
                 const int page = a.batch.page(s, key >> a.batch.page_shift);
-                if (page < 0 || key > pos || (key < row_lo && !(SINKS && key < a.sinks))) continue;
+                const bool unseen = page < 0 || key > pos || (key < row_lo && !(SINKS && key < a.sinks));
+                if constexpr (Q4) {  // with their weights, taken again; a value that is not finite counts whatever its weight is
+                    const int64_t at_head = (page < 0 ? 0 : page) * a.batch.page_stride + head_at;
+                    const float x = weight_again(at_head, key & in_page);
+                    if (unseen) continue;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = 4 * E * g + E * i;
+                        const uint32_t pair = value_pair<D>(a, at_head, key & in_page, d);
+                        if (!q4_not_finite(pair)) continue;
+                        const auto v = value_run<D, Q4, E>(a, at_head, key & in_page, d);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const float y = static_cast<float>(v[e]);
+                            o[e][i] += fabsf(y) < INFINITY ? x * y : y;
+                        }
+                    }
+                    continue;
+                }
+                if (unseen) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const auto v = taken<E>(value_run<D, Q4, E>(a, page * a.batch.page_stride + head_at, key & in_page, 4 * E * g + E * i));
@@ -453,7 +686,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
                     for (int e = 0; e < E; ++e) o[e][i] += static_cast<float>(v[e]);
                 }
             }
-        });
+        }
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -481,7 +714,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
 #pragma unroll
         for (int e = 0; e < E; ++e) num[e] += sm_o[u][r][E * l16 + e] * f;
     }
-    const int rr = at * ROWS + (r < n_rows ? r : n_rows - 1), rtok = rr / a.gqa, rhead = kh * a.gqa + rr - rtok * a.gqa;
+    const int rr = at * ROWS + (r < n_rows ? r : n_rows - 1), rtok = token_of(rr), rhead = kh * a.gqa + rr - rtok * a.gqa;
     const int64_t trow = static_cast<int64_t>(first + rtok) * a.heads + rhead;
     if (r < n_rows) {
         if (span.n > 1) {
@@ -536,13 +769,13 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     const Tile tile = find_tile(a, ROWS, a.few, INT64_MAX, block_no / a.n_kv);
     if (tile.s < 0) return;
     const int s = tile.s, at = tile.at, first = tile.first, n_new = tile.n_new, ctx = tile.ctx, pos0 = ctx - n_new;
-    const Span span(a, s, n_new, ctx);
+    const Span span(a, n_new, ctx, a.chunk);
     const int c = blockIdx.y;
     if (c >= span.n) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
     const int r0 = at * ROWS, n_rows = n_new * a.gqa - r0 < ROWS ? n_new * a.gqa - r0 : ROWS;
     int k0, k1;
-    span.chunk_keys(a, c, k0, k1);
+    span.chunk_keys(a.chunk, c, k0, k1);
     // all of the tile's rows see the keys from `from` to `upto`
     const int upto = pos0 + r0 / a.gqa, from = a.window > 0 ? pos0 + (r0 + n_rows - 1) / a.gqa - a.window + 1 : 0;
     int mid = 0, next = 0;
@@ -616,6 +849,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) gv[j] = *reinterpret_cast<const ve *>(a.v + base + (4 * a4 + j) * D + E * db);
     };
+    const Q4Bits bits;
     auto store = [&](int kb, int buf) {
         // slots that hold no position: 0 times what is there may be NaN
         const bool partly = !g_ok || kb + KT > k1 || (kb < from && !(SINKS && kb + KT <= shown)) || kb + KT - 1 > upto;
@@ -627,7 +861,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
         if constexpr (Q4) {
 #pragma unroll
             for (int i = 0; i < KL; ++i)
-                *reinterpret_cast<half8_t *>(&sk[buf][(16 * w + (lane >> 2)) * KP + 8 * (KL * (lane & 3) + i)]) = q4_values(gkw[i], gks);
+                *reinterpret_cast<half8_t *>(&sk[buf][(16 * w + (lane >> 2)) * KP + 8 * (KL * (lane & 3) + i)]) = q4_values(gkw[i], gks, bits);
             if (partly) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -646,17 +880,26 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
                 sd[t] = __builtin_bit_cast(half2_t, low_halves(gvs[2 * t], gvs[2 * t + 1]));
                 sb[t] = __builtin_bit_cast(half2_t, high_halves(gvs[2 * t], gvs[2 * t + 1]));
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
+            auto value = [&](int e) {
                 half4_t x;
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const half2_t y = __builtin_elementwise_fma(q4_codes(e & 1 ? hi[t] : lo[t], e >> 1), sd[t], sb[t]);
+                    const half2_t y = __builtin_elementwise_fma(q4_codes(e & 1 ? hi[t] : lo[t], e >> 1, bits), sd[t], sb[t]);
                     x[2 * t] = y[0];
                     x[2 * t + 1] = y[1];
                 }
-                if (partly) spoilt |= take_out<4>(x);
-                put(e, x);
+                return x;
+            };
+            if (partly) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    half4_t x = value(e);
+                    spoilt |= take_out<4>(x);
+                    put(e, x);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) put(e, value(e));
             }
         } else {
 #pragma unroll
@@ -874,7 +1117,7 @@ constexpr int kFewChunks = 8;
 // Up to kFewChunks: a wave for R heads of a token, which share its lookups, everything requested at once. 862 tokens of
 // 16 heads over four chunks with 1 / 2 / 4 heads a wave: 7.3 / 5.6 / 6.5 us; with the chunks requested before it is known
 // how many a row has 8.5.
-template <int D, int R>
+template <int D, int R, bool SHARED>
 __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
     constexpr int PER = D / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -885,7 +1128,8 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
     int first, n_new;
     a.batch.rows(s, first, n_new);
     if (t < first || t - first >= n_new) return;
-    const int n = Span(a, s, n_new, a.batch.length(s)).n;
+    const Span span = SHARED ? Span(a, n_new, a.batch.length(s)) : Span(a, n_new, a.batch.length(s), a.chunk);
+    const int n = SHARED ? chunks_of(span.blocks(), shared_blocks(a, Lane(a, lane))) : span.n;
     if (n <= 1) return;
     const float *pr = a.part + trow * a.nsplit * (D + 4);
     float mc[R][kFewChunks], lc[R][kFewChunks], v[R][kFewChunks][PER];
@@ -924,7 +1168,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
 // More: a workgroup a row, wave w taking chunks w, w + 4, ..; 64 of its chunks at a time have their maxima and sums read
 // by a lane each, then their rows follow with U requests in flight (5 tokens of 32 heads, 51 chunks: 19.6 us with a
 // loop that carries the maximum along and waits for each, 5.1 so).
-template <int D>
+template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     constexpr int PER = D / 64, U = 8, W = 4;
     __shared__ float sm[W][D + 2];
@@ -935,7 +1179,8 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     int first, n_new;
     a.batch.rows(s, first, n_new);
     if (t < first || t - first >= n_new) return;
-    const int n = Span(a, s, n_new, a.batch.length(s)).n;
+    const Span span = SHARED ? Span(a, n_new, a.batch.length(s)) : Span(a, n_new, a.batch.length(s), a.chunk);
+    const int n = SHARED ? chunks_of(span.blocks(), shared_blocks(a, Lane(a, lane))) : span.n;
     if (n <= 1) return;
     float num[PER] = {}, den = 0.0f, m = -INFINITY;
     const float *pr = a.part + trow * a.nsplit * (D + 4);
@@ -1006,6 +1251,7 @@ struct Plan {
     int64_t small, large;  // tiles of 16 and of 128 rows, at most
     int64_t few;           // rows of a sequence up to which it goes to the small ones
     int chunk, nsplit;
+    int target;            // units of a kv head where the device shares the keys out, or 0
 };
 
 // Sequences of up to kFew rows go to the 16-row tiles, the others to the 128-row ones: 64 sequences after 2000 keys
@@ -1015,16 +1261,19 @@ struct Plan {
 constexpr int64_t kFew = 32;
 // The keys are cut into chunks until the tiles fill the chip's workgroups, of kMinChunk keys at least. kFillSmall 512 /
 // 1024 / 2048 / 4096: 48 tokens over up to 1536 keys each 40 / 35 / 36 / 37 us, 5 over 65000 82 / 79 / 79 / 84;
-// kFillLarge 256 / 384 / 512: a batch of two chunks and 30 tokens 28.7 / 28.4 / 29.8. kMinChunk 128 / 256 / 512: one
-// token over 1024 keys 8.1 / 9.1 / 11.6. Contexts of up to kWhole keys are not cut, whose second launch costs more than it
+// kFillLarge 256 / 384 / 512: a batch of two chunks and 30 tokens 28.7 / 28.4 / 29.8. Contexts of up to kWhole keys are not cut, whose second launch costs more than it
 // saves. In a captured graph, one token of 8 kv heads over 256 / 384 / 448 / 512 keys: 6.8 / 8.1 / 8.8 / 9.1 us whole,
 // 8.0 / 8.2 / 8.2 / 8.3 cut (4 of D = 64: 5.6 / 6.6 / 7.2 / 7.3 and 7.2 / 7.4 / 7.5 / 7.5). From 128 tiles on, twice that
 // (16 tokens of 8 kv heads over 512 / 768 / 1024: 10.9 / 15.7 / 19.2 whole, 13.1 / 15.7 / 19.0 cut).
-constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kMinChunk = 128, kWhole = 384;
+constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kWhole = 384;
+
+// Where the device shares the keys out (a token or a few of each sequence, over 4-bit pages or with sinks):
+constexpr int64_t kFillShared = 1024, kShareBytes = int64_t(64) << 20;
 
 inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window,
-                    int64_t sinks) {
+                    int64_t sinks, int64_t hd, bool share) {
     Plan p;
+    p.target = 0;
     const int64_t rows = tokens * gqa, live = b < tokens ? b : tokens;
     if (max_q * gqa <= kFew) {
         p.few = INT64_MAX;
@@ -1051,11 +1300,35 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
     if (n > most) n = most;
     p.chunk = static_cast<int>(((span + n - 1) / n + 63) / 64 * 64);
     p.nsplit = static_cast<int>((span + p.chunk - 1) / p.chunk);
+    if (share && p.large == 0 && p.nsplit > 1) {
+        // room for chunks of kMinChunk keys, as many as a kv head has units or kShareBytes of states hold
+        const int64_t left = kFillShared / n_kv - p.small / 2;  // a tile's last chunk is half a one
+        p.target = static_cast<int>(left > p.small ? left : p.small);
+        int64_t room = kFewChunks;
+        if (p.nsplit > kFewChunks / 2) {
+            room = kShareBytes / (tokens * gqa * n_kv * (hd + 4) * static_cast<int64_t>(sizeof(float)));
+            room = room < p.target ? room : p.target;
+        }
+        room = room < most ? room : most;
+        if (room > p.nsplit) p.nsplit = static_cast<int>(room);
+    }
     return p;
 }
 
 inline size_t part_bytes(const Plan &p, int64_t tokens, int64_t heads, int64_t hd) {
     return p.nsplit > 1 ? static_cast<size_t>(tokens * heads * p.nsplit * (hd + 4)) * sizeof(float) : 0;
+}
+
+template <int D, bool SHARED>
+hipError_t merge(const AttnArgs &a, hipStream_t stream) {
+    const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
+    if (a.nsplit <= kFewChunks && a.heads % 2 == 0)
+        paged_attn_merge_few<D, 2, SHARED><<<static_cast<unsigned>((rows / 2 + 3) / 4), 256, 0, stream>>>(a);
+    else if (a.nsplit <= kFewChunks)
+        paged_attn_merge_few<D, 1, SHARED><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+    else
+        paged_attn_merge<D, SHARED><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
+    return hipGetLastError();
 }
 
 template <int D, bool Q4, bool SINKS>
@@ -1064,17 +1337,12 @@ hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
         paged_attn_mixed<D, Q4, SINKS><<<dim3(static_cast<unsigned>((p.large + p.small) * a.n_kv), a.nsplit), 256, 0, stream>>>(
             a, static_cast<int>(p.large * a.n_kv));
     else
-        paged_attn_rows<D, Q4, SINKS><<<dim3(static_cast<unsigned>(p.small * a.n_kv), a.nsplit), 256, 0, stream>>>(a);
+        paged_attn_rows<D, Q4, SINKS><<<
+            a.target > 0 ? dim3(static_cast<unsigned>((p.small + a.target + 1) * a.n_kv)) : dim3(static_cast<unsigned>(p.small * a.n_kv), a.nsplit),
+            256, 0, stream>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
-    const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
-    if (a.nsplit <= kFewChunks && a.heads % 2 == 0)
-        paged_attn_merge_few<D, 2><<<static_cast<unsigned>((rows / 2 + 3) / 4), 256, 0, stream>>>(a);
-    else if (a.nsplit <= kFewChunks)
-        paged_attn_merge_few<D, 1><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
-    else
-        paged_attn_merge<D><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
-    return hipGetLastError();
+    return Q4 && a.target > 0 ? merge<D, Q4>(a, stream) : merge<D, false>(a, stream);
 }
 
 inline bool plannable(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t hd, int64_t max_q, int64_t max_context,
@@ -1111,8 +1379,9 @@ int attention(const char *name, int bits, const dtts_f16 *q, const void *kpages,
                  "%s: misaligned operand", name);
     DTTS_REQUIRE(std::isfinite(scale * kLog2e), "%s: scale %g", name, static_cast<double>(scale));
     if (window == 0) sinks = 0;  // every token sees them
-    Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks);
-    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large) * n_kv < (int64_t(1) << 24), "%s: too many rows", name);
+    const bool share = bits == 4;
+    Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks, head_dim, share);
+    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large + p.target + 1) * n_kv < (int64_t(1) << 24), "%s: too many rows", name);
     const int64_t row = heads * head_dim * static_cast<int64_t>(sizeof(half_t));
     DTTS_REQUIRE(q_stride < (int64_t(1) << 62), "%s: q_stride %lld", name, (long long)q_stride);
     DTTS_REQUIRE(!share_bytes({q, tokens, q_stride * static_cast<int64_t>(sizeof(half_t)), row}, {out, 1, 0, tokens * row}),
@@ -1141,7 +1410,12 @@ int attention(const char *name, int bits, const dtts_f16 *q, const void *kpages,
         a.part = static_cast<float *>(workspace);
     } else {
         p.nsplit = 1;  // one workgroup takes all of a tile's keys
+        p.target = 0;
     }
+    a.target = p.target;
+    a.per_target = 1.0f / static_cast<float>(p.target > 0 ? p.target : 1);
+    a.by_kv = FastDiv(static_cast<uint32_t>(n_kv));
+    a.by_gqa = FastDiv(static_cast<uint32_t>(heads / n_kv));
     a.chunk = p.chunk;
     a.nsplit = p.nsplit;
     const auto fn = bits == 16 ? (a.sinks > 0 ? launch_for<false, true> : launch_for<false, false>)
@@ -1153,16 +1427,19 @@ int attention(const char *name, int bits, const dtts_f16 *q, const void *kpages,
 }  // namespace
 }  // namespace dtts
 
-extern "C" size_t dtts_paged_attention_sinks_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim, int64_t max_q,
-                                             int64_t max_context, int64_t window, int64_t sinks) {
+extern "C" size_t dtts_paged_attention_sinks_workspace_bytes(int32_t bits, int64_t tokens, int64_t b, int64_t heads, int64_t n_kv,
+                                                             int64_t head_dim, int64_t max_q, int64_t max_context, int64_t window,
+                                                             int64_t sinks) {
     using namespace dtts;
-    if (!plannable(tokens, b, heads, n_kv, head_dim, max_q, max_context, window, sinks)) return 0;
-    return part_bytes(plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, window ? sinks : 0), tokens, heads, head_dim);
+    if ((bits != 16 && bits != 4) || !plannable(tokens, b, heads, n_kv, head_dim, max_q, max_context, window, sinks)) return 0;
+    if (window == 0) sinks = 0;
+    const bool share = bits == 4;
+    return part_bytes(plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks, head_dim, share), tokens, heads, head_dim);
 }
 
 extern "C" size_t dtts_paged_attention_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
                                                        int64_t max_q, int64_t max_context, int64_t window) {
-    return dtts_paged_attention_sinks_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window, 0);
+    return dtts_paged_attention_sinks_workspace_bytes(16, tokens, b, heads, n_kv, head_dim, max_q, max_context, window, 0);
 }
 
 extern "C" int dtts_paged_attention(int32_t bits, const dtts_f16 *q, const void *kpages, const void *vpages, const int32_t *q_start,

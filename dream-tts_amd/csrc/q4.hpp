@@ -20,6 +20,14 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kQ4Code = 0x00f000f0u, kQ4Base = 0x54005400u;
+// The two in registers: as literals the and-or became two instructions (a three-operand one takes no literal).
+struct Q4Bits {
+    uint32_t code = kQ4Code, base = kQ4Base;
+    __device__ __forceinline__ Q4Bits() {
+        asm("" : "+s"(code));
+        asm("" : "+v"(base));
+    }
+};
 constexpr float kQ4First = 64.0f, kQ4Last = 79.0f;  // the codes' least and greatest
 
 // Bytes of a row, and byte offsets in a page of a kv head.
@@ -32,9 +40,9 @@ struct Q4Row {
 };
 
 // The i-th pair of codes of a word (i a constant), as f16 numbers.
-__device__ __forceinline__ half2_t q4_codes(uint32_t word, int i) {
+__device__ __forceinline__ half2_t q4_codes(uint32_t word, int i, const Q4Bits &bits) {
     const uint32_t at = i == 0 ? word << 4 : i == 1 ? word : i == 2 ? word >> 4 : word >> 8;
-    return __builtin_bit_cast(half2_t, (at & kQ4Code) | kQ4Base);
+    return __builtin_bit_cast(half2_t, (at & bits.code) | bits.base);
 }
 
 // Halves of two words: the low ones, the high ones.
@@ -42,12 +50,12 @@ __device__ __forceinline__ uint32_t low_halves(uint32_t x, uint32_t y) { return 
 __device__ __forceinline__ uint32_t high_halves(uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); }
 
 // The eight values of a word, in order.
-__device__ __forceinline__ half8_t q4_values(uint32_t word, uint32_t pair) {
+__device__ __forceinline__ half8_t q4_values(uint32_t word, uint32_t pair, const Q4Bits &bits) {
     const half2_t d = __builtin_bit_cast(half2_t, low_halves(pair, pair)), b = __builtin_bit_cast(half2_t, high_halves(pair, pair));
     half8_t y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const half2_t v = __builtin_elementwise_fma(q4_codes(word, i), d, b);
+        const half2_t v = __builtin_elementwise_fma(q4_codes(word, i, bits), d, b);
         y[2 * i] = v[0];
         y[2 * i + 1] = v[1];
     }

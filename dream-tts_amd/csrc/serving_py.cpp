@@ -227,8 +227,8 @@ PyObject *attention(PyObject *const *args) {
     if (!a.ok) return none();
     const int64_t tokens = q->size(0), heads = q->size(1);
     const Tensor out = out_of(a, 10, *q, tokens, heads, p.hd);
-    const size_t need = args[11] == Py_None ? dtts_paged_attention_sinks_workspace_bytes(tokens, p.b, heads, p.n_kv, p.hd, max_q,
-                                                                                         max_context, window, sinks) : 0;
+    const size_t need = args[11] == Py_None ? dtts_paged_attention_sinks_workspace_bytes(p.q4 ? 4 : 16, tokens, p.b, heads, p.n_kv,
+                                                                                         p.hd, max_q, max_context, window, sinks) : 0;
     const Tensor ws = workspace_of(a, 11, need, *q);
     if (!a.ok) return none();
     const int status = dtts_paged_attention(

@@ -27,19 +27,20 @@ __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a, FastDiv piece
     if (id < 0 || id >= a.n_pages) return;
     const uint8_t *x = (values ? a.v : a.k) + id * a.page_stride + static_cast<int64_t>(kv) * page * Q4Row<D>::kBytes;
     half_t *y = (values ? a.v_out : a.k_out) + (head << a.page_shift) * D;
+    const Q4Bits bits;
     const u32x4 words = *reinterpret_cast<const u32x4 *>(x + piece * 16);
     if (values) {
         constexpr int W = Q4Row<D>::kWords;
         const int row = piece / W * 4, w = piece % W;
         const u32x4 pairs = *reinterpret_cast<const u32x4 *>(x + Q4Row<D>::pair(page, row, w / 4));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<half8_t *>(y + (row + k) * D + 8 * w) = q4_values(words[k], pairs[k]);
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<half8_t *>(y + (row + k) * D + 8 * w) = q4_values(words[k], pairs[k], bits);
     } else {
         constexpr int G = D / 32;
         const int row = piece / G, group = piece % G;
         const uint32_t pair = *reinterpret_cast<const uint32_t *>(x + Q4Row<D>::pair(page, row, group));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<half8_t *>(y + row * D + 32 * group + 8 * k) = q4_values(words[k], pair);
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<half8_t *>(y + row * D + 32 * group + 8 * k) = q4_values(words[k], pair, bits);
     }
 }
 

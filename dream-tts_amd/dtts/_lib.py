@@ -74,7 +74,7 @@ SIGNATURES = {
     "dtts_qk_rope_append_paged_f16": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],
     "dtts_paged_attention_workspace_bytes": [_I64] * 8,
     "dtts_paged_attention_f16": [_P] * 7 + [_I64] * 13 + [_F32, _P, _SZ, _P],
-    "dtts_paged_attention_sinks_workspace_bytes": [_I64] * 9,
+    "dtts_paged_attention_sinks_workspace_bytes": [_I32] + [_I64] * 9,
     "dtts_paged_attention": [_I32] + [_P] * 7 + [_I64] * 14 + [_F32, _P, _SZ, _P],
     "dtts_qk_rope_append_paged_q4_f32": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],
     "dtts_qk_rope_append_paged_q4_f16": [_P] * 10 + [_I64] * 6 + [_I32] + [_I64] * 5 + [_F32, _P],

@@ -238,10 +238,10 @@ def qk_rope_append_paged(qkv, cos, sin, k_pages, v_pages, q_start, context, page
 
 
 @functools.lru_cache(maxsize=4096)
-def paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window=0, sinks=0):
-    """Workspace bytes paged_attention splits contexts over workgroups with."""
-    return int(lib().dtts_paged_attention_sinks_workspace_bytes(tokens, b, heads, n_kv, head_dim, int(max_q), int(max_context),
-                                                                int(window), int(sinks)))
+def paged_attention_workspace_bytes(tokens, b, heads, n_kv, head_dim, max_q, max_context, window=0, sinks=0, bits=16):
+    """Workspace bytes paged_attention splits contexts over workgroups with (bits: 16, or 4 for 4-bit pages)."""
+    return int(lib().dtts_paged_attention_sinks_workspace_bytes(int(bits), tokens, b, heads, n_kv, head_dim, int(max_q),
+                                                                int(max_context), int(window), int(sinks)))
 
 
 def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale=1.0, window=0, out=None,
@@ -269,7 +269,7 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
         raise DttsError(f"{name}: q {tuple(q.shape)} over pages of head_dim {hd}")
     out = _out(name, dev, out, q, tokens, heads, hd)
     need = 0 if workspace is not None else paged_attention_workspace_bytes(tokens, b, heads, n_kv, hd, max_q, max_context, window,
-                                                                                      sinks)
+                                                                                      sinks, bits)
     keep = ws = None
     ws_bytes = 0
     if need or workspace is not None:

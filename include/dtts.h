@@ -543,8 +543,9 @@ int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dt
  * 4.27 times its width, where the width is its largest less its least), is NaN, all 32.
  * dtts_unpack_pages_q4: the f16 pages [n, n_kv, page, D] that the pages ids[0 .. n - 1] (DEVICE; NULL: the first n) stand for,
  * whatever their slots hold; an id outside [0, n_pages) leaves its part as it was. */
-size_t dtts_paged_attention_sinks_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
-                                                  int64_t max_q, int64_t max_context, int64_t window, int64_t sinks);
+size_t dtts_paged_attention_sinks_workspace_bytes(int32_t bits, int64_t tokens, int64_t b, int64_t heads, int64_t n_kv,
+                                                  int64_t head_dim, int64_t max_q, int64_t max_context, int64_t window,
+                                                  int64_t sinks);
 int dtts_paged_attention(int32_t bits, const dtts_f16 *q, const void *kpages, const void *vpages, const int32_t *q_start,
                          const int32_t *context, const int32_t *page_table, dtts_f16 *out, int64_t tokens, int64_t b,
                          int64_t heads, int64_t n_kv, int64_t head_dim, int64_t page, int64_t n_pages, int64_t max_pages,

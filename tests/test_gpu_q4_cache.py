@@ -194,13 +194,14 @@ def test_attention_rows_and_pages_apart(dev, path):
     assert not bool(out.any())
 
 
-@pytest.mark.parametrize("n,c", [([1, 2], [50, 70]), ([60], [200])])
+@pytest.mark.parametrize("n,c,back", [([1, 2], [50, 70], 2), ([60], [200], 20), ([5], [60], 3), ([9, 1], [700, 40], 6)])
 @pytest.mark.parametrize("hd", [64, 128])
-def test_a_group_that_is_not_finite_reaches_the_tokens_that_see_it(dev, n, c, hd):
-    """A NaN or infinite pair, and codes past f16's range under a finite one, in the last position but one and in a slot after the last."""
+def test_a_group_that_is_not_finite_reaches_the_tokens_that_see_it(dev, n, c, back, hd):
+    """A NaN or infinite pair, and codes past f16's range under a finite one (the group's other values count with their weights), in a
+    position that the first tokens do not see."""
     b = ref.Batch(n, c, 1, hd, 16, dev, seed=3)
     packed, values = q4(b)
-    p = c[0] - 2 if n[0] == 1 else c[0] - 20
+    p = c[0] - back
     words = packed[1].view(torch.int32).view(b.n_pages, -1)
     at = 16 * hd // 8 + 16 + p % 16  # the pair of group 1
     q = torch.randn((b.tokens, 2, hd), generator=torch.Generator().manual_seed(1)).half()
@@ -215,6 +216,22 @@ def test_a_group_that_is_not_finite_reaches_the_tokens_that_see_it(dev, n, c, hd
         assert bool((~fine).any()) and bool(torch.equal(fine, torch.isfinite(got)))
         assert bool(((got - want).abs()[fine] <= bound[fine]).all())
         assert torch.equal(want.isnan(), got.isnan()) and torch.equal(want[want.isinf()], got[want.isinf()])
+
+
+@pytest.mark.parametrize("b,most", [(70, 900), (200, 300), (130, 2500)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 20)])
+def test_many_sequences_of_unequal_lengths(dev, b, most, window, sinks):
+    """Keys are shared out by what all sequences have: more of them than a wave looks at at once, few long among many short, idle
+    ones; with and without the room to cut, and with less of it than the longest would need."""
+    rng = np.random.RandomState(b)
+    n, c = (rng.rand(b) < 0.9).astype(int), rng.randint(1, 60, b)
+    c[rng.randint(0, b, 5)] = most
+    n[b // 2:b // 2 + 3] = 2
+    batch = ref.Batch(list(n), [int(max(x, y)) for x, y in zip(c, n)], 2, 64, 16, dev, seed=b, extra_tokens=1)
+    packed, values = q4(batch)
+    q = torch.randn((batch.tokens, 4, 64), generator=torch.Generator().manual_seed(b)).half()
+    for max_context, workspace in ((most, None), (64, None), (most, torch.empty(0, dtype=torch.uint8, device=dev)), (10 * most, None)):
+        check(batch, packed, values, q, 2, max_context, 0.2, window, sinks, workspace=workspace)
 
 
 def test_a_captured_step(dev):
