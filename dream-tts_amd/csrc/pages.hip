@@ -67,27 +67,30 @@ __global__ __launch_bounds__(256) void trim_kernel(int32_t *pages, int32_t *refs
 
 constexpr int kNT = 1024, kWaves = kNT / 64;
 
-// The exclusive prefix of x over the workgroup, and the total. `sums` holds kWaves + 1; every thread calls it.
-__device__ __forceinline__ int block_prefix(int x, int *sums, int &total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int inc = x;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int v = __shfl_up(inc, off, 64);
-        if (lane >= off) inc += v;
-    }
+// Inclusive sums over the wave's lanes, by data-parallel moves: no trip through LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int from_before(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int sums_to_here(int x) {
+    x += from_before<0x111, 0xf>(x);
+    x += from_before<0x112, 0xf>(x);
+    x += from_before<0x114, 0xf>(x);
+    x += from_before<0x118, 0xf>(x);
+    x += from_before<0x142, 0xa>(x);
+    return x + from_before<0x143, 0xc>(x);
+}
+
+// The exclusive prefix of x over the workgroup, and the total. `sums` holds 2 * kWaves, used in turn by calls of changing
+// `which`, so that one barrier is enough; every thread calls it.
+__device__ __forceinline__ int block_prefix(int x, int *sums, int which, int &total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, inc = sums_to_here(x);
+    sums += which * kWaves;
     if (lane == 63) sums[w] = inc;
     __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        const int v = sums[i];
-        if (i < w) before += v;
-        total += v;
-    }
-    __syncthreads();
-    return before + inc - x;
+    const int of = sums_to_here(lane < kWaves ? sums[lane] : 0);
+    total = __builtin_amdgcn_readlane(of, kWaves - 1);
+    return (w > 0 ? __shfl(of, w - 1, 64) : 0) + inc - x;
 }
 
 // ---------------------------------------------------------------- claim
@@ -119,32 +122,43 @@ __device__ __forceinline__ void blocks_of(const ClaimArgs &a, int s, int &first,
     partial = (at & ((1 << a.page_shift) - 1)) != 0;
 }
 
+constexpr int kSlots = 2 * kNT;   // of a hash table over the shared pages of up to kNT items
+constexpr int kItemsHere = 4096;  // items whose words, and free pages that, stay in LDS; the workspace has those past them
+
+struct ClaimLds {
+    int start[kNT], first[kNT];  // of kNT sequences: the items before theirs, their first block (and a bit: partly filled)
+    int sums[2 * kWaves];
+    __attribute__((aligned(16))) int items[kItemsHere];
+    int free_pages[kItemsHere];
+    int key[kSlots], writers[kSlots], last[kSlots];  // of a shared page: how many items write to it, and the last of them
+};
+
 // f(item, sequence, block, whether the block holds earlier positions) for all items in order, a workgroup's worth at a
 // time; threads past the last get item -1. Returns the number of items.
 template <typename F>
-__device__ __forceinline__ int for_items(const ClaimArgs &a, int *starts, int *sums, F f) {
+__device__ __forceinline__ int for_items(const ClaimArgs &a, ClaimLds &lds, F f) {
     int base = 0;
     for (int s0 = 0; s0 < a.b; s0 += kNT) {
-        int first = 0, count = 0, total;
+        int total, first = 0, count = 0;
         bool partial = false;
         if (s0 + static_cast<int>(threadIdx.x) < a.b) blocks_of(a, s0 + threadIdx.x, first, count, partial);
-        starts[threadIdx.x] = block_prefix(count, sums, total);
+        __syncthreads();
+        lds.start[threadIdx.x] = block_prefix(count, lds.sums, 0, total);
+        lds.first[threadIdx.x] = first << 1 | partial;
         __syncthreads();
         for (int i0 = 0; i0 < total; i0 += kNT) {
             const int i = i0 + threadIdx.x;
             int s = -1, j = 0;
             bool old = false;
             if (i < total) {  // the last sequence that starts at or before i (those without blocks start where the next does)
-                int lo = 0, hi = kNT - 1;
-                while (lo < hi) {
-                    const int mid = (lo + hi + 1) >> 1;
-                    if (starts[mid] <= i) lo = mid; else hi = mid - 1;
-                }
+                int lo = 0;
+#pragma unroll
+                for (int half = kNT / 2; half >= 1; half >>= 1)
+                    if (lds.start[lo + half] <= i) lo += half;
+                const int first = lds.first[lo], k = i - lds.start[lo];
                 s = s0 + lo;
-                int c;
-                blocks_of(a, s, first, c, partial);
-                j = first + i - starts[lo];
-                old = partial && i == starts[lo];
+                j = (first >> 1) + k;
+                old = (first & 1) && k == 0;
             }
             f(i < total ? base + i : -1, s, j, old);
         }
@@ -154,116 +168,250 @@ __device__ __forceinline__ int for_items(const ClaimArgs &a, int *starts, int *s
     return base;
 }
 
+// How many of four words name page w, those from `end` on (counted from the first of them) left out.
+__device__ __forceinline__ int named(const int *words, int w, int end) {
+    typedef int four __attribute__((ext_vector_type(4)));
+    const four x = *reinterpret_cast<const four *>(words);
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n += ((x[k] ^ w) & ~kKept) == 0 && k < end;  // no page's word differs from it in the sign
+    return n;
+}
+
 // One workgroup. A page of r owners to which c of them write is copied by the first min(c, r - 1), as if they came one
-// after another; a writer's rank among them is counted over the earlier items' words.
+// after another: by all of them where c < r, by all but the last where c = r. Where a table has more entries of a page than its
+// count says (c > r), and for items past the first kNT, a writer's rank is counted over the earlier items' words.
+//
+// Bound by its trips to memory, one after another (the starts, the entries, their counts, the free pages' counts, the answers), and
+// by its instructions, each of which the 16 waves of one CU take turns for. 160 sequences that share pages, over 20011: 23.3
+// us with a barrier for every kNT counts; 18.1 with all ranks counted over words in LDS, of which those took 8.
 __global__ __launch_bounds__(kNT) void claim_kernel(ClaimArgs a) {
-    __shared__ int starts[kNT], sums[kWaves];
+    __shared__ ClaimLds lds;
+    typedef int four __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int U = 4, kWaveCounts = 4 * 64 * U;  // a thread requests U times four counts together, a wave as many neighbours
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    four count[U];
+    auto first_of = [&](int p0, int k) { return p0 + w * kWaveCounts + (k * 64 + lane) * 4; };
+    auto load_counts = [&](int p0) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int p = first_of(p0, k);
+            count[k] = four{1, 1, 1, 1};
+            if (p + 3 < a.n_pages) {
+                count[k] = *reinterpret_cast<const four *>(a.refs + p);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 3; ++c)
+                    if (p + c < a.n_pages) count[k][c] = a.refs[p + c];
+            }
+        }
+    };
     for (int s = threadIdx.x; s < a.b; s += kNT) a.src[s] = a.dst[s] = -1;
-    const int items = for_items(a, starts, sums, [&](int i, int s, int j, bool) {
+    for (int s = threadIdx.x; s < kSlots; s += kNT) {
+        lds.key[s] = lds.last[s] = -1;
+        lds.writers[s] = 0;
+    }
+    int my_s = -1, my_j = 0, my_owners = 0;  // of item threadIdx.x, where there is one round of sequences and of items
+    bool my_old = false;
+    const int items = for_items(a, lds, [&](int i, int s, int j, bool old) {
         if (i < 0) return;
         const int e = a.pages[static_cast<int64_t>(s) * a.m + j];
         const int r = holds(e, a.n_pages) ? a.refs[e] : 0;
-        a.items[i] = r < 1 ? kMissing : r == 1 ? kOwned : e;
+        const int word = r < 1 ? kMissing : r == 1 ? kOwned : e;
+        if (i == static_cast<int>(threadIdx.x)) {
+            my_s = s;
+            my_j = j;
+            my_old = old;
+            my_owners = r;
+        }
+        if (i < kItemsHere) lds.items[i] = word;
+        else a.items[i] = word;
     });
-    __threadfence_block();
+    const bool single = items <= kNT && a.b <= kNT;  // item i was thread i's
+    if (items > kItemsHere) __threadfence_block();
     __syncthreads();
-    int need = 0;
+    load_counts(0);
+    int need = 0, turn = 0, slot = 0;
+    if (items <= kNT) {
+        const int x = static_cast<int>(threadIdx.x) < items ? lds.items[threadIdx.x] : kOwned;
+        if (x >= 0) {
+            slot = static_cast<uint32_t>(x) * 2654435769u >> (32 - 11);
+            static_assert(kSlots == 1 << 11, "the hash takes as many bits");
+            for (;;) {  // at most kNT of the 2 kNT slots are taken, so it meets its key or a free one
+                const int met = atomicCAS(&lds.key[slot], -1, x);
+                if (met == -1 || met == x) break;
+                slot = (slot + 1) & (kSlots - 1);
+            }
+            atomicAdd(&lds.writers[slot], 1);
+            atomicMax(&lds.last[slot], static_cast<int>(threadIdx.x));
+        }
+        __syncthreads();
+    }
     for (int i0 = 0; i0 < items; i0 += kNT) {
         const int i = i0 + threadIdx.x;
         int wants = 0, total;
         if (i < items) {
-            const int w = a.items[i];
-            if (w == kMissing) wants = 1;
-            if (w >= 0) {
-                const int r = a.refs[w];
-                int rank = 0;
-                for (int k = 0; k < i && rank < r - 1; ++k) {
-                    const int x = a.items[k];
-                    rank += x >= 0 && (x & ~kKept) == w;
+            const int x = i < kItemsHere ? lds.items[i] : a.items[i];
+            if (x == kMissing) wants = 1;
+            if (x >= 0) {
+                const int r = single ? my_owners : a.refs[x], here = i < kItemsHere ? i : kItemsHere;
+                if (items <= kNT && lds.writers[slot] <= r) {
+                    wants = lds.writers[slot] < r || lds.last[slot] != i;
+                } else {
+                    int rank = 0;
+                    for (int k = 0; k < here && rank < r - 1; k += 4) rank += named(lds.items + k, x, here - k);
+                    for (int k = kItemsHere; k < i && rank < r - 1; ++k) rank += ((a.items[k] ^ x) & ~kKept) == 0;
+                    wants = rank < r - 1;
                 }
-                wants = rank < r - 1;
-                if (!wants) a.items[i] = w | kKept;
+                if (!wants) {
+                    if (i < kItemsHere) lds.items[i] = x | kKept;
+                    else a.items[i] = x | kKept;
+                }
             }
         }
-        block_prefix(wants, sums, total);
+        block_prefix(wants, lds.sums, turn ^= 1, total);
         need += total;
     }
-    // the lowest free pages
+    // the lowest free pages: a wave's, in order, after those of the waves before
     int found = 0;
-    for (int p0 = 0; p0 < a.n_pages && found < need; p0 += kNT) {
-        const int p = p0 + threadIdx.x;
-        const int is_free = p < a.n_pages && a.refs[p] < 1;
-        int total;
-        const int at = found + block_prefix(is_free, sums, total);
-        if (is_free && at < need) a.free_pages[at] = p;
+    for (int p0 = 0; p0 < a.n_pages && found < need; p0 += kWaves * kWaveCounts) {
+        if (p0 > 0) load_counts(p0);
+        uint64_t is_free[U][4];
+        int mine = 0, total;
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                int x = count[k][c];
+                asm volatile("" : "+v"(x));  // not looked at before here, while the counts are under way
+                is_free[k][c] = __ballot(x < 1);
+                mine += __popcll(is_free[k][c]);
+            }
+        const int before = block_prefix(lane == 0 ? mine : 0, lds.sums, turn ^= 1, total);
+        int at = found + __builtin_amdgcn_readfirstlane(before);
+        if (at < need && mine > 0)
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                int to = at;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    to += __popcll(is_free[k][c] & ((uint64_t(1) << lane) - 1));
+                    at += __popcll(is_free[k][c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (!(is_free[k][c] >> lane & 1)) continue;
+                    if (to < need) {
+                        if (to < kItemsHere) lds.free_pages[to] = first_of(p0, k) + c;
+                        else a.free_pages[to] = first_of(p0, k) + c;
+                    }
+                    ++to;
+                }
+            }
         found += total;
     }
     if (threadIdx.x == 0) a.lacking[0] = need > found ? need - found : 0;
     if (need > found || need == 0) return;
-    __threadfence_block();
+    if (items > kItemsHere || need > kItemsHere) __threadfence_block();
     __syncthreads();
     int given = 0;
-    for_items(a, starts, sums, [&](int i, int s, int j, bool old) {
-        const int w = i < 0 ? kOwned : a.items[i];
-        const bool wants = w == kMissing || (w >= 0 && !(w & kKept));
+    auto give = [&](int i, int s, int j, bool old) {
+        const int x = i < 0 ? kOwned : i < kItemsHere ? lds.items[i] : a.items[i];
+        const bool wants = x == kMissing || (x >= 0 && !(x & kKept));
         int total;
-        const int at = given + block_prefix(wants, sums, total);
+        const int at = given + block_prefix(wants, lds.sums, turn ^= 1, total);
         given += total;
         if (!wants) return;
-        const int p = a.free_pages[at];
+        const int p = at < kItemsHere ? lds.free_pages[at] : a.free_pages[at];
         a.pages[static_cast<int64_t>(s) * a.m + j] = p;
         a.refs[p] = 1;
-        if (w >= 0) {
-            atomicSub(a.refs + w, 1);
+        if (x >= 0) {
+            atomicSub(a.refs + x, 1);
             if (old) {
-                a.src[s] = w;
+                a.src[s] = x;
                 a.dst[s] = p;
             }
         }
-    });
+    };
+    if (single)
+        give(static_cast<int>(threadIdx.x) < items ? static_cast<int>(threadIdx.x) : -1, my_s, my_j, my_old);
+    else
+        for_items(a, lds, give);
 }
 
 // ---------------------------------------------------------------- compact
 
 struct CompactArgs {
     int32_t *pages, *refs, *src, *dst, *used;
-    int32_t *rank;  // workspace [n_pages]: of a used page the used ones before it, of a free one -1 - the free ones before it
-    int32_t *below; // workspace: the used pages under the count of all used ones
+    int32_t *rank;    // workspace [n_pages]: of a used page the used ones before it, of a free one -1 - the free ones before it
+    int32_t *counts;  // workspace: used pages of each kSpan
     int64_t entries;
-    int n_pages;
+    int n_pages, spans;
 };
 
+constexpr int kSpan = 4096;  // pages a workgroup of 1024 threads counts
+
+// The first launch: how many pages of each span are used.
+__global__ __launch_bounds__(kNT) void compact_count_kernel(CompactArgs a) {
+    __shared__ int sums[2 * kWaves];
+    int used = 0, total;
+#pragma unroll
+    for (int k = 0; k < kSpan / kNT; ++k) {
+        const int p = blockIdx.x * kSpan + k * kNT + threadIdx.x;
+        used += p < a.n_pages && a.refs[p] > 0;
+    }
+    block_prefix(used, sums, 0, total);
+    if (threadIdx.x == 0) a.counts[blockIdx.x] = total;
+}
+
+// The second: every workgroup sums the spans' counts for itself (and the used pages before the first one past all of them, in
+// whose span it looks), ranks its span's pages and writes the moves down.
 __global__ __launch_bounds__(kNT) void compact_rank_kernel(CompactArgs a) {
-    __shared__ int sums[kWaves];
-    int count = 0;
-    for (int p0 = 0; p0 < a.n_pages; p0 += kNT) {
-        const int p = p0 + threadIdx.x, is_used = p < a.n_pages && a.refs[p] > 0;
-        int total;
-        const int at = count + block_prefix(is_used, sums, total);
-        if (p < a.n_pages) a.rank[p] = is_used ? at : -1 - (p - at);
-        count += total;
+    __shared__ int sums[2 * kWaves];
+    int used, before, total, mine[kSpan / kNT];
+#pragma unroll
+    for (int k = 0; k < kSpan / kNT; ++k) {
+        const int p = blockIdx.x * kSpan + k * kNT + threadIdx.x;
+        mine[k] = p < a.n_pages && a.refs[p] > 0;
     }
-    if (threadIdx.x == 0) {
-        a.used[0] = count;
-        a.below[0] = count;
+    int all = 0, here = 0;
+    for (int i = threadIdx.x; i < a.spans; i += kNT) {
+        const int c = a.counts[i];
+        all += c;
+        here += i < static_cast<int>(blockIdx.x) ? c : 0;
     }
-    __threadfence_block();
-    __syncthreads();
-    // the rank of the first page past them, whichever kind it is
-    if (threadIdx.x == 0 && count < a.n_pages) a.below[0] = a.rank[count] >= 0 ? a.rank[count] : count - (-1 - a.rank[count]);
+    block_prefix(all, sums, 0, used);
+    block_prefix(here, sums, 1, before);
+    const int at = used / kSpan;  // the span that page `used` is in (or past the last)
+    int low = 0, below;
+    for (int i = threadIdx.x; i < a.spans; i += kNT) low += i < at ? a.counts[i] : 0;
+#pragma unroll
+    for (int k = 0; k < kSpan / kNT; ++k) {
+        const int p = at * kSpan + k * kNT + threadIdx.x;
+        low += p < used && p < a.n_pages && a.refs[p] > 0;
+    }
+    block_prefix(low, sums, 0, below);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        a.used[0] = used;
+        a.counts[a.spans] = below;
+    }
+    const int moves = used - below;
+#pragma unroll
+    for (int k = 0; k < kSpan / kNT; ++k) {
+        const int p = blockIdx.x * kSpan + k * kNT + threadIdx.x;
+        const int r = before + block_prefix(mine[k], sums, (k & 1) ^ 1, total);
+        before += total;
+        if (p >= a.n_pages) continue;
+        a.rank[p] = mine[k] ? r : -1 - (p - r);
+        if (mine[k] && p >= used) a.src[r - below] = p;
+        if (!mine[k] && p < used) a.dst[p - r] = p;
+        if (p >= moves) a.src[p] = a.dst[p] = -1;
+    }
 }
 
-__global__ __launch_bounds__(256) void compact_pairs_kernel(CompactArgs a) {
-    const int p = blockIdx.x * 256 + threadIdx.x;
-    if (p >= a.n_pages) return;
-    const int used = a.used[0], below = a.below[0], r = a.rank[p];
-    if (r >= 0 && p >= used) a.src[r - below] = p;
-    if (r < 0 && p < used) a.dst[-1 - r] = p;
-    if (p >= used - below) a.src[p] = a.dst[p] = -1;
-}
-
+// The third: counts and entries.
 __global__ __launch_bounds__(256) void compact_apply_kernel(CompactArgs a) {
-    const int used = a.used[0], below = a.below[0];
+    const int used = a.used[0], below = a.counts[a.spans];
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i < used - below) {
         const int s = a.src[i];
@@ -285,19 +433,66 @@ constexpr int kMostCaches = 64;
 
 struct CopyArgs {
     uint8_t *cache[kMostCaches];
-    int64_t stride[kMostCaches];  // bytes from page to page
-    int parts[kMostCaches];       // 16-byte parts of a page
+    int64_t stride[kMostCaches];   // bytes from page to page
+    uint32_t units[kMostCaches];   // of 16 bytes in a page
+    uint32_t slices[kMostCaches];  // the caches' pages are cut into slices of at most kSlice units: those before the next cache's
+    FastDiv by_last[kMostCaches];  // by the units of a cache's last slice
+    FastDiv by_slice;
     const int32_t *src, *dst;
     int n, n_pages;
 };
 
+// Units a thread requests together, and a workgroup's at a time.
+constexpr int kRequests = 4, kSlice = 256 * kRequests;
+constexpr int64_t kCopyFill = 4096;  // workgroups
+
+// HBM-bound: every byte read once and written once. A workgroup takes one slice of every gridDim.x-th pair's pages, 256 pairs at
+// a time: those that copy something are put together first, so that a list with few of them, or with all of them in front, is
+// shared out as evenly as a full one, and small pages fill a workgroup.
 __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
-    const int i = blockIdx.x, c = blockIdx.y;
-    const int s = a.src[i], d = a.dst[i];
-    if (!holds(s, a.n_pages) || !holds(d, a.n_pages)) return;
-    const float4_t *x = reinterpret_cast<const float4_t *>(a.cache[c] + s * a.stride[c]);
-    float4_t *y = reinterpret_cast<float4_t *>(a.cache[c] + d * a.stride[c]);
-    for (int k = threadIdx.x; k < a.parts[c]; k += 256) y[k] = x[k];
+    __shared__ int from[256], to[256], waves[4];
+    uint32_t c = 0, slice = blockIdx.y;
+    while (slice >= a.slices[c]) ++c;
+    if (c > 0) slice -= a.slices[c - 1];
+    const uint32_t u0 = slice * kSlice, units = a.units[c] - u0 < kSlice ? a.units[c] - u0 : kSlice;
+    const FastDiv by_units = units == kSlice ? a.by_slice : a.by_last[c];
+    uint8_t *base = a.cache[c] + static_cast<int64_t>(u0) * 16;
+    const int64_t stride = a.stride[c];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int64_t i0 = blockIdx.x; i0 < a.n; i0 += 256 * static_cast<int64_t>(gridDim.x)) {
+        const int64_t i = i0 + static_cast<int64_t>(threadIdx.x) * gridDim.x;
+        const int s = i < a.n ? a.src[i] : -1, d = i < a.n ? a.dst[i] : -1;
+        const bool copies = holds(s, a.n_pages) && holds(d, a.n_pages);
+        const uint64_t mask = __ballot(copies);
+        __syncthreads();
+        if (lane == 0) waves[w] = __popcll(mask);
+        __syncthreads();
+        int at = __popcll(mask & ((uint64_t(1) << lane) - 1)), pairs = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k < w) at += waves[k];
+            pairs += waves[k];
+        }
+        if (copies) {
+            from[at] = s;
+            to[at] = d;
+        }
+        __syncthreads();
+        const uint32_t all = static_cast<uint32_t>(pairs) * units;
+        for (uint32_t t0 = threadIdx.x; t0 < all; t0 += kSlice) {
+            float4_t x[kRequests];
+#pragma unroll
+            for (int k = 0; k < kRequests; ++k) {
+                const uint32_t t = t0 + k * 256, p = by_units.div(t);
+                if (t < all) x[k] = *reinterpret_cast<const float4_t *>(base + from[p] * stride + static_cast<int64_t>(t - p * units) * 16);
+            }
+#pragma unroll
+            for (int k = 0; k < kRequests; ++k) {
+                const uint32_t t = t0 + k * 256, p = by_units.div(t);
+                if (t < all) *reinterpret_cast<float4_t *>(base + to[p] * stride + static_cast<int64_t>(t - p * units) * 16) = x[k];
+            }
+        }
+    }
 }
 
 inline unsigned blocks_for(int64_t n) { return static_cast<unsigned>((n + 255) / 256); }
@@ -406,7 +601,8 @@ extern "C" int dtts_claim_pages(int32_t *pages, int32_t *refs, const int32_t *q_
 }
 
 extern "C" size_t dtts_compact_pages_workspace_bytes(int64_t n_pages) {
-    return n_pages < 1 || n_pages > dtts::kMostPages ? 0 : static_cast<size_t>(n_pages + 1) * 4;
+    using namespace dtts;
+    return n_pages < 1 || n_pages > kMostPages ? 0 : static_cast<size_t>(n_pages + (n_pages + kSpan - 1) / kSpan + 1) * 4;
 }
 
 extern "C" int dtts_compact_pages(int32_t *pages, int32_t *refs, int32_t *src, int32_t *dst, int32_t *used, int64_t b, int64_t max_pages,
@@ -430,13 +626,14 @@ extern "C" int dtts_compact_pages(int32_t *pages, int32_t *refs, int32_t *src, i
     a.src = src;
     a.dst = dst;
     a.used = used;
-    a.below = static_cast<int32_t *>(workspace);
-    a.rank = a.below + 1;
+    a.rank = static_cast<int32_t *>(workspace);
+    a.counts = a.rank + n_pages;
     a.entries = b * max_pages;
     a.n_pages = static_cast<int>(n_pages);
-    compact_rank_kernel<<<1, kNT, 0, stream>>>(a);
+    a.spans = static_cast<int>((n_pages + kSpan - 1) / kSpan);
+    compact_count_kernel<<<a.spans, kNT, 0, stream>>>(a);
     DTTS_LAUNCH_CHECK(name);
-    compact_pairs_kernel<<<blocks_for(n_pages), 256, 0, stream>>>(a);
+    compact_rank_kernel<<<a.spans, kNT, 0, stream>>>(a);
     DTTS_LAUNCH_CHECK(name);
     compact_apply_kernel<<<blocks_for(a.entries > n_pages ? a.entries : n_pages), 256, 0, stream>>>(a);
     DTTS_LAUNCH_CHECK(name);
@@ -454,25 +651,35 @@ extern "C" int dtts_copy_pages(void **caches, const int64_t *page_bytes, const i
     DTTS_REQUIRE(aligned(src, 4) && aligned(dst, 4), "%s: misaligned operand", name);
     for (int64_t c = 0; c < n_caches; ++c) {
         DTTS_REQUIRE(caches[c] && aligned(caches[c], 16), "%s: cache %lld is null or not 16-byte aligned", name, (long long)c);
-        DTTS_REQUIRE(page_bytes[c] > 0 && page_bytes[c] % 16 == 0 && page_bytes[c] < (int64_t(1) << 34) && page_strides[c] % 16 == 0 &&
+        DTTS_REQUIRE(page_bytes[c] > 0 && page_bytes[c] % 16 == 0 && page_bytes[c] < (int64_t(1) << 29) && page_strides[c] % 16 == 0 &&
                          page_strides[c] >= page_bytes[c] && page_strides[c] < (int64_t(1) << 34),
-                     "%s: pages of %lld bytes, %lld apart (multiples of 16 under 2^34)", name, (long long)page_bytes[c],
+                     "%s: pages of %lld bytes, %lld apart (multiples of 16, under 2^29 and 2^34)", name, (long long)page_bytes[c],
                      (long long)page_strides[c]);
     }
-    for (int64_t c0 = 0; c0 < n_caches; c0 += kMostCaches) {
+    for (int64_t c0 = 0; c0 < n_caches;) {
         CopyArgs a;
-        const int64_t left = n_caches - c0, some = left < kMostCaches ? left : kMostCaches;
-        for (int64_t c = 0; c < some; ++c) {
+        int64_t slices = 0, c = 0;
+        for (; c < kMostCaches && c0 + c < n_caches; ++c) {
+            const int64_t units = page_bytes[c0 + c] / 16, more = (units + kSlice - 1) / kSlice;
+            if (c > 0 && slices + more > 65535) break;
+            slices += more;
             a.cache[c] = static_cast<uint8_t *>(caches[c0 + c]);
             a.stride[c] = page_strides[c0 + c];
-            a.parts[c] = static_cast<int>(page_bytes[c0 + c] / 16);
+            a.units[c] = static_cast<uint32_t>(units);
+            a.slices[c] = static_cast<uint32_t>(slices);
+            a.by_last[c] = FastDiv(static_cast<uint32_t>(units - (more - 1) * kSlice));
         }
         a.src = src;
         a.dst = dst;
         a.n = static_cast<int>(n);
         a.n_pages = static_cast<int>(n_pages);
-        copy_kernel<<<dim3(static_cast<unsigned>(n), static_cast<unsigned>(some)), 256, 0, stream>>>(a);
+        a.by_slice = FastDiv(kSlice);
+        // enough workgroups that the pairs which copy something, few or many, keep the chip busy
+        int64_t x = (kCopyFill + slices - 1) / slices;
+        x = x < n ? x : n;
+        copy_kernel<<<dim3(static_cast<unsigned>(x), static_cast<unsigned>(slices)), 256, 0, stream>>>(a);
         DTTS_LAUNCH_CHECK(name);
+        c0 += c;
     }
     return DTTS_OK;
 }
