@@ -83,6 +83,14 @@ struct SinkTiles {
     }
 };
 
+// The keys that the at-th 128-row tile of a sequence sees, in chunks. (Cut by its sequence's, a chunk of 700 tokens of 8 query heads a
+// kv head under a window of 1000 has five chunks for each tile's three: 36 and 31 us.)
+__device__ __forceinline__ Span tile_span(const AttnArgs &a, int at, int n_new, int ctx) {
+    const int rows = n_new * a.gqa, end = (at + 1) * 128 < rows ? (at + 1) * 128 : rows;
+    const int first = static_cast<int>(a.by_gqa.div(at * 128)), last = static_cast<int>(a.by_gqa.div(end - 1));
+    return Span(a, last - first + 1, ctx - n_new + last + 1, a.chunk);
+}
+
 // A tile of rows: its sequence (-1: none), place in it, the sequence's first row and new tokens, context.
 struct Tile {
     int s, at, first, n_new, ctx;
@@ -765,22 +773,23 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     auto &sk = lds.k;
     auto &sv = lds.v;
     auto &s_ok = lds.ok;
-    const int kh = block_no % a.n_kv;
-    const Tile tile = find_tile(a, ROWS, a.few, INT64_MAX, block_no / a.n_kv);
+    const int tile_no = static_cast<int>(a.by_kv.div(static_cast<uint32_t>(block_no))), kh = block_no - tile_no * a.n_kv;
+    const Tile tile = find_tile(a, ROWS, a.few, INT64_MAX, tile_no);
     if (tile.s < 0) return;
     const int s = tile.s, at = tile.at, first = tile.first, n_new = tile.n_new, ctx = tile.ctx, pos0 = ctx - n_new;
-    const Span span(a, n_new, ctx, a.chunk);
+    const Span span = Q4 || SINKS ? tile_span(a, at, n_new, ctx) : Span(a, n_new, ctx, a.chunk);
     const int c = blockIdx.y;
     if (c >= span.n) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
     const int r0 = at * ROWS, n_rows = n_new * a.gqa - r0 < ROWS ? n_new * a.gqa - r0 : ROWS;
     int k0, k1;
     span.chunk_keys(a.chunk, c, k0, k1);
+    const auto token_of = [&](int r) { return static_cast<int>(a.by_gqa.div(static_cast<uint32_t>(r))); };
     // all of the tile's rows see the keys from `from` to `upto`
-    const int upto = pos0 + r0 / a.gqa, from = a.window > 0 ? pos0 + (r0 + n_rows - 1) / a.gqa - a.window + 1 : 0;
+    const int upto = pos0 + token_of(r0), from = a.window > 0 ? pos0 + token_of(r0 + n_rows - 1) - a.window + 1 : 0;
     int mid = 0, next = 0;
     {
-        const int top = pos0 + (r0 + n_rows - 1) / a.gqa + 1, bottom = a.window > 0 ? upto - a.window + 1 : 0;
+        const int top = pos0 + token_of(r0 + n_rows - 1) + 1, bottom = a.window > 0 ? upto - a.window + 1 : 0;
         if constexpr (SINKS) {
             const SinkTiles tiles(span, bottom, KT, k0, k1);
             mid = tiles.mid;
@@ -797,9 +806,9 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     // the wave's rows and the lane's
     const int wrows = n_rows - 32 * w < 32 ? n_rows - 32 * w : 32;
     const int row = r0 + 32 * w + (l32 < wrows ? l32 : wrows > 0 ? wrows - 1 : -32 * w);
-    const int tok = row / a.gqa, head = kh * a.gqa + row - tok * a.gqa, pos = pos0 + tok;
+    const int tok = token_of(row), head = kh * a.gqa + row - tok * a.gqa, pos = pos0 + tok;
     const int row_lo = a.window > 0 ? pos - a.window + 1 : 0;
-    const int wfirst = pos0 + (r0 + 32 * w) / a.gqa, wlast = pos0 + (r0 + 32 * w + wrows - 1) / a.gqa;
+    const int wfirst = pos0 + token_of(r0 + 32 * w), wlast = pos0 + token_of(wrows > 0 ? r0 + 32 * w + wrows - 1 : r0);
     half8_t qf[C];
     {
         const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
@@ -1114,10 +1123,21 @@ __global__ __launch_bounds__(256, 2) void paged_attn_mixed(AttnArgs a, int large
 // Join a row's chunks: out = sum_c num_c w_c / sum_c den_c w_c, w_c = 2^((m_c - M) scale2), M the largest m_c.
 constexpr int kFewChunks = 8;
 
+// How many chunks token t's rows of query head `head` were cut into. OWN: by their tile's keys, or by what the device shared out.
+template <bool OWN>
+__device__ __forceinline__ int chunks_of_row(const AttnArgs &a, int s, int t, int head, int first, int n_new) {
+    const int ctx = a.batch.length(s);
+    if (!OWN) return Span(a, n_new, ctx, a.chunk).n;
+    if (a.target > 0) return chunks_of(Span(a, n_new, ctx).blocks(), shared_blocks(a, Lane(a, threadIdx.x & 63)));
+    if (static_cast<int64_t>(n_new) * a.gqa <= a.few) return Span(a, n_new, ctx, a.chunk).n;
+    const int row = (t - first) * a.gqa + head - static_cast<int>(a.by_gqa.div(head)) * a.gqa;
+    return tile_span(a, row / 128, n_new, ctx).n;
+}
+
 // Up to kFewChunks: a wave for R heads of a token, which share its lookups, everything requested at once. 862 tokens of
 // 16 heads over four chunks with 1 / 2 / 4 heads a wave: 7.3 / 5.6 / 6.5 us; with the chunks requested before it is known
 // how many a row has 8.5.
-template <int D, int R, bool SHARED>
+template <int D, int R, bool OWN>
 __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
     constexpr int PER = D / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1128,16 +1148,21 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
     int first, n_new;
     a.batch.rows(s, first, n_new);
     if (t < first || t - first >= n_new) return;
-    const Span span = SHARED ? Span(a, n_new, a.batch.length(s)) : Span(a, n_new, a.batch.length(s), a.chunk);
-    const int n = SHARED ? chunks_of(span.blocks(), shared_blocks(a, Lane(a, lane))) : span.n;
-    if (n <= 1) return;
+    const int head0 = static_cast<int>(trow - static_cast<int64_t>(t) * a.heads);
+    int n[R], most = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        n[r] = OWN || r == 0 ? chunks_of_row<OWN>(a, s, t, head0 + r, first, n_new) : n[0];
+        most = n[r] > most ? n[r] : most;
+    }
+    if (most <= 1) return;
     const float *pr = a.part + trow * a.nsplit * (D + 4);
     float mc[R][kFewChunks], lc[R][kFewChunks], v[R][kFewChunks][PER];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int c = 0; c < kFewChunks; ++c)
-            if (c < n) {
+            if (c < n[r]) {
                 const float *pc = pr + static_cast<int64_t>(r * a.nsplit + c) * (D + 4);
                 mc[r][c] = pc[D + 1];
                 lc[r][c] = pc[D];
@@ -1146,14 +1171,15 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
             }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+        if (n[r] <= 1) continue;
         float num[PER] = {}, den = 0.0f, m = -INFINITY;
 #pragma unroll
         for (int c = 0; c < kFewChunks; ++c)
-            if (c < n) m = fmaxf(m, mc[r][c]);
+            if (c < n[r]) m = fmaxf(m, mc[r][c]);
         const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int c = 0; c < kFewChunks; ++c)
-            if (c < n) {
+            if (c < n[r]) {
                 const float f = exp2_fast((mc[r][c] - mu) * a.scale2);
                 den += lc[r][c] * f;
 #pragma unroll
@@ -1168,7 +1194,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
 // More: a workgroup a row, wave w taking chunks w, w + 4, ..; 64 of its chunks at a time have their maxima and sums read
 // by a lane each, then their rows follow with U requests in flight (5 tokens of 32 heads, 51 chunks: 19.6 us with a
 // loop that carries the maximum along and waits for each, 5.1 so).
-template <int D, bool SHARED>
+template <int D, bool OWN>
 __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     constexpr int PER = D / 64, U = 8, W = 4;
     __shared__ float sm[W][D + 2];
@@ -1179,8 +1205,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     int first, n_new;
     a.batch.rows(s, first, n_new);
     if (t < first || t - first >= n_new) return;
-    const Span span = SHARED ? Span(a, n_new, a.batch.length(s)) : Span(a, n_new, a.batch.length(s), a.chunk);
-    const int n = SHARED ? chunks_of(span.blocks(), shared_blocks(a, Lane(a, lane))) : span.n;
+    const int n = chunks_of_row<OWN>(a, s, t, static_cast<int>(trow - static_cast<int64_t>(t) * a.heads), first, n_new);
     if (n <= 1) return;
     float num[PER] = {}, den = 0.0f, m = -INFINITY;
     const float *pr = a.part + trow * a.nsplit * (D + 4);
@@ -1265,13 +1290,13 @@ constexpr int64_t kFew = 32;
 // saves. In a captured graph, one token of 8 kv heads over 256 / 384 / 448 / 512 keys: 6.8 / 8.1 / 8.8 / 9.1 us whole,
 // 8.0 / 8.2 / 8.2 / 8.3 cut (4 of D = 64: 5.6 / 6.6 / 7.2 / 7.3 and 7.2 / 7.4 / 7.5 / 7.5). From 128 tiles on, twice that
 // (16 tokens of 8 kv heads over 512 / 768 / 1024: 10.9 / 15.7 / 19.2 whole, 13.1 / 15.7 / 19.0 cut).
-constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kWhole = 384;
+constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kWhole = 384, kSlots = 512, kFillWindow = 320;
 
 // Where the device shares the keys out (a token or a few of each sequence, over 4-bit pages or with sinks):
 constexpr int64_t kFillShared = 1024, kShareBytes = int64_t(64) << 20;
 
 inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window,
-                    int64_t sinks, int64_t hd, bool share) {
+                    int64_t sinks, int64_t hd, bool share, bool own) {
     Plan p;
     p.target = 0;
     const int64_t rows = tokens * gqa, live = b < tokens ? b : tokens;
@@ -1289,13 +1314,16 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
         const int64_t most = rows / (kFew + 1) < live ? rows / (kFew + 1) : live;  // sequences of that many rows
         p.large = (rows + 127 * most) / 128;
     }
-    const int64_t seen = window + max_q + 63 + (sinks > 0 ? sinks + 63 : 0);
+    const int64_t tile = 128 / gqa + 2, q = own && p.large > 0 && tile < max_q ? tile : max_q;  // a 128-row tile's tokens
+    const int64_t seen = window + q + 63 + (sinks > 0 ? sinks + 63 : 0);
     int64_t span = window > 0 && seen < max_context ? seen : max_context;
     if (span < 1) span = 1;
     if (span > int64_t(1) << 30) span = int64_t(1) << 30;  // no table holds more
     // the launch is sized for the most tiles there can be; the chunks go by what a batch of long chunks has
-    const int64_t wgs = (p.large > 0 ? rows / 128 + 1 : p.small) * n_kv, whole = wgs < 128 ? kWhole : 2 * kWhole;
-    int64_t n = ((p.large > 0 ? kFillLarge : kFillSmall) + wgs - 1) / wgs;
+    const int64_t wgs = (p.large > 0 ? (own && b == 1 ? p.large : rows / 128 + 1) : p.small) * n_kv, whole = wgs < 128 ? kWhole : 2 * kWhole;
+    int64_t n = ((p.large > 0 ? (own && window > 0 ? kFillWindow : kFillLarge) : kFillSmall) + wgs - 1) / wgs;
+    // and not so that a few workgroups are left over when all others are done
+    if (own && p.large > 0 && n * wgs > kSlots && n * wgs % kSlots < kSlots / 4) ++n;
     const int64_t most = span <= whole ? 1 : (span + kMinChunk - 1) / kMinChunk;
     if (n > most) n = most;
     p.chunk = static_cast<int>(((span + n - 1) / n + 63) / 64 * 64);
@@ -1319,15 +1347,15 @@ inline size_t part_bytes(const Plan &p, int64_t tokens, int64_t heads, int64_t h
     return p.nsplit > 1 ? static_cast<size_t>(tokens * heads * p.nsplit * (hd + 4)) * sizeof(float) : 0;
 }
 
-template <int D, bool SHARED>
+template <int D, bool OWN>
 hipError_t merge(const AttnArgs &a, hipStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
     if (a.nsplit <= kFewChunks && a.heads % 2 == 0)
-        paged_attn_merge_few<D, 2, SHARED><<<static_cast<unsigned>((rows / 2 + 3) / 4), 256, 0, stream>>>(a);
+        paged_attn_merge_few<D, 2, OWN><<<static_cast<unsigned>((rows / 2 + 3) / 4), 256, 0, stream>>>(a);
     else if (a.nsplit <= kFewChunks)
-        paged_attn_merge_few<D, 1, SHARED><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+        paged_attn_merge_few<D, 1, OWN><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
     else
-        paged_attn_merge<D, SHARED><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
+        paged_attn_merge<D, OWN><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -1342,7 +1370,7 @@ hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
             256, 0, stream>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
-    return Q4 && a.target > 0 ? merge<D, Q4>(a, stream) : merge<D, false>(a, stream);
+    return merge<D, Q4 || SINKS>(a, stream);
 }
 
 inline bool plannable(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t hd, int64_t max_q, int64_t max_context,
@@ -1379,8 +1407,8 @@ int attention(const char *name, int bits, const dtts_f16 *q, const void *kpages,
                  "%s: misaligned operand", name);
     DTTS_REQUIRE(std::isfinite(scale * kLog2e), "%s: scale %g", name, static_cast<double>(scale));
     if (window == 0) sinks = 0;  // every token sees them
-    const bool share = bits == 4;
-    Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks, head_dim, share);
+    const bool share = bits == 4, own = bits == 4 || (sinks > 0 && window < int64_t(1) << 30);
+    Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks, head_dim, share, own);
     DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large + p.target + 1) * n_kv < (int64_t(1) << 24), "%s: too many rows", name);
     const int64_t row = heads * head_dim * static_cast<int64_t>(sizeof(half_t));
     DTTS_REQUIRE(q_stride < (int64_t(1) << 62), "%s: q_stride %lld", name, (long long)q_stride);
@@ -1433,8 +1461,8 @@ extern "C" size_t dtts_paged_attention_sinks_workspace_bytes(int32_t bits, int64
     using namespace dtts;
     if ((bits != 16 && bits != 4) || !plannable(tokens, b, heads, n_kv, head_dim, max_q, max_context, window, sinks)) return 0;
     if (window == 0) sinks = 0;
-    const bool share = bits == 4;
-    return part_bytes(plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks, head_dim, share), tokens, heads, head_dim);
+    const bool share = bits == 4, own = bits == 4 || (sinks > 0 && window < int64_t(1) << 30);
+    return part_bytes(plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks, head_dim, share, own), tokens, heads, head_dim);
 }
 
 extern "C" size_t dtts_paged_attention_workspace_bytes(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t head_dim,
