@@ -350,17 +350,25 @@ struct CompactArgs {
 };
 
 constexpr int kSpan = 4096;  // pages a workgroup of 1024 threads counts
+// Spans up to which every workgroup counts all of them for itself, which saves the launch before (6001 pages: 12.0 -> 9.6 us a call).
+constexpr int kFewSpans = 4;
+
+// Thread's share of span `span`'s pages that are used.
+__device__ __forceinline__ int used_of_span(const CompactArgs &a, int span) {
+    int used = 0;
+#pragma unroll
+    for (int k = 0; k < kSpan / kNT; ++k) {
+        const int p = span * kSpan + k * kNT + threadIdx.x;
+        used += p < a.n_pages && a.refs[p] > 0;
+    }
+    return used;
+}
 
 // The first launch: how many pages of each span are used.
 __global__ __launch_bounds__(kNT) void compact_count_kernel(CompactArgs a) {
     __shared__ int sums[2 * kWaves];
-    int used = 0, total;
-#pragma unroll
-    for (int k = 0; k < kSpan / kNT; ++k) {
-        const int p = blockIdx.x * kSpan + k * kNT + threadIdx.x;
-        used += p < a.n_pages && a.refs[p] > 0;
-    }
-    block_prefix(used, sums, 0, total);
+    int total;
+    block_prefix(used_of_span(a, blockIdx.x), sums, 0, total);
     if (threadIdx.x == 0) a.counts[blockIdx.x] = total;
 }
 
@@ -374,17 +382,32 @@ __global__ __launch_bounds__(kNT) void compact_rank_kernel(CompactArgs a) {
         const int p = blockIdx.x * kSpan + k * kNT + threadIdx.x;
         mine[k] = p < a.n_pages && a.refs[p] > 0;
     }
-    int all = 0, here = 0;
-    for (int i = threadIdx.x; i < a.spans; i += kNT) {
-        const int c = a.counts[i];
-        all += c;
-        here += i < static_cast<int>(blockIdx.x) ? c : 0;
+    int all = 0, here = 0, of[kFewSpans] = {};
+    const bool few = a.spans <= kFewSpans;
+    if (few) {
+#pragma unroll
+        for (int i = 0; i < kFewSpans; ++i) {
+            of[i] = used_of_span(a, i);
+            all += of[i];
+            here += i < static_cast<int>(blockIdx.x) ? of[i] : 0;
+        }
+    } else {
+        for (int i = threadIdx.x; i < a.spans; i += kNT) {
+            const int c = a.counts[i];
+            all += c;
+            here += i < static_cast<int>(blockIdx.x) ? c : 0;
+        }
     }
     block_prefix(all, sums, 0, used);
     block_prefix(here, sums, 1, before);
     const int at = used / kSpan;  // the span that page `used` is in (or past the last)
     int low = 0, below;
-    for (int i = threadIdx.x; i < a.spans; i += kNT) low += i < at ? a.counts[i] : 0;
+    if (few) {
+#pragma unroll
+        for (int i = 0; i < kFewSpans; ++i) low += i < at ? of[i] : 0;
+    } else {
+        for (int i = threadIdx.x; i < a.spans; i += kNT) low += i < at ? a.counts[i] : 0;
+    }
 #pragma unroll
     for (int k = 0; k < kSpan / kNT; ++k) {
         const int p = at * kSpan + k * kNT + threadIdx.x;
@@ -431,25 +454,28 @@ __global__ __launch_bounds__(256) void compact_apply_kernel(CompactArgs a) {
 
 constexpr int kMostCaches = 64;
 
+// MOST: caches there is room for (a launch copies the arguments, and one layer's keys and values need no kilobytes of them).
+template <int MOST>
 struct CopyArgs {
-    uint8_t *cache[kMostCaches];
-    int64_t stride[kMostCaches];   // bytes from page to page
-    uint32_t units[kMostCaches];   // of 16 bytes in a page
-    uint32_t slices[kMostCaches];  // the caches' pages are cut into slices of at most kSlice units: those before the next cache's
-    FastDiv by_last[kMostCaches];  // by the units of a cache's last slice
+    uint8_t *cache[MOST];
+    int64_t stride[MOST];   // bytes from page to page
+    uint32_t units[MOST];   // of 16 bytes in a page
+    uint32_t slices[MOST];  // the caches' pages are cut into slices of at most kSlice units: those before the next cache's
+    FastDiv by_last[MOST];  // by the units of a cache's last slice
     FastDiv by_slice;
     const int32_t *src, *dst;
     int n, n_pages;
 };
 
 // Units a thread requests together, and a workgroup's at a time.
-constexpr int kRequests = 4, kSlice = 256 * kRequests;
-constexpr int64_t kCopyFill = 4096;  // workgroups
+constexpr int kRequests = 2, kSlice = 256 * kRequests;
+constexpr int64_t kCopyFill = 8192;  // workgroups: 1250 pages of 64 KB of 6001, and 4600 of 2.5 KB of 100003, 24.2 and 21.9 us with 4 requests and 4096, 23.6 and 21.1 so
 
 // HBM-bound: every byte read once and written once. A workgroup takes one slice of every gridDim.x-th pair's pages, 256 pairs at
 // a time: those that copy something are put together first, so that a list with few of them, or with all of them in front, is
 // shared out as evenly as a full one, and small pages fill a workgroup.
-__global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
+template <int MOST>
+__global__ __launch_bounds__(256) void copy_kernel(CopyArgs<MOST> a) {
     __shared__ int from[256], to[256], waves[4];
     uint32_t c = 0, slice = blockIdx.y;
     while (slice >= a.slices[c]) ++c;
@@ -493,6 +519,34 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) {
             }
         }
     }
+}
+
+// One launch for the first of the caches, as many as it has room for: how many.
+template <int MOST>
+int64_t copy_some(void **caches, const int64_t *page_bytes, const int64_t *page_strides, int64_t n_caches, const int32_t *src,
+                  const int32_t *dst, int64_t n, int64_t n_pages, hipStream_t stream) {
+    CopyArgs<MOST> a;
+    int64_t slices = 0, c = 0;
+    for (; c < MOST && c < n_caches; ++c) {
+        const int64_t units = page_bytes[c] / 16, more = (units + kSlice - 1) / kSlice;
+        if (c > 0 && slices + more > 65535) break;
+        slices += more;
+        a.cache[c] = static_cast<uint8_t *>(caches[c]);
+        a.stride[c] = page_strides[c];
+        a.units[c] = static_cast<uint32_t>(units);
+        a.slices[c] = static_cast<uint32_t>(slices);
+        a.by_last[c] = FastDiv(static_cast<uint32_t>(units - (more - 1) * kSlice));
+    }
+    a.by_slice = FastDiv(kSlice);
+    a.src = src;
+    a.dst = dst;
+    a.n = static_cast<int>(n);
+    a.n_pages = static_cast<int>(n_pages);
+    // enough workgroups that the pairs which copy something, few or many, keep the chip busy
+    int64_t x = (kCopyFill + slices - 1) / slices;
+    x = x < n ? x : n;
+    copy_kernel<MOST><<<dim3(static_cast<unsigned>(x), static_cast<unsigned>(slices)), 256, 0, stream>>>(a);
+    return c;
 }
 
 inline unsigned blocks_for(int64_t n) { return static_cast<unsigned>((n + 255) / 256); }
@@ -631,8 +685,10 @@ extern "C" int dtts_compact_pages(int32_t *pages, int32_t *refs, int32_t *src, i
     a.entries = b * max_pages;
     a.n_pages = static_cast<int>(n_pages);
     a.spans = static_cast<int>((n_pages + kSpan - 1) / kSpan);
-    compact_count_kernel<<<a.spans, kNT, 0, stream>>>(a);
-    DTTS_LAUNCH_CHECK(name);
+    if (a.spans > kFewSpans) {
+        compact_count_kernel<<<a.spans, kNT, 0, stream>>>(a);
+        DTTS_LAUNCH_CHECK(name);
+    }
     compact_rank_kernel<<<a.spans, kNT, 0, stream>>>(a);
     DTTS_LAUNCH_CHECK(name);
     compact_apply_kernel<<<blocks_for(a.entries > n_pages ? a.entries : n_pages), 256, 0, stream>>>(a);
@@ -657,29 +713,11 @@ extern "C" int dtts_copy_pages(void **caches, const int64_t *page_bytes, const i
                      (long long)page_strides[c]);
     }
     for (int64_t c0 = 0; c0 < n_caches;) {
-        CopyArgs a;
-        int64_t slices = 0, c = 0;
-        for (; c < kMostCaches && c0 + c < n_caches; ++c) {
-            const int64_t units = page_bytes[c0 + c] / 16, more = (units + kSlice - 1) / kSlice;
-            if (c > 0 && slices + more > 65535) break;
-            slices += more;
-            a.cache[c] = static_cast<uint8_t *>(caches[c0 + c]);
-            a.stride[c] = page_strides[c0 + c];
-            a.units[c] = static_cast<uint32_t>(units);
-            a.slices[c] = static_cast<uint32_t>(slices);
-            a.by_last[c] = FastDiv(static_cast<uint32_t>(units - (more - 1) * kSlice));
-        }
-        a.src = src;
-        a.dst = dst;
-        a.n = static_cast<int>(n);
-        a.n_pages = static_cast<int>(n_pages);
-        a.by_slice = FastDiv(kSlice);
-        // enough workgroups that the pairs which copy something, few or many, keep the chip busy
-        int64_t x = (kCopyFill + slices - 1) / slices;
-        x = x < n ? x : n;
-        copy_kernel<<<dim3(static_cast<unsigned>(x), static_cast<unsigned>(slices)), 256, 0, stream>>>(a);
+        const int64_t done = n_caches - c0 <= 2 ? copy_some<2>(caches + c0, page_bytes + c0, page_strides + c0, n_caches - c0, src, dst, n, n_pages, stream)
+                                                : copy_some<kMostCaches>(caches + c0, page_bytes + c0, page_strides + c0, n_caches - c0, src, dst,
+                                                                         n, n_pages, stream);
         DTTS_LAUNCH_CHECK(name);
-        c0 += c;
+        c0 += done;
     }
     return DTTS_OK;
 }

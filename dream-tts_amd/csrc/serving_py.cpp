@@ -7,11 +7,10 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/util/SmallVector.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
-
-#include <vector>
 
 #include "dtts.h"
 
@@ -144,7 +143,20 @@ Tensor workspace_of(Args &a, int i, size_t need, const Tensor &like) {
     return a.ok && need ? at::empty({static_cast<int64_t>(need)}, like.options().dtype(at::kByte).requires_grad(false)) : Tensor();
 }
 
-Tensor ints(const Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kInt).requires_grad(false)); }
+// Several int32 arrays in one allocation: `of` takes the next n of them (each allocation, or view by torch's own way, takes as
+// long as a quarter of a launch).
+struct Ints {
+    Tensor all;
+    int64_t at = 0;
+    Ints(const Tensor &like, int64_t n) : all(at::empty({n}, like.options().dtype(at::kInt).requires_grad(false))) {}
+    Tensor of(int64_t n) {
+        Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+        t.unsafeGetTensorImpl()->set_storage_offset(at);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+        at += n;
+        return t;
+    }
+};
 
 PyObject *tuple_of(std::initializer_list<Tensor> all) {
     PyObject *t = PyTuple_New(static_cast<Py_ssize_t>(all.size()));
@@ -313,12 +325,14 @@ PyObject *claim(PyObject *const *args) {
     const int64_t page = a.integer(4);
     a.need(a.ok && start->numel() == t.b + 1 && context->numel() == t.b);
     if (!a.ok) return none();
-    const Tensor ws = workspace_of(a, 5, args[5] == Py_None ? dtts_claim_pages_workspace_bytes(t.b, t.max_pages, t.n_pages) : 0, *t.pages);
+    const int64_t need = args[5] == Py_None ? static_cast<int64_t>(dtts_claim_pages_workspace_bytes(t.b, t.max_pages, t.n_pages)) / 4 : 0;
+    const Tensor *given = a.maybe(5, at::kByte);
     if (!a.ok) return none();
-    const Tensor src = ints(*t.pages, t.b), dst = ints(*t.pages, t.b), lacking = ints(*t.pages, 1);
+    Ints all(*t.pages, 2 * t.b + 1 + need);
+    const Tensor src = all.of(t.b), dst = all.of(t.b), lacking = all.of(1), ws = given ? *given : all.of(need);
     const int status = dtts_claim_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(start), data<int32_t>(context),
                                         data<int32_t>(&src), data<int32_t>(&dst), data<int32_t>(&lacking), t.b, page, t.max_pages,
-                                        t.n_pages, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, a.stream());
+                                        t.n_pages, ws.data_ptr(), ws.nbytes(), a.stream());
     return status == DTTS_OK ? tuple_of({src, dst, lacking}) : none();
 }
 
@@ -340,12 +354,13 @@ PyObject *trim(PyObject *const *args) {
 PyObject *compact(PyObject *const *args) {
     Args a(args);
     const Table t(a);
-    const Tensor ws = a.ok ? workspace_of(a, 2, dtts_compact_pages_workspace_bytes(t.n_pages), *t.pages) : Tensor();
+    const Tensor *given = a.maybe(2, at::kByte);
     if (!a.ok) return none();
-    const Tensor src = ints(*t.pages, t.n_pages), dst = ints(*t.pages, t.n_pages), used = ints(*t.pages, 1);
+    const int64_t need = given ? 0 : static_cast<int64_t>(dtts_compact_pages_workspace_bytes(t.n_pages)) / 4;
+    Ints all(*t.pages, 2 * t.n_pages + 1 + need);
+    const Tensor src = all.of(t.n_pages), dst = all.of(t.n_pages), used = all.of(1), ws = given ? *given : all.of(need);
     const int status = dtts_compact_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(&src), data<int32_t>(&dst),
-                                          data<int32_t>(&used), t.b, t.max_pages, t.n_pages, ws.defined() ? ws.data_ptr() : nullptr,
-                                          ws.defined() ? ws.numel() : 0, a.stream());
+                                          data<int32_t>(&used), t.b, t.max_pages, t.n_pages, ws.data_ptr(), ws.nbytes(), a.stream());
     return status == DTTS_OK ? tuple_of({src, dst, used}) : none();
 }
 
@@ -358,8 +373,8 @@ PyObject *copy(PyObject *const *args) {
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(args[0]);
     Args of(PySequence_Fast_ITEMS(args[0]));
     of.device = a.device;
-    std::vector<void *> at(n);
-    std::vector<int64_t> size(n), stride(n);
+    c10::SmallVector<void *, 8> at(n);
+    c10::SmallVector<int64_t, 8> size(n), stride(n);
     int64_t n_pages = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
         const Tensor *t = of.tensor(static_cast<int>(i));
