@@ -38,7 +38,7 @@ struct AttnArgs {
     int chunk, nsplit; // keys per chunk, chunks at most (the last takes what is left)
     int target;        // above 0: the chunk is chosen for this many units (tiles' chunks) of a kv head, see shared_blocks
     float per_target;  // 1 / target
-    FastDiv by_kv, by_gqa;
+    FastDiv by_kv, by_gqa, by_chunk;
     int64_t few;       // sequences of at most this many rows go to the 16-row tiles
 };
 
@@ -48,7 +48,7 @@ struct AttnArgs {
 // out: a key past the head is `gap` less there.
 struct Span {
     int lo, hi, n, head, gap;
-    __device__ __forceinline__ Span(const AttnArgs &a, int n_new, int ctx, int chunk) {
+    __device__ __forceinline__ Span(const AttnArgs &a, int n_new, int ctx) {
         const int64_t cap = static_cast<int64_t>(a.batch.max_pages) << a.batch.page_shift;
         hi = ctx < 0 ? 0 : ctx < cap ? ctx : static_cast<int>(cap);
         lo = a.window > 0 && ctx - n_new - a.window + 1 > 0 ? (ctx - n_new - a.window + 1) & ~63 : 0;
@@ -59,9 +59,8 @@ struct Span {
             gap = lo > head ? lo - head : 0;
             lo = 0;
         }
-        cut(a, static_cast<int>((static_cast<uint32_t>(hi - gap - lo) + chunk - 1) / static_cast<uint32_t>(chunk)));
+        cut(a, static_cast<int>(a.by_chunk.div(static_cast<uint32_t>(hi - gap - lo) + a.chunk - 1)));
     }
-    __device__ __forceinline__ Span(const AttnArgs &a, int n_new, int ctx) : Span(a, n_new, ctx, 64) {}
     __device__ __forceinline__ void cut(const AttnArgs &a, int chunks) { n = chunks < 1 ? 1 : chunks > a.nsplit ? a.nsplit : chunks; }
     __device__ __forceinline__ int blocks() const { return (hi - gap - lo + 63) >> 6; }  // of 64 keys
     __device__ __forceinline__ void chunk_keys(int chunk, int c, int &k0, int &k1) const {
@@ -88,7 +87,7 @@ struct SinkTiles {
 __device__ __forceinline__ Span tile_span(const AttnArgs &a, int at, int n_new, int ctx) {
     const int rows = n_new * a.gqa, end = (at + 1) * 128 < rows ? (at + 1) * 128 : rows;
     const int first = static_cast<int>(a.by_gqa.div(at * 128)), last = static_cast<int>(a.by_gqa.div(end - 1));
-    return Span(a, last - first + 1, ctx - n_new + last + 1, a.chunk);
+    return Span(a, last - first + 1, ctx - n_new + last + 1);
 }
 
 // A tile of rows: its sequence (-1: none), place in it, the sequence's first row and new tokens, context.
@@ -471,7 +470,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
     const Tile &tile = unit.tile;
     if (tile.s < 0) return;
     const int s = tile.s, at = tile.at, first = tile.first, n_new = tile.n_new, ctx = tile.ctx;
-    Span span = shared ? Span(a, n_new, ctx) : Span(a, n_new, ctx, unit.chunk);
+    Span span(a, n_new, ctx);
     if (shared) span.cut(a, unit.chunks);
     const int c = unit.c;
     if (c >= span.n) return;
@@ -777,7 +776,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
     const Tile tile = find_tile(a, ROWS, a.few, INT64_MAX, tile_no);
     if (tile.s < 0) return;
     const int s = tile.s, at = tile.at, first = tile.first, n_new = tile.n_new, ctx = tile.ctx, pos0 = ctx - n_new;
-    const Span span = Q4 || SINKS ? tile_span(a, at, n_new, ctx) : Span(a, n_new, ctx, a.chunk);
+    const Span span = Q4 || SINKS ? tile_span(a, at, n_new, ctx) : Span(a, n_new, ctx);
     const int c = blockIdx.y;
     if (c >= span.n) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, g = lane >> 5;
@@ -1123,21 +1122,35 @@ __global__ __launch_bounds__(256, 2) void paged_attn_mixed(AttnArgs a, int large
 // Join a row's chunks: out = sum_c num_c w_c / sum_c den_c w_c, w_c = 2^((m_c - M) scale2), M the largest m_c.
 constexpr int kFewChunks = 8;
 
-// How many chunks token t's rows of query head `head` were cut into. OWN: by their tile's keys, or by what the device shared out.
-template <bool OWN>
-__device__ __forceinline__ int chunks_of_row(const AttnArgs &a, int s, int t, int head, int first, int n_new) {
+// By what a row's keys were cut into chunks.
+enum Cut { kBySequence, kByTile, kShared };
+
+// How many chunks token t's rows of the query heads head .. head + R - 1 were cut into.
+template <Cut CUT, int R>
+__device__ __forceinline__ void chunks_of_rows(const AttnArgs &a, int s, int t, int head, int first, int n_new, int (&n)[R]) {
     const int ctx = a.batch.length(s);
-    if (!OWN) return Span(a, n_new, ctx, a.chunk).n;
-    if (a.target > 0) return chunks_of(Span(a, n_new, ctx).blocks(), shared_blocks(a, Lane(a, threadIdx.x & 63)));
-    if (static_cast<int64_t>(n_new) * a.gqa <= a.few) return Span(a, n_new, ctx, a.chunk).n;
-    const int row = (t - first) * a.gqa + head - static_cast<int>(a.by_gqa.div(head)) * a.gqa;
-    return tile_span(a, row / 128, n_new, ctx).n;
+    if (CUT == kShared)
+        n[0] = chunks_of(Span(a, n_new, ctx).blocks(), shared_blocks(a, Lane(a, threadIdx.x & 63)));
+    else if (CUT == kBySequence || static_cast<int64_t>(n_new) * a.gqa <= a.few)
+        n[0] = Span(a, n_new, ctx).n;
+    else {
+        int tile = -1;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int h = head + r, row = (t - first) * a.gqa + h - static_cast<int>(a.by_gqa.div(h)) * a.gqa;
+            n[r] = r > 0 && row / 128 == tile ? n[r - 1] : tile_span(a, row / 128, n_new, ctx).n;
+            tile = row / 128;
+        }
+        return;
+    }
+#pragma unroll
+    for (int r = 1; r < R; ++r) n[r] = n[0];
 }
 
 // Up to kFewChunks: a wave for R heads of a token, which share its lookups, everything requested at once. 862 tokens of
 // 16 heads over four chunks with 1 / 2 / 4 heads a wave: 7.3 / 5.6 / 6.5 us; with the chunks requested before it is known
 // how many a row has 8.5.
-template <int D, int R, bool OWN>
+template <int D, int R, Cut CUT>
 __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
     constexpr int PER = D / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1150,11 +1163,9 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
     if (t < first || t - first >= n_new) return;
     const int head0 = static_cast<int>(trow - static_cast<int64_t>(t) * a.heads);
     int n[R], most = 0;
+    chunks_of_rows<CUT, R>(a, s, t, head0, first, n_new, n);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        n[r] = OWN || r == 0 ? chunks_of_row<OWN>(a, s, t, head0 + r, first, n_new) : n[0];
-        most = n[r] > most ? n[r] : most;
-    }
+    for (int r = 0; r < R; ++r) most = n[r] > most ? n[r] : most;
     if (most <= 1) return;
     const float *pr = a.part + trow * a.nsplit * (D + 4);
     float mc[R][kFewChunks], lc[R][kFewChunks], v[R][kFewChunks][PER];
@@ -1194,7 +1205,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_few(AttnArgs a) {
 // More: a workgroup a row, wave w taking chunks w, w + 4, ..; 64 of its chunks at a time have their maxima and sums read
 // by a lane each, then their rows follow with U requests in flight (5 tokens of 32 heads, 51 chunks: 19.6 us with a
 // loop that carries the maximum along and waits for each, 5.1 so).
-template <int D, bool OWN>
+template <int D, Cut CUT>
 __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     constexpr int PER = D / 64, U = 8, W = 4;
     __shared__ float sm[W][D + 2];
@@ -1205,7 +1216,9 @@ __global__ __launch_bounds__(256) void paged_attn_merge(AttnArgs a) {
     int first, n_new;
     a.batch.rows(s, first, n_new);
     if (t < first || t - first >= n_new) return;
-    const int n = chunks_of_row<OWN>(a, s, t, static_cast<int>(trow - static_cast<int64_t>(t) * a.heads), first, n_new);
+    int of[1];
+    chunks_of_rows<CUT, 1>(a, s, t, static_cast<int>(trow - static_cast<int64_t>(t) * a.heads), first, n_new, of);
+    const int n = of[0];
     if (n <= 1) return;
     float num[PER] = {}, den = 0.0f, m = -INFINITY;
     const float *pr = a.part + trow * a.nsplit * (D + 4);
@@ -1290,10 +1303,41 @@ constexpr int64_t kFew = 32;
 // saves. In a captured graph, one token of 8 kv heads over 256 / 384 / 448 / 512 keys: 6.8 / 8.1 / 8.8 / 9.1 us whole,
 // 8.0 / 8.2 / 8.2 / 8.3 cut (4 of D = 64: 5.6 / 6.6 / 7.2 / 7.3 and 7.2 / 7.4 / 7.5 / 7.5). From 128 tiles on, twice that
 // (16 tokens of 8 kv heads over 512 / 768 / 1024: 10.9 / 15.7 / 19.2 whole, 13.1 / 15.7 / 19.0 cut).
-constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kWhole = 384, kSlots = 512, kFillWindow = 320;
+constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kWhole = 384;
 
 // Where the device shares the keys out (a token or a few of each sequence, over 4-bit pages or with sinks):
 constexpr int64_t kFillShared = 1024, kShareBytes = int64_t(64) << 20;
+
+// How far to cut 128-row tiles over 4-bit pages or with sinks. A tile's time is a fixed part and one for each 64 keys, which
+// depend on how many workgroups share its CU (us; 128 and 1152 keys on 2, 256 and 512 workgroups, D = 64 then 128, three
+// of D = 64 taken to go on like that): cut, more of them run at once, but each begins anew, and their states are joined. Of the
+// cuts that fill the chip once or a few times, the cheapest by that. 700 and 615 tokens of 8 query heads under a window of 1000
+// (166 tiles): 46 us in two, 38 uncut; 1025 of 4 after 5975 (264 tiles): 202 in two, 179 in three.
+inline int64_t cheapest_cut(int64_t wgs, int64_t blocks, int64_t rows, int64_t hd) {
+    struct Tile {
+        float fixed, block;
+    };
+    constexpr Tile kNarrow[] = {{7.0f, 1.05f}, {9.0f, 1.57f}, {11.0f, 2.2f}}, kWide[] = {{9.5f, 1.45f}, {13.0f, 2.4f}};
+    const int full = hd == 64 ? 3 : 2;  // workgroups a CU holds
+    const Tile *of = hd == 64 ? kNarrow : kWide;
+    int64_t best = 1;
+    float least = 0.0f;
+    for (int64_t fill = 0; fill <= 5; ++fill) {
+        const int64_t n = fill == 0 ? 1 : kNumCUs * fill / wgs;
+        if (n < 1 || (n == 1 && fill > 0)) continue;
+        const int64_t all = wgs * n, rounds = all / (kNumCUs * full), left = all - rounds * kNumCUs * full;
+        const float keys = static_cast<float>((blocks + n - 1) / n);
+        const auto time = [&](int share) { return of[share - 1].fixed + of[share - 1].block * keys; };
+        float t = static_cast<float>(rounds) * time(full);
+        if (left > 0) t += time(static_cast<int>((left + kNumCUs - 1) / kNumCUs));
+        if (n > 1) t += 3.0f + static_cast<float>(rows * n * (hd + 4) * 4) / 5e6f;  // joined at 5 TB/s
+        if (fill == 0 || t < least) {
+            least = t;
+            best = n;
+        }
+    }
+    return best;
+}
 
 inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_t max_q, int64_t max_context, int64_t window,
                     int64_t sinks, int64_t hd, bool share, bool own) {
@@ -1321,10 +1365,9 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
     if (span > int64_t(1) << 30) span = int64_t(1) << 30;  // no table holds more
     // the launch is sized for the most tiles there can be; the chunks go by what a batch of long chunks has
     const int64_t wgs = (p.large > 0 ? (own && b == 1 ? p.large : rows / 128 + 1) : p.small) * n_kv, whole = wgs < 128 ? kWhole : 2 * kWhole;
-    int64_t n = ((p.large > 0 ? (own && window > 0 ? kFillWindow : kFillLarge) : kFillSmall) + wgs - 1) / wgs;
-    // and not so that a few workgroups are left over when all others are done
-    if (own && p.large > 0 && n * wgs > kSlots && n * wgs % kSlots < kSlots / 4) ++n;
+    int64_t n = ((p.large > 0 ? kFillLarge : kFillSmall) + wgs - 1) / wgs;
     const int64_t most = span <= whole ? 1 : (span + kMinChunk - 1) / kMinChunk;
+    if (own && p.large > 0) n = cheapest_cut(wgs, (span + 63) / 64, rows * n_kv, hd);
     if (n > most) n = most;
     p.chunk = static_cast<int>(((span + n - 1) / n + 63) / 64 * 64);
     p.nsplit = static_cast<int>((span + p.chunk - 1) / p.chunk);
@@ -1347,15 +1390,15 @@ inline size_t part_bytes(const Plan &p, int64_t tokens, int64_t heads, int64_t h
     return p.nsplit > 1 ? static_cast<size_t>(tokens * heads * p.nsplit * (hd + 4)) * sizeof(float) : 0;
 }
 
-template <int D, bool OWN>
+template <int D, Cut CUT>
 hipError_t merge(const AttnArgs &a, hipStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.batch.tokens) * a.heads;
     if (a.nsplit <= kFewChunks && a.heads % 2 == 0)
-        paged_attn_merge_few<D, 2, OWN><<<static_cast<unsigned>((rows / 2 + 3) / 4), 256, 0, stream>>>(a);
+        paged_attn_merge_few<D, 2, CUT><<<static_cast<unsigned>((rows / 2 + 3) / 4), 256, 0, stream>>>(a);
     else if (a.nsplit <= kFewChunks)
-        paged_attn_merge_few<D, 1, OWN><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+        paged_attn_merge_few<D, 1, CUT><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
     else
-        paged_attn_merge<D, OWN><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
+        paged_attn_merge<D, CUT><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -1370,7 +1413,8 @@ hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
             256, 0, stream>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
-    return merge<D, Q4 || SINKS>(a, stream);
+    if (Q4 && a.target > 0) return merge<D, Q4 ? kShared : kBySequence>(a, stream);
+    return merge<D, Q4 || SINKS ? kByTile : kBySequence>(a, stream);
 }
 
 inline bool plannable(int64_t tokens, int64_t b, int64_t heads, int64_t n_kv, int64_t hd, int64_t max_q, int64_t max_context,
@@ -1445,6 +1489,7 @@ int attention(const char *name, int bits, const dtts_f16 *q, const void *kpages,
     a.by_kv = FastDiv(static_cast<uint32_t>(n_kv));
     a.by_gqa = FastDiv(static_cast<uint32_t>(heads / n_kv));
     a.chunk = p.chunk;
+    a.by_chunk = FastDiv(static_cast<uint32_t>(p.chunk));
     a.nsplit = p.nsplit;
     const auto fn = bits == 16 ? (a.sinks > 0 ? launch_for<false, true> : launch_for<false, false>)
                                : (a.sinks > 0 ? launch_for<true, true> : launch_for<true, false>);

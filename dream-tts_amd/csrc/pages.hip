@@ -469,7 +469,7 @@ struct CopyArgs {
 
 // Units a thread requests together, and a workgroup's at a time.
 constexpr int kRequests = 2, kSlice = 256 * kRequests;
-constexpr int64_t kCopyFill = 8192;  // workgroups: 1250 pages of 64 KB of 6001, and 4600 of 2.5 KB of 100003, 24.2 and 21.9 us with 4 requests and 4096, 23.6 and 21.1 so
+constexpr int64_t kCopyFill = 8192;  // workgroups: 866 pages of 64 KB and 18980 of 2.5 KB 24.2 and 21.9 us with 4 requests and 4096, 23.6 and 21.1 so (4.8 and 4.6 TB/s)
 
 // HBM-bound: every byte read once and written once. A workgroup takes one slice of every gridDim.x-th pair's pages, 256 pairs at
 // a time: those that copy something are put together first, so that a list with few of them, or with all of them in front, is
