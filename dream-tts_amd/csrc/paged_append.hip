@@ -62,15 +62,14 @@ struct Four<half_t> {
 // Eight neighbours of a row, of a group that four lanes share: their word, and the group's pair. A group with a value that is
 // not finite, or whose values pass f16's range, is NaN, all of it.
 __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair) {
-    float lo = z[0], hi = z[0];
-    bool finite = true;
+    float lo = z[0], hi = z[0], none = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         lo = fminf(lo, z[i]);
         hi = fmaxf(hi, z[i]);
-        finite = finite && fabsf(z[i]) < INFINITY;
+        none = __builtin_fmaf(z[i], 0.0f, none);  // NaN from a value that is not finite on
     }
-    if (!finite) hi = INFINITY;
+    if (none != 0.0f) hi = INFINITY;
 #pragma unroll
     for (int off = 1; off <= 2; off <<= 1) {
         lo = fminf(lo, __shfl_xor(lo, off, 64));
@@ -85,8 +84,11 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
     const float per = step > 0.0f ? 1.0f / step : 0.0f;
     uint32_t word = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        word |= static_cast<uint32_t>(fminf(fmaxf(rintf((z[i] - first) * per), 0.0f), 15.0f)) << (4 * (i >> 1) + 16 * (i & 1));
+    for (int i = 0; i < 8; ++i) {
+        // the quotient with its error taken off once: where it lies between two codes exactly, as f16 values often do, it comes out so
+        const float x = z[i] - first, q = x * per, n = __builtin_fmaf(__builtin_fmaf(-q, step, x), per, q);
+        word |= static_cast<uint32_t>(fminf(fmaxf(rintf(n), 0.0f), 15.0f)) << (4 * (i >> 1) + 16 * (i & 1));
+    }
     return word;
 }
 

@@ -150,7 +150,7 @@ def _cache(name, device, k_pages, v_pages):
     """Checks the cache's pages [n_pages, n_kv, page, D] f16 or [n_pages, n_kv, page, 5 D / 8] uint8 (each contiguous): n_kv, D,
     page, n_pages, the elements (bytes) between pages, and the bits of a value."""
     for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not isinstance(t, _Tensor) or t.get_device() != device or (t.dtype is not _F16 and t.dtype is not _U8):
+        if not isinstance(t, _Tensor) or device < 0 or t.get_device() != device or (t.dtype is not _F16 and t.dtype is not _U8):
             _need(name, device, what, t, (_F16, _U8), contiguous=False)
     shape = k_pages.shape
     if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype:

@@ -101,6 +101,21 @@ def test_append(dev, path, hd, rot, interleaved, dtype, norm):
             assert np.array_equal(x0[kept], x1[kept])
 
 
+def test_append_of_f16_values_takes_the_codes_of_the_definition(dev):
+    """Values of f16 rows go into their pages without arithmetic before it, so their codes and pairs are the definition's, ties
+    between two codes (which the f16 grid has many of) included."""
+    n_kv, page = 2, 64
+    for hd in (64, 128):
+        x = (torch.randn((page, (1 + 2 * n_kv) * hd), generator=torch.Generator().manual_seed(hd)) * 2).half()
+        x[:, -hd:] = (x[:, -hd:] * 8).round() / 8  # a coarse grid: a tie every few values
+        cos, sin = tables(dev, page, hd)
+        k, v = (torch.zeros((1, n_kv, page, 5 * hd // 8), dtype=torch.uint8, device=dev) for _ in range(2))
+        i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+        serving.qk_rope_append_paged(x.to(dev), cos, sin, k, v, i32([0, page]), i32([page]), i32([[0]]), 1)
+        want = pref.pack(x[:, -n_kv * hd:].double().numpy().reshape(page, n_kv, hd).transpose(1, 0, 2)[None], True)
+        assert np.array_equal(v.cpu().numpy(), want), hd
+
+
 def slots(raw, values):
     """The words [n_pages, page, n_kv, D / 8] and pairs [n_pages, page, n_kv, D / 32] of uint8 pages."""
     n, n_kv, page, row = raw.shape
@@ -232,6 +247,94 @@ def test_many_sequences_of_unequal_lengths(dev, b, most, window, sinks):
     q = torch.randn((batch.tokens, 4, 64), generator=torch.Generator().manual_seed(b)).half()
     for max_context, workspace in ((most, None), (64, None), (most, torch.empty(0, dtype=torch.uint8, device=dev)), (10 * most, None)):
         check(batch, packed, values, q, 2, max_context, 0.2, window, sinks, workspace=workspace)
+
+
+@pytest.mark.parametrize("n,c", [([5, 3], [3, 0]), ([40, 1], [7, 1]), ([2, 1, 60], [1, 0, 200])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2, 1)])
+def test_tokens_before_the_first_position(dev, n, c, window, sinks):
+    """More new tokens than positions: those before position 0 see nothing and get zeros, and write nothing."""
+    b = ref.Batch(n, c, 2, 64, 16, dev, seed=1)
+    packed, values = q4(b)
+    q = torch.randn((b.tokens, 4, 64), generator=torch.Generator().manual_seed(1)).half()
+    for max_context in (200, 3000):
+        out = check(b, packed, values, q, max(n), max_context, 0.1, window, sinks)
+        for s in range(len(n)):
+            first = int(b.start[s])
+            assert not bool(out[first:first + max(0, n[s] - c[s])].any())
+    _, _, start, ctx, table = b.device()
+    before = [t.clone() for t in packed]
+    cos, sin = tables(dev, 256, 64)
+    out = torch.full((b.tokens, 4, 64), 9.0, dtype=torch.float16, device=dev)
+    serving.qk_rope_append_paged(torch.randn((b.tokens, 8 * 64), device=dev), cos, sin, *packed, start, ctx, table, 4, out=out)
+    for s in range(len(n)):
+        first, none = int(b.start[s]), max(0, n[s] - c[s])
+        assert bool((out[first:first + none] == 9.0).all()) and not bool((out[first + none:int(b.start[s + 1])] == 9.0).all(-1).any())
+    if sum(c) == 3:  # a sequence of three positions, all new
+        changed = [bool((x != y).view(x.shape[0], -1).any(1)[p]) for x, y in zip(packed, before) for p in range(x.shape[0])]
+        assert changed.count(True) <= 2
+
+
+@pytest.mark.parametrize("max_context", [60, 5000])
+def test_starts_that_select_nothing_write_nothing(dev, path, max_context):
+    """Starts that fall, lie outside the batch or are all alike: rows of `out` that no sequence has stay as they were."""
+    c = [30, 400, 2000]
+    b = ref.Batch([4, 3, 2], c, 2, 64, 16, dev, extra_tokens=2)
+    packed, _ = q4(b)
+    q = torch.randn((b.tokens, 2, 64), generator=torch.Generator().manual_seed(4)).half().to(dev)
+    _, _, _, ctx, table = b.device()
+    for starts, rows in (([9, 4, 2, 0], []), ([5, 3, -9, -9], []), ([100, 200, 300, 400], []), ([-8, -8, -8, 0], []),
+                         ([11, 11, 11, 2 ** 31 - 1], []), ([6, 2, 2, 5], [2, 3, 4]), ([0, 0, 0, 3], [0, 1, 2]), ([3, 1, 4, 4], [1, 2, 3])):
+        start = torch.tensor(starts, dtype=torch.int32, device=dev)
+        for max_q in (4, 200):
+            out = torch.full((b.tokens, 2, 64), 9.0, dtype=torch.float16, device=dev)
+            serving.paged_attention(q, *packed, start, ctx, table, max_q, max_context, 0.1, out=out)
+            assert bool((out[[t for t in range(b.tokens) if t not in rows]] == 9.0).all()), starts
+            serving.paged_attention(q, *packed, start, ctx, table, max_q, max_context, 0.1, window=70, sinks=3, out=out)
+            assert bool((out[[t for t in range(b.tokens) if t not in rows]] == 9.0).all()), starts
+
+
+def test_a_captured_call_shares_out_the_lengths_of_each_replay(dev):
+    """Cut contexts, whose cut the device chooses: one graph, other lengths and idle sequences at each replay, against the eager call."""
+    b = ref.Batch([1] * 9, [3000] * 9, 2, 128, 16, dev, seed=3)
+    packed, _ = q4(b)
+    _, _, start, ctx, table = b.device()
+    q = torch.randn((9, 8, 128), generator=torch.Generator().manual_seed(1)).half().to(dev)
+    call = lambda: serving.paged_attention(q, *packed, start, ctx, table, 1, 3000, 0.1)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    rng = np.random.RandomState(2)
+    for i in range(6):
+        ctx.copy_(torch.from_numpy(np.minimum(3000, rng.choice([1, 20, 700, 3000], 9) + i)))
+        start.copy_(torch.from_numpy(np.concatenate([[0], np.cumsum(rng.rand(9) < 0.8)]).astype(np.int32)))
+        rows = int(start[-1])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got[:rows], call()[:rows]), i
+
+
+def test_two_calls_at_once(dev):
+    """Two streams with calls that are cut, in flight together: the bits of each alone."""
+    bs = [ref.Batch([1] * 5, [c] * 5, 2, 64, 16, dev, seed=c) for c in (1500, 2500)]
+    args = []
+    for b in bs:
+        packed, _ = q4(b)
+        _, _, start, ctx, table = b.device()
+        q = torch.randn((5, 4, 64), generator=torch.Generator().manual_seed(b.c[0])).half().to(dev)
+        args.append((q, *packed, start, ctx, table, 1, b.c[0], 0.1))
+    want = [serving.paged_attention(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for a, s, g in zip(args, streams, got):
+            with torch.cuda.stream(s):
+                g.append(serving.paged_attention(*a))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
 
 
 def test_a_captured_step(dev):
