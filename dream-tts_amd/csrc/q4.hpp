@@ -1,7 +1,8 @@
 // 4-bit pages: rows of D values in groups of 32, value = f16(c d + b) with c = 64 + n, n the value's 4 bits, d and b the
 // group's f16 pair. As an f16, 64 + n is the bits 0x5400 | n << 4, so two codes of a word become two numbers with one
 // and-or (after a shift, for three of four), and one packed fma makes them the two values with their one rounding. With codes
-// from 0 on, a subtraction would come between.
+// from 0 on, a subtraction would come between. (11 instructions for 8 values against 13; an attention tile of 32 keys of 128
+// dimensions spends 192 of its 350 on them, and over 5 x 65000 keys vector issue, 0.63 of the cycles, is what it waits for most.)
 //
 // A page of a kv head (5 D / 8 bytes a row, against 2 D) is first the rows' codes, D / 8 words of 32 a row: element 8 w + 2 i
 // of a row in bits 4 i of its word w, element 8 w + 2 i + 1 in bits 16 + 4 i, so that a pair of neighbours is one number apart
