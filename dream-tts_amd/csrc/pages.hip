@@ -184,7 +184,8 @@ __device__ __forceinline__ int named(const int *words, int w, int end) {
 //
 // Bound by its trips to memory, one after another (the starts, the entries, their counts, the free pages' counts, the answers), and
 // by its instructions, each of which the 16 waves of one CU take turns for. 160 sequences that share pages, over 20011: 23.3
-// us with a barrier for every kNT counts; 18.1 with all ranks counted over words in LDS, of which those took 8.
+// us with a barrier for every kNT counts; 18.1 with all ranks counted over words in LDS, of which those took 8; 11.1 with the
+// hash, while the compiler compared the counts (and so waited for them) where they were requested; 6.7 so.
 __global__ __launch_bounds__(kNT) void claim_kernel(ClaimArgs a) {
     __shared__ ClaimLds lds;
     typedef int four __attribute__((ext_vector_type(4), aligned(4)));
@@ -469,6 +470,7 @@ struct CopyArgs {
 
 // Units a thread requests together, and a workgroup's at a time.
 constexpr int kRequests = 2, kSlice = 256 * kRequests;
+constexpr int64_t kMostSlices = 65535, kMostPageBytes = kMostSlices * kSlice * 16;  // of a launch, a slice a row of its grid
 constexpr int64_t kCopyFill = 8192;  // workgroups: 866 pages of 64 KB and 18980 of 2.5 KB 24.2 and 21.9 us with 4 requests and 4096, 23.6 and 21.1 so (4.8 and 4.6 TB/s)
 
 // HBM-bound: every byte read once and written once. A workgroup takes one slice of every gridDim.x-th pair's pages, 256 pairs at
@@ -529,7 +531,7 @@ int64_t copy_some(void **caches, const int64_t *page_bytes, const int64_t *page_
     int64_t slices = 0, c = 0;
     for (; c < MOST && c < n_caches; ++c) {
         const int64_t units = page_bytes[c] / 16, more = (units + kSlice - 1) / kSlice;
-        if (c > 0 && slices + more > 65535) break;
+        if (c > 0 && slices + more > kMostSlices) break;
         slices += more;
         a.cache[c] = static_cast<uint8_t *>(caches[c]);
         a.stride[c] = page_strides[c];
@@ -707,10 +709,10 @@ extern "C" int dtts_copy_pages(void **caches, const int64_t *page_bytes, const i
     DTTS_REQUIRE(aligned(src, 4) && aligned(dst, 4), "%s: misaligned operand", name);
     for (int64_t c = 0; c < n_caches; ++c) {
         DTTS_REQUIRE(caches[c] && aligned(caches[c], 16), "%s: cache %lld is null or not 16-byte aligned", name, (long long)c);
-        DTTS_REQUIRE(page_bytes[c] > 0 && page_bytes[c] % 16 == 0 && page_bytes[c] < (int64_t(1) << 29) && page_strides[c] % 16 == 0 &&
+        DTTS_REQUIRE(page_bytes[c] > 0 && page_bytes[c] % 16 == 0 && page_bytes[c] <= kMostPageBytes && page_strides[c] % 16 == 0 &&
                          page_strides[c] >= page_bytes[c] && page_strides[c] < (int64_t(1) << 34),
-                     "%s: pages of %lld bytes, %lld apart (multiples of 16, under 2^29 and 2^34)", name, (long long)page_bytes[c],
-                     (long long)page_strides[c]);
+                     "%s: pages of %lld bytes, %lld apart (multiples of 16, up to %lld and under 2^34)", name, (long long)page_bytes[c],
+                     (long long)page_strides[c], (long long)kMostPageBytes);
     }
     for (int64_t c0 = 0; c0 < n_caches;) {
         const int64_t done = n_caches - c0 <= 2 ? copy_some<2>(caches + c0, page_bytes + c0, page_strides + c0, n_caches - c0, src, dst, n, n_pages, stream)

@@ -160,6 +160,13 @@ def test_copy(match, bad):
             at(2 * BIG), a["n"], a["n_pages"], None)
 
 
+@pytest.mark.parametrize("size", [(1 << 29) - 8192 + 16, (1 << 29) - 16])
+def test_copy_of_pages_with_more_slices_than_a_grid_has_rows(size):
+    c = (ctypes.c_void_p * 2)(at(0).value, at(BIG).value)
+    refused("dtts_copy_pages", "apart", c, (ctypes.c_int64 * 2)(1280, size), (ctypes.c_int64 * 2)(1280, 1 << 30), 2, at(2 * BIG),
+            at(3 * BIG), 5, 9, None)
+
+
 def test_tensors_that_are_not_on_a_gpu():
     i, x = torch.zeros((2, 2), dtype=torch.int32), torch.zeros((4, 2, 16, 40), dtype=torch.uint8)
     for call in (lambda: serving.fork_pages(i, i[0], i[0]), lambda: serving.claim_pages(i, i[0], torch.zeros(3, dtype=torch.int32), i[0], 16),
