@@ -409,3 +409,47 @@ def test_refusals(dev, path):
         serving.qk_rope_append_paged(torch.zeros((2, 8 * 64), device=dev), cos, sin, k, k, start, ctx, table, 4)
     with pytest.raises(DttsError, match="dtype"):
         serving.unpack_pages(k.view(torch.float16), v.view(torch.float16))
+
+
+@pytest.mark.parametrize("apart", [(1 << 31) + 4096, (1 << 32) - 16])
+def test_pages_far_apart(dev, apart):
+    """Offsets past 31 and 32 bits: the append, attention of single tokens and of a chunk, with sinks and without, the values read
+    back and the copy give what they give over neighbouring pages, bit for bit."""
+    n, c, n_kv, hd, page = [1, 3, 40], [30, 17, 45], 2, 64, 16
+    b = ref.Batch(n, c, n_kv, hd, page, dev, seed=2, spare=0)
+    _, _, start, ctx, table = b.device()
+    cos, sin = tables(dev, 128, hd)
+    qkv = torch.randn((b.tokens, (4 + 2 * n_kv) * hd), generator=torch.Generator().manual_seed(3)).to(dev)
+    room = (b.n_pages - 1) * apart + n_kv * page * 40
+    near, _ = q4(b)
+    far = [torch.empty(room, dtype=torch.uint8, device=dev).as_strided(t.shape, (apart, *t.stride()[1:])) for t in near]
+    for f, t in zip(far, near):
+        f.copy_(t)
+    out = []
+    for pages in (near, far):
+        q = serving.qk_rope_append_paged(qkv, cos, sin, *pages, start, ctx, table, 4)
+        got = [q, *serving.unpack_pages(*pages)]
+        for window, sinks in ((0, 0), (20, 5)):
+            got.append(serving.paged_attention(q, *pages, start, ctx, table, max(n), max(c), 0.125, window, sinks=sinks))
+        ones = torch.arange(3, dtype=torch.int32, device=dev)
+        got.append(serving.paged_attention(q[:2].contiguous(), *pages, ones, ctx[[0, 2]], table[[0, 2]], 1, max(c), 0.125))
+        move = torch.tensor([b.n_pages - 1, 1], dtype=torch.int32, device=dev), torch.tensor([0, b.n_pages - 2], dtype=torch.int32, device=dev)
+        serving.copy_pages(pages, *move)
+        got += [t.clone(memory_format=torch.contiguous_format) for t in pages]
+        out.append(got)
+    for x, y in zip(*out):
+        assert torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+
+
+def test_no_tokens(dev, path):
+    b = ref.Batch([1], [20], 1, 64, 16, dev, seed=1)
+    packed, _ = q4(b)
+    before = [t.clone() for t in packed]
+    _, _, start, ctx, table = b.device()
+    cos, sin = tables(dev, 32, 64)
+    q = serving.qk_rope_append_paged(torch.empty((0, 4 * 64), device=dev), cos, sin, *packed, start, ctx, table, 2)
+    assert q.shape == (0, 2, 64) and serving.paged_attention(q, *packed, start, ctx, table, 1, 20).shape == q.shape
+    none = [torch.zeros(k, dtype=torch.int32, device=dev) for k in (1, 0)]
+    q = torch.full((3, 2, 64), 5.0, dtype=torch.float16, device=dev)
+    out = serving.paged_attention(q, *packed, *none, table[:0], 1, 20, out=torch.full_like(q, 7.0))
+    assert bool((out == 7.0).all()) and all(torch.equal(x, y) for x, y in zip(before, packed))
