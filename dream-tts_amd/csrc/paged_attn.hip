@@ -348,7 +348,8 @@ struct KvTile {
 
 // Of 4-bit pages a lane has 16 or 32 neighbouring dimensions of its key (one load and their pair), and of the values a word
 // of four keys at once (one load) with their pairs (another). The words are turned before they become numbers: halves of two
-// keys' words make pairs of keys, which is what the product's operand holds.
+// keys' words make pairs of keys, which is what the product's operand holds. 5 tokens of 32 heads over 4 and up to 65000 keys (132
+// MB): 29 us, 4.5 TB/s, vector issue 0.63 of the cycles; 48 of 16 over 8 and up to 1536 (49 MB): 15.8, of which one key each takes 6.
 template <int D>
 struct KvTile<D, true> {
     static constexpr int E = D / 16, W = D / 32;  // W: key words a lane holds
