@@ -26,8 +26,8 @@ struct PagedBatch {
 
     // Sequence s's first row and row count: clipped to the batch, so that no value of q_start reaches
     // outside it.
-    __device__ __forceinline__ void rows(int s, int &first, int &n) const {
-        const int lo = q_start[s], hi = q_start[s + 1];
+    __device__ __forceinline__ void rows(int s, int &first, int &n) const { clip(q_start[s], q_start[s + 1], first, n); }
+    __device__ __forceinline__ void clip(int lo, int hi, int &first, int &n) const {
         first = lo < 0 ? 0 : lo > tokens ? tokens : lo;
         const int end = hi > tokens ? tokens : hi;
         n = end > first ? end - first : 0;
@@ -35,9 +35,9 @@ struct PagedBatch {
 
     // Sequence s's length. A table holds 2^30 positions at most and a batch 2^24 tokens: clipped so that positions,
     // and a kernel's look ahead of them, stay ints, and none of an impossible length's is in a table.
-    __device__ __forceinline__ int length(int s) const {
+    __device__ __forceinline__ int length(int s) const { return clip(context[s]); }
+    __device__ __forceinline__ static int clip(int c) {
         constexpr int kMost = (1 << 30) + (1 << 24);
-        const int c = context[s];
         return c < 0 ? 0 : c > kMost ? kMost : c;
     }
 
@@ -60,6 +60,31 @@ struct PagedBatch {
             ended += __popcll(__ballot(end <= t));
         }
         return ended;
+    }
+
+    // The same with the sequence's rows and length (nothing for b). Of up to 64 sequences a lane each has read all of them along
+    // with their ends, which saves a trip to memory.
+    __device__ __forceinline__ int sequence_of(int t, int &first, int &n, int &len) const {
+        first = n = len = 0;
+        if (b > 64) {
+            const int s = sequence_of(t);
+            if (s >= b) return s;
+            rows(s, first, n);
+            len = length(s);
+            return s;
+        }
+        const int lane = threadIdx.x & 63;
+        int lo = 0, hi = 0x7fffffff, c = 0;
+        if (lane < b) {
+            lo = q_start[lane];
+            hi = q_start[lane + 1];
+            c = context[lane];
+        }
+        const int s = __popcll(__ballot(hi <= t));
+        if (s >= b) return s;
+        clip(__builtin_amdgcn_readlane(lo, s), __builtin_amdgcn_readlane(hi, s), first, n);
+        len = clip(__builtin_amdgcn_readlane(c, s));
+        return s;
     }
 };
 

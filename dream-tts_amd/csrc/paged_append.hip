@@ -17,7 +17,8 @@
 // half-split, four pairs' first and second members; interleaved, eight neighbours (four pairs), so
 // both layouts turn in registers and the norm is a shuffle sum over D/8 lanes. At a decode step's
 // sizes it is the chain of dependent reads that counts (q_start -> context -> page id and table
-// rows): qkv is requested before it, and its ends overlap.
+// rows): qkv is requested before it, and its ends overlap. Into 4-bit pages: 48 f32 tokens of 32 rows of 128 (2.6 MB) 3.9 us;
+// 4436 f16 tokens of 32 rows of 64 (30 MB) 9.9 us, half of it vector issue, the rest the chain, which a wave a token meets once.
 #include <cmath>
 
 #include "norm_rope.hpp"
@@ -59,6 +60,20 @@ struct Four<half_t> {
     }
 };
 
+// x / y from per, about 1 / y, with the error taken off once: right to a last place, and where the quotient is a float (half
+// way between two codes, as f16 values often are) it is that one.
+__device__ __forceinline__ float quotient(float x, float y, float per) {
+    const float q = x * per;
+    return __builtin_fmaf(__builtin_fmaf(-q, y, x), per, q);
+}
+
+// x of the lane OFF (1 or 2) away among four.
+template <int OFF>
+__device__ __forceinline__ float other_of_four(float x) {
+    constexpr int kSwap = OFF == 1 ? 0xb1 : 0x4e;  // quad_perm [1, 0, 3, 2], [2, 3, 0, 1]
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(x), kSwap, 0xf, 0xf, false));
+}
+
 // Eight neighbours of a row, of a group that four lanes share: their word, and the group's pair. A group with a value that is
 // not finite, or whose values pass f16's range, is NaN, all of it.
 __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair) {
@@ -70,26 +85,22 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
         none = __builtin_fmaf(z[i], 0.0f, none);  // NaN from a value that is not finite on
     }
     if (none != 0.0f) hi = INFINITY;
-#pragma unroll
-    for (int off = 1; off <= 2; off <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, off, 64));
-        hi = fmaxf(hi, __shfl_xor(hi, off, 64));
-    }
-    half_t d = static_cast<half_t>((hi - lo) / 15.0f), b = static_cast<half_t>(lo - kQ4First * static_cast<float>(d));
+    lo = fminf(lo, other_of_four<1>(lo));
+    hi = fmaxf(hi, other_of_four<1>(hi));
+    lo = fminf(lo, other_of_four<2>(lo));
+    hi = fmaxf(hi, other_of_four<2>(hi));
+    half_t d = static_cast<half_t>(quotient(hi - lo, 15.0f, 1.0f / 15.0f)), b = static_cast<half_t>(lo - kQ4First * static_cast<float>(d));
     const float step = static_cast<float>(d), first = __builtin_fmaf(kQ4First, step, static_cast<float>(b));
     const float last = __builtin_fmaf(kQ4Last, step, static_cast<float>(b));
     constexpr float kOver = 65520.0f;  // what f16 rounds to infinity
     if (!(fabsf(first) < kOver && fabsf(last) < kOver)) d = b = static_cast<half_t>(NAN);
     pair = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, d)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
-    const float per = step > 0.0f ? 1.0f / step : 0.0f;
-    uint32_t word = 0;
+    const float per = step > 0.0f ? __builtin_amdgcn_rcpf(step) : 0.0f;
+    float half[2] = {};  // of the word, as numbers
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        // the quotient with its error taken off once: where it lies between two codes exactly, as f16 values often do, it comes out so
-        const float x = z[i] - first, q = x * per, n = __builtin_fmaf(__builtin_fmaf(-q, step, x), per, q);
-        word |= static_cast<uint32_t>(fminf(fmaxf(rintf(n), 0.0f), 15.0f)) << (4 * (i >> 1) + 16 * (i & 1));
-    }
-    return word;
+    for (int i = 7; i >= 0; --i)
+        half[i & 1] = __builtin_fmaf(half[i & 1], 16.0f, __builtin_amdgcn_fmed3f(rintf(quotient(z[i] - first, step, per)), 0.0f, 15.0f));
+    return static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
 }
 
 // A wave takes one token, or one of its `parts`: rows part * RW + its lane group's, then parts * RW further.
@@ -97,7 +108,10 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
 // read once for all of them.
 template <typename T, int D, bool INTERLEAVED, bool Q4>
 __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv, AppendArgs a) {
-    constexpr int L = D / 8, RW = 64 / L, U = 4;  // lanes per head row, head rows per wave step, steps requested together
+    // Lanes per head row, head rows per wave step, steps requested together. Making 4-bit groups takes 130 instructions a step, which
+    // are not unrolled (4 / 3 / 2 / 1 steps: 4000 f16 tokens of 32 rows of 64 9.5 / 9.5 / 9.3 / 8.8 us, 400 of 128 5.8 / 5.6 / 5.3 / 5.1,
+    // 8000 of 48 rows 36.2 / 36.5 / 37.6 / 35.1).
+    constexpr int L = D / 8, RW = 64 / L, U = Q4 ? 1 : 4;
     const uint32_t wid = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const int t = static_cast<int>(a.parts.div(wid)), part = static_cast<int>(wid - static_cast<uint32_t>(t) * a.parts.d);
     if (t >= a.batch.tokens) return;
@@ -119,11 +133,10 @@ __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv,
     };
     int r0 = part * RW + lane / L;
     load(r0);
-    const int s = a.batch.sequence_of(t);
+    int first, n, len;
+    const int s = a.batch.sequence_of(t, first, n, len);
     if (s >= a.batch.b) return;
-    int first, n;
-    a.batch.rows(s, first, n);
-    const int pos = a.batch.length(s) - n + (t - first);
+    const int pos = len - n + (t - first);
     if (t < first || t >= first + n || pos < 0 || pos >= a.table_len) return;
     const int page = a.batch.page(s, pos >> a.batch.page_shift);
     if (page < 0) return;
