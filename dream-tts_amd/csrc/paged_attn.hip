@@ -332,7 +332,7 @@ struct KvTile {
         for (int j = 0; j < 4; ++j) v[4 * u + j] = *reinterpret_cast<const ve *>(a.v + base + (4 * at.g + j) * D + E * at.l16);
     }
     __device__ __forceinline__ half8_t key(int u, int i, const Q4Bits &) const { return k[u][i]; }
-    __device__ __forceinline__ void drop(int j) { v[j] = ve{}; }
+    __device__ __forceinline__ void drop(int j, bool out) { v[j] = out ? ve{} : v[j]; }
     __device__ __forceinline__ void turn(int) {}
     __device__ __forceinline__ void take_out_values(uint32_t &spoilt) {
 #pragma unroll
@@ -387,7 +387,7 @@ struct KvTile<D, true> {
         vs[u] = *reinterpret_cast<const u32x4 *>(vp + pairs + at.vs);
     }
     __device__ __forceinline__ half8_t key(int u, int i, const Q4Bits &bits) const { return q4_values(k[u][i], ks[u], bits); }
-    __device__ __forceinline__ void drop(int j) { vs[j >> 2][j & 3] = 0; }  // 64 + n times 0
+    __device__ __forceinline__ void drop(int j, bool out) { vs[j >> 2][j & 3] = out ? 0 : vs[j >> 2][j & 3]; }  // 64 + n times 0
     __device__ __forceinline__ void turn(int l16) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -605,12 +605,14 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
                 p[4 * u + i] = static_cast<half_t>(x);
             }
         l += sum;
-        // what no row sees holds anything: 0 times it may be NaN
+        // what no row sees holds anything: 0 times it may be NaN. Selected without a branch: of nested ones (k1, window, sinks, page)
+        // around a register's part the compiler kept only the first and the zero of a missing page was lost.
         if (__builtin_expect(partly || t.ok != 3, 0)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
-                if (key >= k1 || (key < bottom && !(SINKS && key < a.sinks)) || !(t.ok >> (j >> 2) & 1)) t.drop(j);
+                const bool sunk = SINKS & (key < a.sinks), there = t.ok >> (j >> 2) & 1;
+                t.drop(j, (key >= k1) | ((key < bottom) & !sunk) | !there);
             }
         }
         t.turn(l16);
@@ -874,7 +876,7 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
             if (partly) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (!g_ok || kb + 16 * w + 4 * a4 + j >= k1) gvs[j] = 0;
+                    gvs[j] = (!g_ok | (kb + 16 * w + 4 * a4 + j >= k1)) ? 0 : gvs[j];
             }
             uint32_t lo[2], hi[2];
             half2_t sd[2], sb[2];

@@ -453,3 +453,24 @@ def test_no_tokens(dev, path):
     q = torch.full((3, 2, 64), 5.0, dtype=torch.float16, device=dev)
     out = serving.paged_attention(q, *packed, *none, table[:0], 1, 20, out=torch.full_like(q, 7.0))
     assert bool((out == 7.0).all()) and all(torch.equal(x, y) for x, y in zip(before, packed))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,c", [([1], [300]), ([3], [300]), ([40], [300]), ([1, 50, 2], [200, 300, 100])])
+@pytest.mark.parametrize("where", ["keys", "values"])
+def test_a_missing_page_stands_for_nothing(dev, bits, hd, n, c, where):
+    """Blocks without a page, inside the sinks, before and in the window, while page 0 (of no sequence) holds NaN."""
+    b = ref.Batch(n, c, 2, hd, 16, dev, seed=hd, extra_tokens=1)
+    k, v = (torch.nan_to_num(t, nan=0.5) for t in (b.k, b.v))
+    b.table[b.table == 0] = next(i for i in range(1, b.n_pages) if i not in b.table)
+    (k if where == "keys" else v)[0] = float("nan")
+    b.k, b.v = k, v
+    packed, values = q4(b) if bits == 4 else (list(b.device()[:2]), (k, v))
+    q = torch.randn((b.tokens, 4, hd), generator=torch.Generator().manual_seed(hd)).half()
+    table = b.table
+    for block in (0, 1, 2, 5, table.shape[1] - 2):
+        b.table = table.copy()
+        b.table[:, block] = -1
+        for window, sinks in ((0, 0), (1000, 5), (60, 0), (60, 7), (60, 100), (1000, 64)):
+            check(b, packed, values, q, max(n), max(c), 0.15, window, sinks)
