@@ -306,7 +306,13 @@ __device__ __forceinline__ half_t __attribute__((ext_vector_type(E))) taken(half
 // hundred keys are a chain of trips to memory (starts, page ids, keys, 32 keys a wave and step): one token over 300
 // 7.7 us. Two tiles in flight a wave halve the waves a SIMD holds (74 -> 81); page ids a tile ahead win half a
 // microsecond under 1000 keys and lose 1 % of the long ones.
-template <int D, bool Q4>
+template <bool ONCE, typename T>
+__device__ __forceinline__ T fetch(const T *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    return *p;
+}
+
+template <int D, bool Q4, bool ONCE>
 struct KvTile {
     static constexpr int E = D / 16;  // dimensions a lane holds of each of its 8 value rows
     typedef half_t ve __attribute__((ext_vector_type(E)));
@@ -324,12 +330,12 @@ struct KvTile {
     __device__ __forceinline__ void load_keys(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
         base += static_cast<int64_t>(slot) * D;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) k[u][i] = *reinterpret_cast<const half8_t *>(a.k + base + at.l16 * D + dim(i, at.g));
+        for (int i = 0; i < D / 32; ++i) k[u][i] = fetch<ONCE>(reinterpret_cast<const half8_t *>(a.k + base + at.l16 * D + dim(i, at.g)));
     }
     __device__ __forceinline__ void load_values(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
         base += static_cast<int64_t>(slot) * D;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * u + j] = *reinterpret_cast<const ve *>(a.v + base + (4 * at.g + j) * D + E * at.l16);
+        for (int j = 0; j < 4; ++j) v[4 * u + j] = fetch<ONCE>(reinterpret_cast<const ve *>(a.v + base + (4 * at.g + j) * D + E * at.l16));
     }
     __device__ __forceinline__ half8_t key(int u, int i, const Q4Bits &) const { return k[u][i]; }
     __device__ __forceinline__ void drop(int j, bool out) { v[j] = out ? ve{} : v[j]; }
@@ -349,9 +355,9 @@ struct KvTile {
 // Of 4-bit pages a lane has 16 or 32 neighbouring dimensions of its key (one load and their pair), and of the values a word
 // of four keys at once (one load) with their pairs (another). The words are turned before they become numbers: halves of two
 // keys' words make pairs of keys, which is what the product's operand holds. 5 tokens of 32 heads over 4 and up to 65000 keys (132
-// MB): 29 us, 4.5 TB/s, vector issue 0.63 of the cycles; 48 of 16 over 8 and up to 1536 (49 MB): 15.8, of which one key each takes 6.
-template <int D>
-struct KvTile<D, true> {
+// MB): 27.6 us, 4.8 TB/s, vector issue 0.63 of the cycles; 48 of 16 over 8 and up to 1536 (49 MB): 15.8, of which one key each takes 6.
+template <int D, bool ONCE>
+struct KvTile<D, true, ONCE> {
     static constexpr int E = D / 16, W = D / 32;  // W: key words a lane holds
     typedef half_t ve __attribute__((ext_vector_type(E)));
     typedef uint32_t kw __attribute__((ext_vector_type(W)));
@@ -377,14 +383,14 @@ struct KvTile<D, true> {
     __device__ __forceinline__ void load_keys(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
         const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.k) + base;
         const uint32_t words = slot * (Q4Row<D>::kWords * 4), pairs = Q4Row<D>::pair(1 << a.batch.page_shift, slot, 0);
-        k[u] = *reinterpret_cast<const kw *>(kp + words + at.k);
-        ks[u] = *reinterpret_cast<const uint32_t *>(kp + pairs + at.ks);
+        k[u] = fetch<ONCE>(reinterpret_cast<const kw *>(kp + words + at.k));
+        ks[u] = fetch<ONCE>(reinterpret_cast<const uint32_t *>(kp + pairs + at.ks));
     }
     __device__ __forceinline__ void load_values(const AttnArgs &a, int u, int64_t base, int slot, const Lane &at) {
         const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.v) + base;
         const uint32_t words = slot * (Q4Row<D>::kWords * 4), pairs = Q4Row<D>::pair(1 << a.batch.page_shift, slot, 0);
-        v[u] = *reinterpret_cast<const u32x4 *>(vp + words + at.v);
-        vs[u] = *reinterpret_cast<const u32x4 *>(vp + pairs + at.vs);
+        v[u] = fetch<ONCE>(reinterpret_cast<const u32x4 *>(vp + words + at.v));
+        vs[u] = fetch<ONCE>(reinterpret_cast<const u32x4 *>(vp + pairs + at.vs));
     }
     __device__ __forceinline__ half8_t key(int u, int i, const Q4Bits &bits) const { return q4_values(k[u][i], ks[u], bits); }
     __device__ __forceinline__ void drop(int j, bool out) { vs[j >> 2][j & 3] = out ? 0 : vs[j >> 2][j & 3]; }  // 64 + n times 0
@@ -459,7 +465,7 @@ struct RowsLds {
     float o[4][16][D + 4], m[4][16], l[4][16];
 };
 
-template <int D, bool Q4, bool SINKS>
+template <int D, bool Q4, bool SINKS, bool ONCE>
 __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, int block) {
     constexpr int C = D / 32, E = D / 16, ROWS = 16;
     auto &sm_o = lds.o;
@@ -508,13 +514,13 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
         const half_t *qr = a.q + (first + tok) * a.q_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            qf[i] = *reinterpret_cast<const half8_t *>(qr + KvTile<D, Q4>::dim(i, g));
+            qf[i] = *reinterpret_cast<const half8_t *>(qr + KvTile<D, Q4, ONCE>::dim(i, g));
             if (a.negate) qf[i] = -qf[i];
         }
     }
     const int in_page = (1 << a.batch.page_shift) - 1;
     const int64_t head_at = head_offset<D, Q4>(a, kh);
-    const typename KvTile<D, Q4>::Lane lane_at(a, l16, g);
+    const typename KvTile<D, Q4, ONCE>::Lane lane_at(a, l16, g);
     // the wave's key tiles are every fourth: the i-th begins at key_of(i)
     const int base = SINKS ? k0 : k0 & ~31;
     const int heads_tiles = SINKS ? (mid - k0 + 31) >> 5 : 0, rest_at = SINKS ? next : base;
@@ -527,14 +533,14 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
         id_lane = i + 4 * (lane >> 1) < n_tiles && key < k1 ? a.batch.page(s, key >> a.batch.page_shift) : -1;
     };
     auto page_of = [&](int i, int u) { return __builtin_amdgcn_readlane(id_lane, ((i - w) >> 1 & 62) + u); };  // i: w and every fourth
-    auto load_keys = [&](int i, KvTile<D, Q4> &t) {
+    auto load_keys = [&](int i, KvTile<D, Q4, ONCE> &t) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int page = page_of(i, u);
             t.load_keys(a, u, (page < 0 ? 0 : page) * a.batch.page_stride + head_at, (key_of(i) + 16 * u) & in_page, lane_at);
         }
     };
-    auto load_values = [&](int i, KvTile<D, Q4> &t) {
+    auto load_values = [&](int i, KvTile<D, Q4, ONCE> &t) {
         t.ok = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -550,7 +556,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
     const Q4Bits bits;
-    auto compute = [&](int kb, KvTile<D, Q4> &t, auto after_scores) {
+    auto compute = [&](int kb, KvTile<D, Q4, ONCE> &t, auto after_scores) {
         float4_t sc[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -623,7 +629,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             if (Q4 && (e & 1)) __builtin_amdgcn_sched_barrier(0);
         }
     };
-    KvTile<D, Q4> t;
+    KvTile<D, Q4, ONCE> t;
     if constexpr (Q4) {
         // the next tile's keys are requested as soon as this one's have made their scores, in the same registers; past the last
         // key page 0 is read, for nothing, so that no branch holds a request
@@ -653,7 +659,7 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
         float x = 0.0f;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int d = KvTile<D, Q4>::dim(i, g);
+            const int d = KvTile<D, Q4, ONCE>::dim(i, g);
             const half8_t k = q4_values(*reinterpret_cast<const uint32_t *>(kp + Q4Row<D>::key_word(slot, d / 8)),
                                         *reinterpret_cast<const uint32_t *>(kp + Q4Row<D>::pair(in_page + 1, slot, d / 32)), bits);
 #pragma unroll
@@ -738,10 +744,10 @@ __device__ __forceinline__ void rows_tile(const AttnArgs &a, RowsLds<D> &lds, in
             }
         } else {
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // a row that sees no key is zero
-            typename KvTile<D, Q4>::ve y;
+            typename KvTile<D, Q4, ONCE>::ve y;
 #pragma unroll
             for (int e = 0; e < E; ++e) y[e] = static_cast<half_t>(num[e] * inv);
-            *reinterpret_cast<typename KvTile<D, Q4>::ve *>(a.out + trow * D + E * l16) = y;
+            *reinterpret_cast<typename KvTile<D, Q4, ONCE>::ve *>(a.out + trow * D + E * l16) = y;
         }
     }
 }
@@ -1099,10 +1105,10 @@ __device__ __forceinline__ void chunk_tile(const AttnArgs &a, ChunkLds<D> &lds, 
 
 // ---------------------------------------------------------------- the kernels
 
-template <int D, bool Q4, bool SINKS>
+template <int D, bool Q4, bool SINKS, bool ONCE>
 __global__ __launch_bounds__(256, 2) void paged_attn_rows(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
-    rows_tile<D, Q4, SINKS>(a, lds, blockIdx.x);
+    rows_tile<D, Q4, SINKS, ONCE>(a, lds, blockIdx.x);
 }
 
 // Batches with long chunks: the first `large` blocks are 128-row tiles, the rest the short chunks' 16-row
@@ -1117,7 +1123,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_mixed(AttnArgs a, int large
     if (static_cast<int>(blockIdx.x) < large)
         chunk_tile<D, Q4, SINKS>(a, lds.chunk, blockIdx.x);
     else
-        rows_tile<D, Q4, SINKS>(a, lds.rows, static_cast<int>(blockIdx.x) - large);
+        rows_tile<D, Q4, SINKS, false>(a, lds.rows, static_cast<int>(blockIdx.x) - large);
 }
 
 // ---------------------------------------------------------------- the chunks' states
@@ -1293,6 +1299,7 @@ struct Plan {
     int64_t few;           // rows of a sequence up to which it goes to the small ones
     int chunk, nsplit;
     int target;            // units of a kv head where the device shares the keys out, or 0
+    bool once;             // keys and values are read once and not kept
 };
 
 // Sequences of up to kFew rows go to the 16-row tiles, the others to the 128-row ones: 64 sequences after 2000 keys
@@ -1310,6 +1317,13 @@ constexpr int64_t kFillSmall = 1024, kFillLarge = 384, kWhole = 384;
 
 // Where the device shares the keys out (a token or a few of each sequence, over 4-bit pages or with sinks):
 constexpr int64_t kFillShared = 1024, kShareBytes = int64_t(64) << 20;
+
+// Where one tile of a sequence reads its keys, and all of them are too many for two such calls (two layers) in turn to find them
+// in the 256 MB cache before the memory, they are read past it. Over others' data in between, 64 tokens under a window of 2048 (f16,
+// D = 64, 134 MB) 32.5 us kept and 28.5 so, 5 over up to 65000 (4 bits, 132 MB) 34.4 and 32.4; again over the same data 27.7 and
+// 28.5, 27.1 and 27.8; 48 over up to 1536 (4 bits, 49 MB) 17.6 and 17.9. With two tiles (30 sequences of 6 tokens of 4 heads over 20000,
+// f16) 530 and 711. f16 pages without sinks are kept: 5 over up to 65000 of D = 64 33.0 and 39.4 over the same data.
+constexpr double kKeptBytes = 128 << 20;
 
 // How far to cut 128-row tiles over 4-bit pages or with sinks. A tile's time is a fixed part and one for each 64 keys, which
 // depend on how many workgroups share its CU (us; 128 and 1152 keys on 2, 256 and 512 workgroups, D = 64 then 128, three
@@ -1374,6 +1388,8 @@ inline Plan plan_of(int64_t tokens, int64_t b, int64_t gqa, int64_t n_kv, int64_
     if (n > most) n = most;
     p.chunk = static_cast<int>(((span + n - 1) / n + 63) / 64 * 64);
     p.nsplit = static_cast<int>((span + p.chunk - 1) / p.chunk);
+    const int64_t row_bytes = share ? 5 * hd / 4 : 4 * hd;  // a key's and its value's; share: of 4-bit pages
+    p.once = own && p.large == 0 && max_q * gqa <= 16 && static_cast<double>(live * n_kv * row_bytes) * static_cast<double>(span) > kKeptBytes;
     if (share && p.large == 0 && p.nsplit > 1) {
         // room for chunks of kMinChunk keys, as many as a kv head has units or kShareBytes of states hold
         const int64_t left = kFillShared / n_kv - p.small / 2;  // a tile's last chunk is half a one
@@ -1410,10 +1426,14 @@ hipError_t launch(const AttnArgs &a, const Plan &p, hipStream_t stream) {
     if (p.large > 0)
         paged_attn_mixed<D, Q4, SINKS><<<dim3(static_cast<unsigned>((p.large + p.small) * a.n_kv), a.nsplit), 256, 0, stream>>>(
             a, static_cast<int>(p.large * a.n_kv));
-    else
-        paged_attn_rows<D, Q4, SINKS><<<
-            a.target > 0 ? dim3(static_cast<unsigned>((p.small + a.target + 1) * a.n_kv)) : dim3(static_cast<unsigned>(p.small * a.n_kv), a.nsplit),
-            256, 0, stream>>>(a);
+    else {
+        const dim3 grid = a.target > 0 ? dim3(static_cast<unsigned>((p.small + a.target + 1) * a.n_kv))
+                                       : dim3(static_cast<unsigned>(p.small * a.n_kv), a.nsplit);
+        if ((Q4 || SINKS) && p.once)
+            paged_attn_rows<D, Q4, SINKS, Q4 || SINKS><<<grid, 256, 0, stream>>>(a);
+        else
+            paged_attn_rows<D, Q4, SINKS, false><<<grid, 256, 0, stream>>>(a);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     if (Q4 && a.target > 0) return merge<D, Q4 ? kShared : kBySequence>(a, stream);

@@ -471,7 +471,7 @@ struct CopyArgs {
 // Units a thread requests together, and a workgroup's at a time.
 constexpr int kRequests = 2, kSlice = 256 * kRequests;
 constexpr int64_t kMostSlices = 65535, kMostPageBytes = kMostSlices * kSlice * 16;  // of a launch, a slice a row of its grid
-constexpr int64_t kCopyFill = 8192;  // workgroups: 866 pages of 64 KB and 18980 of 2.5 KB 24.2 and 21.9 us with 4 requests and 4096, 23.6 and 21.1 so (4.8 and 4.6 TB/s)
+constexpr int64_t kCopyFill = 8192;  // workgroups: 866 pages of 64 KB and 18980 of 2.5 KB 24.2 and 21.9 us with 4 requests and 4096, 23.6 and 21.1 so; each 4 us less with stores past the caches, which a list of pages fills
 
 // HBM-bound: every byte read once and written once. A workgroup takes one slice of every gridDim.x-th pair's pages, 256 pairs at
 // a time: those that copy something are put together first, so that a list with few of them, or with all of them in front, is
@@ -517,7 +517,7 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyArgs<MOST> a) {
 #pragma unroll
             for (int k = 0; k < kRequests; ++k) {
                 const uint32_t t = t0 + k * 256, p = by_units.div(t);
-                if (t < all) *reinterpret_cast<float4_t *>(base + to[p] * stride + static_cast<int64_t>(t - p * units) * 16) = x[k];
+                if (t < all) __builtin_nontemporal_store(x[k], reinterpret_cast<float4_t *>(base + to[p] * stride + static_cast<int64_t>(t - p * units) * 16));
             }
         }
     }

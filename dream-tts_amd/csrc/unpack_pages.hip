@@ -17,6 +17,8 @@ struct UnpackArgs {
 // blockIdx.y: keys or values; blockIdx.x walks (page, kv head, 16-byte piece of its codes). A wave's stores are runs of whole
 // rows either way: of values a thread takes eight dimensions of four rows, one load; of keys words 64 apart, so that each
 // store of the wave is 64 neighbouring words' values (with 16 bytes a thread, stores of 64 bytes apart: 13.9 us for 57 MB).
+// Values are stored past the caches, keys are not: both kept / keys past / values past / both 13.0 / 12.9 / 12.6 / 13.2 us (with the append of
+// 48 tokens before, 43 MB) and 14.2 / 13.9 / 13.85 / 13.65 (4436 tokens, 16 MB).
 template <int D>
 __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a, FastDiv pieces, FastDiv heads, uint32_t most) {
     constexpr int W = Q4Row<D>::kWords;
@@ -39,7 +41,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a, FastDiv piece
         const u32x4 pairs = *reinterpret_cast<const u32x4 *>(x + Q4Row<D>::pair(page, row, w / 4));
         half_t *y = a.v_out + (static_cast<int64_t>(head) << a.page_shift) * D + row * D + 8 * w;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<half8_t *>(y + k * D) = q4_values(words[k], pairs[k], bits);
+        for (int k = 0; k < 4; ++k) __builtin_nontemporal_store(q4_values(words[k], pairs[k], bits), reinterpret_cast<half8_t *>(y + k * D));
     } else {
         const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;  // the wave's pieces; its words are four times as many
         uint32_t word[4], pair[4];

@@ -474,3 +474,18 @@ def test_a_missing_page_stands_for_nothing(dev, bits, hd, n, c, where):
         b.table[:, block] = -1
         for window, sinks in ((0, 0), (1000, 5), (60, 0), (60, 7), (60, 100), (1000, 64)):
             check(b, packed, values, q, max(n), max(c), 0.15, window, sinks)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,c", [([1], [300]), ([1, 2, 4, 0, 3], [700, 2, 90, 40, 333])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200000, 5), (60, 7)])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_keys_that_no_cache_holds(dev, hd, n, c, window, sinks, bits):
+    """A longest context of a million positions makes a call that is taken to read more than the caches keep (short sequences all the
+    same), with room for its chunks and without; unseen and missing pages among them."""
+    b = ref.Batch(n, c, 2, hd, 16, dev, seed=len(n) + hd, extra_tokens=1)
+    b.table[-1, 1:2] = -1
+    packed, values = q4(b) if bits == 4 else (list(b.device()[:2]), (b.k, b.v))
+    q = torch.randn((b.tokens, 8, hd), generator=torch.Generator().manual_seed(hd)).half()
+    for workspace in (None, torch.empty(0, dtype=torch.uint8, device=dev)):
+        check(b, packed, values, q, max(n), 1 << 20, 0.15, window, sinks, workspace=workspace)
