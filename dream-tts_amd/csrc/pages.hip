@@ -624,19 +624,21 @@ extern "C" int dtts_claim_pages(int32_t *pages, int32_t *refs, const int32_t *q_
     const char *name = "dtts_claim_pages";
     DTTS_REQUIRE_TABLE(name, b, max_pages, n_pages);
     DTTS_REQUIRE_PAGE(name, page, max_pages);
-    DTTS_REQUIRE(lacking && aligned(lacking, 4), "%s: null or misaligned pointer", name);
-    const size_t need = dtts_claim_pages_workspace_bytes(b, max_pages, n_pages);
+    // counts and `lacking` are read and written without sequences too
+    DTTS_REQUIRE(lacking && refs && aligned(lacking, 4) && aligned(refs, 4), "%s: counts or lacking null or misaligned", name);
+    const size_t need = b > 0 ? dtts_claim_pages_workspace_bytes(b, max_pages, n_pages) : 0;
     if (b > 0) {
-        DTTS_REQUIRE(pages && refs && q_start && context && src && dst, "%s: null pointer", name);
-        DTTS_REQUIRE(aligned(pages, 4) && aligned(refs, 4) && aligned(q_start, 4) && aligned(context, 4) && aligned(src, 4) && aligned(dst, 4),
+        DTTS_REQUIRE(pages && q_start && context && src && dst, "%s: null pointer", name);
+        DTTS_REQUIRE(aligned(pages, 4) && aligned(q_start, 4) && aligned(context, 4) && aligned(src, 4) && aligned(dst, 4),
                      "%s: misaligned operand", name);
         DTTS_REQUIRE(workspace && ws_bytes >= need && aligned(workspace, 4), "%s: a workspace of %zu bytes is needed", name, need);
-        const ByteRows of[] = {{pages, 1, 0, b * max_pages * 4}, {refs, 1, 0, n_pages * 4}, {src, 1, 0, b * 4}, {dst, 1, 0, b * 4},
-                               {lacking, 1, 0, 4}, {workspace, 1, 0, static_cast<int64_t>(need)}, {q_start, 1, 0, (b + 1) * 4},
-                               {context, 1, 0, b * 4}};
-        for (int i = 0; i < 6; ++i)
-            for (int j = i + 1; j < 8; ++j) DTTS_REQUIRE(!share_bytes(of[i], of[j]), "%s: operands share memory", name);
     }
+    const int64_t rows = b > 0 ? 1 : 0;  // arrays of a batch without sequences are not looked at
+    const ByteRows of[] = {{refs, 1, 0, n_pages * 4}, {lacking, 1, 0, 4}, {pages, rows, 0, b * max_pages * 4}, {src, rows, 0, b * 4},
+                           {dst, rows, 0, b * 4}, {workspace, rows, 0, static_cast<int64_t>(need)}, {q_start, rows, 0, (b + 1) * 4},
+                           {context, rows, 0, b * 4}};
+    for (int i = 0; i < 6; ++i)
+        for (int j = i + 1; j < 8; ++j) DTTS_REQUIRE(!share_bytes(of[i], of[j]), "%s: operands share memory", name);
     ClaimArgs a;
     a.pages = pages;
     a.refs = refs;

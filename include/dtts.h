@@ -583,7 +583,8 @@ int dtts_unpack_pages_q4(const void *kpages, const void *vpages, const int32_t *
  * gets a free one; a page with other owners is replaced by one, so that the writes of one do not reach the others (of c writers
  * to a page of r owners the first min(c, r - 1) in order). src[s] and dst[s] [b]: where positions before the new ones are in
  * that page, what to copy, or -1. lacking[0]: how many free pages there are too few; above 0 nothing was changed, src and dst
- * are -1, and the step must wait. workspace of dtts_claim_pages_workspace_bytes (refused without it).
+ * are -1, and the step must wait. workspace of dtts_claim_pages_workspace_bytes (refused without it). Without sequences refs and
+ * lacking alone are needed.
  * 6.7 us for 160 sequences over 20011 pages; where a step writes to more than 1024 blocks, each writer to a shared page is ranked
  * among the earlier blocks, one after another.
  *

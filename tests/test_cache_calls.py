@@ -123,6 +123,15 @@ def test_claim(match, bad):
     claim(match, **bad)
 
 
+@pytest.mark.parametrize("match,refs,lacking", [
+    ("counts or lacking", None, BIG), ("counts or lacking", 2, BIG), ("counts or lacking", 0, None), ("share memory", 0, 32),
+])
+def test_claim_without_sequences_needs_its_counts(match, refs, lacking):
+    """They are read whatever the batch is; the arrays of sequences are not."""
+    p = [None if x is None else at(x) for x in (refs, lacking)]
+    refused("dtts_claim_pages", match, None, p[0], None, None, None, None, p[1], 0, 16, 4, 9, None, 0, None)
+
+
 @pytest.mark.parametrize("match,args", [
     ("window 0", (16, 4, 9, 0, 0)), ("window", (16, 4, 9, 1 << 31, 0)), ("sinks", (16, 4, 9, 5, -1)), ("positions", (17, 4, 9, 5, 0)),
     ("a table of", (16, 0, 9, 5, 0)),
