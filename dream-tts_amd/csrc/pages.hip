@@ -8,6 +8,10 @@
 // on nothing but the arguments, and the calls of a step can be captured.
 //
 // All but the copy are a few dependent trips to memory over some hundred kilobytes at most.
+#include <algorithm>
+#include <memory>
+#include <new>
+
 #include "paged.hpp"
 
 namespace dtts {
@@ -551,6 +555,31 @@ int64_t copy_some(void **caches, const int64_t *page_bytes, const int64_t *page_
     return c;
 }
 
+// Two pools that share memory without being one and the same (which is then copied twice, to the same end), or false. In order
+// of address each meets those alone that begin before its end: none where every pool is an allocation, all where the layers'
+// pages lie side by side in one, and there strides that are equal tell.
+inline bool pools_meet(const ByteRows *pools, int32_t *order, int64_t n, int32_t &one, int32_t &other) {
+    const auto from = [&](int64_t i) { return reinterpret_cast<uintptr_t>(pools[order[i]].p); };
+    for (int64_t i = 0; i < n; ++i) order[i] = static_cast<int32_t>(i);
+    std::sort(order, order + n, [&](int32_t i, int32_t j) { return pools[i].p < pools[j].p; });
+    for (int64_t i = 0; i + 1 < n; ++i) {
+        const ByteRows &x = pools[order[i]];
+        const __int128 end = static_cast<__int128>(from(i)) + static_cast<__int128>(x.n - 1) * x.stride + x.width;
+        for (int64_t j = i + 1; j < n && static_cast<__int128>(from(j)) < end; ++j) {
+            const ByteRows &y = pools[order[j]];
+            const uintptr_t apart = from(j) - from(i);
+            const bool alike = x.stride == y.stride;
+            if (alike && apart >= static_cast<uintptr_t>(x.width) && apart + static_cast<uintptr_t>(y.width) <= static_cast<uintptr_t>(x.stride)) continue;
+            if (apart == 0 && alike && x.width == y.width) continue;
+            if (!share_bytes(x, y)) continue;
+            one = order[i];
+            other = order[j];
+            return true;
+        }
+    }
+    return false;
+}
+
 inline unsigned blocks_for(int64_t n) { return static_cast<unsigned>((n + 255) / 256); }
 
 }  // namespace
@@ -716,6 +745,16 @@ extern "C" int dtts_copy_pages(void **caches, const int64_t *page_bytes, const i
                      "%s: pages of %lld bytes, %lld apart (multiples of 16, up to %lld and under 2^34)", name, (long long)page_bytes[c],
                      (long long)page_strides[c], (long long)kMostPageBytes);
     }
+    const std::unique_ptr<ByteRows[]> pools(new (std::nothrow) ByteRows[n_caches]);
+    const std::unique_ptr<int32_t[]> order(new (std::nothrow) int32_t[n_caches]);
+    DTTS_REQUIRE(pools && order, "%s: no host memory for %lld caches", name, (long long)n_caches);
+    for (int64_t c = 0; c < n_caches; ++c) {
+        pools[c] = {caches[c], n_pages, page_strides[c], page_bytes[c]};
+        DTTS_REQUIRE(!share_bytes(pools[c], {src, 1, 0, n * 4}) && !share_bytes(pools[c], {dst, 1, 0, n * 4}),
+                     "%s: cache %lld and the pairs share memory", name, (long long)c);
+    }
+    int32_t one, other;
+    DTTS_REQUIRE(!pools_meet(pools.get(), order.get(), n_caches, one, other), "%s: caches %d and %d share memory", name, one, other);
     for (int64_t c0 = 0; c0 < n_caches;) {
         const int64_t done = n_caches - c0 <= 2 ? copy_some<2>(caches + c0, page_bytes + c0, page_strides + c0, n_caches - c0, src, dst, n, n_pages, stream)
                                                 : copy_some<kMostCaches>(caches + c0, page_bytes + c0, page_strides + c0, n_caches - c0, src, dst,

@@ -406,7 +406,8 @@ def compact_pages(pages, refs, workspace=None):
 def copy_pages(caches, src, dst):
     """Page src[i] to page dst[i] (int32) in each of `caches`, tensors [n_pages, ...] whose pages are contiguous and some
     multiple of 16 bytes: f16 and 4-bit pages of any number of layers at once. Pairs with an id outside the pool (the -1 of
-    claim_pages and compact_pages) copy nothing. A page is the destination of one pair at most, and then no source."""
+    claim_pages and compact_pages) copy nothing. A page is the destination of one pair at most, and then no source. Two caches share
+    no memory, unless they are the same, nor does one with src or dst."""
     if isinstance(caches, _Tensor):
         caches = (caches,)
     if _serving.copy_pages(caches, src, dst) is not None:

@@ -597,7 +597,8 @@ int dtts_unpack_pages_q4(const void *kpages, const void *vpages, const int32_t *
  *
  * dtts_copy_pages: in each of n_caches pools (HOST arrays: its address, bytes of a page, bytes from page to page; multiples of
  * 16) page src[i] to page dst[i], i < n (DEVICE arrays; pairs with an id outside [0, n_pages) copy nothing). No page is the
- * destination of two pairs, nor of one and the source of another: what such pages hold afterwards is not said. */
+ * destination of two pairs, nor of one and the source of another: what such pages hold afterwards is not said. Two pools are one
+ * and the same or share no memory. */
 int dtts_fork_pages(const int32_t *page_table, int32_t *refs, const int32_t *parent, int32_t *out, int64_t b, int64_t n,
                     int64_t max_pages, int64_t n_pages, void *workspace, size_t ws_bytes, hipStream_t stream);
 size_t dtts_claim_pages_workspace_bytes(int64_t b, int64_t max_pages, int64_t n_pages);

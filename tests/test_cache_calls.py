@@ -176,6 +176,41 @@ def test_copy_of_pages_with_more_slices_than_a_grid_has_rows(size):
             at(3 * BIG), 5, 9, None)
 
 
+def copy_of(match, *pools, src=8 * BIG, dst=9 * BIG, n=5, n_pages=9):
+    """Pools (address, bytes of a page, bytes from page to page)."""
+    addresses, sizes, strides = zip(*pools)
+    caches = (ctypes.c_void_p * len(pools))(*(at(a).value for a in addresses))
+    refused("dtts_copy_pages", match, caches, *((ctypes.c_int64 * len(pools))(*x) for x in (sizes, strides)), len(pools), at(src), at(dst),
+            n, n_pages, None)
+
+
+ONE = (BIG, 1280, 2560)
+
+
+@pytest.mark.parametrize("match,pools,pairs", [
+    ("pairs share memory", [ONE], dict(src=BIG)), ("pairs share memory", [ONE], dict(dst=BIG + 8 * 2560 + 1276)),
+    ("pairs share memory", [ONE], dict(src=BIG - 16)), ("pairs share memory", [(0, 64, 64), ONE], dict(dst=BIG + 2560 - 4)),
+    ("share memory", [ONE, (BIG + 16, 1280, 2560)], {}), ("share memory", [(BIG + 1264, 1280, 2560), ONE], {}),
+    ("share memory", [ONE, (BIG + 1280 + 16, 1280, 2560)], {}), ("share memory", [ONE, (BIG, 1264, 2560)], {}),
+    ("share memory", [ONE, (BIG, 1280, 1280)], {}), ("share memory", [ONE, (BIG + 1280, 1280, 1280)], {}),
+    ("share memory", [ONE, (BIG - 8 * 2560 - 1264, 1280, 2560)], {}), ("share memory", [ONE, (BIG + 8 * 2560 + 1264, 16, 16)], {}),
+    ("share memory", [(BIG + 1280, 1280, 2560), (3 * BIG, 64, 64), ONE, (2 * BIG, 64, 80), (BIG + 1264, 16, 2560)], {}),
+])
+def test_copy_of_shared_memory(match, pools, pairs):
+    copy_of(match, *pools, **pairs)
+
+
+@pytest.mark.parametrize("pools,pairs", [
+    ([ONE, ONE], {}), ([ONE, (BIG + 1280, 1280, 2560)], {}), ([ONE, (BIG + 8 * 2560 + 1280, 64, 64)], {}), ([(BIG - 9 * 64, 64, 64), ONE], {}),
+    ([ONE], dict(src=BIG + 1280)), ([ONE], dict(src=BIG + 8 * 2560 + 1280, dst=BIG - 20)),
+    ([(BIG + 80 * i, 80, 80 * 64) for i in reversed(range(64))], {}), ([(BIG + 640, 640, 1280), (BIG, 320, 640)], dict(n_pages=1)),
+])
+def test_copy_of_pools_that_lie_apart(pools, pairs):
+    """Told by what is refused after them: two pools past all others."""
+    n = len(pools)
+    copy_of(f"caches {n} and {n + 1} share memory", *pools, (7 * BIG, 64, 64), (7 * BIG + 32, 64, 64), **pairs)
+
+
 def test_tensors_that_are_not_on_a_gpu():
     i, x = torch.zeros((2, 2), dtype=torch.int32), torch.zeros((4, 2, 16, 40), dtype=torch.uint8)
     for call in (lambda: serving.fork_pages(i, i[0], i[0]), lambda: serving.claim_pages(i, i[0], torch.zeros(3, dtype=torch.int32), i[0], 16),
