@@ -1476,7 +1476,8 @@ int attention(const char *name, int bits, const dtts_f16 *q, const void *kpages,
     if (window == 0) sinks = 0;  // every token sees them
     const bool share = bits == 4, own = bits == 4 || (sinks > 0 && window < int64_t(1) << 30);
     Plan p = plan_of(tokens, b, heads / n_kv, n_kv, max_q, max_context, window, sinks, head_dim, share, own);
-    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large + p.target + 1) * n_kv < (int64_t(1) << 24), "%s: too many rows", name);
+    DTTS_REQUIRE(tokens * heads < (int64_t(1) << 31) && (p.small + p.large + (p.target > 0 ? p.target + 1 : 0)) * n_kv < (int64_t(1) << 24),
+                 "%s: too many rows", name);
     const int64_t row = heads * head_dim * static_cast<int64_t>(sizeof(half_t));
     DTTS_REQUIRE(q_stride < (int64_t(1) << 62), "%s: q_stride %lld", name, (long long)q_stride);
     DTTS_REQUIRE(!share_bytes({q, tokens, q_stride * static_cast<int64_t>(sizeof(half_t)), row}, {out, 1, 0, tokens * row}),

@@ -40,6 +40,14 @@ def test_attention(match, bad):
     attention(match, **bad)
 
 
+@pytest.mark.parametrize("tokens,match", [(65520, "may not be the queries"), (65521, "too many rows")])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_attention_of_as_many_tiles_as_a_launch_has(bits, tokens, match):
+    """4095 and 4096 tiles of 16 rows of 4096 kv heads, under 2^24 workgroups and not: told by what is refused after that."""
+    attention(match, bits=bits, tokens=tokens, b=1, heads=4096, n_kv=4096, stride=4096 * 16 * (64 if bits == 16 else 40), q_stride=4096 * 64,
+              max_q=1, out=512)
+
+
 def test_attention_of_nothing_is_taken():
     p = at(0)
     for tokens, b in ((0, 3), (3, 0)):
