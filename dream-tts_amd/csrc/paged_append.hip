@@ -9,8 +9,9 @@
 //
 // 4-bit pages (q4.hpp) take k = turn(x') and v in groups of 32 instead:
 //   d = f16((max - min) / 15), b = f16(min - 64 d), n = rint((x - (64 d + b)) / d) from 0 to 15
-// 64 d + b is exact in f32 (two f16 numbers that nearly cancel) and b is rounded before the codes are chosen, so the
-// steps lie where the values read back do. A lane needs eight neighbours of a row, a group being four lanes: half-split
+// The pair's two roundings are those of the exact numbers, and b is rounded before the codes are chosen, so the steps lie where
+// the values read back do. 64 d + b takes two f32 numbers (one where they nearly cancel; a narrow group far from zero needs the
+// other). A code is the definition's unless its value lies within 2^-18 of a step of the border between two. A lane needs eight neighbours of a row, a group being four lanes: half-split
 // rows, whose lanes hold two groups of four apart, meet in LDS, a wave's rows in its own.
 //
 // HBM-bound: qkv in, q, k and v out, once. D/8 lanes own a head row, two groups of four elements each:
@@ -67,6 +68,21 @@ __device__ __forceinline__ float quotient(float x, float y, float per) {
     return __builtin_fmaf(__builtin_fmaf(-q, y, x), per, q);
 }
 
+// x - y rounded, and what that leaves of it: exact together.
+__device__ __forceinline__ float difference(float x, float y, float &rest) {
+    const float s = x - y, v = s - x;
+    rest = (x - (s - v)) - (y + v);
+    return s;
+}
+
+// x + rest, less than a last place from x, as the f16 number next to it. Rounded to f32 before, the sum could fall half way between
+// two f16 numbers; of x and its neighbours the odd one on the sum's side is on the same side of every such place.
+__device__ __forceinline__ half_t half_of(float x, float rest) {
+    const int bits = static_cast<int>(__float_as_uint(x)), away = ((bits ^ static_cast<int>(__float_as_uint(rest))) >> 31) | 1;
+    const bool moves = (rest != 0.0f) & ((bits & 1) == 0);
+    return static_cast<half_t>(__uint_as_float(static_cast<uint32_t>(bits + (moves ? away : 0))));
+}
+
 // x of the lane OFF (1 or 2) away among four.
 template <int OFF>
 __device__ __forceinline__ float other_of_four(float x) {
@@ -89,8 +105,14 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
     hi = fmaxf(hi, other_of_four<1>(hi));
     lo = fminf(lo, other_of_four<2>(lo));
     hi = fmaxf(hi, other_of_four<2>(hi));
-    half_t d = static_cast<half_t>(quotient(hi - lo, 15.0f, 1.0f / 15.0f)), b = static_cast<half_t>(lo - kQ4First * static_cast<float>(d));
-    const float step = static_cast<float>(d), first = __builtin_fmaf(kQ4First, step, static_cast<float>(b));
+    constexpr float kPer = 1.0f / 15.0f;
+    float rest;
+    const float width = difference(hi, lo, rest), about = width * kPer;
+    const float fifteenth = __builtin_fmaf(__builtin_fmaf(-about, 15.0f, width) + rest, kPer, about);
+    half_t d = half_of(fifteenth, __builtin_fmaf(-fifteenth, 15.0f, width) + rest);
+    const float step = static_cast<float>(d), least = difference(lo, kQ4First * step, rest);
+    half_t b = half_of(least, rest);
+    const float first = difference(kQ4First * step, -static_cast<float>(b), rest);  // and rest: where code 64 is
     const float last = __builtin_fmaf(kQ4Last, step, static_cast<float>(b));
     constexpr float kOver = 65520.0f;  // what f16 rounds to infinity
     if (!(fabsf(first) < kOver && fabsf(last) < kOver)) d = b = static_cast<half_t>(NAN);
@@ -99,7 +121,7 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
     float half[2] = {};  // of the word, as numbers
 #pragma unroll
     for (int i = 7; i >= 0; --i)
-        half[i & 1] = __builtin_fmaf(half[i & 1], 16.0f, __builtin_amdgcn_fmed3f(rintf(quotient(z[i] - first, step, per)), 0.0f, 15.0f));
+        half[i & 1] = __builtin_fmaf(half[i & 1], 16.0f, __builtin_amdgcn_fmed3f(rintf(quotient(z[i] - first - rest, step, per)), 0.0f, 15.0f));
     return static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
 }
 

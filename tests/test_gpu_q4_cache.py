@@ -116,6 +116,57 @@ def test_append_of_f16_values_takes_the_codes_of_the_definition(dev):
         assert np.array_equal(v.cpu().numpy(), want), hd
 
 
+def hard_groups(rng, n):
+    """Groups [5 n, 32] of f32 numbers: whose width over 15, and whose least number less 64 steps, are next to half way between two
+    f16 numbers, nearer than f32 can tell; narrow ones far from zero, whose first code is no f32 number; wider ones; ordinary ones."""
+    f = np.float32
+    d = rng.randint(1024, 2048, n) * 2.0 ** rng.randint(-13, -3, n)
+    sign = rng.choice([-1, 1], n)
+    mid = rng.rand(n, 32)
+
+    def ends(lo, hi):
+        g = (lo[:, None] + mid * (hi - lo)[:, None]).astype(f)
+        g = g.clip(lo.astype(f)[:, None], hi.astype(f)[:, None])
+        g[:, 3], g[:, 7] = lo, hi
+        return g
+
+    tie = 15 * (d + 2.0 ** (np.floor(np.log2(d)) - 11))
+    low = sign * tie * 2.0 ** -26
+    least = (-64 * d * (1 + rng.uniform(-0.02, 0.02, n))).astype(np.float16)
+    half = np.spacing(np.abs(least)).astype(np.float64) / 2
+    lo = np.nextafter((least.astype(np.float64) + half + 64 * d).astype(f), (sign * 1e9).astype(f)).astype(np.float64)
+    at = sign * 10 ** rng.uniform(-2, 3.3, n)
+    wide = rng.randn(n) * 3
+    return np.concatenate([ends(low, tie), ends(lo, lo + 15 * d), ends(at, at + 10 ** rng.uniform(-5, -1, n)),
+                           ends(wide, wide + 10 ** rng.uniform(-3, 1, n)), rng.randn(n, 32).astype(f)])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_of_f32_values_takes_the_pairs_and_codes_of_the_definition(dev, interleaved):
+    """Rows that the rotation leaves as they are: pairs bit for bit, codes but for those of values within 2^-18 of a step of the border
+    between two (three f32 roundings of 16 steps at most)."""
+    n_kv, page, hd = 4, 64, 128
+    rng = np.random.RandomState(5)
+    g = rng.permutation(hard_groups(rng, page * n_kv * 2))[:page * n_kv * 8]
+    rows = torch.from_numpy(g.reshape(page, 2 * n_kv, hd))
+    x = torch.cat([torch.zeros((page, 1, hd)), rows], 1).view(page, -1)
+    cos, sin = torch.ones((page, hd // 2), device=dev), torch.zeros((page, hd // 2), device=dev)
+    pages = [torch.zeros((1, n_kv, page, 80), dtype=torch.uint8, device=dev) for _ in range(2)]
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    serving.qk_rope_append_paged(x.to(dev), cos, sin, *pages, i32([0, page]), i32([page]), i32([[0]]), 1, interleaved=interleaved)
+    for i, t in enumerate(pages):
+        want = rows[:, i * n_kv:(i + 1) * n_kv].double().numpy()  # [page, n_kv, D]
+        n, d, b = pref.quantise(want)
+        words, pairs = slots(t.cpu().numpy(), i)
+        pairs = np.ascontiguousarray(pairs[0]).view(np.float16).reshape(page, n_kv, hd // 32, 2)
+        assert np.array_equal(pairs[..., 0].view(np.int16), d.view(np.int16)) and np.array_equal(pairs[..., 1].view(np.int16), b.view(np.int16))
+        got = np.stack([words[0] >> np.uint32(4 * (e // 2) + 16 * (e % 2)) & np.uint32(15) for e in range(8)], -1).reshape(want.shape)
+        d, b = (np.repeat(y.astype(np.float64), 32, -1) for y in (d, b))
+        step = (want.astype(np.longdouble) - b - 64 * d) / np.where(d > 0, d, 1)
+        border = np.abs(step - np.floor(step) - 0.5)
+        assert (border[got != n] <= 2.0 ** -18).all(), (got != n).sum()
+
+
 def slots(raw, values):
     """The words [n_pages, page, n_kv, D / 8] and pairs [n_pages, page, n_kv, D / 32] of uint8 pages."""
     n, n_kv, page, row = raw.shape
