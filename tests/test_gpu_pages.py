@@ -91,6 +91,43 @@ def test_claim(dev, path, b, m, n_pages, page):
         assert int(lacking) == want[4], kind
 
 
+def written(start, c, m, page):
+    """The blocks that each row writes to."""
+    n, c = np.maximum(np.diff(start), 0), np.minimum(np.maximum(c, 0), m * page)
+    first = np.maximum(c - n, 0) // page
+    return np.where((n > 0) & (c > 0), -(-c // page) - first, 0)
+
+
+@pytest.mark.parametrize("b,m,n_pages,share,free_from,n,c,items,need", [
+    (3000, 8, 40000, 0.6, 0, (30, 64), (64, 129), (9000, 24000), 4097),  # words and free ids past what LDS holds, shared pages throughout
+    (3000, 8, 24000, 0.9, 0, (60, 64), (64, 129), (9000, 24000), 4097),  # most pages shared by many
+    (700, 8, 40000, 0.4, 33000, (1, 40), (20, 129), (1025, 4096), 500),  # the free ids far behind, rounds of counts without any
+    (1500, 5, 20000, 0.8, 16000, (0, 2), (1, 81), (300, 1024), 100),  # more rows than threads, fewer blocks
+    (5000, 3, 60000, 0.5, 50000, (1, 2), (1, 49), (4097, 5000), 1000),  # a token each
+])
+def test_claim_of_many_blocks(dev, b, m, n_pages, share, free_from, n, c, items, need):
+    """Past the sizes that stay in LDS, in a round of threads and in a round of counts; and with a page too few, and with as many as are
+    needed to the last."""
+    table, refs, rng = pool(b, b, m, n_pages, share=share, waste=0.0)
+    refs[:free_from][refs[:free_from] < 1] = 1  # held by other tables
+    tokens, ctx = rng.randint(*n, b), rng.randint(*c, b)
+    if n == (0, 2):
+        tokens = (rng.rand(b) < 0.4).astype(int)
+    start = np.concatenate([[0], np.cumsum(tokens)])
+    want = ref.claim(table, refs, start, ctx, 16)
+    given = int((want[0] != table).sum())
+    assert items[0] <= written(start, ctx, m, 16).sum() <= items[1] and given >= need and want[4] == 0
+    free = np.flatnonzero(refs < 1)
+    for lacking in (0, 1, given // 2):
+        r0 = refs.copy()
+        r0[free[given - lacking:]] = 1  # held by others
+        again = ref.claim(table, r0, start, ctx, 16)
+        assert again[4] == lacking
+        t, r = up(table, dev), up(r0, dev)
+        src, dst, short = serving.claim_pages(t, r, up(start, dev), up(ctx, dev), 16)
+        assert all(np.array_equal(x, y) for x, y in zip(host(t, r, src, dst), again)) and int(short) == lacking
+
+
 def test_claim_of_too_few_pages_changes_nothing(dev):
     table, refs, _ = pool(3, 40, 6, 160, waste=0.0)
     free = int((refs < 1).sum())
