@@ -78,9 +78,8 @@ __device__ __forceinline__ float difference(float x, float y, float &rest) {
 // x + rest, less than a last place from x, as the f16 number next to it. Rounded to f32 before, the sum could fall half way between
 // two f16 numbers; of x and its neighbours the odd one on the sum's side is on the same side of every such place.
 __device__ __forceinline__ half_t half_of(float x, float rest) {
-    const int bits = static_cast<int>(__float_as_uint(x)), away = ((bits ^ static_cast<int>(__float_as_uint(rest))) >> 31) | 1;
-    const bool moves = (rest != 0.0f) & ((bits & 1) == 0);
-    return static_cast<half_t>(__uint_as_float(static_cast<uint32_t>(bits + (moves ? away : 0))));
+    const int bits = static_cast<int>(__float_as_uint(x)), under = (bits ^ static_cast<int>(__float_as_uint(rest))) >> 31;
+    return static_cast<half_t>(__uint_as_float(static_cast<uint32_t>(rest != 0.0f ? (bits + under) | 1 : bits)));
 }
 
 // x of the lane OFF (1 or 2) away among four.
@@ -112,16 +111,24 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
     half_t d = half_of(fifteenth, __builtin_fmaf(-fifteenth, 15.0f, width) + rest);
     const float step = static_cast<float>(d), least = difference(lo, kQ4First * step, rest);
     half_t b = half_of(least, rest);
-    const float first = difference(kQ4First * step, -static_cast<float>(b), rest);  // and rest: where code 64 is
+    const float first = __builtin_fmaf(kQ4First, step, static_cast<float>(b));
+    rest = __builtin_fmaf(kQ4First, step, static_cast<float>(b) - first);  // code 64 is at first and rest, which few groups have
     const float last = __builtin_fmaf(kQ4Last, step, static_cast<float>(b));
     constexpr float kOver = 65520.0f;  // what f16 rounds to infinity
     if (!(fabsf(first) < kOver && fabsf(last) < kOver)) d = b = static_cast<half_t>(NAN);
     pair = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, d)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
     const float per = step > 0.0f ? __builtin_amdgcn_rcpf(step) : 0.0f;
     float half[2] = {};  // of the word, as numbers
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = z[i] - first;
+    if (__any(rest != 0.0f)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] -= rest;
+    }
 #pragma unroll
     for (int i = 7; i >= 0; --i)
-        half[i & 1] = __builtin_fmaf(half[i & 1], 16.0f, __builtin_amdgcn_fmed3f(rintf(quotient(z[i] - first - rest, step, per)), 0.0f, 15.0f));
+        half[i & 1] = __builtin_fmaf(half[i & 1], 16.0f, __builtin_amdgcn_fmed3f(rintf(quotient(t[i], step, per)), 0.0f, 15.0f));
     return static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
 }
 
@@ -130,7 +137,7 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
 // read once for all of them.
 template <typename T, int D, bool INTERLEAVED, bool Q4>
 __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv, AppendArgs a) {
-    // Lanes per head row, head rows per wave step, steps requested together. Making 4-bit groups takes 130 instructions a step, which
+    // Lanes per head row, head rows per wave step, steps requested together. Making 4-bit groups takes 150 instructions a step, which
     // are not unrolled (4 / 3 / 2 / 1 steps: 4000 f16 tokens of 32 rows of 64 9.5 / 9.5 / 9.3 / 8.8 us, 400 of 128 5.8 / 5.6 / 5.3 / 5.1,
     // 8000 of 48 rows 36.2 / 36.5 / 37.6 / 35.1).
     constexpr int L = D / 8, RW = 64 / L, U = Q4 ? 1 : 4;
