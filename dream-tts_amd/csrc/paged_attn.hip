@@ -6,9 +6,11 @@
 // workgroup: 16 rows where a sequence has few, 128 where it has a chunk. A query's scores, softmax state (running maximum,
 // running sum) and output sums are f32; q, k, v are f16 as the cache and the matrix cores hold them;
 // the weights e^(s - max) are rounded to f16 for the second product, and the output is rounded once. The weights are
-// held times 2^kBias (it cancels in the division by their sum), at the upper end of f16's range: down to 2^(-14 - kBias) of
-// the largest each is off by 2^-11 relative at most, as the output's own rounding is, and below that by 2^(-25 - kBias) of
-// the largest. Without it a flat tail far under one leading key would leave the numerator and stay in the denominator
+// held times 2^bias (it cancels in the division by their sum), the largest of a tile at 2^bias at least, toward the upper end of
+// f16's range: down to 2^(-14 - bias) of the largest each is off by 2^-11 relative at most, as the output's own rounding is,
+// and below that by 2^(-25 - bias) of the largest. The bias is kBias = 15 in the 16-row tiles over f16 pages, kChunkBias = 11 in
+// those over 4-bit pages and in the 128-row ones, whose maximum may lag. Without it a flat tail far under one leading key would
+// leave the numerator and stay in the denominator
 // (65000 keys e^-17.5 below one: all of their 0.16 %). For the same reason a tile's weights are summed before they meet
 // the running sum, next to which a single one may be nothing.
 #include <cfloat>
@@ -234,9 +236,9 @@ __device__ __forceinline__ float max_16_32_apart(float x) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// What the exponents of the weights are raised by. The 16-row tiles' largest weight is 2^15, the 128-row ones' up to
-// 2^kSlack times 2^kChunkBias (their maximum may lag behind by that): both under f16's 65504. kSlack 1 / 4 / 8 (and a
-// bias that goes with it): 2048 tokens after 7952 335 / 333 / 335 us.
+// What the exponents of the weights are raised by. The largest weight of the 16-row tiles over f16 pages is 2^kBias; of those over
+// 4-bit pages and of the 128-row ones it is 2^kChunkBias to 2^(kChunkBias + kSlack), as their maximum may lag behind by kSlack: all
+// under f16's 65504. kSlack 1 / 4 / 8 (and a bias that goes with it): 2048 tokens after 7952 335 / 333 / 335 us.
 constexpr float kBias = 15.0f, kSlack = 4.0f, kChunkBias = 11.0f;
 // A weight's exponent is fma(q . k, scale2, -m2), m2 the rounded product of the maximum: off by half of m2's last place,
 // alike for all keys that a wave takes relative to one maximum, so that it cancels among them as a bias does, but not
