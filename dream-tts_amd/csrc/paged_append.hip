@@ -162,9 +162,18 @@ __global__ __launch_bounds__(256) void qk_rope_append_paged_kernel(const T *qkv,
     };
     int r0 = part * RW + lane / L;
     load(r0);
-    int first, n, len;
-    const int s = a.batch.sequence_of(t, first, n, len);
-    if (s >= a.batch.b) return;
+    // Starts and lengths in one trip where a step is long (4-bit rows: 4436 tokens 11.0 -> 9.7 us); with four rows under way the trip
+    // that this saves is hidden, and its instructions are not (f16 rows: 800 tokens 5.71 -> 5.96, 300 of as many sequences 4.6 -> 4.73).
+    int first, n, len, s;
+    if constexpr (Q4) {
+        s = a.batch.sequence_of(t, first, n, len);
+        if (s >= a.batch.b) return;
+    } else {
+        s = a.batch.sequence_of(t);
+        if (s >= a.batch.b) return;
+        a.batch.rows(s, first, n);
+        len = a.batch.length(s);
+    }
     const int pos = len - n + (t - first);
     if (t < first || t >= first + n || pos < 0 || pos >= a.table_len) return;
     const int page = a.batch.page(s, pos >> a.batch.page_shift);
