@@ -653,6 +653,8 @@ extern "C" int dtts_claim_pages(int32_t *pages, int32_t *refs, const int32_t *q_
     const char *name = "dtts_claim_pages";
     DTTS_REQUIRE_TABLE(name, b, max_pages, n_pages);
     DTTS_REQUIRE_PAGE(name, page, max_pages);
+    DTTS_REQUIRE(b * max_pages <= (int64_t(1) << 31) - kNT, "%s: a table of %lld x %lld has items past an int in its last round", name,
+                 (long long)b, (long long)max_pages);
     // counts and `lacking` are read and written without sequences too
     DTTS_REQUIRE(lacking && refs && aligned(lacking, 4) && aligned(refs, 4), "%s: counts or lacking null or misaligned", name);
     const size_t need = b > 0 ? dtts_claim_pages_workspace_bytes(b, max_pages, n_pages) : 0;

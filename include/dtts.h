@@ -571,7 +571,7 @@ int dtts_unpack_pages_q4(const void *kpages, const void *vpages, const int32_t *
  * hold each page; under 1 the page is free. What each call reads and writes is on the device, so all of them can be captured; a
  * result depends on its arguments alone (free pages are given out from the lowest id on, sequences are served in order). One
  * table serves every layer's pools: ids are decided once, and dtts_copy_pages carries out what has to be copied in all of them.
- * n_pages <= 2^24, b <= 65536, b * max_pages < 2^31. Calls on one table or refs are ordered by the caller, and a call's
+ * n_pages <= 2^24, b <= 65536, b * max_pages < 2^31 (claims: up to 2^31 - 1024). Calls on one table or refs are ordered by the caller, and a call's
  * operands share no memory (refused).
  *
  * dtts_fork_pages: row i of `out` [n, max_pages] takes the entries of row parent[i] of page_table [b, max_pages] (outside

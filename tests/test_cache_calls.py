@@ -131,6 +131,12 @@ def test_claim(match, bad):
     claim(match, **bad)
 
 
+@pytest.mark.parametrize("b,m,match", [(2047, 1049088, "past an int"), (2047, 1049087, "workspace of")])
+def test_claim_of_tables_whose_last_round_passes_an_int(b, m, match):
+    """2^31 - 512 entries; and 2^31 - 2559, which is told by what is refused next."""
+    claim(match, b=b, m=m, ws_bytes=0)
+
+
 @pytest.mark.parametrize("match,refs,lacking", [
     ("counts or lacking", None, BIG), ("counts or lacking", 2, BIG), ("counts or lacking", 0, None), ("share memory", 0, 32),
 ])
