@@ -144,11 +144,15 @@ Tensor workspace_of(Args &a, int i, size_t need, const Tensor &like) {
 }
 
 // Several int32 arrays in one allocation: `of` takes the next n of them (each allocation, or view by torch's own way, takes as
-// long as a quarter of a launch).
+// long as a quarter of a launch). Whoever keeps one of them keeps all, so scratch of more than kScratchHere is apart.
+constexpr int64_t kScratchHere = 1 << 18;
 struct Ints {
     Tensor all;
     int64_t at = 0;
     Ints(const Tensor &like, int64_t n) : all(at::empty({n}, like.options().dtype(at::kInt).requires_grad(false))) {}
+    // The last of the arrays: n ints of scratch, of which `all` was made with scratch_here(n).
+    Tensor scratch(int64_t n) { return n > kScratchHere ? at::empty({n}, all.options()) : of(n); }
+    static int64_t scratch_here(int64_t n) { return n > kScratchHere ? 0 : n; }
     Tensor of(int64_t n) {
         Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
         t.unsafeGetTensorImpl()->set_storage_offset(at);
@@ -328,8 +332,8 @@ PyObject *claim(PyObject *const *args) {
     const int64_t need = args[5] == Py_None ? static_cast<int64_t>(dtts_claim_pages_workspace_bytes(t.b, t.max_pages, t.n_pages)) / 4 : 0;
     const Tensor *given = a.maybe(5, at::kByte);
     if (!a.ok) return none();
-    Ints all(*t.pages, 2 * t.b + 1 + need);
-    const Tensor src = all.of(t.b), dst = all.of(t.b), lacking = all.of(1), ws = given ? *given : all.of(need);
+    Ints all(*t.pages, 2 * t.b + 1 + Ints::scratch_here(need));
+    const Tensor src = all.of(t.b), dst = all.of(t.b), lacking = all.of(1), ws = given ? *given : all.scratch(need);
     const int status = dtts_claim_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(start), data<int32_t>(context),
                                         data<int32_t>(&src), data<int32_t>(&dst), data<int32_t>(&lacking), t.b, page, t.max_pages,
                                         t.n_pages, ws.data_ptr(), ws.nbytes(), a.stream());
@@ -357,8 +361,8 @@ PyObject *compact(PyObject *const *args) {
     const Tensor *given = a.maybe(2, at::kByte);
     if (!a.ok) return none();
     const int64_t need = given ? 0 : static_cast<int64_t>(dtts_compact_pages_workspace_bytes(t.n_pages)) / 4;
-    Ints all(*t.pages, 2 * t.n_pages + 1 + need);
-    const Tensor src = all.of(t.n_pages), dst = all.of(t.n_pages), used = all.of(1), ws = given ? *given : all.of(need);
+    Ints all(*t.pages, 2 * t.n_pages + 1 + Ints::scratch_here(need));
+    const Tensor src = all.of(t.n_pages), dst = all.of(t.n_pages), used = all.of(1), ws = given ? *given : all.scratch(need);
     const int status = dtts_compact_pages(data<int32_t>(t.pages), data<int32_t>(t.refs), data<int32_t>(&src), data<int32_t>(&dst),
                                           data<int32_t>(&used), t.b, t.max_pages, t.n_pages, ws.data_ptr(), ws.nbytes(), a.stream());
     return status == DTTS_OK ? tuple_of({src, dst, used}) : none();

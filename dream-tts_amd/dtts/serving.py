@@ -4,8 +4,9 @@ pages' forks, claims, trims, moves and copies, and sampling.
 
 A step of a batch is: project to qkv, ``qk_rope_append_paged`` (queries turned, keys and values into
 their pages), ``paged_attention``, the output projection, and after the last layer logits to
-``sample``. Before a step, ``claim_pages`` gives each sequence the pages that its new tokens go to. Lengths, positions, page tables and sampling settings are device tensors, so a step
-captured into a graph is replayed while they change. Outputs are allocated unless given.
+``sample``. Before a step, ``claim_pages`` gives each sequence the pages that its new tokens go to. Lengths, positions,
+page tables and sampling settings are device tensors, so a step captured into a graph is replayed while they change. Outputs
+are allocated unless given.
 
 Every tensor of a call is on one device; the work goes to that device's current stream.
 
@@ -249,7 +250,8 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
     """Attention of a ragged batch's new tokens over their pages (f16, or 4-bit ones as qk_rope_append_paged
     writes them), their own keys included: q [tokens, heads, D] f16 (rows may be strided) -> [tokens, heads,
     D] f16. Each token attends to its sequence's positions up to its own, when `window` is set to the last
-    `window` of them and to the sequence's first `sinks`. max_q and max_context (the longest chunk and context)
+    `window` of them and to the sequence's first `sinks` (whose keys stay turned by their own positions, as the append wrote
+    them: a token is as far from them as its position says, not as its window does). max_q and max_context (the longest chunk and context)
     size the launch and never change what is computed. `workspace`: a device byte tensor of
     paged_attention_workspace_bytes (allocated when not given). Rows of `out` that belong to no sequence are
     left as they were; a token that sees no position gets zeros. `out` shares no memory with q."""
@@ -357,7 +359,7 @@ def claim_pages(pages, refs, q_start, context, page, workspace=None):
     ones come from the free pages (refs under 1), lowest first, and a page that other sequences hold too is replaced.
     pages [b, max_pages] and refs [n_pages] change in place; returns (src, dst, lacking) int32 [b], [b], [1]: copy_pages carries
     src and dst out in every layer's pools, and where lacking is above 0 there were that many free pages too few and nothing was
-    changed: the step must wait."""
+    changed: the step must wait. The three are parts of one allocation, with up to 1 MB of the call's scratch: a clone keeps less."""
     y = _serving.claim_pages(pages, refs, q_start, context, page, workspace)
     if y is not None:
         return y
@@ -389,7 +391,8 @@ def compact_pages_workspace_bytes(n_pages):
 def compact_pages(pages, refs, workspace=None):
     """Gives the pages in use the first ids, so that a pool can end after them: pages and refs change in place; returns (src, dst,
     used) int32 [n_pages], [n_pages], [1]: the moves that copy_pages carries out in every layer's pools, and how many pages are
-    in use. Other tables over the same pools hold none of these ids any more."""
+    in use. Other tables over the same pools hold none of these ids any more. The three are parts of one allocation, with up to 1 MB
+    of the call's scratch: a clone keeps less."""
     y = _serving.compact_pages(pages, refs, workspace)
     if y is not None:
         return y

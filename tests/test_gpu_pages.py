@@ -174,6 +174,16 @@ def test_compact_of_no_and_of_all_pages(dev):
         assert all(np.array_equal(x, y) for x, y in zip(host(t, r, src, dst), want)) and int(used) == want[4]
 
 
+def test_results_that_are_kept_hold_little_else(dev, path):
+    """The parts of one allocation, and a megabyte of scratch at most."""
+    table, refs = up(np.full((400, 1000), -1), dev), up(np.zeros(300000), dev)
+    start, c = up(np.arange(401), dev), up(np.ones(400), dev)
+    for got in (serving.claim_pages(table, refs, start, c, 16), serving.compact_pages(table, refs)):
+        for t in got:
+            assert t.untyped_storage().nbytes() <= 4 * sum(x.numel() for x in got) + (1 << 20)
+    assert sorted(table[:, 0].tolist()) == list(range(400)) and int(refs.sum()) == 400
+
+
 def test_tables_without_rows(dev, path):
     t, r, one = up(np.zeros((0, 4)), dev), up([1, 0, 2], dev), up([0], dev)
     assert [x.numel() for x in serving.claim_pages(t, r, one, t.view(-1), 16)] == [0, 0, 1]
