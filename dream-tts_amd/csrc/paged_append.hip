@@ -18,8 +18,8 @@
 // half-split, four pairs' first and second members; interleaved, eight neighbours (four pairs), so
 // both layouts turn in registers and the norm is a shuffle sum over D/8 lanes. At a decode step's
 // sizes it is the chain of dependent reads that counts (q_start -> context -> page id and table
-// rows): qkv is requested before it, and its ends overlap. Into 4-bit pages: 48 f32 tokens of 32 rows of 128 (2.6 MB) 3.9 us;
-// 4436 f16 tokens of 32 rows of 64 (30 MB) 9.9 us, half of it vector issue, the rest the chain, which a wave a token meets once.
+// rows): qkv is requested before it, and its ends overlap. Into 4-bit pages: 48 f32 tokens of 32 rows of 128 (2.6 MB) 3.7 us;
+// 4436 f16 tokens of 32 rows of 64 (30 MB) 9.9 us (launches one after another of a graph 3.4 and 9.15), half of it vector issue, the rest the chain, which a wave a token meets once.
 #include <cmath>
 
 #include "norm_rope.hpp"

@@ -357,7 +357,7 @@ struct KvTile {
 // Of 4-bit pages a lane has 16 or 32 neighbouring dimensions of its key (one load and their pair), and of the values a word
 // of four keys at once (one load) with their pairs (another). The words are turned before they become numbers: halves of two
 // keys' words make pairs of keys, which is what the product's operand holds. 5 tokens of 32 heads over 4 and up to 65000 keys (132
-// MB): 27.6 us, 4.8 TB/s, vector issue 0.63 of the cycles; 48 of 16 over 8 and up to 1536 (49 MB): 15.8, of which one key each takes 6.
+// MB): 27.4 us, 4.8 TB/s, vector issue 0.63 of the cycles; 48 of 16 over 8 and up to 1536 (49 MB): 15.5, of which one key each takes 6.
 template <int D, bool ONCE>
 struct KvTile<D, true, ONCE> {
     static constexpr int E = D / 16, W = D / 32;  // W: key words a lane holds
@@ -1324,13 +1324,15 @@ constexpr int64_t kFillShared = 1024, kShareBytes = int64_t(64) << 20;
 // in the 256 MB cache before the memory, they are read past it. Over others' data in between, 64 tokens under a window of 2048 (f16,
 // D = 64, 134 MB) 32.5 us kept and 28.5 so, 5 over up to 65000 (4 bits, 132 MB) 34.4 and 32.4; again over the same data 27.7 and
 // 28.5, 27.1 and 27.8; 48 over up to 1536 (4 bits, 49 MB) 17.6 and 17.9. With two tiles (30 sequences of 6 tokens of 4 heads over 20000,
-// f16) 530 and 711. f16 pages without sinks are kept: 5 over up to 65000 of D = 64 33.0 and 39.4 over the same data.
+// f16) 530 and 711. The host knows the longest context alone, which stands for all of them: a batch with one long sequence among short
+// ones is read past the caches although its keys would stay there, at those 3 %. f16 pages without sinks are kept: 5 over up to 65000 of D = 64 33.0 and 39.4 over the same data.
 constexpr double kKeptBytes = 128 << 20;
 
 // How far to cut 128-row tiles over 4-bit pages or with sinks. A tile's time is a fixed part and one for each 64 keys, which
 // depend on how many workgroups share its CU (us; 128 and 1152 keys on 2, 256 and 512 workgroups, D = 64 then 128, three
 // of D = 64 taken to go on like that): cut, more of them run at once, but each begins anew, and their states are joined. Of the
-// cuts that fill the chip once or a few times, the cheapest by that. 700 and 615 tokens of 8 query heads under a window of 1000
+// cuts that fill the chip once or a few times, the cheapest by that. (Fitted on one card: another one's times would choose other
+// cuts, never other results but for their last bits. Batches over f16 pages without sinks keep kFillLarge.) 700 and 615 tokens of 8 query heads under a window of 1000
 // (166 tiles): 46 us in two, 38 uncut; 1025 of 4 after 5975 (264 tiles): 202 in two, 179 in three.
 inline int64_t cheapest_cut(int64_t wgs, int64_t blocks, int64_t rows, int64_t hd) {
     struct Tile {
