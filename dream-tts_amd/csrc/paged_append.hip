@@ -111,8 +111,7 @@ __device__ __forceinline__ uint32_t quantise(const float (&z)[8], uint32_t &pair
     half_t d = half_of(fifteenth, __builtin_fmaf(-fifteenth, 15.0f, width) + rest);
     const float step = static_cast<float>(d), least = difference(lo, kQ4First * step, rest);
     half_t b = half_of(least, rest);
-    const float first = __builtin_fmaf(kQ4First, step, static_cast<float>(b));
-    rest = __builtin_fmaf(kQ4First, step, static_cast<float>(b) - first);  // code 64 is at first and rest, which few groups have
+    const float first = difference(kQ4First * step, -static_cast<float>(b), rest);  // code 64 is at first and rest, which few groups have
     const float last = __builtin_fmaf(kQ4Last, step, static_cast<float>(b));
     constexpr float kOver = 65520.0f;  // what f16 rounds to infinity
     if (!(fabsf(first) < kOver && fabsf(last) < kOver)) d = b = static_cast<half_t>(NAN);

@@ -118,7 +118,8 @@ def test_append_of_f16_values_takes_the_codes_of_the_definition(dev):
 
 def hard_groups(rng, n):
     """Groups [5 n, 32] of f32 numbers: whose width over 15, and whose least number less 64 steps, are next to half way between two
-    f16 numbers, nearer than f32 can tell; narrow ones far from zero, whose first code is no f32 number; wider ones; ordinary ones."""
+    f16 numbers, nearer than f32 can tell; narrow ones far from zero, whose first code is no f32 number; ones whose least number is 64
+    steps and next to nothing; ordinary ones."""
     f = np.float32
     d = rng.randint(1024, 2048, n) * 2.0 ** rng.randint(-13, -3, n)
     sign = rng.choice([-1, 1], n)
@@ -136,9 +137,9 @@ def hard_groups(rng, n):
     half = np.spacing(np.abs(least)).astype(np.float64) / 2
     lo = np.nextafter((least.astype(np.float64) + half + 64 * d).astype(f), (sign * 1e9).astype(f)).astype(np.float64)
     at = sign * 10 ** rng.uniform(-2, 3.3, n)
-    wide = rng.randn(n) * 3
+    near = 64 * d + sign * 2.0 ** rng.uniform(-24, -10, n)
     return np.concatenate([ends(low, tie), ends(lo, lo + 15 * d), ends(at, at + 10 ** rng.uniform(-5, -1, n)),
-                           ends(wide, wide + 10 ** rng.uniform(-3, 1, n)), rng.randn(n, 32).astype(f)])
+                           ends(near, near + 15 * d), rng.randn(n, 32).astype(f)])
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
