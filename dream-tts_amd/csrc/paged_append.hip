@@ -11,15 +11,17 @@
 //   d = f16((max - min) / 15), b = f16(min - 64 d), n = rint((x - (64 d + b)) / d) from 0 to 15
 // The pair's two roundings are those of the exact numbers, and b is rounded before the codes are chosen, so the steps lie where
 // the values read back do. 64 d + b takes two f32 numbers (one where they nearly cancel; a narrow group far from zero needs the
-// other). A code is the definition's unless its value lies within 2^-18 of a step of the border between two. A lane needs eight neighbours of a row, a group being four lanes: half-split
-// rows, whose lanes hold two groups of four apart, meet in LDS, a wave's rows in its own.
+// other). A code is the definition's unless its value lies within 2^-18 of a step of the border between two. A lane needs eight
+// neighbours of a row, a group being four lanes: half-split rows, whose lanes hold two groups of four apart, meet in LDS, a wave's
+// rows in its own.
 //
 // HBM-bound: qkv in, q, k and v out, once. D/8 lanes own a head row, two groups of four elements each:
 // half-split, four pairs' first and second members; interleaved, eight neighbours (four pairs), so
 // both layouts turn in registers and the norm is a shuffle sum over D/8 lanes. At a decode step's
 // sizes it is the chain of dependent reads that counts (q_start -> context -> page id and table
 // rows): qkv is requested before it, and its ends overlap. Into 4-bit pages: 48 f32 tokens of 32 rows of 128 (2.6 MB) 3.7 us;
-// 4436 f16 tokens of 32 rows of 64 (30 MB) 9.9 us (launches one after another of a graph 3.4 and 9.15), half of it vector issue, the rest the chain, which a wave a token meets once.
+// 4436 f16 tokens of 32 rows of 64 (30 MB) 9.9 us (launches one after another of a graph 3.4 and 9.15), half of it vector issue,
+// the rest the chain, which a wave a token meets once.
 #include <cmath>
 
 #include "norm_rope.hpp"
@@ -78,8 +80,8 @@ __device__ __forceinline__ float difference(float x, float y, float &rest) {
 // x + rest, less than a last place from x, as the f16 number next to it. Rounded to f32 before, the sum could fall half way between
 // two f16 numbers; of x and its neighbours the odd one on the sum's side is on the same side of every such place.
 __device__ __forceinline__ half_t half_of(float x, float rest) {
-    const int bits = static_cast<int>(__float_as_uint(x)), under = (bits ^ static_cast<int>(__float_as_uint(rest))) >> 31;
-    return static_cast<half_t>(__uint_as_float(static_cast<uint32_t>(rest != 0.0f ? (bits + under) | 1 : bits)));
+    const uint32_t bits = __float_as_uint(x), away = (bits ^ __float_as_uint(rest)) >> 31;  // 1: the sum is nearer to zero than x
+    return static_cast<half_t>(__uint_as_float(rest != 0.0f ? (bits - away) | 1u : bits));
 }
 
 // x of the lane OFF (1 or 2) away among four.

@@ -10,9 +10,8 @@
 // f16's range: down to 2^(-14 - bias) of the largest each is off by 2^-11 relative at most, as the output's own rounding is,
 // and below that by 2^(-25 - bias) of the largest. The bias is kBias = 15 in the 16-row tiles over f16 pages, kChunkBias = 11 in
 // those over 4-bit pages and in the 128-row ones, whose maximum may lag. Without it a flat tail far under one leading key would
-// leave the numerator and stay in the denominator
-// (65000 keys e^-17.5 below one: all of their 0.16 %). For the same reason a tile's weights are summed before they meet
-// the running sum, next to which a single one may be nothing.
+// leave the numerator and stay in the denominator (65000 keys e^-17.5 below one: all of their 0.16 %). For the same reason a
+// tile's weights are summed before they meet the running sum, next to which a single one may be nothing.
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -1325,15 +1324,16 @@ constexpr int64_t kFillShared = 1024, kShareBytes = int64_t(64) << 20;
 // D = 64, 134 MB) 32.5 us kept and 28.5 so, 5 over up to 65000 (4 bits, 132 MB) 34.4 and 32.4; again over the same data 27.7 and
 // 28.5, 27.1 and 27.8; 48 over up to 1536 (4 bits, 49 MB) 17.6 and 17.9. With two tiles (30 sequences of 6 tokens of 4 heads over 20000,
 // f16) 530 and 711. The host knows the longest context alone, which stands for all of them: a batch with one long sequence among short
-// ones is read past the caches although its keys would stay there, at those 3 %. f16 pages without sinks are kept: 5 over up to 65000 of D = 64 33.0 and 39.4 over the same data.
+// ones is read past the caches although its keys would stay there, at those 3 %. f16 pages without sinks are kept: 5 over up to
+// 65000 of D = 64 33.0 and 39.4 over the same data.
 constexpr double kKeptBytes = 128 << 20;
 
 // How far to cut 128-row tiles over 4-bit pages or with sinks. A tile's time is a fixed part and one for each 64 keys, which
 // depend on how many workgroups share its CU (us; 128 and 1152 keys on 2, 256 and 512 workgroups, D = 64 then 128, three
 // of D = 64 taken to go on like that): cut, more of them run at once, but each begins anew, and their states are joined. Of the
 // cuts that fill the chip once or a few times, the cheapest by that. (Fitted on one card: another one's times would choose other
-// cuts, never other results but for their last bits. Batches over f16 pages without sinks keep kFillLarge.) 700 and 615 tokens of 8 query heads under a window of 1000
-// (166 tiles): 46 us in two, 38 uncut; 1025 of 4 after 5975 (264 tiles): 202 in two, 179 in three.
+// cuts, never other results but for their last bits. Batches over f16 pages without sinks keep kFillLarge.) 700 and 615 tokens of 8
+// query heads under a window of 1000 (166 tiles): 46 us in two, 38 uncut; 1025 of 4 after 5975 (264 tiles): 202 in two, 179 in three.
 inline int64_t cheapest_cut(int64_t wgs, int64_t blocks, int64_t rows, int64_t hd) {
     struct Tile {
         float fixed, block;

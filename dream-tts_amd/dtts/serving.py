@@ -251,10 +251,10 @@ def paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_con
     writes them), their own keys included: q [tokens, heads, D] f16 (rows may be strided) -> [tokens, heads,
     D] f16. Each token attends to its sequence's positions up to its own, when `window` is set to the last
     `window` of them and to the sequence's first `sinks` (whose keys stay turned by their own positions, as the append wrote
-    them: a token is as far from them as its position says, not as its window does). max_q and max_context (the longest chunk and context)
-    size the launch and never change what is computed. `workspace`: a device byte tensor of
-    paged_attention_workspace_bytes (allocated when not given). Rows of `out` that belong to no sequence are
-    left as they were; a token that sees no position gets zeros. `out` shares no memory with q."""
+    them: a token is as far from them as its position says, not as its window does). max_q and max_context (the
+    longest chunk and context) size the launch and never change what is computed. `workspace`: a device byte tensor
+    of paged_attention_workspace_bytes (allocated when not given). Rows of `out` that belong to no sequence are left
+    as they were; a token that sees no position gets zeros. `out` shares no memory with q."""
     y = _serving.paged_attention(q, k_pages, v_pages, q_start, context, pages, max_q, max_context, scale, window, out, workspace,
                                  sinks)
     if y is not None:

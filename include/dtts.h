@@ -528,8 +528,9 @@ int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dt
                              int64_t window, float scale, void *workspace, size_t ws_bytes, hipStream_t stream);
 
 /* The same with `sinks`: beside its window a token sees the sequence's first `sinks` positions (those up to its own), so a stream can
- * run on past its window over the first tokens that its attention rests on. Their keys stay turned by their own positions. Pages that hold neither may be freed
- * (dtts_trim_pages). Without a window sinks count for nothing. And over pages of `bits`: 16, as above, or 4.
+ * run on past its window over the first tokens that its attention rests on. Their keys stay turned by their own positions. Pages
+ * that hold neither may be freed (dtts_trim_pages). Without a window sinks count for nothing. And over pages of `bits`: 16, as
+ * above, or 4.
  *
  * 4-bit pages take 5 D / 8 bytes a row in the place of 2 D. kpages and vpages are bytes, 16-byte aligned; page_stride counts
  * bytes (a multiple of 16, at least n_kv * page * 5 D / 8, under 2^32). A row's values in groups of 32 share an f16 pair
@@ -539,8 +540,9 @@ int dtts_paged_attention_f16(const dtts_f16 *q, const dtts_f16 *kpages, const dt
  *
  * dtts_qk_rope_append_paged_q4_*: dtts_qk_rope_append_paged_* into 4-bit pages. Of a group's f32 values
  * d = f16((max - min) / 15), b = f16(min - 64 d), n = (x - (64 d + b)) / d rounded to the nearest (ties to even) from 0 to 15
- * (0 where d is 0; a value within 2^-18 of a step of the border between two codes may take either). A group with a value that is not finite, or whose values pass f16's range in this form (its least minus
- * 4.27 times its width, where the width is its largest less its least), is NaN, all 32.
+ * (0 where d is 0; a value within 2^-18 of a step of the border between two codes may take either). A group with a value that
+ * is not finite, or whose values pass f16's range in this form (its least minus 4.27 times its width, where the width is its
+ * largest less its least), is NaN, all 32.
  * dtts_unpack_pages_q4: the f16 pages [n, n_kv, page, D] that the pages ids[0 .. n - 1] (DEVICE; NULL: the first n) stand for,
  * whatever their slots hold; an id outside [0, n_pages) leaves its part as it was. */
 size_t dtts_paged_attention_sinks_workspace_bytes(int32_t bits, int64_t tokens, int64_t b, int64_t heads, int64_t n_kv,
@@ -571,8 +573,8 @@ int dtts_unpack_pages_q4(const void *kpages, const void *vpages, const int32_t *
  * hold each page; under 1 the page is free. What each call reads and writes is on the device, so all of them can be captured; a
  * result depends on its arguments alone (free pages are given out from the lowest id on, sequences are served in order). One
  * table serves every layer's pools: ids are decided once, and dtts_copy_pages carries out what has to be copied in all of them.
- * n_pages <= 2^24, b <= 65536, b * max_pages < 2^31 (claims: up to 2^31 - 1024). Calls on one table or refs are ordered by the caller, and a call's
- * operands share no memory (refused).
+ * n_pages <= 2^24, b <= 65536, b * max_pages < 2^31 (claims: up to 2^31 - 1024). Calls on one table or refs are ordered by the
+ * caller, and a call's operands share no memory (refused).
  *
  * dtts_fork_pages: row i of `out` [n, max_pages] takes the entries of row parent[i] of page_table [b, max_pages] (outside
  * [0, b): -1 in all of them), and refs follow: forks, reorders beams and frees rows in one step. out is another table, or
